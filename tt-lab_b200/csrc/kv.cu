@@ -1,0 +1,1127 @@
+// kv.cu -- the paged key/value cache: the batch's plan, append with rotation,
+// read, and the C ABI of include/ttl_kv.h.  The attention kernels are in
+// kv_attend.cu.
+//
+// Reference: store_kv and apply_rope of tt-lab (src/model.cpp:230-253), there
+// for one token of one sequence in a contiguous f32 cache.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <string>
+
+#include "internal.h"
+#include "kv.cuh"
+#include "kv_internal.h"
+#include "ttl_kv.h"
+
+namespace {
+
+using namespace ttl::kv;
+
+// ---- plan ----
+
+struct PlanArgs {
+    Plan *plan;
+    Tile *tiles[2][2];
+    int32_t *prefix[2][2];
+    Cut *cuts[2][2];
+    int4 *row[2];
+    int4 *seq;
+    uint32_t *counters;
+    uint32_t *status;
+    const int32_t *row_start, *length, *pages, *first, *prefix_len;
+    uint32_t page_stride;
+    int seqs, rows, max_new, group, kv_heads, window, page_tokens;
+    int width[2], gran[2], ctas[2];  // ctas 0: no sequence goes to this kind
+    int few;                         // sequences of at most this many columns go to kind 0
+    int tile_cap[2];
+};
+
+constexpr int kPlanThreads = 1024;
+constexpr int kMaxPosition = 1 << 30;
+
+struct SeqState {
+    int row0, n, len;
+    bool good;
+};
+
+__device__ SeqState load_seq(const PlanArgs &a, int s) {
+    SeqState r;
+    r.row0 = a.row_start[s];
+    const int end = a.row_start[s + 1];
+    r.len = a.length[s];
+    const bool order = r.row0 >= 0 && end >= r.row0 && end <= a.rows;
+    r.n = order ? end - r.row0 : 0;
+    const long long room = (long long)(a.page_stride) * a.page_tokens;
+    r.good = order && r.len >= r.n && r.len <= room && r.len <= kMaxPosition && r.n <= a.max_new;
+    if (!r.good) {
+        r.n = 0;
+        r.len = 0;
+    }
+    return r;
+}
+
+// Exclusive scan of one int per thread over the block; total in *sum.
+__device__ int block_scan(int v, int *sum, int *warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        x += lane >= o ? y : 0;
+    }
+    if (lane == 31) {
+        warp_sums[warp] = x;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int y = warp_sums[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, y, o);
+            y += lane >= o ? z : 0;
+        }
+        warp_sums[lane] = y;
+    }
+    __syncthreads();
+    const int base = warp ? warp_sums[warp - 1] : 0;
+    *sum = warp_sums[31];
+    __syncthreads();
+    return base + x - v;
+}
+
+// CTAs 0 .. 3 build the tile list of (kind, window); the others write the rows'
+// visible ranges.  Everything is read from the caller's arrays, so no CTA
+// waits for another.  Latency-bound: a few dependent loads and three scans.
+__global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
+    __shared__ int sums[32];
+    __shared__ int starts[4096 + 1];  // first tile of a sequence
+    __shared__ Cut shared_cuts[kMaxCtas + 1];
+    const int tid = threadIdx.x;
+    if (blockIdx.x >= 4) {
+        const int r = (blockIdx.x - 4) * kPlanThreads + tid;
+        if (r >= a.rows) {
+            return;
+        }
+        int lo = 0, hi = a.seqs;  // last sequence with row_start <= r
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (a.row_start[mid] <= r) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        SeqState s = load_seq(a, lo);
+        if (!(s.good && r >= s.row0 && r < s.row0 + s.n) && r < a.row_start[a.seqs]) {
+            // row_start is out of order: the first good sequence that claims the row
+            for (lo = 0; lo < a.seqs - 1; ++lo) {
+                s = load_seq(a, lo);
+                if (s.good && r >= s.row0 && r < s.row0 + s.n) {
+                    break;
+                }
+            }
+            s = load_seq(a, lo);
+        }
+        int4 full = make_int4(0, 0, 0, -1), slide = full;
+        if (s.good && r >= s.row0 && r < s.row0 + s.n) {
+            const int p = s.len - s.n + r - s.row0;
+            const int first = a.first ? a.first[r] : 0;
+            const int end = a.prefix_len ? min(max(p + 1, a.prefix_len[lo]), s.len) : p + 1;
+            full = make_int4(p, max(first, 0), end, lo);
+            slide = make_int4(p, max(max(first, 0), p - a.window + 1), end, lo);
+        }
+        a.row[0][r] = full;
+        a.row[1][r] = slide;
+        return;
+    }
+    const int kind = blockIdx.x >> 1, sliding = blockIdx.x & 1;
+    if (blockIdx.x == 0 && tid == 0) {
+        a.plan->pages = a.pages;
+        a.plan->page_stride = a.page_stride;
+        a.plan->seqs = a.seqs;
+        if (a.row_start[0] != 0) {
+            ttl::set_status(a.status, kKvBadBatch);
+        }
+    }
+    if (!sliding) {  // the merge counters of the kind start at zero
+        for (int i = tid; i < kMaxCtas; i += kPlanThreads) {
+            a.counters[kind * kMaxCtas + i] = 0;
+        }
+    }
+    if (sliding && a.window == 0) {
+        if (tid == 0) {
+            a.plan->list[kind][1] = List{0, 0, 0, 0, 0, {0, 0, 0}};
+        }
+        return;
+    }
+    const int width = a.width[kind], gran = a.gran[kind];
+    Tile *tiles = a.tiles[kind][sliding];
+    int32_t *prefix = a.prefix[kind][sliding];
+    Cut *cuts = a.cuts[kind][sliding];
+    // tiles of each sequence
+    int total = 0;
+    for (int base = 0; base < a.seqs; base += kPlanThreads) {
+        const int s = base + tid;
+        int count = 0;
+        if (s < a.seqs) {
+            const SeqState q = load_seq(a, s);
+            if (!q.good && blockIdx.x == 0) {
+                ttl::set_status(a.status, kKvBadBatch);
+            }
+            const int columns = q.n * a.group;
+            const bool mine = (columns <= a.few) == (kind == 0);
+            count = (mine && columns > 0) ? (columns + width - 1) / width : 0;
+            if (blockIdx.x == 0) {
+                a.seq[s] = make_int4(q.row0, q.n, q.len, 0);
+            }
+        }
+        int sum;
+        const int at = block_scan(count, &sum, sums);
+        if (s < a.seqs) {
+            starts[s] = total + at;
+        }
+        total += sum;
+    }
+    if (a.ctas[kind] == 0) {
+        total = 0;  // no launch of this kind follows
+    }
+    if (total > a.tile_cap[kind]) {
+        if (tid == 0) {
+            ttl::set_status(a.status, kKvBadBatch);
+        }
+        total = 0;
+    }
+    if (tid == 0) {
+        starts[a.seqs] = total;
+    }
+    __syncthreads();
+    // their key ranges
+    int line = 0;
+    for (int base = 0; base < total; base += kPlanThreads) {
+        const int t = base + tid;
+        int n = 0;
+        if (t < total) {
+            int lo = 0, hi = a.seqs;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (starts[mid] <= t) {
+                    lo = mid;
+                } else {
+                    hi = mid;
+                }
+            }
+            const SeqState q = load_seq(a, lo);
+            const int col0 = (t - starts[lo]) * width;
+            const int ncols = min(width, q.n * a.group - col0);
+            const int r0 = col0 / a.group, r1 = (col0 + ncols - 1) / a.group;
+            const int p0 = q.len - q.n + r0, p1 = q.len - q.n + r1;
+            const int pre = a.prefix_len ? min(a.prefix_len[lo], q.len) : 0;
+            int begin, end;
+            if (a.first) {
+                begin = q.len, end = 0;
+                for (int r = r0; r <= r1; ++r) {  // rows that see something
+                    const int p = q.len - q.n + r;
+                    const int b = max(max(a.first[q.row0 + r], 0), sliding ? p - a.window + 1 : 0);
+                    const int e = max(p + 1, pre);
+                    if (b < e) {
+                        begin = min(begin, b);
+                        end = max(end, e);
+                    }
+                }
+            } else {
+                begin = sliding ? max(0, p0 - a.window + 1) : 0;
+                end = max(p1 + 1, pre);
+            }
+            const int g0 = begin < end ? begin / gran : 0;
+            // at least one granule: a tile whose rows see nothing is written too
+            n = begin < end ? (end + gran - 1) / gran - g0 : 1;
+            tiles[t] = Tile{lo, col0, ncols, g0};
+        }
+        int sum;
+        const int at = block_scan(n, &sum, sums);
+        if (t < total) {
+            prefix[t] = line + at;
+        }
+        line += sum;
+    }
+    if (tid == 0) {
+        prefix[total] = line;
+        a.plan->list[kind][sliding] = List{total, a.ctas[kind], width, gran, line, {0, 0, 0}};
+    }
+    __syncthreads();
+    // the cuts: equal shares of the line of all heads; a tile of few granules
+    // is not cut, and no tile is cut next to its ends
+    const long long all = (long long)(line) * a.kv_heads;
+    // at least one granule per share, so that cuts inside a tile differ
+    const int shares = int(min((long long)(a.ctas[kind]), all));
+    for (int c = tid; c <= a.ctas[kind]; c += kPlanThreads) {
+        Cut cut{total == 0 ? 0 : a.kv_heads, 0, 0, 0u};
+        if (c < shares) {
+            const long long pos = all * c / shares;
+            cut.head = int(pos / line);
+            const int rest = int(pos - (long long)(cut.head) * line);
+            int lo = 0, hi = total;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (prefix[mid] <= rest) {
+                    lo = mid;
+                } else {
+                    hi = mid;
+                }
+            }
+            const int g = rest - prefix[lo], n = prefix[lo + 1] - prefix[lo];
+            cut.tile = lo;
+            if (n <= kNoSplit ? 2 * g < n : g < 2) {
+                cut.gran = 0;
+            } else if (n <= kNoSplit || n - g < 2) {
+                cut.gran = 0;
+                if (++cut.tile == total) {
+                    cut.tile = 0;
+                    ++cut.head;
+                }
+            } else {
+                cut.gran = g;
+            }
+        }
+        shared_cuts[c] = cut;
+    }
+    __syncthreads();
+    // a cut inside a tile knows the CTAs that share the tile: those of the
+    // neighbouring cuts inside it
+    for (int c = tid; c <= a.ctas[kind]; c += kPlanThreads) {
+        Cut cut = shared_cuts[c];
+        if (cut.gran > 0) {
+            int first = c - 1, last = c;
+            while (shared_cuts[first].head == cut.head && shared_cuts[first].tile == cut.tile && shared_cuts[first].gran > 0) {
+                --first;
+            }
+            while (shared_cuts[last + 1].head == cut.head && shared_cuts[last + 1].tile == cut.tile) {
+                ++last;
+            }
+            cut.span = uint32_t(first) | uint32_t(last) << 16;
+        }
+        cuts[c] = cut;
+    }
+}
+
+// ---- append ----
+
+struct AppendArgs {
+    const Plan *plan;
+    const int4 *row;
+    const void *k, *v, *q;
+    void *q_out;
+    size_t k_stride, v_stride, q_stride, q_out_stride;
+    uint8_t *pool;  // this layer
+    const double *turns;
+    float rope_scale;
+    uint32_t *status;
+    int rows, q_heads, kv_heads, page_shift, pages, half, interleaved;  // half: rotated pairs (0: none)
+    uint32_t block_bytes;
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kMaxPairs = 64;
+
+// The slot of a row: the block of (page, head 0) and the token in it, or
+// nullptr for padding and for a page outside the pool.
+template <class Args> __device__ __forceinline__ uint8_t *row_slot(const Args &a, const int4 &ri, int &token) {
+    if (ri.w < 0) {
+        return nullptr;
+    }
+    const int id = a.plan->pages[size_t(ri.w) * a.plan->page_stride + size_t(ri.x >> a.page_shift)];
+    token = ri.x & ((1 << a.page_shift) - 1);
+    if (uint32_t(id) >= uint32_t(a.pages)) {
+        ttl::set_status(a.status, kKvBadPage);
+        return nullptr;
+    }
+    return const_cast<uint8_t *>(a.pool) + size_t(id) * a.kv_heads * a.block_bytes;
+}
+
+// E2M1 codes of two values that are already divided by their scale.
+__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+    uint32_t out;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(out) : "f"(lo), "f"(hi));
+    return out;
+}
+
+// f64 -> f32 rounded to odd: keeps the order against every f32 with an even
+// last bit, so that rounding the result to E2M1 (whose borders are such
+// numbers) equals rounding the f64 at once.
+__device__ __forceinline__ float to_odd(double x) {
+    const float f = __double2float_rz(x);
+    return double(f) == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
+// 32 values -> a 16-byte code block and its scale.
+template <class T> __device__ __forceinline__ void quantize_block(const T (&x)[32], uint8_t *codes, uint8_t *scale) {
+    T top = 0;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const T m = x[i] < 0 ? -x[i] : x[i];
+        top = m > top ? m : top;
+        finite = finite && (m < T(INFINITY));
+    }
+    int e = -127;
+    if constexpr (sizeof(T) == 8) {
+        const int b = int(__double_as_longlong(top) >> 52) & 0x7ff;
+        e = max(b - 1023 - 2, -127);
+    } else {
+        // a subnormal maximum has a scale below the smallest: -127 all the same
+        e = max(int(__float_as_uint(top) >> 23) - 127 - 2, -127);
+    }
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (finite && top > 0) {
+        // x * 2^-e is exact: e is at most 125 and at least -127
+        T inv;
+        if constexpr (sizeof(T) == 8) {
+            inv = __longlong_as_double((long long)(1023 - e) << 52);
+        } else {
+            inv = __uint_as_float(uint32_t(127 - e) << 23);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            float lo, hi;
+            if constexpr (sizeof(T) == 8) {
+                lo = to_odd(x[i] * inv), hi = to_odd(x[i + 1] * inv);
+            } else {
+                lo = x[i] * inv, hi = x[i + 1] * inv;
+            }
+            w[i / 8] |= e2m1x2(lo, hi) << (4 * (i % 8));
+        }
+    }
+    *reinterpret_cast<uint4 *>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
+    *scale = finite ? uint8_t(e + 127) : uint8_t(255);
+}
+
+// One CTA takes kAppendRows rows: the cosines and sines of the rows' pairs
+// once, for all heads, then every head in units of 16 values (two runs of 8
+// that are rotated with one another).  The angle is a fraction of a
+// revolution in 64 bits (a position times a frequency has lost 7 bits of its
+// fraction at position 131072 in 32), cut to its fractional part there, and
+// its cosine and sine are then good to 32 bits.
+// Memory-bound: every row is read and written once.
+template <int kRows>
+__device__ __forceinline__ void rotate_unit(const void *src, size_t base, int u, int half, int interleaved, const float2 *cs,
+                                            float (&x)[8], float (&y)[8], int &at_x, int &at_y) {
+    // rotated dims are a multiple of 16, so a unit is rotated whole or not at all
+    if (half && !interleaved && 8 * u < half) {
+        at_x = 8 * u, at_y = half + 8 * u;
+    } else {
+        at_x = 16 * u, at_y = 16 * u + 8;
+    }
+    load8<kRows>(src, base + at_x, x);
+    load8<kRows>(src, base + at_y, y);
+    if (16 * u >= 2 * half) {
+        return;
+    }
+    if (!interleaved) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 t = cs[8 * u + j];
+            const float a = x[j], b = y[j];
+            x[j] = a * t.x - b * t.y;
+            y[j] = a * t.y + b * t.x;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 t = cs[8 * u + j], s = cs[8 * u + 4 + j];
+            float a = x[2 * j], b = x[2 * j + 1];
+            x[2 * j] = a * t.x - b * t.y;
+            x[2 * j + 1] = a * t.y + b * t.x;
+            a = y[2 * j], b = y[2 * j + 1];
+            y[2 * j] = a * s.x - b * s.y;
+            y[2 * j + 1] = a * s.y + b * s.x;
+        }
+    }
+}
+
+template <int kRows, int kCache, int D>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(AppendArgs a, int rows_per_cta) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    // [rows_per_cta][half]: f64 where the cache is 4 bits (K is rounded to codes
+    // once, from 64 bits), then f32
+    double2 *cs64 = reinterpret_cast<double2 *>(smem);
+    float2 *cs = reinterpret_cast<float2 *>(smem + (kCache == kMxfp4 ? size_t(rows_per_cta) * a.half * sizeof(double2) : 0));
+    const int r0 = blockIdx.x * rows_per_cta;
+    const int count = min(rows_per_cta, a.rows - r0);
+    for (int i = threadIdx.x; i < count * a.half; i += kAppendThreads) {
+        const int r = i / a.half, pair = i - r * a.half;
+        const int4 ri = a.row[r0 + r];
+        const double turn = double(ri.x) * a.turns[pair];
+        const double part = 2.0 * (turn - rint(turn));  // half turns in [-1, 1]
+        if constexpr (kCache == kMxfp4) {
+            double s, c;
+            sincospi(part, &s, &c);
+            cs64[i] = make_double2(c * a.rope_scale, s * a.rope_scale);
+            cs[i] = make_float2(float(c * a.rope_scale), float(s * a.rope_scale));
+        } else {
+            float s, c;
+            sincospif(float(part), &s, &c);
+            cs[i] = make_float2(c * a.rope_scale, s * a.rope_scale);
+        }
+    }
+    __syncthreads();
+    constexpr int kUnits = D / 16;
+    // Q, and K and V where the cache holds the rows' type
+    const int qu = a.q ? a.q_heads * kUnits : 0;
+    const int per_row = qu + (kCache == kMxfp4 ? 0 : 2 * a.kv_heads * kUnits);
+    for (int i = threadIdx.x; i < count * per_row; i += kAppendThreads) {
+        const int r = i / per_row;
+        int u = i - r * per_row;
+        const int row = r0 + r;
+        const int4 ri = a.row[row];
+        if (ri.w < 0) {
+            continue;
+        }
+        float x[8], y[8];
+        int ax, ay;
+        const float2 *rot = cs + r * a.half;
+        if (u < qu) {
+            const int head = u / kUnits;
+            u -= head * kUnits;
+            rotate_unit<kRows>(a.q, size_t(row) * a.q_stride + size_t(head) * D, u, a.half, a.interleaved, rot, x, y, ax, ay);
+            const size_t to = size_t(row) * a.q_out_stride + size_t(head) * D;
+            store8<kRows>(a.q_out, to + ax, x);
+            store8<kRows>(a.q_out, to + ay, y);
+            continue;
+        }
+        if constexpr (kCache != kMxfp4) {
+            u -= qu;
+            const bool is_v = u >= a.kv_heads * kUnits;
+            u -= is_v ? a.kv_heads * kUnits : 0;
+            const int head = u / kUnits;
+            u -= head * kUnits;
+            int token = 0;
+            uint8_t *slot = row_slot(a, ri, token);
+            if (!slot) {
+                continue;
+            }
+            slot += size_t(head) * a.block_bytes + (is_v ? a.block_bytes >> 1 : 0);
+            if (is_v) {
+                rotate_unit<kRows>(a.v, size_t(row) * a.v_stride + size_t(head) * D, u, 0, 0, rot, x, y, ax, ay);
+            } else {
+                rotate_unit<kRows>(a.k, size_t(row) * a.k_stride + size_t(head) * D, u, a.half, a.interleaved, rot, x, y, ax, ay);
+            }
+            store8<kRows>(slot, size_t(token) * D + ax, x);
+            store8<kRows>(slot, size_t(token) * D + ay, y);
+        }
+    }
+    if constexpr (kCache == kMxfp4) {
+        // a thread per block of 32 values
+        constexpr int kBlocks = D / 32;
+        const int blocks = 2 * a.kv_heads * kBlocks;
+        for (int i = threadIdx.x; i < count * blocks; i += kAppendThreads) {
+            const int r = i / blocks;
+            int u = i - r * blocks;
+            const int row = r0 + r;
+            const int4 ri = a.row[row];
+            int token = 0;
+            uint8_t *slot = row_slot(a, ri, token);
+            if (!slot) {
+                continue;
+            }
+            const bool is_v = u >= a.kv_heads * kBlocks;
+            u -= is_v ? a.kv_heads * kBlocks : 0;
+            const int head = u / kBlocks, b = u - head * kBlocks;
+            slot += size_t(head) * a.block_bytes + (is_v ? a.block_bytes >> 1 : 0);
+            uint8_t *codes = slot + size_t(token) * (D / 2) + b * 16;
+            uint8_t *scale = slot + (size_t(1) << a.page_shift) * (D / 2) + size_t(token) * (D / 32) + b;
+            float x[32], w[8];
+            if (is_v || a.half == 0 || 32 * b >= 2 * a.half) {
+                const size_t at = is_v ? size_t(row) * a.v_stride : size_t(row) * a.k_stride;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    load8<kRows>(is_v ? a.v : a.k, at + size_t(head) * D + 32 * b + 8 * j, w);
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        x[8 * j + t] = w[t];
+                    }
+                }
+                quantize_block(x, codes, scale);
+                continue;
+            }
+            double z[32];
+            const double2 *rot = cs64 + r * a.half;
+            const size_t at = size_t(row) * a.k_stride + size_t(head) * D;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d0 = 32 * b + 8 * j;
+                load8<kRows>(a.k, at + d0, w);
+                if (d0 >= 2 * a.half) {
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        z[8 * j + t] = w[t];
+                    }
+                } else if (a.interleaved) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const double2 c = rot[d0 / 2 + t];
+                        const double p = w[2 * t], q = w[2 * t + 1];
+                        z[8 * j + 2 * t] = p * c.x - q * c.y;
+                        z[8 * j + 2 * t + 1] = p * c.y + q * c.x;
+                    }
+                } else {
+                    const bool second = d0 >= a.half;
+                    float o[8];
+                    load8<kRows>(a.k, at + (second ? d0 - a.half : d0 + a.half), o);
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        const double2 c = rot[(second ? d0 - a.half : d0) + t];
+                        z[8 * j + t] = second ? double(o[t]) * c.y + double(w[t]) * c.x : double(w[t]) * c.x - double(o[t]) * c.y;
+                    }
+                }
+            }
+            quantize_block(z, codes, scale);
+        }
+    }
+}
+
+// ---- read ----
+
+struct ReadArgs {
+    const Plan *plan;
+    const int4 *row;
+    void *k, *v;
+    size_t k_stride, v_stride;
+    const uint8_t *pool;
+    uint32_t *status;
+    int rows, kv_heads, page_shift, pages;
+    uint32_t block_bytes;
+};
+
+template <int kRows, int kCache, int D> __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
+    constexpr int kUnits = D / 8;
+    const int per_row = 2 * a.kv_heads * kUnits;
+    const long long all = (long long)(a.rows) * per_row;
+    for (long long i = (long long)(blockIdx.x) * 256 + threadIdx.x; i < all; i += (long long)(gridDim.x) * 256) {
+        const int row = int(i / per_row);
+        int u = int(i - (long long)(row)*per_row);
+        const int4 ri = a.row[row];
+        int token = 0;
+        const uint8_t *slot = row_slot(a, ri, token);
+        if (!slot) {
+            continue;
+        }
+        const bool is_v = u >= a.kv_heads * kUnits;
+        u -= is_v ? a.kv_heads * kUnits : 0;
+        const int head = u / kUnits, d = 8 * (u - head * kUnits);
+        slot += size_t(head) * a.block_bytes + (is_v ? a.block_bytes >> 1 : 0);
+        float x[8];
+        if constexpr (kCache != kMxfp4) {
+            load8<kCache>(slot, size_t(token) * D + d, x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = pool_value<kCache, D>(slot, 1 << a.page_shift, token, d + j);
+            }
+        }
+        store8<kRows>(is_v ? a.v : a.k, size_t(row) * (is_v ? a.v_stride : a.k_stride) + size_t(head) * D + d, x);
+    }
+}
+
+// ---- host ----
+
+int kv_fail(ttl_kv *h, int code, const std::string &msg) {
+    if (h) {
+        h->error = msg;
+    }
+    return ttl::fail(nullptr, code, msg);
+}
+
+#define TTL_KV_CUDA(h, expr)                                                                           \
+    do {                                                                                               \
+        const cudaError_t e_ = (expr);                                                                 \
+        if (e_ != cudaSuccess) {                                                                       \
+            cudaGetLastError();                                                                        \
+            return kv_fail((h), TTL_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e_));     \
+        }                                                                                              \
+    } while (0)
+
+// Makes the handle's device current and the caller's again on return.
+struct DeviceGuard {
+    int before = -1;
+    cudaError_t error;
+    explicit DeviceGuard(int device) {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != device) {
+            error = cudaSetDevice(device);
+        } else {
+            before = -1;
+        }
+    }
+    ~DeviceGuard() {
+        if (before >= 0) {
+            cudaSetDevice(before);
+        }
+    }
+};
+
+template <class T> int kv_alloc(ttl_kv *h, T **p, size_t count) {
+    void *q = nullptr;
+    const cudaError_t e = cudaMalloc(&q, std::max<size_t>(count, 1) * sizeof(T));
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return kv_fail(h, TTL_ERR_CUDA, "device allocation of " + std::to_string(count * sizeof(T)) + " bytes failed");
+    }
+    h->allocations.push_back(q);
+    *p = static_cast<T *>(q);
+    return TTL_OK;
+}
+
+size_t type_size(int t) {
+    return t == kF32 ? 4 : 2;
+}
+
+// A device array the kernels will read or write.
+int check_pointer(ttl_kv *h, const void *p, const char *name, size_t align) {
+    if (!p) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, std::string("null ") + name);
+    }
+    if (reinterpret_cast<uintptr_t>(p) % align) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, std::string(name) + " is not aligned to " + std::to_string(align) + " bytes");
+    }
+    cudaPointerAttributes at{};
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return kv_fail(h, TTL_ERR_ARGUMENT, std::string(name) + " is not a device pointer");
+    }
+    if (at.type == cudaMemoryTypeManaged) {
+        return TTL_OK;
+    }
+    if (at.type != cudaMemoryTypeDevice || at.device != h->device) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, std::string(name) + " is not memory of the handle's GPU");
+    }
+    return TTL_OK;
+}
+
+// A row array: pointer, and a stride that holds a row and keeps its alignment.
+int check_rows(ttl_kv *h, const void *p, size_t stride, int heads, const char *name) {
+    if (h->rows == 0) {
+        return TTL_OK;
+    }
+    const int rc = check_pointer(h, p, name, 16);
+    if (rc) {
+        return rc;
+    }
+    if (stride < size_t(heads) * h->dim || stride > (size_t(1) << 40) || stride * type_size(h->rows_type) % 16) {
+        return kv_fail(h, TTL_ERR_ARGUMENT,
+                       std::string(name) + ": a row stride is at least heads * head_dim and a multiple of 16 bytes");
+    }
+    return TTL_OK;
+}
+
+int check_layer(ttl_kv *h, int layer) {
+    if (layer < 0 || layer >= h->layers) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "layer " + std::to_string(layer) + " out of range");
+    }
+    if (!h->batched) {
+        return kv_fail(h, TTL_ERR_STATE, "no batch: call ttl_kv_batch_async first");
+    }
+    return TTL_OK;
+}
+
+template <int kRows, int kCache, int D> cudaError_t launch_append(ttl_kv *h, const AppendArgs &a) {
+    // enough rows for a few hundred units of 16 values, and cosines that fit
+    // 48 KB; one row each while that does not fill the GPU
+    int per = a.rows <= 2 * h->sms ? 1 : 4;
+    const size_t smem = size_t(per) * a.half * (sizeof(float2) + (kCache == kMxfp4 ? sizeof(double2) : 0));
+    kv_append_kernel<kRows, kCache, D><<<(a.rows + per - 1) / per, kAppendThreads, smem, h->stream>>>(a, per);
+    return cudaGetLastError();
+}
+
+template <int kRows, int kCache, int D> cudaError_t launch_read(ttl_kv *h, const ReadArgs &a) {
+    const long long all = (long long)(a.rows) * 2 * a.kv_heads * (D / 8);
+    const long long ctas = std::min<long long>((all + 255) / 256, (long long)(h->sms) * 32);
+    kv_read_kernel<kRows, kCache, D><<<unsigned(ctas), 256, 0, h->stream>>>(a);
+    return cudaGetLastError();
+}
+
+std::string config_error(const ttl_kv_config &c) {
+    auto in = [](uint32_t v, uint32_t lo, uint32_t hi) { return v >= lo && v <= hi; };
+    if (!in(c.layers, 1, 256)) return "layers must be 1..256";
+    if (!in(c.pages, 1, 1u << 24)) return "pages must be 1..2^24";
+    if (c.page_tokens != 16 && c.page_tokens != 32 && c.page_tokens != 64 && c.page_tokens != 128)
+        return "page_tokens must be 16, 32, 64 or 128";
+    if (!in(c.q_heads, 1, 256) || !in(c.kv_heads, 1, 256) || c.q_heads % c.kv_heads)
+        return "q_heads must be 1..256 and a multiple of kv_heads";
+    if (c.head_dim != 64 && c.head_dim != 128) return "head_dim must be 64 or 128";
+    if (c.rows_type > TTL_KV_BF16) return "rows_type must be TTL_KV_F32, TTL_KV_F16 or TTL_KV_BF16";
+    if (c.cache_type != c.rows_type && c.cache_type != TTL_KV_MXFP4) return "cache_type must be rows_type or TTL_KV_MXFP4";
+    if (!in(c.max_seqs, 1, 4096)) return "max_seqs must be 1..4096";
+    if (!in(c.max_rows, 1, 1u << 20)) return "max_rows must be 1..2^20";
+    if (c.window > (1u << 30)) return "window must be at most 2^30";
+    if (c.rope_dims % 16 || c.rope_dims > c.head_dim) return "rope_dims must be a multiple of 16 up to head_dim";
+    if (c.rope_interleaved > 1) return "rope_interleaved must be 0 or 1";
+    if (c.rope_dims && !c.rope_freq) return "rope_dims without rope_freq";
+    if (!std::isfinite(c.rope_scale)) return "rope_scale must be finite";
+    for (uint32_t i = 0; i < c.rope_dims / 2; ++i) {
+        if (!std::isfinite(c.rope_freq[i])) return "rope_freq must be finite";
+    }
+    return "";
+}
+
+int kv_create(const ttl_kv_config *c, ttl_kv **out) {
+    if (!c || !out) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, "null argument");
+    }
+    *out = nullptr;
+    const std::string bad = config_error(*c);
+    if (!bad.empty()) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, bad);
+    }
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
+        cudaGetLastError();
+        return kv_fail(nullptr, TTL_ERR_UNSUPPORTED, "no CUDA device");
+    }
+    int device = c->device;
+    if (device < 0 && cudaGetDevice(&device) != cudaSuccess) {
+        return kv_fail(nullptr, TTL_ERR_CUDA, "cudaGetDevice failed");
+    }
+    if (device >= count) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, "device ordinal out of range");
+    }
+    cudaDeviceProp prop{};
+    if (cudaGetDeviceProperties(&prop, device) != cudaSuccess || prop.major != 10) {
+        cudaGetLastError();
+        return kv_fail(nullptr, TTL_ERR_UNSUPPORTED, "the kernels are built for sm_100a (B200)");
+    }
+    DeviceGuard guard(device);
+    if (guard.error != cudaSuccess) {
+        return kv_fail(nullptr, TTL_ERR_CUDA, "cudaSetDevice failed");
+    }
+    ttl_kv *h = new ttl_kv();
+    auto bail = [&](int rc, const std::string &why) {
+        ttl_kv_destroy(h);
+        return kv_fail(nullptr, rc, why);
+    };
+    h->device = device;
+    h->sms = prop.multiProcessorCount;
+    h->layers = int(c->layers), h->pages = int(c->pages), h->page_tokens = int(c->page_tokens);
+    h->page_shift = c->page_tokens == 16 ? 4 : c->page_tokens == 32 ? 5 : c->page_tokens == 64 ? 6 : 7;
+    h->q_heads = int(c->q_heads), h->kv_heads = int(c->kv_heads), h->dim = int(c->head_dim);
+    h->rows_type = int(c->rows_type), h->cache_type = int(c->cache_type);
+    h->max_seqs = int(c->max_seqs), h->max_rows = int(c->max_rows), h->window = int(c->window);
+    h->rope_dims = int(c->rope_dims), h->interleaved = int(c->rope_interleaved);
+    h->rope_scale = c->rope_scale == 0.0 ? 1.0f : float(c->rope_scale);
+    h->block_bytes = 2 * uint32_t(h->page_tokens) * row_bytes(h->cache_type, h->dim);
+    h->layer_bytes = size_t(h->pages) * h->kv_heads * h->block_bytes;
+    if (c->stream) {
+        h->stream = static_cast<cudaStream_t>(c->stream);
+    } else {
+        if (cudaStreamCreateWithFlags(&h->stream, cudaStreamNonBlocking) != cudaSuccess) {
+            cudaGetLastError();
+            return bail(TTL_ERR_CUDA, "cannot create a stream");
+        }
+        h->own_stream = true;
+    }
+    const int group = h->q_heads / h->kv_heads;
+    // tiles of the narrowest width a list can have; see choose_shapes
+    h->tile_cap[0] = int(std::min<long long>((long long)(h->max_rows) * group / kNarrow + h->max_seqs, 1 << 28));
+    h->tile_cap[1] = int((long long)(h->max_rows) * group / kPromptWidth + h->max_seqs);
+    const size_t part = kv_part_floats(*h);
+    int rc = kv_alloc(h, &h->pool, h->layer_bytes * h->layers);
+    rc = rc ? rc : kv_alloc(h, &h->turns, size_t(h->rope_dims / 2));
+    rc = rc ? rc : kv_alloc(h, &h->plan, 1);
+    for (int k = 0; k < kKinds && !rc; ++k) {
+        for (int w = 0; w < (h->window ? 2 : 1) && !rc; ++w) {
+            rc = rc ? rc : kv_alloc(h, &h->tiles[k][w], size_t(h->tile_cap[k]));
+            rc = rc ? rc : kv_alloc(h, &h->prefix[k][w], size_t(h->tile_cap[k]) + 1);
+            rc = rc ? rc : kv_alloc(h, &h->cuts[k][w], kMaxCtas + 1);
+        }
+    }
+    rc = rc ? rc : kv_alloc(h, &h->row[0], size_t(h->max_rows));
+    rc = rc ? rc : kv_alloc(h, &h->row[1], size_t(h->max_rows));
+    rc = rc ? rc : kv_alloc(h, &h->seq, size_t(h->max_seqs));
+    rc = rc ? rc : kv_alloc(h, &h->part, part);
+    rc = rc ? rc : kv_alloc(h, &h->counters, size_t(kKinds) * kMaxCtas);
+    rc = rc ? rc : kv_alloc(h, &h->status, 1);
+    if (rc) {
+        return bail(rc, h->error);
+    }
+    double turns[kMaxPairs] = {};
+    for (int i = 0; i < h->rope_dims / 2; ++i) {
+        turns[i] = c->rope_freq[i] / 6.283185307179586476925286766559;
+    }
+    cudaError_t e = cudaMemsetAsync(h->pool, 0, h->layer_bytes * h->layers, h->stream);
+    e = e ? e : cudaMemsetAsync(h->plan, 0, sizeof(Plan), h->stream);
+    e = e ? e : cudaMemsetAsync(h->counters, 0, sizeof(uint32_t) * kKinds * kMaxCtas, h->stream);
+    e = e ? e : cudaMemsetAsync(h->status, 0, sizeof(uint32_t), h->stream);
+    e = e ? e : cudaMemcpyAsync(h->turns, turns, sizeof(double) * size_t(h->rope_dims / 2), cudaMemcpyHostToDevice, h->stream);
+    e = e ? e : cudaStreamSynchronize(h->stream);
+    e = e ? e : kv_configure(*h);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return bail(TTL_ERR_CUDA, std::string("device initialisation: ") + cudaGetErrorString(e));
+    }
+    *out = h;
+    return TTL_OK;
+}
+
+int kv_batch(ttl_kv *h, uint32_t seqs, uint32_t rows, uint32_t max_new, const int32_t *row_start, const int32_t *length,
+             const int32_t *pages, uint32_t page_stride, const int32_t *first, const int32_t *prefix) {
+    if (!h) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, "null handle");
+    }
+    if (seqs == 0 || seqs > uint32_t(h->max_seqs)) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "seqs must be 1..max_seqs");
+    }
+    if (rows > uint32_t(h->max_rows)) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "rows exceed max_rows");
+    }
+    if (page_stride == 0 || page_stride > (1u << 26)) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "page_stride must be 1..2^26");
+    }
+    DeviceGuard guard(h->device);
+    TTL_KV_CUDA(h, guard.error);
+    int rc = check_pointer(h, row_start, "row_start", 4);
+    rc = rc ? rc : check_pointer(h, length, "length", 4);
+    rc = rc ? rc : check_pointer(h, pages, "pages", 4);
+    rc = (rc || !first) ? rc : check_pointer(h, first, "first", 4);
+    rc = (rc || !prefix) ? rc : check_pointer(h, prefix, "prefix", 4);
+    if (rc) {
+        return rc;
+    }
+    max_new = std::min(max_new, rows);
+    PlanArgs a{};
+    a.plan = h->plan;
+    for (int k = 0; k < kKinds; ++k) {
+        for (int w = 0; w < 2; ++w) {
+            a.tiles[k][w] = h->tiles[k][w];
+            a.prefix[k][w] = h->prefix[k][w];
+            a.cuts[k][w] = h->cuts[k][w];
+        }
+    }
+    a.row[0] = h->row[0], a.row[1] = h->row[1], a.seq = h->seq;
+    a.counters = h->counters, a.status = h->status;
+    a.row_start = row_start, a.length = length, a.pages = pages, a.first = first, a.prefix_len = prefix;
+    a.page_stride = page_stride;
+    a.seqs = int(seqs), a.rows = int(rows), a.max_new = int(max_new);
+    a.group = h->q_heads / h->kv_heads, a.kv_heads = h->kv_heads, a.window = h->window, a.page_tokens = h->page_tokens;
+    Shape shape[kKinds];
+    a.few = choose_shapes(*h, int(seqs), int(rows), int(max_new), shape);
+    for (int k = 0; k < kKinds; ++k) {
+        a.width[k] = h->width[k] = shape[k].width;
+        a.gran[k] = shape[k].gran;
+        a.ctas[k] = h->ctas[k] = shape[k].ctas;
+        a.tile_cap[k] = h->tile_cap[k];
+    }
+    kv_plan_kernel<<<4 + (rows + kPlanThreads - 1) / kPlanThreads, kPlanThreads, 0, h->stream>>>(a);
+    TTL_KV_CUDA(h, cudaGetLastError());
+    h->batched = true;
+    h->seqs = int(seqs), h->rows = int(rows);
+    return TTL_OK;
+}
+
+int kv_append(ttl_kv *h, int layer, int rotate, const void *k, size_t k_stride, const void *v, size_t v_stride, const void *q,
+              size_t q_stride, void *q_out, size_t q_out_stride) {
+    if (!h) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, "null handle");
+    }
+    int rc = check_layer(h, layer);
+    if (rc) {
+        return rc;
+    }
+    if ((q == nullptr) != (q_out == nullptr)) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "q and q_out go together");
+    }
+    if (q && q == q_out && q_stride != q_out_stride) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "q rotated in place has one stride");
+    }
+    DeviceGuard guard(h->device);
+    TTL_KV_CUDA(h, guard.error);
+    rc = check_rows(h, k, k_stride, h->kv_heads, "k");
+    rc = rc ? rc : check_rows(h, v, v_stride, h->kv_heads, "v");
+    rc = (rc || !q) ? rc : check_rows(h, q, q_stride, h->q_heads, "q");
+    rc = (rc || !q) ? rc : check_rows(h, q_out, q_out_stride, h->q_heads, "q_out");
+    if (rc || h->rows == 0) {
+        return rc;
+    }
+    AppendArgs a{};
+    a.plan = h->plan, a.row = h->row[0];
+    a.k = k, a.v = v, a.q = q, a.q_out = q_out;
+    a.k_stride = k_stride, a.v_stride = v_stride, a.q_stride = q_stride, a.q_out_stride = q_out_stride;
+    a.pool = h->pool + size_t(layer) * h->layer_bytes;
+    a.turns = h->turns, a.rope_scale = h->rope_scale, a.status = h->status;
+    a.rows = h->rows, a.q_heads = h->q_heads, a.kv_heads = h->kv_heads, a.page_shift = h->page_shift, a.pages = h->pages;
+    a.half = rotate ? h->rope_dims / 2 : 0, a.interleaved = h->interleaved, a.block_bytes = h->block_bytes;
+    TTL_KV_CUDA(h, TTL_KV_DISPATCH(h, launch_append, h, a));
+    return TTL_OK;
+}
+
+int kv_read(ttl_kv *h, int layer, void *k, size_t k_stride, void *v, size_t v_stride) {
+    if (!h) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, "null handle");
+    }
+    int rc = check_layer(h, layer);
+    if (rc) {
+        return rc;
+    }
+    DeviceGuard guard(h->device);
+    TTL_KV_CUDA(h, guard.error);
+    rc = check_rows(h, k, k_stride, h->kv_heads, "k");
+    rc = rc ? rc : check_rows(h, v, v_stride, h->kv_heads, "v");
+    if (rc || h->rows == 0) {
+        return rc;
+    }
+    ReadArgs a{h->plan, h->row[0], k, v, k_stride, v_stride, h->pool + size_t(layer) * h->layer_bytes, h->status,
+               h->rows, h->kv_heads, h->page_shift, h->pages, h->block_bytes};
+    TTL_KV_CUDA(h, TTL_KV_DISPATCH(h, launch_read, h, a));
+    return TTL_OK;
+}
+
+int kv_attend(ttl_kv *h, int layer, uint32_t flags, const void *q, size_t q_stride, void *out, size_t out_stride, float scale,
+              float cap, const float *sinks, const float *slopes) {
+    if (!h) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, "null handle");
+    }
+    int rc = check_layer(h, layer);
+    if (rc) {
+        return rc;
+    }
+    if (flags & ~TTL_KV_SLIDING) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "unknown flags");
+    }
+    if ((flags & TTL_KV_SLIDING) && h->window == 0) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "a sliding call on a handle without a window");
+    }
+    if (!std::isfinite(scale) || !std::isfinite(cap) || cap < 0.0f) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "scale must be finite, cap finite and not negative");
+    }
+    if (q == out && h->rows > 0) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "out must not be q");
+    }
+    DeviceGuard guard(h->device);
+    TTL_KV_CUDA(h, guard.error);
+    rc = check_rows(h, q, q_stride, h->q_heads, "q");
+    rc = rc ? rc : check_rows(h, out, out_stride, h->q_heads, "out");
+    rc = (rc || !sinks) ? rc : check_pointer(h, sinks, "sinks", 4);
+    rc = (rc || !slopes) ? rc : check_pointer(h, slopes, "slopes", 4);
+    if (rc || h->rows == 0) {
+        return rc;
+    }
+    const int w = (flags & TTL_KV_SLIDING) ? 1 : 0;
+    for (int kind = 0; kind < kKinds; ++kind) {
+        if (h->ctas[kind] == 0) {
+            continue;
+        }
+        AttendArgs a{};
+        a.walk = Walk{h->plan, &h->plan->list[kind][w], h->tiles[kind][w], h->prefix[kind][w], h->cuts[kind][w], h->row[w], h->seq};
+        a.pool = h->pool + size_t(layer) * h->layer_bytes;
+        a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+        a.sinks = sinks, a.slopes = slopes;
+        a.part = h->part, a.counters = h->counters + kind * kMaxCtas, a.status = h->status;
+        a.scale = scale == 0.0f ? 1.0f / std::sqrt(float(h->dim)) : scale;
+        a.cap = cap;
+        a.rows = h->rows, a.group = h->q_heads / h->kv_heads, a.page_shift = h->page_shift, a.pages = h->pages;
+        a.kv_heads = h->kv_heads, a.block_bytes = h->block_bytes;
+        TTL_KV_CUDA(h, launch_attend(*h, a, kind, layer));
+    }
+    return TTL_OK;
+}
+
+int kv_sync(ttl_kv *h) {
+    if (!h) {
+        return kv_fail(nullptr, TTL_ERR_ARGUMENT, "null handle");
+    }
+    DeviceGuard guard(h->device);
+    TTL_KV_CUDA(h, guard.error);
+    uint32_t st = 0;
+    TTL_KV_CUDA(h, cudaMemcpyAsync(&st, h->status, sizeof(st), cudaMemcpyDeviceToHost, h->stream));
+    TTL_KV_CUDA(h, cudaStreamSynchronize(h->stream));
+    if (!st) {
+        return TTL_OK;
+    }
+    // a kernel that gave up leaves counters behind: both start again at zero
+    TTL_KV_CUDA(h, cudaMemsetAsync(h->status, 0, sizeof(uint32_t), h->stream));
+    TTL_KV_CUDA(h, cudaMemsetAsync(h->counters, 0, sizeof(uint32_t) * kKinds * kMaxCtas, h->stream));
+    TTL_KV_CUDA(h, cudaStreamSynchronize(h->stream));
+    std::string why = "device status:";
+    why += (st & kKvBadBatch) ? " row_start or length out of order or range;" : "";
+    why += (st & kKvBadPage) ? " a page id outside the pool;" : "";
+    why += (st & kKvWait) ? " bounded-wait-timeout;" : "";
+    why += (st & kKvStalePlan) ? " the plan on the device has another shape than the call;" : "";
+    return kv_fail(h, TTL_ERR_DEVICE, why);
+}
+
+// No exception (an allocation of a message) leaves a C entry.
+template <class F> int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return TTL_ERR_STATE;
+    } catch (...) {
+        return TTL_ERR_STATE;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int ttl_kv_create(const ttl_kv_config *config, ttl_kv **handle_out) {
+    return guarded([&] { return kv_create(config, handle_out); });
+}
+
+void ttl_kv_destroy(ttl_kv *h) {
+    if (!h) {
+        return;
+    }
+    DeviceGuard guard(h->device);
+    if (h->stream || !h->own_stream) {
+        cudaStreamSynchronize(h->stream);
+    }
+    for (void *p : h->allocations) {
+        cudaFree(p);
+    }
+    if (h->own_stream && h->stream) {
+        cudaStreamDestroy(h->stream);
+    }
+    delete h;
+}
+
+const char *ttl_kv_last_error(const ttl_kv *h) {
+    return h ? h->error.c_str() : ttl::thread_error().c_str();
+}
+
+size_t ttl_kv_page_bytes(const ttl_kv *h) {
+    return h ? size_t(h->kv_heads) * h->block_bytes : 0;
+}
+
+int ttl_kv_batch_async(ttl_kv *h, uint32_t seqs, uint32_t rows, uint32_t max_new, const int32_t *row_start,
+                       const int32_t *length, const int32_t *pages, uint32_t page_stride, const int32_t *first,
+                       const int32_t *prefix) {
+    return guarded([&] { return kv_batch(h, seqs, rows, max_new, row_start, length, pages, page_stride, first, prefix); });
+}
+
+int ttl_kv_append_async(ttl_kv *h, int layer, int rotate, const void *k, size_t k_stride, const void *v, size_t v_stride,
+                        const void *q, size_t q_stride, void *q_out, size_t q_out_stride) {
+    return guarded([&] { return kv_append(h, layer, rotate, k, k_stride, v, v_stride, q, q_stride, q_out, q_out_stride); });
+}
+
+int ttl_kv_read_async(ttl_kv *h, int layer, void *k, size_t k_stride, void *v, size_t v_stride) {
+    return guarded([&] { return kv_read(h, layer, k, k_stride, v, v_stride); });
+}
+
+int ttl_kv_attend_async(ttl_kv *h, int layer, uint32_t flags, const void *q, size_t q_stride, void *out, size_t out_stride,
+                        float scale, float cap, const float *sinks, const float *slopes) {
+    return guarded([&] { return kv_attend(h, layer, flags, q, q_stride, out, out_stride, scale, cap, sinks, slopes); });
+}
+
+int ttl_kv_sync(ttl_kv *h) {
+    return guarded([&] { return kv_sync(h); });
+}
+
+void *ttl_kv_stream(ttl_kv *h) {
+    return h ? static_cast<void *>(h->stream) : nullptr;
+}
+
+}  // extern "C"

@@ -1,0 +1,448 @@
+// kv.cuh -- what the kernels of the paged cache share: the plan that a batch
+// call leaves on the device, the walk over it, the pool's layout, and the end
+// of a tile (merge of partial results, sink, rounding, rows with infinities).
+//
+// Columns.  The query rows of one sequence and one KV head are n x group
+// vectors over the same keys; they are numbered c = i * group + g (row i,
+// query head kv * group + g).  A tile is up to `width` columns of a sequence.
+//
+// Plan.  A tile's visible key range is counted in granules (of 64 or 128
+// keys); tiles are laid end to end, once per KV head, and the line is cut into
+// one piece of equal length per CTA.  So every CTA gets the same number of
+// key granules whatever the batch's shape, in one wave; a tile cut by a CTA
+// border leaves partial sums in the workspace, and the CTA that arrives last
+// merges them, in the order of the keys, so results do not depend on timing.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace ttl {
+namespace kv {
+
+enum : int { kF32 = 0, kF16 = 1, kBf16 = 2, kMxfp4 = 3 };
+
+// Status bits (device word of a ttl_kv handle).
+enum : uint32_t {
+    kKvBadBatch = 1u << 0,   // row_start / length out of order or range
+    kKvBadPage = 1u << 1,    // a page id outside the pool
+    kKvWait = 1u << 2,       // a bounded wait gave up
+    kKvStalePlan = 1u << 3,  // the plan on the device is not of this launch's shape
+};
+
+constexpr int kKinds = 2;          // tiles of few columns, tiles of a prompt
+constexpr int kMaxCtas = 1024;     // CTAs of a list (cuts)
+constexpr int kNoSplit = 4;        // a tile of at most this many granules is not cut
+
+struct Tile {
+    int32_t seq, col0, ncols, gran0;
+};
+struct __align__(16) Cut {
+    int32_t head, tile, gran;      // gran: granules into the tile
+    uint32_t span;                 // gran > 0: first and last CTA (<< 16) that hold a part of the tile
+};
+struct List {
+    int32_t tiles, ctas, width, gran;
+    int32_t line;                  // granules of one head's line
+    int32_t pad[3];
+};
+struct Plan {
+    const int32_t *pages;
+    uint32_t page_stride;
+    int32_t seqs;
+    List list[kKinds][2];          // [kind][0 full, 1 sliding]
+};
+
+// What one list's walk reads.
+struct Walk {
+    const Plan *plan;
+    const List *list;
+    const Tile *tiles;
+    const int32_t *prefix;         // [tiles + 1] granules before a tile
+    const Cut *cuts;               // [ctas + 1]
+    const int4 *row;               // [rows] {position, lo, hi, seq} of this window; seq -1: padding
+    const int4 *seq;               // [seqs] {row0, rows, length, 0}
+};
+
+struct AttendArgs {
+    Walk walk;
+    const uint8_t *pool;           // this layer
+    const void *q;
+    void *out;
+    size_t q_stride, out_stride;   // elements
+    const float *sinks, *slopes;
+    float *part;                   // [2 * ctas][width][D + 2]
+    uint32_t *counters;            // [ctas]
+    uint32_t *status;
+    float scale, cap;              // natural units; cap 0: none
+    int rows, group, page_shift, pages, kv_heads;
+    uint32_t block_bytes;          // one KV head of a page
+};
+
+__host__ __device__ constexpr uint32_t row_bytes(int cache, int d) {
+    return cache == kMxfp4 ? uint32_t(d / 2 + d / 32) : uint32_t(cache == kF32 ? 4 * d : 2 * d);
+}
+
+// ---- the pool: [page][KV head][K rows, V rows] ----
+// f32, f16, bf16: [page_tokens][D].  MXFP4: codes [page_tokens][D / 2] (value k
+// in byte k / 2, low nibble for even k), then scales [page_tokens][D / 32].
+
+template <int kCache, int D> __device__ __forceinline__ float pool_value(const uint8_t *rows, int tokens, int t, int d) {
+    if constexpr (kCache == kF32) {
+        return reinterpret_cast<const float *>(rows)[size_t(t) * D + d];
+    } else if constexpr (kCache == kF16) {
+        return __half2float(reinterpret_cast<const __half *>(rows)[size_t(t) * D + d]);
+    } else if constexpr (kCache == kBf16) {
+        return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(rows)[size_t(t) * D + d]);
+    } else {
+        const uint32_t byte = rows[t * (D / 2) + d / 2];
+        const uint32_t code = (d & 1) ? byte >> 4 : byte & 15u;
+        const uint32_t e = rows[tokens * (D / 2) + t * (D / 32) + d / 32];
+        const float2 v = __half22float2(e2m1x2_to_half2(code));
+        // 2^(e - 127); 0 is the smallest scale (a subnormal float), 255 NaN
+        const float s = e == 255u ? __uint_as_float(0x7fffffffu) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
+        return v.x * s;
+    }
+}
+
+template <int kRows> __device__ __forceinline__ float row_value(const void *base, size_t i) {
+    if constexpr (kRows == kF32) {
+        return static_cast<const float *>(base)[i];
+    } else if constexpr (kRows == kF16) {
+        return __half2float(static_cast<const __half *>(base)[i]);
+    } else {
+        return __bfloat162float(static_cast<const __nv_bfloat16 *>(base)[i]);
+    }
+}
+template <int kRows> __device__ __forceinline__ void store_value(void *base, size_t i, float v) {
+    if constexpr (kRows == kF32) {
+        static_cast<float *>(base)[i] = v;
+    } else if constexpr (kRows == kF16) {
+        static_cast<__half *>(base)[i] = __float2half_rn(v);
+    } else {
+        static_cast<__nv_bfloat16 *>(base)[i] = __float2bfloat16_rn(v);
+    }
+}
+// Eight values as 16-bit or 32-bit rows (16-byte aligned).
+template <int kRows> __device__ __forceinline__ void store8(void *base, size_t i, const float (&v)[8]) {
+    if constexpr (kRows == kF32) {
+        float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(base) + i);
+        p[0] = make_float4(v[0], v[1], v[2], v[3]);
+        p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (kRows == kF16) {
+                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+template <int kRows> __device__ __forceinline__ void load8(const void *base, size_t i, float (&v)[8]) {
+    if constexpr (kRows == kF32) {
+        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + i);
+        const float4 a = p[0], b = p[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + i);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float2 f;
+            if constexpr (kRows == kF16) {
+                f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
+            } else {
+                f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u[j]));
+            }
+            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+    }
+}
+
+// Page id of position `pos` of a sequence; an id outside the pool is reported
+// and read as page 0.  The caller keeps pos below the sequence's length.
+__device__ __forceinline__ int page_of(const Plan &plan, int seq, int pos, int page_shift, int pages, uint32_t *status) {
+    const int id = plan.pages[size_t(seq) * plan.page_stride + size_t(pos >> page_shift)];
+    if (uint32_t(id) >= uint32_t(pages)) {
+        set_status(status, kKvBadPage);
+        return 0;
+    }
+    return id;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A score in log2 units from the raw product: scaled, capped, with the
+// distance bias.  tanh as 1 - 2 / (e^2x + 1): absolute error about 1e-7 of the
+// cap, where the hardware's tanh.approx has 5e-4.
+__device__ __forceinline__ float score_log2(float dot, float scale_log2, float cap_log2, float two_over_cap, float slope_log2,
+                                            int distance) {
+    float t;
+    if (cap_log2 != 0.0f) {
+        // scale_log2 here is scale * log2(e); two_over_cap * (dot * scale) in log2 units
+        const float e = exp2f(dot * scale_log2 * two_over_cap);
+        t = cap_log2 - __fdividef(2.0f * cap_log2, e + 1.0f);
+        if (e > 1e30f) {  // __fdividef returns 0 from 2^126 on, and NaN for an infinite divisor is ruled out here
+            t = cap_log2;
+        }
+        if (dot != dot) {
+            t = dot;
+        }
+    } else {
+        t = dot * scale_log2;
+    }
+    return t - slope_log2 * float(distance);
+}
+
+// ---- the walk ----
+
+struct Piece {
+    int head, tile, seq, col0, ncols;
+    int k0, k1;        // keys of the piece (k1 <= the tile's last granule; clip to the sequence's length)
+    int first, last;   // first and last CTA that hold a part of the tile (equal: the whole tile is here)
+};
+
+struct Walker {
+    const Walk &w;
+    int head, tile, gran;  // next piece
+    Cut end;
+    uint32_t start_span;   // of the tile that the CTA's range begins in, where it begins inside
+    int cta;
+
+    __device__ __forceinline__ Walker(const Walk &walk, int cta_) : w(walk), cta(cta_) {
+        const Cut a = w.cuts[cta];
+        end = w.cuts[cta + 1];
+        head = a.head, tile = a.tile, gran = a.gran;
+        start_span = a.span;
+    }
+    // -1, 0, 1: (head, tile, gran) against a cut
+    __device__ __forceinline__ static bool before(int h, int t, int g, const Cut &c) {
+        return h != c.head ? h < c.head : (t != c.tile ? t < c.tile : g < c.gran);
+    }
+    __device__ __forceinline__ bool next(Piece &p) {
+        if (!before(head, tile, gran, end)) {
+            return false;
+        }
+        const Tile t = w.tiles[tile];
+        const int n = w.prefix[tile + 1] - w.prefix[tile];
+        int stop = n;
+        if (end.head == head && end.tile == tile) {
+            stop = end.gran;  // > gran
+        }
+        p.head = head, p.tile = tile, p.seq = t.seq, p.col0 = t.col0, p.ncols = t.ncols;
+        const int gsize = w.list->gran;
+        p.k0 = (t.gran0 + gran) * gsize;
+        p.k1 = (t.gran0 + stop) * gsize;
+        p.first = p.last = cta;
+        const uint32_t span = gran > 0 ? start_span : end.span;
+        if (gran > 0 || stop < n) {
+            p.first = int(span & 0xffffu);
+            p.last = int(span >> 16);
+        }
+        if (stop == n) {
+            gran = 0;
+            if (++tile == w.list->tiles) {
+                tile = 0;
+                ++head;
+            }
+        } else {
+            gran = stop;
+        }
+        return true;
+    }
+};
+
+// Slot of the partial result that CTA c keeps for a tile whose parts begin in
+// CTA `first`: its own first tile (slot 2c) or the one it begins (2c + 1).
+__device__ __forceinline__ int part_slot(int c, int first) {
+    return 2 * c + (c == first ? 1 : 0);
+}
+
+// ---- rows with infinities or NaN ----
+// One column computed key by key by a warp, over the keys it sees and no
+// others.  The matrix products multiply every value of a tile, so an infinity
+// or NaN in a place that a column does not see reaches its sum as 0 * x; any
+// column whose result is not finite is computed again here, where unseen keys
+// are not touched.
+template <int kRows, int kCache, int D>
+__device__ __noinline__ void attend_column(const AttendArgs &a, const Plan &plan, int head, int seq, int row, int qhead) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kPer = D / 32;
+    const int4 ri = a.walk.row[row];
+    const int len = a.walk.seq[seq].z;
+    const int lo = max(ri.y, 0), hi = min(ri.z, len);
+    const float scale_log2 = a.scale * kLog2e;
+    const float slope = a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
+    const int tokens = 1 << a.page_shift;
+    float q[kPer], o[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        q[i] = row_value<kRows>(a.q, size_t(row) * a.q_stride + size_t(qhead) * D + lane + 32 * i);
+        o[i] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    if (a.sinks) {
+        m = a.sinks[qhead] * kLog2e;
+        l = m == -INFINITY ? 0.0f : 1.0f;
+    }
+    for (int j = lo; j < hi; ++j) {
+        const int page = page_of(plan, seq, j, a.page_shift, a.pages, a.status);
+        const uint8_t *kb = a.pool + (size_t(page) * a.kv_heads + head) * a.block_bytes;
+        const uint8_t *vb = kb + (a.block_bytes >> 1);
+        const int t = j & (tokens - 1);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s = fmaf(q[i], pool_value<kCache, D>(kb, tokens, t, lane + 32 * i), s);
+        }
+        s = warp_sum(s);
+        const float x = a.cap != 0.0f ? a.cap * tanhf(s * a.scale / a.cap) * kLog2e : s * scale_log2;
+        const float z = x - slope * float(abs(ri.x - j));
+        const float mn = (z > m || z != z) ? z : m;
+        const float safe = mn == -INFINITY ? 0.0f : mn;
+        const float up = exp2f(m - safe), p = exp2f(z - safe);
+        l = l * up + p;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            o[i] = o[i] * up + p * pool_value<kCache, D>(vb, tokens, t, lane + 32 * i);
+        }
+        m = mn;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        store_value<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + lane + 32 * i,
+                           lo < hi ? o[i] / l : 0.0f);
+    }
+}
+
+// ---- the end of a tile ----
+
+// Adds the sink, divides, rounds and stores columns [c0, ncols) step `step` of
+// a tile, by warps: D / 8 lanes per column, eight values a lane.  value(c, d,
+// v) gives the eight unnormalised sums, stats(c) {max, sum} in log2 units.
+template <int kRows, int kCache, int D, class Value, class Stats>
+__device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps,
+                                              Value value, Stats stats) {
+    constexpr int kLanes = D / 8, kCols = 32 / kLanes;
+    const int lane = threadIdx.x & 31;
+    const int4 si = a.walk.seq[p.seq];
+    for (int base = warp * kCols; base < p.ncols; base += warps * kCols) {
+        const int c = base + lane / kLanes;
+        bool bad = false;
+        int row = 0, qhead = 0;
+        if (c < p.ncols) {
+            const int cc = p.col0 + c;
+            const int i = cc / a.group;
+            qhead = p.head * a.group + cc - i * a.group;
+            row = si.x + i;
+            const int4 ri = a.walk.row[row];
+            const bool sees = max(ri.y, 0) < min(ri.z, si.z);
+            const float2 ml = stats(c);
+            float m = ml.x, l = ml.y, f = 1.0f;
+            if (a.sinks) {
+                const float sink = a.sinks[qhead] * kLog2e;
+                const float mn = fmaxf(m, sink);
+                const float safe = mn == -INFINITY ? 0.0f : mn;
+                f = exp2f(m - safe);
+                l = l * f + exp2f(sink - safe);
+            }
+            f = f / l;
+            float v[8];
+            value(c, (lane % kLanes) * 8, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = sees ? v[j] * f : 0.0f;
+                bad = bad || !(fabsf(v[j]) < INFINITY);
+            }
+            if (row < a.rows && ri.w == p.seq) {  // a row that two sequences claim belongs to the first
+                store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + (lane % kLanes) * 8, v);
+            } else {
+                bad = false;
+            }
+        }
+        uint32_t redo = __ballot_sync(0xffffffffu, bad);
+        while (redo) {
+            const int src = __ffs(redo) - 1;
+            const int r = __shfl_sync(0xffffffffu, row, src), h = __shfl_sync(0xffffffffu, qhead, src);
+            attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, r, h);
+            const int first = src / kLanes * kLanes;
+            redo &= ~(((kLanes == 32 ? 0u : (1u << kLanes)) - 1u) << first);
+        }
+    }
+}
+
+// Merges the partial results of a tile over the CTAs [first, last] that hold
+// them and stores its columns.  part: [slot][width][D + 2] with {max, sum}
+// after the D sums.
+template <int kRows, int kCache, int D>
+__device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps, int width) {
+    const size_t pitch = D + 2;
+    store_columns<kRows, kCache, D>(
+        a, plan, p, warp, warps,
+        [&](int c, int d, float(&v)[8]) {
+            float m = -INFINITY;
+            for (int k = p.first; k <= p.last; ++k) {
+                m = fmaxf(m, __ldcg(a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch + D));
+            }
+            const float safe = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = 0.0f;
+            }
+            for (int k = p.first; k <= p.last; ++k) {
+                const float *src = a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch;
+                const float f = exp2f(__ldcg(src + D) - safe);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 x = __ldcg(reinterpret_cast<const float2 *>(src + d) + j);
+                    v[2 * j] = fmaf(x.x, f, v[2 * j]);
+                    v[2 * j + 1] = fmaf(x.y, f, v[2 * j + 1]);
+                }
+            }
+        },
+        [&](int c) {
+            float m = -INFINITY;
+            for (int k = p.first; k <= p.last; ++k) {
+                m = fmaxf(m, __ldcg(a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch + D));
+            }
+            const float safe = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f;
+            for (int k = p.first; k <= p.last; ++k) {
+                const float *src = a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch + D;
+                l = fmaf(__ldcg(src + 1), exp2f(__ldcg(src) - safe), l);
+            }
+            return make_float2(m, l);
+        });
+}
+
+// After a CTA wrote its partial result of a tile: counts it, and returns true
+// in the CTA that arrived last (all threads), with the others' results
+// visible.  That CTA leaves the tile's counter at zero for the next launch.
+__device__ __forceinline__ bool arrive_last(const AttendArgs &a, const Piece &p, int *flag) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t parts = uint32_t(p.last - p.first + 1);
+        const bool is_last = atomicAdd(&a.counters[p.first], 1u) + 1u == parts;
+        if (is_last) {
+            a.counters[p.first] = 0;
+        }
+        *flag = is_last;
+        __threadfence();
+    }
+    __syncthreads();
+    return *flag != 0;
+}
+
+}  // namespace kv
+}  // namespace ttl

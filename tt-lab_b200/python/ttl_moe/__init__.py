@@ -87,6 +87,16 @@ def lib():
         "ttl_attn_forward": (i32, [vp, i32, sz, vp, vp, vp]),
         "ttl_attn_sync": (i32, [vp]),
         "ttl_attn_stream": (vp, [vp]),
+        "ttl_kv_create": (i32, [vp, ctypes.POINTER(vp)]),
+        "ttl_kv_destroy": (None, [vp]),
+        "ttl_kv_last_error": (ctypes.c_char_p, [vp]),
+        "ttl_kv_page_bytes": (sz, [vp]),
+        "ttl_kv_batch_async": (i32, [vp, u32, u32, u32, vp, vp, vp, u32, vp, vp]),
+        "ttl_kv_append_async": (i32, [vp, i32, i32, vp, sz, vp, sz, vp, sz, vp, sz]),
+        "ttl_kv_read_async": (i32, [vp, i32, vp, sz, vp, sz]),
+        "ttl_kv_attend_async": (i32, [vp, i32, u32, vp, sz, vp, sz, ctypes.c_float, ctypes.c_float, vp, vp]),
+        "ttl_kv_sync": (i32, [vp]),
+        "ttl_kv_stream": (vp, [vp]),
         "ttl_moe_set_timeout": (i32, [vp, u32]),
         "ttl_moe_serve": (i32, [vp, u32]),
         "ttl_moe_decode": (i32, [vp, i32, fp, fp, vp, fp]),
@@ -462,6 +472,163 @@ class Attention:
 
     def stream(self) -> int:
         return lib().ttl_attn_stream(self.h) or 0
+
+
+class KvConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "layers", "pages", "page_tokens", "q_heads", "kv_heads", "head_dim", "rows_type", "cache_type", "max_seqs",
+        "max_rows", "window", "rope_dims", "rope_interleaved")] + [
+        ("rope_freq", ctypes.c_void_p), ("rope_scale", ctypes.c_double), ("device", ctypes.c_int32),
+        ("stream", ctypes.c_void_p)]
+
+
+KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2, "mxfp4": 3}
+KV_SLIDING = 1
+STREAM_LEGACY = 1  # cudaStreamLegacy: the default stream, by a handle that is not NULL
+
+
+def gptoss_rope():
+    """(rope_freq [32] f64, rope_scale) of gpt-oss: the YaRN table and
+    magnitude of the GptOssModel constructor and apply_rope (src/model.cpp:123-138,
+    :231), as ttl_attn applies them."""
+    head, base, scale, original, fast, slow = 64, 150000.0, 1.0 / 32.0, 4096.0, 32.0, 1.0
+
+    def corr(turns):
+        return head * np.log(original / (turns * 2.0 * np.pi)) / (2.0 * np.log(base))
+
+    low, high = max(0.0, np.floor(corr(fast))), min(head - 1.0, np.ceil(corr(slow)))
+    pair = np.arange(head // 2, dtype=np.float64)
+    extrap = base ** (-2.0 * pair / head)
+    ramp = 1.0 - np.clip((pair - low) / max(0.001, high - low), 0.0, 1.0)
+    return scale * extrap * (1.0 - ramp) + extrap * ramp, 1.0 + 0.1 * float(np.log(1.0 / scale))
+
+
+class KvCache:
+    """One ttl_kv handle (include/ttl_kv.h): a paged key/value cache of many
+    sequences, in the rows' type or in 4 bits, and the attention over it.
+
+    Arrays are torch tensors of the handle's GPU.  Work goes to the handle's
+    stream: `stream` is a torch stream or a cudaStream_t, None an own one.  The
+    caller keeps the tensors of a call alive until its work is done."""
+
+    def __init__(self, layers=1, pages=64, page_tokens=64, q_heads=64, kv_heads=8, head_dim=64, rows="bf16",
+                 cache=None, max_seqs=1, max_rows=1, window=0, rope_freq=None, rope_scale=1.0,
+                 rope_interleaved=False, device=-1, stream=None):
+        self.h = None
+        for name, t in (("rows", rows), ("cache", cache or rows)):
+            if t not in KV_TYPES:
+                raise ValueError(f"{name} must be one of {', '.join(KV_TYPES)}")
+        freq = np.ascontiguousarray(rope_freq, np.float64).reshape(-1) if rope_freq is not None else np.zeros(0)
+        if stream is not None and not isinstance(stream, int):
+            stream = stream.cuda_stream or STREAM_LEGACY
+        cfg = KvConfig(layers, pages, page_tokens, q_heads, kv_heads, head_dim, KV_TYPES[rows],
+                       KV_TYPES[cache or rows], max_seqs, max_rows, window, 2 * freq.size, int(bool(rope_interleaved)),
+                       freq.ctypes.data if freq.size else None, rope_scale, device, stream)
+        h = ctypes.c_void_p()
+        rc = lib().ttl_kv_create(ctypes.byref(cfg), ctypes.byref(h))
+        if rc != TTL_OK:
+            msg = lib().ttl_kv_last_error(None)
+            raise RuntimeError(f"cuda kv cache ({rc}): {msg.decode() if msg else ''}")
+        self.h = h
+        self.rows_type, self.cache_type = rows, cache or rows
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self._dtype = {"f32": "torch.float32", "f16": "torch.float16", "bf16": "torch.bfloat16"}[rows]
+        self._rows = 0
+
+    def _check(self, rc):
+        if rc != TTL_OK:
+            msg = lib().ttl_kv_last_error(self.h)
+            raise RuntimeError(f"cuda kv cache ({rc}): {msg.decode() if msg else ''}")
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().ttl_kv_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    @staticmethod
+    def _array(t, name, dtype, shape):
+        """Address of an optional contiguous tensor of the given type and shape."""
+        if t is None:
+            return None
+        if str(t.dtype) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
+        return t.data_ptr()
+
+    def _row_array(self, t, name, heads):
+        """(address, row stride) of [rows, heads, head_dim] rows, each contiguous."""
+        shape, stride = t.shape, t.stride()
+        d = self.head_dim
+        if str(t.dtype) != self._dtype or len(shape) != 3 or shape[0] < self._rows or shape[1] != heads or shape[2] != d:
+            raise ValueError(f"{name} must be a {self._dtype} tensor [{self._rows} rows, {heads}, {d}]")
+        if stride[2] != 1 or (stride[1] != d and heads > 1):
+            raise ValueError(f"{name}: the heads of a row must be contiguous")
+        return t.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], heads * d)
+
+    def batch_async(self, row_start, length, pages, rows, max_new=None, first=None, prefix=None):
+        """The batch of the next calls: int32 device tensors row_start
+        [seqs + 1], length [seqs], pages [seqs, n], first [rows], prefix
+        [seqs]; `rows` in all, at most `max_new` of one sequence (None: rows)."""
+        seqs = length.shape[0]
+        i32 = "torch.int32"
+        if pages.dim() != 2 or str(pages.dtype) != i32 or pages.shape[0] < seqs or pages.stride(1) != 1:
+            raise ValueError("pages must be an int32 tensor [seqs, n] with contiguous rows")
+        stride = pages.stride(0) if pages.shape[0] > 1 else pages.shape[1]
+        if stride != pages.shape[1]:
+            raise ValueError("pages must be contiguous")
+        self._check(lib().ttl_kv_batch_async(
+            self.h, seqs, rows, rows if max_new is None else max_new, self._array(row_start, "row_start", i32, (seqs + 1,)),
+            self._array(length, "length", i32, (seqs,)), pages.data_ptr(), stride,
+            self._array(first, "first", i32, (rows,)), self._array(prefix, "prefix", i32, (seqs,))))
+        self._rows = rows
+        self._kept = (row_start, length, pages, first, prefix)  # the batch's arrays live until the next batch
+
+    def append_async(self, layer, k, v, q=None, q_out=None, rotate=True):
+        """Stores the batch's K and V rows, K rotated; Q rotated goes to q_out."""
+        kp, ks = self._row_array(k, "k", self.kv_heads)
+        vp, vs = self._row_array(v, "v", self.kv_heads)
+        qp = op = None
+        qs = os_ = 0
+        if q is not None:
+            qp, qs = self._row_array(q, "q", self.q_heads)
+        if q_out is not None:
+            op, os_ = self._row_array(q_out, "q_out", self.q_heads)
+        self._check(lib().ttl_kv_append_async(self.h, layer, 1 if rotate else 0, kp, ks, vp, vs, qp, qs, op, os_))
+
+    def read_async(self, layer, k, v):
+        """The batch's rows of K and V as the cache holds them."""
+        kp, ks = self._row_array(k, "k", self.kv_heads)
+        vp, vs = self._row_array(v, "v", self.kv_heads)
+        self._check(lib().ttl_kv_read_async(self.h, layer, kp, ks, vp, vs))
+
+    def attend_async(self, layer, q, out, scale=0.0, cap=0.0, sinks=None, slopes=None, sliding=False):
+        """out = attention of the (rotated) Q rows over the layer's cache."""
+        qp, qs = self._row_array(q, "q", self.q_heads)
+        op, os_ = self._row_array(out, "out", self.q_heads)
+        self._check(lib().ttl_kv_attend_async(
+            self.h, layer, KV_SLIDING if sliding else 0, qp, qs, op, os_, scale or 0.0, cap,
+            self._array(sinks, "sinks", "torch.float32", (self.q_heads,)),
+            self._array(slopes, "slopes", "torch.float32", (self.q_heads,))))
+
+    def page_bytes(self) -> int:
+        return lib().ttl_kv_page_bytes(self.h)
+
+    def sync(self):
+        self._check(lib().ttl_kv_sync(self.h))
+
+    def stream(self) -> int:
+        return lib().ttl_kv_stream(self.h) or 0
 
 
 class TtqWriter:
