@@ -61,7 +61,14 @@ def attend(q, k, v, pos, rows, cache, scale=None, cap=0.0, slopes=None, sinks=No
     scale; the transforms after it by a few units of the score's own size; so a
     weight by twice that (the maximum is off as well), and the sum of L weighted
     values by (L + 16) 2^-23 more.  Rows of 16 bits round each weight once (half
-    a step) and, like every type, the result once."""
+    a step) and, like every type, the result once.
+
+    f16 weights (f16 rows, and every 16-bit row over a 4-bit cache, where the
+    weight carries the block's scale) have a smallest step of 2^-24, half of
+    which is an absolute error; the kernels lift the largest weight to 2^9 or
+    more, so it is at most 2^-34 of the largest weight, for each seen value of
+    up to |v| (4 bits: 6 times the largest seen scale of the block, which is at
+    most twice the block's largest |v|, so 2^-33 * 6 * max|v|)."""
     n, H, D = q.shape
     L, KV = k.shape[0], k.shape[1]
     G = H // KV
@@ -103,5 +110,12 @@ def attend(q, k, v, pos, rows, cache, scale=None, cap=0.0, slopes=None, sinks=No
             e = err[torch.isfinite(err)]
             e = float(e.max()) if len(e) else 0.0
             size = p @ vs.abs()
-            tol[i, h] = (2 * e + (L + 16) * ulp + (u if rows != "f32" else 0.0)) * 1.01 * size + u * out[i, h].abs() + least
+            if rows != "f32" and cache == "mxfp4":
+                top_v = vs.abs().reshape(len(vs), -1, 32).amax((0, 2)).repeat_interleave(32)
+                floor = len(vs) * 2.0 ** -33 * float(p.max()) * 6 * torch.nan_to_num(top_v, 0, 0)
+            elif rows == "f16":
+                floor = 2.0 ** -34 * float(p.max()) * vs.abs().sum(0)
+            else:
+                floor = 0.0
+            tol[i, h] = (2 * e + (L + 16) * ulp + (u if rows != "f32" else 0.0)) * 1.01 * size + u * out[i, h].abs() + least + floor
     return out, tol

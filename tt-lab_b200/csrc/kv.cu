@@ -744,6 +744,43 @@ template <int kRows, int kCache, int D> cudaError_t launch_read(ttl_kv *h, const
     return cudaGetLastError();
 }
 
+// Tensor maps of a 16-bit pool, one per layer: rows of head_dim values (K and V
+// of a head's page follow one another), boxes of 64 values x up to 64 rows, with
+// the 128-byte swizzle that ldmatrix and the matrix instructions read.
+int build_maps(ttl_kv *h) {
+    if (h->rows_type == kF32 || h->cache_type == kMxfp4) {
+        h->maps.resize(size_t(h->layers));
+        return TTL_OK;
+    }
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+        cudaGetLastError();
+        return kv_fail(h, TTL_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    }
+    h->maps.resize(size_t(h->layers));
+    const cuuint64_t rows = cuuint64_t(h->pages) * h->kv_heads * 2 * h->page_tokens;
+    if (rows > (cuuint64_t(1) << 31)) {
+        return kv_fail(h, TTL_ERR_ARGUMENT, "pages * kv_heads * page_tokens must be at most 2^30");  // coordinates are 32 bits
+    }
+    const cuuint64_t dims[2] = {cuuint64_t(h->dim), rows}, strides[1] = {cuuint64_t(h->dim) * 2};
+    const cuuint32_t box[2] = {64, cuuint32_t(std::min(h->page_tokens, 64))}, ones[2] = {1, 1};
+    for (int i = 0; i < h->layers; ++i) {
+        const CUresult r = reinterpret_cast<Encode>(fn)(
+            &h->maps[size_t(i)], h->rows_type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+            h->pool + size_t(i) * h->layer_bytes, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) {
+            return kv_fail(h, TTL_ERR_CUDA, "cuTensorMapEncodeTiled rejected the pool's map");
+        }
+    }
+    return TTL_OK;
+}
+
 std::string config_error(const ttl_kv_config &c) {
     auto in = [](uint32_t v, uint32_t lo, uint32_t hi) { return v >= lo && v <= hi; };
     if (!in(c.layers, 1, 256)) return "layers must be 1..256";
@@ -827,6 +864,11 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
     // tiles of the narrowest width a list can have; see choose_shapes
     h->tile_cap[0] = int(std::min<long long>((long long)(h->max_rows) * group / kNarrow + h->max_seqs, 1 << 28));
     h->tile_cap[1] = int((long long)(h->max_rows) * group / kPromptWidth + h->max_seqs);
+    const cudaError_t ec = kv_configure(*h);
+    if (ec != cudaSuccess) {
+        cudaGetLastError();
+        return bail(TTL_ERR_CUDA, std::string("cannot configure the kernels: ") + cudaGetErrorString(ec));
+    }
     const size_t part = kv_part_floats(*h);
     int rc = kv_alloc(h, &h->pool, h->layer_bytes * h->layers);
     rc = rc ? rc : kv_alloc(h, &h->turns, size_t(h->rope_dims / 2));
@@ -844,6 +886,7 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
     rc = rc ? rc : kv_alloc(h, &h->part, part);
     rc = rc ? rc : kv_alloc(h, &h->counters, size_t(kKinds) * kMaxCtas);
     rc = rc ? rc : kv_alloc(h, &h->status, 1);
+    rc = rc ? rc : build_maps(h);
     if (rc) {
         return bail(rc, h->error);
     }
@@ -857,7 +900,6 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
     e = e ? e : cudaMemsetAsync(h->status, 0, sizeof(uint32_t), h->stream);
     e = e ? e : cudaMemcpyAsync(h->turns, turns, sizeof(double) * size_t(h->rope_dims / 2), cudaMemcpyHostToDevice, h->stream);
     e = e ? e : cudaStreamSynchronize(h->stream);
-    e = e ? e : kv_configure(*h);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return bail(TTL_ERR_CUDA, std::string("device initialisation: ") + cudaGetErrorString(e));

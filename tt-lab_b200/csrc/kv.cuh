@@ -426,11 +426,11 @@ __device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan
 }
 
 // After a CTA wrote its partial result of a tile: counts it, and returns true
-// in the CTA that arrived last (all threads), with the others' results
-// visible.  That CTA leaves the tile's counter at zero for the next launch.
-__device__ __forceinline__ bool arrive_last(const AttendArgs &a, const Piece &p, int *flag) {
+// in the CTA that arrived last (all threads that `sync` joins, thread 0 among
+// them), with the others' results visible.  That CTA leaves the tile's counter at zero for the next launch.
+template <class Sync> __device__ __forceinline__ bool arrive_last(const AttendArgs &a, const Piece &p, int *flag, Sync sync) {
     __threadfence();
-    __syncthreads();
+    sync();
     if (threadIdx.x == 0) {
         const uint32_t parts = uint32_t(p.last - p.first + 1);
         const bool is_last = atomicAdd(&a.counters[p.first], 1u) + 1u == parts;
@@ -440,7 +440,7 @@ __device__ __forceinline__ bool arrive_last(const AttendArgs &a, const Piece &p,
         *flag = is_last;
         __threadfence();
     }
-    __syncthreads();
+    sync();
     return *flag != 0;
 }
 

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
                 const int c = i / (D + 2), d = i - c * (D + 2);
                 part[i] = d < D ? sum[c * D + d] : (d == D ? sm.m[c] : sm.l[c]);
             }
-            if (arrive_last(a, p, &sm.last)) {
+            if (arrive_last(a, p, &sm.last, [] { __syncthreads(); })) {
                 merge_tile<kRows, kCache, D>(a, plan, p, warp, kSimpleThreads / 32, CT);
             }
         }
@@ -246,37 +246,63 @@ template <int kRows, int kCache, int D, int CT> cudaError_t launch_simple_ct(con
 }
 
 template <int kRows, int kCache, int D> cudaError_t launch_simple(const ttl_kv &h, const AttendArgs &a) {
-    return h.width[0] == 8 ? launch_simple_ct<kRows, kCache, D, 8>(h, a, h.ctas[0])
+    if constexpr (kRows != kF32) {
+        return cudaErrorInvalidValue;
+    } else {
+        return h.width[0] == 8 ? launch_simple_ct<kRows, kCache, D, 8>(h, a, h.ctas[0])
                            : launch_simple_ct<kRows, kCache, D, 32>(h, a, h.ctas[0]);
+    }
 }
 
 template <int kRows, int kCache, int D> cudaError_t configure_simple(const ttl_kv &) {
+    if constexpr (kRows != kF32) {
+        return cudaErrorInvalidValue;
+    } else {
     cudaError_t e = cudaFuncSetAttribute(kv_attend_simple_kernel<kRows, kCache, D, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          int(sizeof(SimpleSmem<8, D>)));
     return e ? e
              : cudaFuncSetAttribute(kv_attend_simple_kernel<kRows, kCache, D, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     int(sizeof(SimpleSmem<32, D>)));
+    }
 }
 
 }  // namespace
 
+namespace {
+int token_index(int columns, int dim) {
+    return columns <= 8 ? 0 : (columns <= 16 || dim == 128 ? 1 : 2);
+}
+}  // namespace
+
 int choose_shapes(const ttl_kv &h, int, int, int max_new, Shape shape[kKinds]) {
     const int columns = max_new * (h.q_heads / h.kv_heads);
-    shape[0] = Shape{columns <= 8 ? 8 : 32, kSimpleGran, 2 * h.sms};
+    if (h.rows_type == kF32) {
+        shape[0] = Shape{columns <= 8 ? 8 : 32, kSimpleGran, 2 * h.sms};
+    } else {
+        const int i = token_index(columns, h.dim);
+        shape[0] = Shape{8 << i, 64, h.token_ctas[i]};
+    }
     shape[1] = Shape{kPromptWidth, 128, 0};
     return 1 << 30;
 }
 
 size_t kv_part_floats(const ttl_kv &h) {
-    return size_t(2 * 2 * h.sms) * 32 * (h.dim + 2);
+    size_t most = h.rows_type == kF32 ? size_t(2 * h.sms) * 32 : 0;
+    for (int i = 0; i < 3; ++i) {
+        most = std::max(most, size_t(h.token_ctas[i]) * (8 << i));
+    }
+    return 2 * most * (h.dim + 2);
 }
 
 cudaError_t kv_configure(ttl_kv &h) {
-    return TTL_KV_DISPATCH(&h, configure_simple, h);
+    if (h.rows_type == kF32) {
+        return TTL_KV_DISPATCH(&h, configure_simple, h);
+    }
+    return tokens_configure(h);
 }
 
-cudaError_t launch_attend(const ttl_kv &h, const AttendArgs &a, int, int) {
-    return TTL_KV_DISPATCH(&h, launch_simple, h, a);
+cudaError_t launch_attend(const ttl_kv &h, const AttendArgs &a, int, int layer) {
+    return h.rows_type == kF32 ? TTL_KV_DISPATCH(&h, launch_simple, h, a) : launch_tokens(h, a, layer);
 }
 
 }  // namespace kv

@@ -1,6 +1,7 @@
 // kv_internal.h -- the handle of ttl_kv and the launchers of its kernels.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <string>
@@ -30,6 +31,8 @@ struct ttl_kv {
     float *part = nullptr;
     uint32_t *counters = nullptr;  // [2 kinds][kMaxCtas]
     uint32_t *status = nullptr;
+    std::vector<CUtensorMap> maps; // per layer: the 16-bit pool as rows of head_dim values
+    int token_ctas[3] = {};        // CTAs that are resident at once, tiles of 8, 16, 32 columns
     // the last batch call
     bool batched = false;
     int seqs = 0, rows = 0;
@@ -65,6 +68,8 @@ int choose_shapes(const ttl_kv &h, int seqs, int rows, int max_new, Shape shape[
 size_t kv_part_floats(const ttl_kv &h);
 // Sets the kernels' attributes once per handle.
 cudaError_t kv_configure(ttl_kv &h);
+cudaError_t tokens_configure(ttl_kv &h);
+cudaError_t launch_tokens(const ttl_kv &h, const AttendArgs &a, int layer);
 cudaError_t launch_attend(const ttl_kv &h, const AttendArgs &a, int kind, int layer);
 
 }  // namespace kv

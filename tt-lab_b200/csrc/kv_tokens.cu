@@ -1,0 +1,775 @@
+// kv_tokens.cu -- attention of a few columns per KV head (single tokens, a few
+// rows) over the paged cache, for f16 and bf16 rows: the decode side of
+// ttl_kv_attend_async.
+//
+// What it must do is read K and V once: 2 x D x 2 bytes per key and KV head
+// (17/64 of that in 4 bits) against 4 x group x D operations, so HBM bounds it
+// and the work per byte has to stay small.
+//
+// Both products are taken with the keys as the rows of the matrix instruction
+// (mma.sync m16n8k16) and the columns as its N, 8 to a step: the 8 query heads
+// of a KV head fill it, where they would fill half of an M = 16.
+//   S^T [16 keys x 8 cols] = K [16 x D] Q^T       A = K rows as they lie in memory
+//   O^T [D x 8 cols]      += V^T [D x 16 keys] P^T  A = V^T by ldmatrix.trans
+// The weights go from S^T's accumulator layout to the B operand by one 8 x 8
+// transpose in registers (movmatrix).  tcgen05 has nothing to give here: its M
+// is 128 rows for 8 columns, and the tensor pipe is not what bounds.
+//
+// A CTA is four warps that compute and one that loads.  The loader walks the
+// CTA's piece of the plan and keeps kStages granules of 64 keys in flight (TMA
+// boxes with the 128-byte swizzle, or bulk copies of 4-bit pages), across
+// tiles.  Each computing warp takes 16 keys of a granule with its own running
+// maximum, sum and accumulators; the four are merged when the tile ends.  The
+// maximum moves only when a weight would pass 2^8 (bf16) or 2^4 (f16) times 1,
+// so that most granules need one vote instead of shuffles and a rescaling;
+// weights that large are as exact as weights up to 1.  f16 weights are lifted
+// by a power of two, so that the smallest step of f16 (2^-24) is 2^-35 (4 bits:
+// 2^-33) of the largest weight.
+//
+// 4 bits.  K's codes become f16 exactly (cvt e2m1x2 -> f16x2); a block's scale
+// multiplies the 32-term partial score of the block, in f32.  V's codes are
+// gathered to key pairs (ldmatrix.trans moves 4 codes of a key as one b16) and
+// the scale of (key, block) is multiplied into the weight, taken relative to the
+// largest scale a column has seen in the block, so that it stays in f16's
+// range whatever the values' size.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "kv.cuh"
+#include "kv_internal.h"
+#include "tc.cuh"
+
+namespace ttl {
+namespace kv {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kGran = 64;
+
+template <int kRows, int kCache, int D, int NT> struct TokenShape {
+    static constexpr int kCols = 8 * NT;
+    static constexpr bool kFour = kCache == kMxfp4;
+    static constexpr uint32_t kStageBytes = kFour ? 2 * kGran * row_bytes(kMxfp4, D) : 2 * kGran * D * 2;
+    // enough in flight to cover HBM's latency at its full rate over the CTAs of an SM (about 48 KB per SM)
+    static constexpr int kStages = kFour ? 6 : (D == 64 ? 4 : 3);
+    static constexpr int kOPitch = D + 4;
+};
+
+template <int kRows, int kCache, int D, int NT> struct TokenSmem {
+    using T = TokenShape<kRows, kCache, D, NT>;
+    alignas(1024) uint8_t stage[T::kStages][(T::kStageBytes + 1023) / 1024 * 1024];
+    float o[kWarps][T::kCols][T::kOPitch];
+    float m[kWarps][T::kCols], l[kWarps][T::kCols];
+    int lo[T::kCols], hi[T::kCols], pos[T::kCols];
+    float slope[T::kCols], scale[T::kCols];
+    uint64_t full[T::kStages], empty[T::kStages];
+    int last, abort;
+};
+
+__device__ __forceinline__ void consumer_sync() {
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix2_trans(uint32_t &r0, uint32_t &r1, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// C += A B, 16 x 8 x 16, f16 or bf16 operands, f32 sums.
+template <int kType> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (kType == kF16) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+template <int kType> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (kType == kF16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+__device__ __forceinline__ uint32_t half2_of_codes(uint32_t byte) {
+    const __half2 h = e2m1x2_to_half2(byte);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 2^(e - 127) of an E8M0 byte; 255 is NaN.
+__device__ __forceinline__ float e8m0(uint32_t e) {
+    return e == 255u ? __uint_as_float(0x7fffffffu) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
+}
+// 2^d for |d| beyond f32's exponents too (0 or infinity there).
+__device__ __forceinline__ float pow2i(int d) {
+    return ex2(float(max(d, -1000)));
+}
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     tc::smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+
+// Waits for a phase of a barrier unless the CTA has given up; a wait that runs
+// out gives the CTA up (every later wait returns at once, so that all warps
+// still meet at their barriers and leave).
+__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *status) {
+    if (tc::mbar_try_wait(bar, parity)) {
+        return true;
+    }
+    if (*abort) {
+        return false;
+    }
+    if (!tc::mbar_wait(bar, parity)) {
+        set_status(status, kKvWait);
+        *abort = 1;
+        return false;
+    }
+    return true;
+}
+
+// The loader: one warp, 64 keys a step.
+template <class Smem, int kCache, int D, int kStages, uint32_t kStageBytes>
+__device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &plan, const CUtensorMap *map, Smem &sm) {
+    const int lane = threadIdx.x & 31;
+    const int seg = min(1 << a.page_shift, kGran);       // keys of one copy
+    const int segs = kGran / seg;
+    int stage = 0;
+    uint32_t phase = 0;
+    Walker walk(a.walk, int(blockIdx.x));
+    Piece p;
+    while (walk.next(p)) {
+        const int len = a.walk.seq[p.seq].z;
+        const int32_t *table = plan.pages + size_t(p.seq) * plan.page_stride;
+        const int last = max(len - 1, 0) >> a.page_shift;
+        // page ids of 32 pages at a time; past the end the last page stands in
+        int base = -64, id = 0;
+        for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
+            const int first = k0 >> a.page_shift;
+            const int need = (k0 + kGran - 1) >> a.page_shift;
+            if (need >= base + 32 || base < 0) {
+                base = first;
+                id = len > 0 ? table[min(base + lane, last)] : 0;
+                if (uint32_t(id) >= uint32_t(a.pages)) {
+                    if (base + lane <= last && base + lane <= ((p.k1 - 1) >> a.page_shift)) {
+                        set_status(a.status, kKvBadPage);
+                    }
+                    id = 0;
+                }
+            }
+            const bool free = wait_or_abort(&sm.empty[stage], phase ^ 1, &sm.abort, a.status);
+            if (__all_sync(0xffffffffu, free)) {
+                if (lane == 0) {
+                    tc::mbar_expect_tx(&sm.full[stage], kStageBytes);
+                }
+                __syncwarp();
+                if constexpr (kCache != kMxfp4) {
+                    // copy c: (segment, K or V, 64 values of the head)
+                    const int copies = segs * 2 * (D / 64);
+                    const int c = lane;
+                    const int s = c / (2 * (D / 64)), is_v = c / (D / 64) & 1, x = c & (D / 64 - 1);
+                    const int key = k0 + (c < copies ? s : 0) * seg;
+                    const int page = __shfl_sync(0xffffffffu, id, (key >> a.page_shift) - base);
+                    if (c < copies) {
+                        const int y = ((page * a.kv_heads + p.head) * 2 + is_v) * (1 << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+                        tc::tma_load_2d(sm.stage[stage] + ((is_v * (D / 64) + x) * kGran + s * seg) * 128, map, 64 * x, y, &sm.full[stage]);
+                    }
+                } else {
+                    // pages of up to 64 keys: one copy of a head's block; of 128: its four parts
+                    const bool whole = (1 << a.page_shift) <= kGran;
+                    const int copies = whole ? segs : 4;
+                    const int c = lane;
+                    const int key = k0 + (whole && c < copies ? c * seg : 0);
+                    const int page = __shfl_sync(0xffffffffu, id, (key >> a.page_shift) - base);
+                    if (c < copies) {
+                        const uint8_t *src = a.pool + (size_t(page) * a.kv_heads + p.head) * a.block_bytes;
+                        if (whole) {
+                            bulk_load(sm.stage[stage] + c * a.block_bytes, src, a.block_bytes, &sm.full[stage]);
+                        } else {
+                            const uint32_t codes = kGran * (D / 2), scales = kGran * (D / 32);
+                            const uint32_t t0 = uint32_t(key & ((1 << a.page_shift) - 1));
+                            const uint32_t from = (c >> 1) * (a.block_bytes >> 1) + ((c & 1) ? 128u * (D / 2) + t0 * (D / 32) : t0 * (D / 2));
+                            const uint32_t to = (c >> 1) * (codes + scales) + (c & 1) * codes;
+                            bulk_load(sm.stage[stage] + to, src + from, (c & 1) ? scales : codes, &sm.full[stage]);
+                        }
+                    }
+                }
+            }
+            if (++stage == kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+    }
+    if (*const_cast<volatile int *>(&sm.abort)) {
+        // what is still in flight lands before the shared memory goes away
+        for (int i = 0; i < kStages; ++i) {
+            tc::mbar_wait(&sm.full[i], 0, 1000000ull);
+            tc::mbar_wait(&sm.full[i], 1, 1000000ull);
+        }
+    }
+}
+
+template <int kRows, int kCache, int D, int NT>
+__global__ void __launch_bounds__(kThreads)
+    kv_attend_tokens_kernel(AttendArgs a, const __grid_constant__ CUtensorMap map) {
+    using T = TokenShape<kRows, kCache, D, NT>;
+    using Smem = TokenSmem<kRows, kCache, D, NT>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
+    constexpr int kCols = T::kCols;
+    constexpr int kBlocks = D / 32;
+    constexpr int kMma = kCache == kMxfp4 ? kF16 : kRows;
+    constexpr int kMTiles = D / 16;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Plan &plan = *a.walk.plan;
+    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kCols || a.walk.list->gran != kGran) {
+        if (tid == 0) {
+            set_status(a.status, kKvStalePlan);
+        }
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < T::kStages; ++i) {
+            tc::mbar_init(&sm.full[i], 1);
+            tc::mbar_init(&sm.empty[i], kWarps);
+        }
+        sm.abort = 0;
+        tc::fence_mbar_init();
+    }
+    __syncthreads();
+    if (warp == kWarps) {
+        load_granules<Smem, kCache, D, T::kStages, T::kStageBytes>(a, plan, &map, sm);
+        return;
+    }
+    const int g = lane >> 2, t = lane & 3;
+    const float cap_log2 = a.cap * kLog2e;
+    const float two_over_cap = a.cap != 0.0f ? 2.0f / a.cap : 0.0f;
+    const int seg_shift = min(a.page_shift, 6), seg = 1 << seg_shift;
+    // largest weight 2^(kSlack + kLift), times 2^kScaleSlack over a 4-bit cache: 2^15 in f16
+    constexpr float kSlack = kMma == kF16 ? 4.0f : 8.0f;
+    constexpr int kScaleSlack = 2;
+    constexpr float kLift = kMma != kF16 ? 0.0f : (kCache == kMxfp4 ? 9.0f : 11.0f);
+    int stage = 0;
+    uint32_t phase = 0;
+    Walker walk(a.walk, int(blockIdx.x));
+    Piece p;
+    while (walk.next(p)) {
+        const int4 si = a.walk.seq[p.seq];
+        // ---- the columns ----
+        if (tid < kCols) {
+            int4 ri = make_int4(0, 0, 1 << 30, -1);  // a column past the tile: all keys, so that it asks for no mask
+            float slope = 0.0f;
+            if (tid < p.ncols) {
+                const int cc = p.col0 + tid, r = cc / a.group;
+                ri = a.walk.row[si.x + r];
+                slope = a.slopes ? a.slopes[p.head * a.group + cc - r * a.group] * kLog2e : 0.0f;
+                ri.y = max(ri.y, 0), ri.z = min(ri.z, si.z);
+            }
+            sm.pos[tid] = ri.x, sm.lo[tid] = ri.y, sm.hi[tid] = ri.z;
+            sm.slope[tid] = slope;
+        }
+        uint32_t q[NT][D / 16][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int c = 8 * n + g;
+            const int cc = p.col0 + c, r = cc / a.group, row = si.x + r;
+            const bool have = c < p.ncols && row < a.rows;
+            const uint16_t *src = static_cast<const uint16_t *>(a.q) + size_t(row) * a.q_stride +
+                                  size_t(p.head * a.group + cc - r * a.group) * D;
+            if constexpr (kCache != kMxfp4) {
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s) {
+                    q[n][s][0] = have ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * t) : 0u;
+                    q[n][s][1] = have ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * t) : 0u;
+                }
+            } else {
+                // values 8t .. 8t + 7 of each block of 32, as the codes' words lie
+                uint4 w[kBlocks];
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    w[b] = have ? *reinterpret_cast<const uint4 *>(src + 32 * b + 8 * t) : make_uint4(0, 0, 0, 0);
+                }
+                float unscale = 1.0f;
+                if constexpr (kRows == kBf16) {
+                    // bf16 -> f16 by a power of two per column: exact down to 2^-39 of its largest value
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        const uint32_t u[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            top = max(top, max(u[j] & 0x7fffu, (u[j] >> 16) & 0x7fffu));
+                        }
+                    }
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const int e = int(top >> 7);  // biased exponent of the largest value
+                    // to [2^14, 2^15); infinities and NaN as they are
+                    const int up = e == 255 ? 0 : min(14 - (e - 127), 120);
+                    const float f = __uint_as_float(uint32_t(127 + max(up, -120)) << 23);
+                    unscale = __uint_as_float(uint32_t(127 - max(up, -120)) << 23);
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        uint32_t u[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            u[j] = pack2<kF16>(__uint_as_float(u[j] << 16) * f, __uint_as_float(u[j] & 0xffff0000u) * f);
+                        }
+                        w[b] = make_uint4(u[0], u[1], u[2], u[3]);
+                    }
+                }
+                if (t == 0 && warp == 0) {
+                    sm.scale[c] = a.scale * kLog2e * unscale;
+                }
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    q[n][2 * b][0] = w[b].x, q[n][2 * b][1] = w[b].y;
+                    q[n][2 * b + 1][0] = w[b].z, q[n][2 * b + 1][1] = w[b].w;
+                }
+            }
+        }
+        consumer_sync();
+        // lowest and highest borders over the columns
+        int lo_min, lo_max, hi_min, hi_max;
+        {
+            const int l = lane < kCols ? sm.lo[lane] : 0, h = lane < kCols ? sm.hi[lane] : 0;
+            const bool real = lane < p.ncols;
+            lo_max = __reduce_max_sync(0xffffffffu, real ? l : 0);
+            hi_min = __reduce_min_sync(0xffffffffu, real ? h : 1 << 30);
+            lo_min = __reduce_min_sync(0xffffffffu, real && l < h ? l : 1 << 30);
+            hi_max = __reduce_max_sync(0xffffffffu, real && l < h ? h : 0);
+        }
+        float scale[NT][2], m[NT][2], l[NT][2];
+        float o[NT][kMTiles][4];
+        int ref[kCache == kMxfp4 ? NT : 1][2][kBlocks];  // 4 bits: the scale exponent that o is in units of
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                scale[n][c] = kCache == kMxfp4 ? sm.scale[8 * n + 2 * t + c] : a.scale * kLog2e;
+                m[n][c] = -INFINITY, l[n][c] = 0.0f;
+                if constexpr (kCache == kMxfp4) {
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        ref[n][c][b] = -1000;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kMTiles; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    o[n][i][j] = 0.0f;
+                }
+            }
+        }
+        for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
+            wait_or_abort(&sm.full[stage], phase, &sm.abort, a.status);
+            const int key0 = k0 + 16 * warp;
+            if (key0 < hi_max && key0 + 16 > lo_min) {
+                const uint32_t buf = tc::smem_u32(sm.stage[stage]);
+                float s[NT][4];
+                uint32_t sv[kCache == kMxfp4 ? 2 : 1][kBlocks];  // V's scale bytes of keys g, g + 8
+                uint32_t vcodes = 0;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[n][j] = 0.0f;
+                    }
+                }
+                if constexpr (kCache != kMxfp4) {
+                    const int row = 16 * warp + (lane & 15);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        uint32_t ka[4];
+                        const int chunk = (2 * ks + (lane >> 4)) & 7, x = ks >> 2;
+                        ldmatrix4(ka, buf + (x * kGran + row) * 128 + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma<kMma>(s[n], ka, q[n][ks][0], q[n][ks][1]);
+                        }
+                    }
+                } else {
+                    const int in_seg = (16 * warp) & (seg - 1);
+                    const uint32_t block = 2u * uint32_t(seg) * row_bytes(kMxfp4, D);
+                    const uint32_t kc = buf + uint32_t(16 * warp >> seg_shift) * block;
+                    const uint32_t ksc = kc + uint32_t(seg) * (D / 2);
+                    vcodes = kc + (block >> 1);
+                    const uint32_t vsc = vcodes + uint32_t(seg) * (D / 2);
+                    vcodes += uint32_t(in_seg) * (D / 2);
+                    float sk[2][kBlocks];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t at = uint32_t(in_seg + g + 8 * h) * kBlocks;
+                        uint32_t bk, bv;
+                        if constexpr (kBlocks == 2) {
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bk) : "r"(ksc + at));
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bv) : "r"(vsc + at));
+                        } else {
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bk) : "r"(ksc + at));
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bv) : "r"(vsc + at));
+                        }
+#pragma unroll
+                        for (int b = 0; b < kBlocks; ++b) {
+                            sk[h][b] = e8m0((bk >> (8 * b)) & 255u);
+                            sv[h][b] = (bv >> (8 * b)) & 255u;
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        uint32_t w0, w1;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(kc + uint32_t(in_seg + g) * (D / 2) + 16 * b + 4 * t));
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(kc + uint32_t(in_seg + g + 8) * (D / 2) + 16 * b + 4 * t));
+                        const uint32_t a0[4] = {half2_of_codes(w0 & 255u), half2_of_codes(w1 & 255u), half2_of_codes((w0 >> 8) & 255u),
+                                                half2_of_codes((w1 >> 8) & 255u)};
+                        const uint32_t a1[4] = {half2_of_codes((w0 >> 16) & 255u), half2_of_codes((w1 >> 16) & 255u),
+                                                half2_of_codes(w0 >> 24), half2_of_codes(w1 >> 24)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma<kMma>(c, a0, q[n][2 * b][0], q[n][2 * b][1]);
+                            mma<kMma>(c, a1, q[n][2 * b + 1][0], q[n][2 * b + 1][1]);
+                            s[n][0] = fmaf(c[0], sk[0][b], s[n][0]);
+                            s[n][1] = fmaf(c[1], sk[0][b], s[n][1]);
+                            s[n][2] = fmaf(c[2], sk[1][b], s[n][2]);
+                            s[n][3] = fmaf(c[3], sk[1][b], s[n][3]);
+                        }
+                    }
+                }
+                // ---- scores in log2 units ----
+                const bool masked = key0 < lo_max || key0 + 16 > hi_min;
+                if (cap_log2 == 0.0f && !a.slopes) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            s[n][j] *= scale[n][j & 1];
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int c = 8 * n + 2 * t + (j & 1), key = key0 + g + (j >> 1) * 8;
+                            s[n][j] = score_log2(s[n][j], scale[n][j & 1], cap_log2, two_over_cap, sm.slope[c], abs(sm.pos[c] - key));
+                        }
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int c = 8 * n + 2 * t + (j & 1), key = key0 + g + (j >> 1) * 8;
+                            s[n][j] = key >= sm.lo[c] && key < sm.hi[c] ? s[n][j] : -INFINITY;
+                        }
+                    }
+                }
+                // ---- the running maximum ----
+                bool move = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        move = move || fmaxf(s[n][c], s[n][c + 2]) > m[n][c] + (kSlack + kLift);
+                        if constexpr (kCache == kMxfp4) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                                for (int b = 0; b < kBlocks; ++b) {
+                                    move = move || (int(sv[h][b]) > ref[n][c][b] + kScaleSlack && sv[h][b] != 255u && s[n][c + 2 * h] != -INFINITY);
+                                }
+                            }
+                        }
+                    }
+                }
+                if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float up[2];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float top = fmaxf(s[n][c], s[n][c + 2]);
+#pragma unroll
+                            for (int off = 4; off < 32; off <<= 1) {
+                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                            }
+                            // m is what weights are relative to: the maximum less the lift
+                            const float mn = fmaxf(m[n][c], top - kLift);
+                            up[c] = ex2(m[n][c] - (mn == -INFINITY ? 0.0f : mn));
+                            m[n][c] = mn;
+                            l[n][c] *= up[c];
+                        }
+                        if constexpr (kCache == kMxfp4) {
+#pragma unroll
+                            for (int b = 0; b < kBlocks; ++b) {
+                                float f[2];
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    int e = -1000;
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) {
+                                        e = sv[h][b] != 255u && s[n][c + 2 * h] != -INFINITY ? max(e, int(sv[h][b])) : e;
+                                    }
+#pragma unroll
+                                    for (int off = 4; off < 32; off <<= 1) {
+                                        e = max(e, __shfl_xor_sync(0xffffffffu, e, off));
+                                    }
+                                    const int r = max(ref[n][c][b], e);
+                                    f[c] = up[c] * pow2i(ref[n][c][b] - r);
+                                    ref[n][c][b] = r;
+                                }
+#pragma unroll
+                                for (int i = 2 * b; i < 2 * b + 2; ++i) {
+                                    o[n][i][0] *= f[0], o[n][i][1] *= f[1], o[n][i][2] *= f[0], o[n][i][3] *= f[1];
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kMTiles; ++i) {
+                                o[n][i][0] *= up[0], o[n][i][1] *= up[1], o[n][i][2] *= up[0], o[n][i][3] *= up[1];
+                            }
+                        }
+                    }
+                }
+                // ---- weights, and their products with V ----
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float mm = m[n][j & 1];
+                        s[n][j] = ex2(s[n][j] - (mm == -INFINITY ? 0.0f : mm));
+                        l[n][j & 1] += s[n][j];
+                    }
+                }
+                if constexpr (kCache != kMxfp4) {
+                    uint32_t w[NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        w[n][0] = transpose8(pack2<kMma>(s[n][0], s[n][1]));
+                        w[n][1] = transpose8(pack2<kMma>(s[n][2], s[n][3]));
+                    }
+                    const uint32_t vbuf = buf + (D / 64) * kGran * 128;
+                    const int row = 16 * warp + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                    for (int i = 0; i < kMTiles; ++i) {
+                        uint32_t va[4];
+                        const int chunk = (2 * i + ((lane >> 3) & 1)) & 7, x = i >> 2;
+                        ldmatrix4_trans(va, vbuf + (x * kGran + row) * 128 + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma<kMma>(o[n][i], va, w[n][0], w[n][1]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) {
+                        // 8 x 8 b16 of 4 codes each: keys 0-7 and 8-15, the block's 32 values
+                        uint32_t r0, r1;
+                        ldmatrix2_trans(r0, r1, vcodes + uint32_t(lane & 15) * (D / 2) + 16 * b);
+                        // r: codes 4g .. 4g + 3 of keys 2t (low half) and 2t + 1; to bytes of (key 2t, key 2t + 1)
+                        const uint32_t x0 = (r0 & 0x0F0Fu) | ((r0 >> 12) & 0xF0F0u), y0 = ((r0 >> 4) & 0x0F0Fu) | ((r0 >> 16) & 0xF0F0u);
+                        const uint32_t x1 = (r1 & 0x0F0Fu) | ((r1 >> 12) & 0xF0F0u), y1 = ((r1 >> 4) & 0x0F0Fu) | ((r1 >> 16) & 0xF0F0u);
+                        // rows 0-7: value 4g + 2i, rows 8-15: value 4g + 2i + 1
+                        const uint32_t va0[4] = {half2_of_codes(x0 & 255u), half2_of_codes(y0 & 255u), half2_of_codes(x1 & 255u), half2_of_codes(y1 & 255u)};
+                        const uint32_t va1[4] = {half2_of_codes(x0 >> 8), half2_of_codes(y0 >> 8), half2_of_codes(x1 >> 8), half2_of_codes(y1 >> 8)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float z[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t e = sv[j >> 1][b];
+                                // 2^(e - ref), at most 2^kScaleSlack where the weight is not 0 (a NaN scale of an unseen
+                                // key makes the column NaN, and so computed again)
+                                const int d = int(e) - ref[n][j & 1][b];
+                                const float f = e == 255u ? __uint_as_float(0x7fffffffu)
+                                                          : (d < -126 ? 0.0f : __uint_as_float(uint32_t(min(d, 100) + 127) << 23));
+                                z[j] = s[n][j] * f;
+                            }
+                            const uint32_t w0 = transpose8(pack2<kF16>(z[0], z[1])), w1 = transpose8(pack2<kF16>(z[2], z[3]));
+                            mma<kF16>(o[n][2 * b], va0, w0, w1);
+                            mma<kF16>(o[n][2 * b + 1], va1, w0, w1);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) {
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&sm.empty[stage])) : "memory");
+            }
+            if (++stage == T::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+        // ---- the four warps' results ----
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], off);
+                }
+                if (g == 0) {
+                    sm.m[warp][8 * n + 2 * t + c] = m[n][c];
+                    sm.l[warp][8 * n + 2 * t + c] = l[n][c];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kMTiles; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = 8 * n + 2 * t + (j & 1);
+                    if constexpr (kCache == kMxfp4) {
+                        const int d = 32 * (i >> 1) + 4 * g + 2 * (i & 1) + (j >> 1);
+                        sm.o[warp][c][d] = o[n][i][j] * pow2i(ref[n][j & 1][i >> 1] - 127);
+                    } else {
+                        sm.o[warp][c][16 * i + g + 8 * (j >> 1)] = o[n][i][j];
+                    }
+                }
+            }
+        }
+        consumer_sync();
+        auto top = [&](int c) {
+            return fmaxf(fmaxf(sm.m[0][c], sm.m[1][c]), fmaxf(sm.m[2][c], sm.m[3][c]));
+        };
+        auto stats = [&](int c) {
+            const float mm = top(c), safe = mm == -INFINITY ? 0.0f : mm;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                sum = fmaf(sm.l[w][c], ex2(sm.m[w][c] - safe), sum);
+            }
+            return make_float2(mm, sum);
+        };
+        auto value = [&](int c, int d, float(&v)[8]) {
+            const float mm = top(c), safe = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = 0.0f;
+            }
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = ex2(sm.m[w][c] - safe);
+                const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][c][d]);
+                const float4 y = *reinterpret_cast<const float4 *>(&sm.o[w][c][d + 4]);
+                v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]), v[2] = fmaf(x.z, f, v[2]), v[3] = fmaf(x.w, f, v[3]);
+                v[4] = fmaf(y.x, f, v[4]), v[5] = fmaf(y.y, f, v[5]), v[6] = fmaf(y.z, f, v[6]), v[7] = fmaf(y.w, f, v[7]);
+            }
+        };
+        if (p.first == p.last) {
+            store_columns<kRows, kCache, D>(a, plan, p, warp, kWarps, value, stats);
+        } else {
+            float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * kCols * (D + 2);
+            for (int i = tid; i < p.ncols * (D / 8); i += 32 * kWarps) {
+                const int c = i / (D / 8), d = 8 * (i % (D / 8));
+                float v[8];
+                value(c, d, v);
+                float2 *dst = reinterpret_cast<float2 *>(part + size_t(c) * (D + 2) + d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    dst[j] = make_float2(v[2 * j], v[2 * j + 1]);
+                }
+                if (d == 0) {
+                    *reinterpret_cast<float2 *>(part + size_t(c) * (D + 2) + D) = stats(c);
+                }
+            }
+            if (arrive_last(a, p, &sm.last, consumer_sync)) {
+                merge_tile<kRows, kCache, D>(a, plan, p, warp, kWarps, kCols);
+            }
+        }
+    }
+}
+
+template <int kRows, int kCache, int D, int NT> cudaError_t launch_nt(const ttl_kv &h, const AttendArgs &a, int layer) {
+    kv_attend_tokens_kernel<kRows, kCache, D, NT>
+        <<<h.ctas[0], kThreads, sizeof(TokenSmem<kRows, kCache, D, NT>), h.stream>>>(a, h.maps[size_t(layer)]);
+    return cudaGetLastError();
+}
+
+template <int kRows, int kCache, int D> cudaError_t launch(const ttl_kv &h, const AttendArgs &a, int layer) {
+    if constexpr (kRows == kF32) {
+        return cudaErrorInvalidValue;
+    } else {
+        if (h.width[0] == 8) {
+            return launch_nt<kRows, kCache, D, 1>(h, a, layer);
+        }
+        if (h.width[0] == 16) {
+            return launch_nt<kRows, kCache, D, 2>(h, a, layer);
+        }
+        if constexpr (D == 64) {
+            return launch_nt<kRows, kCache, D, 4>(h, a, layer);
+        }
+        return cudaErrorInvalidValue;
+    }
+}
+
+template <int kRows, int kCache, int D, int NT> cudaError_t configure_nt(ttl_kv &h, int i) {
+    const int bytes = int(sizeof(TokenSmem<kRows, kCache, D, NT>));
+    cudaError_t e = cudaFuncSetAttribute(kv_attend_tokens_kernel<kRows, kCache, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    int n = 0;
+    e = e ? e : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attend_tokens_kernel<kRows, kCache, D, NT>, kThreads, size_t(bytes));
+    h.token_ctas[i] = std::min(std::max(n, 1) * h.sms, kMaxCtas);
+    return e;
+}
+
+template <int kRows, int kCache, int D> cudaError_t configure(ttl_kv &h) {
+    if constexpr (kRows == kF32) {
+        return cudaSuccess;
+    } else {
+        cudaError_t e = configure_nt<kRows, kCache, D, 1>(h, 0);
+        e = e ? e : configure_nt<kRows, kCache, D, 2>(h, 1);
+        if constexpr (D == 64) {
+            e = e ? e : configure_nt<kRows, kCache, D, 4>(h, 2);
+        }
+        return e;
+    }
+}
+
+}  // namespace
+
+cudaError_t tokens_configure(ttl_kv &h) {
+    return TTL_KV_DISPATCH(&h, configure, h);
+}
+
+cudaError_t launch_tokens(const ttl_kv &h, const AttendArgs &a, int layer) {
+    return TTL_KV_DISPATCH(&h, launch, h, a, layer);
+}
+
+}  // namespace kv
+}  // namespace ttl
