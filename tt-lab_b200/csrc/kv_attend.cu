@@ -268,26 +268,36 @@ template <int kRows, int kCache, int D> cudaError_t configure_simple(const ttl_k
 
 }  // namespace
 
+// Sequences of more columns than this go to the prompt kernel.
+constexpr int kFewColumns = 64;
+
 namespace {
 int token_index(int columns, int dim) {
     return columns <= 8 ? 0 : (columns <= 16 || dim == 128 ? 1 : 2);
 }
 }  // namespace
 
-int choose_shapes(const ttl_kv &h, int, int, int max_new, Shape shape[kKinds]) {
-    const int columns = max_new * (h.q_heads / h.kv_heads);
+int choose_shapes(const ttl_kv &h, int seqs, int, int max_new, Shape shape[kKinds]) {
+    const int group = h.q_heads / h.kv_heads, columns = max_new * group;
+    shape[0] = shape[1] = Shape{kPromptWidth, 128, 0};
     if (h.rows_type == kF32) {
         shape[0] = Shape{columns <= 8 ? 8 : 32, kSimpleGran, 2 * h.sms};
-    } else {
-        const int i = token_index(columns, h.dim);
-        shape[0] = Shape{8 << i, 64, h.token_ctas[i]};
+        return 1 << 30;
     }
-    shape[1] = Shape{kPromptWidth, 128, 0};
-    return 1 << 30;
+    const bool prompt = h.prompt_ctas > 0 && columns > kFewColumns;
+    if (prompt) {
+        shape[1].ctas = h.prompt_ctas;
+    }
+    if (prompt && seqs == 1) {
+        return 0;  // one launch: whatever the sequence's rows turn out to be
+    }
+    const int i = token_index(columns, h.dim);
+    shape[0] = Shape{8 << i, 64, h.token_ctas[i]};
+    return prompt ? kFewColumns : 1 << 30;
 }
 
 size_t kv_part_floats(const ttl_kv &h) {
-    size_t most = h.rows_type == kF32 ? size_t(2 * h.sms) * 32 : 0;
+    size_t most = h.rows_type == kF32 ? size_t(2 * h.sms) * 32 : size_t(h.prompt_ctas) * kPromptWidth;
     for (int i = 0; i < 3; ++i) {
         most = std::max(most, size_t(h.token_ctas[i]) * (8 << i));
     }
@@ -298,11 +308,15 @@ cudaError_t kv_configure(ttl_kv &h) {
     if (h.rows_type == kF32) {
         return TTL_KV_DISPATCH(&h, configure_simple, h);
     }
-    return tokens_configure(h);
+    const cudaError_t e = tokens_configure(h);
+    return e ? e : prompt_configure(h);
 }
 
-cudaError_t launch_attend(const ttl_kv &h, const AttendArgs &a, int, int layer) {
-    return h.rows_type == kF32 ? TTL_KV_DISPATCH(&h, launch_simple, h, a) : launch_tokens(h, a, layer);
+cudaError_t launch_attend(const ttl_kv &h, const AttendArgs &a, int kind, int layer) {
+    if (h.rows_type == kF32) {
+        return TTL_KV_DISPATCH(&h, launch_simple, h, a);
+    }
+    return kind == 0 ? launch_tokens(h, a, layer) : launch_prompt(h, a, layer);
 }
 
 }  // namespace kv

@@ -33,6 +33,7 @@ struct ttl_kv {
     uint32_t *status = nullptr;
     std::vector<CUtensorMap> maps; // per layer: the 16-bit pool as rows of head_dim values
     int token_ctas[3] = {};        // CTAs that are resident at once, tiles of 8, 16, 32 columns
+    int prompt_ctas = 0;           // 0: no prompt kernel for the handle's types
     // the last batch call
     bool batched = false;
     int seqs = 0, rows = 0;
@@ -70,6 +71,8 @@ size_t kv_part_floats(const ttl_kv &h);
 cudaError_t kv_configure(ttl_kv &h);
 cudaError_t tokens_configure(ttl_kv &h);
 cudaError_t launch_tokens(const ttl_kv &h, const AttendArgs &a, int layer);
+cudaError_t prompt_configure(ttl_kv &h);
+cudaError_t launch_prompt(const ttl_kv &h, const AttendArgs &a, int layer);
 cudaError_t launch_attend(const ttl_kv &h, const AttendArgs &a, int kind, int layer);
 
 }  // namespace kv

@@ -1,0 +1,567 @@
+// kv_prompt.cu -- attention of many columns per KV head (prompts and chunks of
+// prompts) over the paged cache on tcgen05, for f16 and bf16 rows.
+//
+//   S [128 cols x 128 keys] = Q K^T      A = Q, B = K from shared memory (K-major)
+//   O [128 cols x D]       += P V        A = P from tensor memory, B = V (D-major)
+//
+// What bounds it is neither of these: per score the tensor pipe does 4 D
+// operations (at D = 64, 256 of its 8192 a clock) and the special-function unit
+// one exponential (16 a clock), so 128 x 128 scores take 512 clocks of the one
+// and 1024 of the other.  So the exponentials must never wait:
+//   - a tile is 2 x 128 columns, each with a warpgroup of its own: while one
+//     turns its scores into weights, the tensor pipe works for the other;
+//   - a thread owns a column: its 128 scores of a granule come from tensor
+//     memory into registers once, the maximum and the sum need no shuffles, and
+//     the weights go back over the scores as P;
+//   - the maximum moves only when a weight would pass 2^8 (f16: 2^4), and only
+//     then are the sums in tensor memory read, rescaled and written.
+// One warp loads K and V (TMA, 128-byte swizzle, a ring of granules), one thread
+// issues the matrix instructions.  The scores of granule j + 1 are issued right
+// behind the product of granule j, over the weights it has just read.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "kv.cuh"
+#include "kv_internal.h"
+#include "tc.cuh"
+
+namespace ttl {
+namespace kv {
+
+namespace {
+
+constexpr int kGran = 128;
+constexpr int kHalf = 128;                 // columns of a warpgroup
+constexpr int kLoader = 8, kIssuer = 9;    // warps
+constexpr int kThreads = 384;
+// Registers a thread: 168 at launch (384 threads); the softmax warpgroups keep a
+// granule's 128 scores in them.  256 * 208 + 128 * 80 = 63488 <= 384 * 168.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+constexpr uint32_t kTmemCols = 512;
+
+template <int D> struct PromptSmem {
+    static constexpr int kStages = D == 64 ? 3 : 2;
+    alignas(1024) uint8_t q[2][kHalf * D * 2];
+    alignas(1024) uint8_t k[kStages][kGran * D * 2];
+    alignas(1024) uint8_t v[kStages][kGran * D * 2];
+    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    uint32_t tmem;
+    int last, abort;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *status) {
+    if (tc::mbar_try_wait(bar, parity)) {
+        return true;
+    }
+    if (*abort) {
+        return false;
+    }
+    if (!tc::mbar_wait(bar, parity)) {
+        set_status(status, kKvWait);
+        *abort = 1;
+        return false;
+    }
+    return true;
+}
+
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void softmax_sync() {
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
+// kind::f16: D f32, A and B f16 or bf16, M = 128; b_mn: B is N-major.
+template <int kType> __device__ __forceinline__ constexpr uint32_t f16_desc(uint32_t n, bool b_mn) {
+    const uint32_t t = kType == kBf16 ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// N-major, 128-byte swizzle: rows of 64 N-values (128 bytes), 8-row groups 1024
+// bytes apart along K (SBO), 64-value blocks `lbo` bytes apart along N.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
+    return uint64_t((saddr >> 4) & 0x3FFFu) | uint64_t((lbo >> 4) & 0x3FFFu) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 |
+           uint64_t(2) << 61;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+
+#define KV_R8(a, i) "=f"(a[i]), "=f"(a[i + 1]), "=f"(a[i + 2]), "=f"(a[i + 3]), "=f"(a[i + 4]), "=f"(a[i + 5]), "=f"(a[i + 6]), "=f"(a[i + 7])
+// This warp's 32 lanes, 32 consecutive f32 columns into v[0 .. 31].
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : KV_R8(v, 0), KV_R8(v, 8), KV_R8(v, 16), KV_R8(v, 24)
+        : "r"(taddr)
+        : "memory");
+}
+#undef KV_R8
+#define KV_F8(a, i) "f"(a[i]), "f"(a[i + 1]), "f"(a[i + 2]), "f"(a[i + 3]), "f"(a[i + 4]), "f"(a[i + 5]), "f"(a[i + 6]), "f"(a[i + 7])
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        KV_F8(v, 0), KV_F8(v, 8), KV_F8(v, 16), KV_F8(v, 24)
+        : "memory");
+}
+#undef KV_F8
+
+template <int kType> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (kType == kF16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+template <int D> __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &plan, const CUtensorMap *map, PromptSmem<D> &sm) {
+    const int lane = threadIdx.x & 31;
+    const int seg = min(1 << a.page_shift, 64), segs = kGran / seg, copies = segs * (D / 64);
+    const int s = lane / (D / 64), x = lane % (D / 64);
+    int stage = 0;
+    uint32_t phase = 0;
+    Walker walk(a.walk, int(blockIdx.x));
+    Piece p;
+    while (walk.next(p)) {
+        const int len = a.walk.seq[p.seq].z;
+        const int32_t *table = plan.pages + size_t(p.seq) * plan.page_stride;
+        const int last = max(len - 1, 0) >> a.page_shift;
+        int base = -64, id = 0;
+        for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
+            const int first = k0 >> a.page_shift;
+            if (((k0 + kGran - 1) >> a.page_shift) >= base + 32) {
+                base = first;
+                id = len > 0 ? table[min(base + lane, last)] : 0;
+                if (uint32_t(id) >= uint32_t(a.pages)) {
+                    if (base + lane <= min(last, (p.k1 - 1) >> a.page_shift)) {
+                        set_status(a.status, kKvBadPage);
+                    }
+                    id = 0;
+                }
+            }
+            const int key = k0 + (lane < copies ? s : 0) * seg;
+            const int page = __shfl_sync(0xffffffffu, id, (key >> a.page_shift) - base);
+            const int y = ((page * a.kv_heads + p.head) * 2) * (1 << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+            const uint32_t to = uint32_t(x * kGran + s * seg) * 128;
+            bool ok = wait_or_abort(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
+            if (__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) {
+                    tc::mbar_expect_tx(&sm.k_full[stage], kGran * D * 2);
+                }
+                __syncwarp();
+                if (lane < copies) {
+                    tc::tma_load_2d(sm.k[stage] + to, map, 64 * x, y, &sm.k_full[stage]);
+                }
+            }
+            ok = wait_or_abort(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
+            if (__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) {
+                    tc::mbar_expect_tx(&sm.v_full[stage], kGran * D * 2);
+                }
+                __syncwarp();
+                if (lane < copies) {
+                    tc::tma_load_2d(sm.v[stage] + to, map, 64 * x, y + (1 << a.page_shift), &sm.v_full[stage]);
+                }
+            }
+            if (++stage == PromptSmem<D>::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+    }
+}
+
+// The matrix instructions, from one thread.
+template <int kRows, int D> __device__ __forceinline__ void issue(const AttendArgs &a, PromptSmem<D> &sm, uint32_t tmem) {
+    constexpr int kStages = PromptSmem<D>::kStages;
+    constexpr uint32_t kSDesc = f16_desc<kRows>(kGran, false), kODesc = f16_desc<kRows>(D, true);
+    const uint32_t s_at[2] = {tmem, tmem + 128}, o_at[2] = {tmem + 256, tmem + 256 + D};
+    int ks = 0, vs = 0;
+    uint32_t k_phase = 0, v_phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+    auto scores = [&](int w) {
+        const uint32_t q = tc::smem_u32(sm.q[w]), k = tc::smem_u32(sm.k[ks]);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const uint32_t off = uint32_t(i / 4) * 128 * 128 + uint32_t(i % 4) * 32;
+            mma_ss(s_at[w], tc::smem_desc_sw128(q + off), tc::smem_desc_sw128(k + off), kSDesc, i > 0);
+        }
+        tc::mma_commit(&sm.s_full[w]);
+    };
+    Walker walk(a.walk, int(blockIdx.x));
+    Piece p;
+    while (walk.next(p)) {
+        const int n = (p.k1 - p.k0) / kGran, halves = p.ncols > kHalf ? 2 : 1;
+        wait_or_abort(&sm.k_full[ks], k_phase, &sm.abort, a.status);
+        for (int w = 0; w < halves; ++w) {
+            wait_or_abort(&sm.q_full[w], q_phase[w], &sm.abort, a.status);
+            q_phase[w] ^= 1;
+            tc::fence_after_sync();
+            if (!*const_cast<volatile int *>(&sm.abort)) {
+                scores(w);
+            }
+        }
+        tc::mma_commit(&sm.k_empty[ks]);
+        if (++ks == kStages) {
+            ks = 0;
+            k_phase ^= 1;
+        }
+        for (int j = 0; j < n; ++j) {
+            wait_or_abort(&sm.v_full[vs], v_phase, &sm.abort, a.status);
+            const uint32_t v = tc::smem_u32(sm.v[vs]);
+            for (int w = 0; w < halves; ++w) {
+                wait_or_abort(&sm.p_full[w], p_phase[w], &sm.abort, a.status);
+                p_phase[w] ^= 1;
+                tc::fence_after_sync();
+                if (j + 1 < n && w == 0) {
+                    wait_or_abort(&sm.k_full[ks], k_phase, &sm.abort, a.status);
+                }
+                if (*const_cast<volatile int *>(&sm.abort)) {
+                    continue;
+                }
+#pragma unroll
+                for (int i = 0; i < kGran / 16; ++i) {
+                    mma_ts(o_at[w], s_at[w] + 8 * i, desc_mn(v + uint32_t(i) * 2048, kGran * 128), kODesc, j > 0 || i > 0);
+                }
+                if (j + 1 < n) {
+                    scores(w);
+                } else {
+                    tc::mma_commit(&sm.o_full[w]);
+                }
+            }
+            tc::mma_commit(&sm.v_empty[vs]);
+            if (++vs == kStages) {
+                vs = 0;
+                v_phase ^= 1;
+            }
+            if (j + 1 < n) {
+                tc::mma_commit(&sm.k_empty[ks]);
+                if (++ks == kStages) {
+                    ks = 0;
+                    k_phase ^= 1;
+                }
+            }
+        }
+    }
+}
+
+// A warpgroup: the columns [128 w, 128 w + 128) of each tile, one per thread.
+template <int kRows, int D>
+__device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, PromptSmem<D> &sm, uint32_t tmem) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w = warp >> 2;
+    const uint32_t lanes = uint32_t(warp & 3) << 21;  // (32 * quadrant) << 16
+    const uint32_t s_at = tmem + 128 * w + lanes, o_at = tmem + 256 + D * w + lanes;
+    constexpr float kSlack = kRows == kF16 ? 4.0f : 8.0f;
+    constexpr float kLift = kRows == kF16 ? 11.0f : 0.0f;
+    const float scale = a.scale * kLog2e, cap_log2 = a.cap * kLog2e, two_over_cap = a.cap != 0.0f ? 2.0f / a.cap : 0.0f;
+    uint32_t s_phase = 0, o_phase = 0;
+    Walker walk(a.walk, int(blockIdx.x));
+    Piece p;
+    while (walk.next(p)) {
+        const int4 si = a.walk.seq[p.seq];
+        const int c = tid;  // column of the tile
+        const bool active = w == 0 || p.ncols > kHalf;
+        const bool have = c < p.ncols;
+        int row = 0, qhead = 0;
+        int4 ri = make_int4(0, 0, 1 << 30, -1);
+        float slope = 0.0f;
+        if (have) {
+            const int cc = p.col0 + c, r = cc / a.group;
+            qhead = p.head * a.group + cc - r * a.group;
+            row = si.x + r;
+            ri = a.walk.row[row];
+            ri.y = max(ri.y, 0), ri.z = min(ri.z, si.z);
+            slope = a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
+        }
+        const bool sees = ri.y < ri.z;
+        float m = -INFINITY, l = 0.0f;
+        if (active) {
+            // Q, 16 bytes at a time, swizzled as the matrix instruction reads it
+            {
+                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + size_t(row) * a.q_stride +
+                                                                   size_t(qhead) * D);
+                const bool read = have && row < a.rows;
+                const int r = c & (kHalf - 1);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint4 x = read ? src[i] : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(sm.q[w] + (i / 8) * (kHalf * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tc::fence_before_sync();
+                arrive(&sm.q_full[w]);
+            }
+            for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
+                const bool ok = wait_or_abort(&sm.s_full[w], s_phase, &sm.abort, a.status);
+                s_phase ^= 1;
+                if (!__all_sync(0xffffffffu, ok)) {
+                    continue;
+                }
+                tc::fence_after_sync();
+                float s[kGran];
+#pragma unroll
+                for (int i = 0; i < kGran / 32; ++i) {
+                    tmem_ld32(s_at + 32 * i, s + 32 * i);
+                }
+                tc::wait_ld();
+                const bool plain = a.cap == 0.0f && !a.slopes;
+                float f = scale;
+                if (!plain) {
+                    f = 1.0f;
+#pragma unroll
+                    for (int i = 0; i < kGran; ++i) {
+                        s[i] = score_log2(s[i], scale, cap_log2, two_over_cap, slope, abs(ri.x - k0 - i));
+                    }
+                }
+                if (__any_sync(0xffffffffu, k0 < ri.y || k0 + kGran > ri.z)) {
+                    const int from = ri.y - k0, to = ri.z - k0;
+                    const float out = f < 0.0f ? INFINITY : -INFINITY;  // a negative scale turns it
+#pragma unroll
+                    for (int i = 0; i < kGran; ++i) {
+                        s[i] = i >= from && i < to ? s[i] : out;
+                    }
+                }
+                float top0 = s[0], top1 = s[1], top2 = s[2], top3 = s[3];
+                if (f >= 0.0f) {
+#pragma unroll
+                    for (int i = 4; i < kGran; i += 4) {
+                        top0 = fmaxf(top0, s[i]), top1 = fmaxf(top1, s[i + 1]), top2 = fmaxf(top2, s[i + 2]), top3 = fmaxf(top3, s[i + 3]);
+                    }
+                    top0 = fmaxf(fmaxf(top0, top1), fmaxf(top2, top3));
+                } else {
+#pragma unroll
+                    for (int i = 4; i < kGran; i += 4) {
+                        top0 = fminf(top0, s[i]), top1 = fminf(top1, s[i + 1]), top2 = fminf(top2, s[i + 2]), top3 = fminf(top3, s[i + 3]);
+                    }
+                    top0 = fminf(fminf(top0, top1), fminf(top2, top3));
+                }
+                const float top = top0 * f;
+                if (__any_sync(0xffffffffu, top > m + (kSlack + kLift))) {
+                    const float mn = fmaxf(m, top - kLift);
+                    const float up = ex2(m - (mn == -INFINITY ? 0.0f : mn));
+                    m = mn;
+                    l *= up;
+                    if (k0 != p.k0) {
+                        // the product before has ended: its scores came behind it
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            float o[32];
+                            tmem_ld32(o_at + 32 * i, o);
+                            tc::wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                o[j] *= up;
+                            }
+                            tmem_st32(o_at + 32 * i, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kGran / 32; ++i) {
+                    uint32_t w2[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float p0 = ex2(fmaf(s[32 * i + j], f, -base)), p1 = ex2(fmaf(s[32 * i + j + 1], f, -base));
+                        const float p2 = ex2(fmaf(s[32 * i + j + 2], f, -base)), p3 = ex2(fmaf(s[32 * i + j + 3], f, -base));
+                        l0 += p0, l1 += p1, l2 += p2, l3 += p3;
+                        w2[j / 2] = pack2<kRows>(p0, p1);
+                        w2[j / 2 + 1] = pack2<kRows>(p2, p3);
+                    }
+                    tc::tmem_st16(s_at + 16 * i, w2);
+                }
+                l += (l0 + l1) + (l2 + l3);
+                tc::wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    arrive(&sm.p_full[w]);
+                }
+            }
+        }
+        // ---- the end of the tile ----
+        const bool whole = p.first == p.last;
+        bool bad = false;
+        if (active) {
+            const bool ok = wait_or_abort(&sm.o_full[w], o_phase, &sm.abort, a.status);
+            o_phase ^= 1;
+            tc::fence_after_sync();
+            float g = 1.0f;
+            float *part = a.part + (size_t(part_slot(int(blockIdx.x), p.first)) * kPromptWidth + c) * (D + 2);
+            if (whole) {
+                float mm = m, ll = l;
+                if (a.sinks && have) {
+                    const float sink = a.sinks[qhead] * kLog2e;
+                    mm = fmaxf(m, sink);
+                    const float safe = mm == -INFINITY ? 0.0f : mm;
+                    g = exp2f(m - safe);
+                    ll = l * g + exp2f(sink - safe);
+                }
+                g = g / ll;
+            } else if (have) {
+                part[D] = m, part[D + 1] = l;
+            }
+            const bool write = have && row < a.rows && ri.w == p.seq;
+            if (__all_sync(0xffffffffu, ok)) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    float o[32];
+                    tmem_ld32(o_at + 32 * i, o);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int t = 0; t < 8; ++t) {
+                            v[t] = whole ? (sees ? o[j + t] * g : 0.0f) : o[j + t];
+                            bad = bad || !(fabsf(v[t]) < INFINITY);
+                        }
+                        if (whole && write) {
+                            store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + 32 * i + j, v);
+                        } else if (!whole && have) {
+#pragma unroll
+                            for (int t = 0; t < 8; t += 2) {
+                                *reinterpret_cast<float2 *>(part + 32 * i + j + t) = make_float2(v[t], v[t + 1]);
+                            }
+                        }
+                    }
+                }
+            }
+            tc::fence_before_sync();
+            uint32_t redo = __ballot_sync(0xffffffffu, bad && whole && write);
+            while (redo) {
+                const int src = __ffs(redo) - 1;
+                redo &= redo - 1;
+                attend_column<kRows, kRows, D>(a, plan, p.head, p.seq, __shfl_sync(0xffffffffu, row, src),
+                                               __shfl_sync(0xffffffffu, qhead, src));
+            }
+        }
+        if (!whole) {
+            if (arrive_last(a, p, &sm.last, softmax_sync)) {
+                merge_tile<kRows, kRows, D>(a, plan, p, warp, 8, kPromptWidth);
+            }
+            softmax_sync();
+        }
+    }
+}
+
+template <int kRows, int D>
+__global__ void __launch_bounds__(kThreads, 1) kv_attend_prompt_kernel(AttendArgs a, const __grid_constant__ CUtensorMap map) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    PromptSmem<D> &sm = *reinterpret_cast<PromptSmem<D> *>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const Plan &plan = *a.walk.plan;
+    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kPromptWidth || a.walk.list->gran != kGran) {
+        if (tid == 0) {
+            set_status(a.status, kKvStalePlan);
+        }
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < PromptSmem<D>::kStages; ++i) {
+            tc::mbar_init(&sm.k_full[i], 1);
+            tc::mbar_init(&sm.k_empty[i], 1);
+            tc::mbar_init(&sm.v_full[i], 1);
+            tc::mbar_init(&sm.v_empty[i], 1);
+        }
+        for (int w = 0; w < 2; ++w) {
+            tc::mbar_init(&sm.q_full[w], kHalf);
+            tc::mbar_init(&sm.s_full[w], 1);
+            tc::mbar_init(&sm.p_full[w], 4);
+            tc::mbar_init(&sm.o_full[w], 1);
+        }
+        sm.abort = 0;
+        tc::fence_mbar_init();
+    }
+    if (warp == kIssuer) {
+        tc::tmem_alloc(&sm.tmem, kTmemCols);
+        tc::tmem_relinquish();
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = sm.tmem;
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        soften<kRows, D>(a, plan, sm, tmem);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kLoader) {
+            load_granules<D>(a, plan, &map, sm);
+        } else if (threadIdx.x == 32 * kIssuer) {
+            issue<kRows, D>(a, sm, tmem);
+        }
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == kIssuer) {
+        if (*const_cast<volatile int *>(&sm.abort)) {
+            // copies and products that are still in flight end before their memory goes
+            for (int i = 0; i < PromptSmem<D>::kStages; ++i) {
+                for (uint32_t ph = 0; ph < 2; ++ph) {
+                    tc::mbar_wait(&sm.k_full[i], ph, 1000000ull);
+                    tc::mbar_wait(&sm.v_full[i], ph, 1000000ull);
+                    tc::mbar_wait(&sm.k_empty[i], ph, 1000000ull);
+                    tc::mbar_wait(&sm.v_empty[i], ph, 1000000ull);
+                }
+            }
+        }
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <int kRows, int kCache, int D> cudaError_t launch(const ttl_kv &h, const AttendArgs &a, int layer) {
+    if constexpr (kRows == kF32 || kCache == kMxfp4) {
+        return cudaErrorInvalidValue;
+    } else {
+        kv_attend_prompt_kernel<kRows, D><<<h.ctas[1], kThreads, sizeof(PromptSmem<D>), h.stream>>>(a, h.maps[size_t(layer)]);
+        return cudaGetLastError();
+    }
+}
+
+template <int kRows, int kCache, int D> cudaError_t configure(ttl_kv &h) {
+    if constexpr (kRows == kF32 || kCache == kMxfp4) {
+        return cudaSuccess;
+    } else {
+        h.prompt_ctas = std::min(h.sms, kMaxCtas);
+        return cudaFuncSetAttribute(kv_attend_prompt_kernel<kRows, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PromptSmem<D>)));
+    }
+}
+
+}  // namespace
+
+cudaError_t prompt_configure(ttl_kv &h) {
+    return TTL_KV_DISPATCH(&h, configure, h);
+}
+
+cudaError_t launch_prompt(const ttl_kv &h, const AttendArgs &a, int layer) {
+    return TTL_KV_DISPATCH(&h, launch, h, a, layer);
+}
+
+}  // namespace kv
+}  // namespace ttl
