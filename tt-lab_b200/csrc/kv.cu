@@ -35,13 +35,13 @@ struct PlanArgs {
     const int32_t *row_start, *length, *pages, *first, *prefix_len;
     uint32_t page_stride;
     int seqs, rows, max_new, group, kv_heads, window, page_tokens;
-    int width[2], gran[2], ctas[2];  // ctas 0: no sequence goes to this kind
+    int width[2], gran[2], cost[2], ctas[2];  // ctas 0: no sequence goes to this kind
     int few;                         // sequences of at most this many columns go to kind 0
     int tile_cap[2];
 };
 
 constexpr int kPlanThreads = 1024;
-constexpr int kMaxPosition = 1 << 30;
+constexpr int kMaxPosition = 1 << 29;  // a tile counts up to 2^23 granules
 
 struct SeqState {
     int row0, n, len;
@@ -154,11 +154,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     }
     if (sliding && a.window == 0) {
         if (tid == 0) {
-            a.plan->list[kind][1] = List{0, 0, 0, 0, 0, {0, 0, 0}};
+            a.plan->list[kind][1] = List{0, 0, 0, 0, {0, 0, 0, 0}};
         }
         return;
     }
-    const int width = a.width[kind], gran = a.gran[kind];
+    const int width = a.width[kind], gran = a.gran[kind], cost = a.cost[kind];
     Tile *tiles = a.tiles[kind][sliding];
     int32_t *prefix = a.prefix[kind][sliding];
     Cut *cuts = a.cuts[kind][sliding];
@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             const int g0 = begin < end ? begin / gran : 0;
             // at least one granule: a tile whose rows see nothing is written too
             n = begin < end ? (end + gran - 1) / gran - g0 : 1;
-            tiles[t] = Tile{lo, col0, ncols, g0};
+            tiles[t] = Tile{lo, col0, g0, uint32_t(ncols) | uint32_t(n) << 9};
+            n += cost;
         }
         int sum;
         const int at = block_scan(n, &sum, sums);
@@ -250,13 +251,13 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     }
     if (tid == 0) {
         prefix[total] = line;
-        a.plan->list[kind][sliding] = List{total, a.ctas[kind], width, gran, line, {0, 0, 0}};
+        a.plan->list[kind][sliding] = List{total, a.ctas[kind], width, gran, {0, 0, 0, 0}};
     }
     __syncthreads();
     // the cuts: equal shares of the line of all heads; a tile of few granules
     // is not cut, and no tile is cut next to its ends
     const long long all = (long long)(line) * a.kv_heads;
-    // at least one granule per share, so that cuts inside a tile differ
+    // at least one unit per share, so that cuts inside a tile differ
     const int shares = int(min((long long)(a.ctas[kind]), all));
     for (int c = tid; c <= a.ctas[kind]; c += kPlanThreads) {
         Cut cut{total == 0 ? 0 : a.kv_heads, 0, 0, 0u};
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
                     hi = mid;
                 }
             }
-            const int g = rest - prefix[lo], n = prefix[lo + 1] - prefix[lo];
+            const int g = rest - prefix[lo] - cost, n = prefix[lo + 1] - prefix[lo] - cost;
             cut.tile = lo;
             if (n <= kNoSplit ? 2 * g < n : g < 2) {
                 cut.gran = 0;
@@ -953,6 +954,7 @@ int kv_batch(ttl_kv *h, uint32_t seqs, uint32_t rows, uint32_t max_new, const in
     for (int k = 0; k < kKinds; ++k) {
         a.width[k] = h->width[k] = shape[k].width;
         a.gran[k] = shape[k].gran;
+        a.cost[k] = shape[k].cost;
         a.ctas[k] = h->ctas[k] = shape[k].ctas;
         a.tile_cap[k] = h->tile_cap[k];
     }
@@ -1056,7 +1058,7 @@ int kv_attend(ttl_kv *h, int layer, uint32_t flags, const void *q, size_t q_stri
             continue;
         }
         AttendArgs a{};
-        a.walk = Walk{h->plan, &h->plan->list[kind][w], h->tiles[kind][w], h->prefix[kind][w], h->cuts[kind][w], h->row[w], h->seq};
+        a.walk = Walk{h->plan, &h->plan->list[kind][w], h->tiles[kind][w], h->cuts[kind][w], h->row[w], h->seq};
         a.pool = h->pool + size_t(layer) * h->layer_bytes;
         a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
         a.sinks = sinks, a.slopes = slopes;

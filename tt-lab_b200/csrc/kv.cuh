@@ -7,10 +7,10 @@
 // query head kv * group + g).  A tile is up to `width` columns of a sequence.
 //
 // Plan.  A tile's visible key range is counted in granules (of 64 or 128
-// keys); tiles are laid end to end, once per KV head, and the line is cut into
-// one piece of equal length per CTA.  So every CTA gets the same number of
-// key granules whatever the batch's shape, in one wave; a tile cut by a CTA
-// border leaves partial sums in the workspace, and the CTA that arrives last
+// keys); tiles are laid end to end, once per KV head, each as long as its
+// granules and the few that its start and end cost, and the line is cut into
+// one piece of equal length per CTA.  So every CTA gets the same work
+// whatever the batch's shape, in one wave; a tile cut by a CTA border leaves partial sums in the workspace, and the CTA that arrives last
 // merges them, in the order of the keys, so results do not depend on timing.
 #pragma once
 
@@ -38,8 +38,9 @@ constexpr int kKinds = 2;          // tiles of few columns, tiles of a prompt
 constexpr int kMaxCtas = 1024;     // CTAs of a list (cuts)
 constexpr int kNoSplit = 4;        // a tile of at most this many granules is not cut
 
-struct Tile {
-    int32_t seq, col0, ncols, gran0;
+struct __align__(16) Tile {
+    int32_t seq, col0, gran0;
+    uint32_t size;                 // columns (9 bits), granules
 };
 struct __align__(16) Cut {
     int32_t head, tile, gran;      // gran: granules into the tile
@@ -47,8 +48,7 @@ struct __align__(16) Cut {
 };
 struct List {
     int32_t tiles, ctas, width, gran;
-    int32_t line;                  // granules of one head's line
-    int32_t pad[3];
+    int32_t pad[4];
 };
 struct Plan {
     const int32_t *pages;
@@ -62,7 +62,6 @@ struct Walk {
     const Plan *plan;
     const List *list;
     const Tile *tiles;
-    const int32_t *prefix;         // [tiles + 1] granules before a tile
     const Cut *cuts;               // [ctas + 1]
     const int4 *row;               // [rows] {position, lo, hi, seq} of this window; seq -1: padding
     const int4 *seq;               // [seqs] {row0, rows, length, 0}
@@ -182,26 +181,20 @@ __device__ __forceinline__ int page_of(const Plan &plan, int seq, int pos, int p
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A score in log2 units from the raw product: scaled, capped, with the
-// distance bias.  tanh as 1 - 2 / (e^2x + 1): absolute error about 1e-7 of the
-// cap, where the hardware's tanh.approx has 5e-4.
-__device__ __forceinline__ float score_log2(float dot, float scale_log2, float cap_log2, float two_over_cap, float slope_log2,
-                                            int distance) {
-    float t;
-    if (cap_log2 != 0.0f) {
-        // scale_log2 here is scale * log2(e); two_over_cap * (dot * scale) in log2 units
-        const float e = exp2f(dot * scale_log2 * two_over_cap);
-        t = cap_log2 - __fdividef(2.0f * cap_log2, e + 1.0f);
-        if (e > 1e30f) {  // __fdividef returns 0 from 2^126 on, and NaN for an infinite divisor is ruled out here
-            t = cap_log2;
-        }
-        if (dot != dot) {
-            t = dot;
-        }
-    } else {
-        t = dot * scale_log2;
-    }
-    return t - slope_log2 * float(distance);
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// cap * tanh(x / cap) in log2 units, from the raw product: `in` is the scale
+// times 2 log2(e) / cap, `out` cap * log2(e).  tanh y = 1 - 2 / (e^2y + 1): its
+// absolute error is about 2^-22, where the hardware's tanh.approx has 2^-11;
+// e^2y = infinity gives 1.
+__device__ __forceinline__ float capped(float dot, float in, float out) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(dot * in) + 1.0f));
+    return fmaf(-2.0f * out, r, out);
 }
 
 // ---- the walk ----
@@ -234,12 +227,12 @@ struct Walker {
             return false;
         }
         const Tile t = w.tiles[tile];
-        const int n = w.prefix[tile + 1] - w.prefix[tile];
+        const int n = int(t.size >> 9);
         int stop = n;
         if (end.head == head && end.tile == tile) {
             stop = end.gran;  // > gran
         }
-        p.head = head, p.tile = tile, p.seq = t.seq, p.col0 = t.col0, p.ncols = t.ncols;
+        p.head = head, p.tile = tile, p.seq = t.seq, p.col0 = t.col0, p.ncols = int(t.size & 511u);
         const int gsize = w.list->gran;
         p.k0 = (t.gran0 + gran) * gsize;
         p.k1 = (t.gran0 + stop) * gsize;

@@ -279,9 +279,9 @@ int token_index(int columns, int dim) {
 
 int choose_shapes(const ttl_kv &h, int seqs, int, int max_new, Shape shape[kKinds]) {
     const int group = h.q_heads / h.kv_heads, columns = max_new * group;
-    shape[0] = shape[1] = Shape{kPromptWidth, 128, 0};
+    shape[0] = shape[1] = Shape{kPromptWidth, 128, 2, 0};
     if (h.rows_type == kF32) {
-        shape[0] = Shape{columns <= 8 ? 8 : 32, kSimpleGran, 2 * h.sms};
+        shape[0] = Shape{columns <= 8 ? 8 : 32, kSimpleGran, 1, 2 * h.sms};
         return 1 << 30;
     }
     const bool prompt = h.prompt_ctas > 0 && columns > kFewColumns;
@@ -292,7 +292,7 @@ int choose_shapes(const ttl_kv &h, int seqs, int, int max_new, Shape shape[kKind
         return 0;  // one launch: whatever the sequence's rows turn out to be
     }
     const int i = token_index(columns, h.dim);
-    shape[0] = Shape{8 << i, 64, h.token_ctas[i]};
+    shape[0] = Shape{8 << i, 64, 1, h.token_ctas[i]};
     return prompt ? kFewColumns : 1 << 30;
 }
 

@@ -59,7 +59,7 @@ constexpr int kPromptWidth = 256;  // columns of a prompt tile
 
 // Shape of one kind's launch.
 struct Shape {
-    int width, gran, ctas;         // columns per tile, keys per granule, CTAs (0: no launch)
+    int width, gran, cost, ctas;   // columns per tile, keys per granule, granules a tile's ends cost, CTAs (0: no launch)
 };
 
 // Chooses the kernels of a batch; returns the most columns of a sequence that

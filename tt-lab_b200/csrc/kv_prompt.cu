@@ -52,12 +52,6 @@ template <int D> struct PromptSmem {
     int last, abort;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *status) {
     if (tc::mbar_try_wait(bar, parity)) {
         return true;
@@ -211,8 +205,10 @@ template <int kRows, int D> __device__ __forceinline__ void issue(const AttendAr
         tc::mma_commit(&sm.s_full[w]);
     };
     Walker walk(a.walk, int(blockIdx.x));
-    Piece p;
-    while (walk.next(p)) {
+    Piece p, ahead;
+    bool any = walk.next(p), more;
+    for (; any; any = more, p = ahead) {
+        more = walk.next(ahead);
         const int n = (p.k1 - p.k0) / kGran, halves = p.ncols > kHalf ? 2 : 1;
         wait_or_abort(&sm.k_full[ks], k_phase, &sm.abort, a.status);
         for (int w = 0; w < halves; ++w) {
@@ -275,44 +271,78 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
     const uint32_t s_at = tmem + 128 * w + lanes, o_at = tmem + 256 + D * w + lanes;
     constexpr float kSlack = kRows == kF16 ? 4.0f : 8.0f;
     constexpr float kLift = kRows == kF16 ? 11.0f : 0.0f;
-    const float scale = a.scale * kLog2e, cap_log2 = a.cap * kLog2e, two_over_cap = a.cap != 0.0f ? 2.0f / a.cap : 0.0f;
+    const float scale = a.scale * kLog2e, cap_log2 = a.cap * kLog2e;
+    const float cap_in = a.cap != 0.0f ? scale * 2.0f / a.cap : 0.0f;
+    const float sign = scale < 0.0f ? -1.0f : 1.0f;  // the largest score is the smallest product where the scale is negative
+    const bool special = a.cap != 0.0f || a.slopes;
     uint32_t s_phase = 0, o_phase = 0;
     Walker walk(a.walk, int(blockIdx.x));
-    Piece p;
-    while (walk.next(p)) {
-        const int4 si = a.walk.seq[p.seq];
-        const int c = tid;  // column of the tile
-        const bool active = w == 0 || p.ncols > kHalf;
-        const bool have = c < p.ncols;
-        int row = 0, qhead = 0;
-        int4 ri = make_int4(0, 0, 1 << 30, -1);
-        float slope = 0.0f;
-        if (have) {
-            const int cc = p.col0 + c, r = cc / a.group;
-            qhead = p.head * a.group + cc - r * a.group;
-            row = si.x + r;
-            ri = a.walk.row[row];
-            ri.y = max(ri.y, 0), ri.z = min(ri.z, si.z);
-            slope = a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
+    // The tile after the one in hand is looked up while that one runs, and its Q
+    // rows are copied as soon as the last scores of this one are there, so that
+    // its first scores are under way before this one has ended.
+    struct Column {
+        Piece p;
+        bool any, active, have;
+        int row, qhead;
+        int4 ri;
+        float slope;
+    };
+    auto look_up = [&](Column &c) {
+        c.any = walk.next(c.p);
+        c.active = c.any && (w == 0 || c.p.ncols > kHalf);
+        c.have = c.any && tid < c.p.ncols;
+        c.row = 0, c.qhead = 0, c.slope = 0.0f;
+        c.ri = make_int4(0, 0, 1 << 30, -1);
+        if (c.have) {
+            const int4 si = a.walk.seq[c.p.seq];
+            const int cc = c.p.col0 + tid, r = cc / a.group;
+            c.qhead = c.p.head * a.group + cc - r * a.group;
+            c.row = si.x + r;
+            c.ri = a.walk.row[c.row];
+            c.ri.y = max(c.ri.y, 0), c.ri.z = min(c.ri.z, si.z);
+            c.slope = a.slopes ? a.slopes[c.qhead] * kLog2e : 0.0f;
         }
+    };
+    // Q, 16 bytes at a time, swizzled as the matrix instruction reads it
+    auto copy_q = [&](const Column &c) {
+        const bool read = c.have && c.row < a.rows;
+        const uint16_t *src = static_cast<const uint16_t *>(a.q) + (read ? size_t(c.row) * a.q_stride + size_t(c.qhead) * D : 0);
+        const int r = tid & (kHalf - 1);
+        const uint32_t to = tc::smem_u32(sm.q[w]) + r * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + uint32_t(i / 8) * (kHalf * 128) + (((i & 7) ^ (r & 7)) << 4)),
+                         "l"(src + (read ? 8 * i : 0)), "r"(read ? 16 : 0)
+                         : "memory");
+        }
+    };
+    auto publish_q = [&] {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc::fence_before_sync();
+        arrive(&sm.q_full[w]);
+    };
+    Column cur, next;
+    look_up(cur);
+    if (cur.active) {
+        copy_q(cur);
+        publish_q();
+    }
+    for (; cur.any; cur = next) {
+        look_up(next);
+        const Piece &p = cur.p;
+        const int c = tid;  // column of the tile
+        const bool active = cur.active, have = cur.have;
+        const int row = cur.row, qhead = cur.qhead;
+        const int4 ri = cur.ri;
+        const float slope = cur.slope;
         const bool sees = ri.y < ri.z;
         float m = -INFINITY, l = 0.0f;
+        if (!active && next.active) {
+            copy_q(next);
+            publish_q();
+        }
         if (active) {
-            // Q, 16 bytes at a time, swizzled as the matrix instruction reads it
-            {
-                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + size_t(row) * a.q_stride +
-                                                                   size_t(qhead) * D);
-                const bool read = have && row < a.rows;
-                const int r = c & (kHalf - 1);
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint4 x = read ? src[i] : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4 *>(sm.q[w] + (i / 8) * (kHalf * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = x;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                tc::fence_before_sync();
-                arrive(&sm.q_full[w]);
-            }
             for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
                 const bool ok = wait_or_abort(&sm.s_full[w], s_phase, &sm.abort, a.status);
                 s_phase ^= 1;
@@ -320,77 +350,109 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                     continue;
                 }
                 tc::fence_after_sync();
-                float s[kGran];
-#pragma unroll
-                for (int i = 0; i < kGran / 32; ++i) {
-                    tmem_ld32(s_at + 32 * i, s + 32 * i);
+                if (k0 + kGran >= p.k1 && next.active) {
+                    copy_q(next);  // the last scores of this tile: its Q has been read
                 }
-                tc::wait_ld();
-                const bool plain = a.cap == 0.0f && !a.slopes;
-                float f = scale;
-                if (!plain) {
+                // ---- the maximum; scores that are capped, biased or masked go back as they then are ----
+                float f = scale, top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                const bool mask = __any_sync(0xffffffffu, k0 < ri.y || k0 + kGran > ri.z);
+                if (mask || special) {
                     f = 1.0f;
-#pragma unroll
-                    for (int i = 0; i < kGran; ++i) {
-                        s[i] = score_log2(s[i], scale, cap_log2, two_over_cap, slope, abs(ri.x - k0 - i));
-                    }
-                }
-                if (__any_sync(0xffffffffu, k0 < ri.y || k0 + kGran > ri.z)) {
                     const int from = ri.y - k0, to = ri.z - k0;
-                    const float out = f < 0.0f ? INFINITY : -INFINITY;  // a negative scale turns it
+#pragma unroll 1
+                    for (int i = 0; i < kGran; i += 32) {
+                        float s[32];
+                        tmem_ld32(s_at + i, s);
+                        tc::wait_ld();
+                        if (a.cap != 0.0f) {
 #pragma unroll
-                    for (int i = 0; i < kGran; ++i) {
-                        s[i] = i >= from && i < to ? s[i] : out;
-                    }
-                }
-                float top0 = s[0], top1 = s[1], top2 = s[2], top3 = s[3];
-                if (f >= 0.0f) {
+                            for (int j = 0; j < 32; ++j) {
+                                s[j] = capped(s[j], cap_in, cap_log2);
+                            }
+                        } else {
 #pragma unroll
-                    for (int i = 4; i < kGran; i += 4) {
-                        top0 = fmaxf(top0, s[i]), top1 = fmaxf(top1, s[i + 1]), top2 = fmaxf(top2, s[i + 2]), top3 = fmaxf(top3, s[i + 3]);
+                            for (int j = 0; j < 32; ++j) {
+                                s[j] *= scale;
+                            }
+                        }
+                        if (a.slopes) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                s[j] = fmaf(-slope, fabsf(float(ri.x - k0 - i - j)), s[j]);
+                            }
+                        }
+                        if (mask) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                s[j] = i + j >= from && i + j < to ? s[j] : -INFINITY;
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            top[j & 3] = fmaxf(top[j & 3], s[j]);
+                        }
+                        tmem_st32(s_at + i, s);
                     }
-                    top0 = fmaxf(fmaxf(top0, top1), fmaxf(top2, top3));
+                    tc::wait_st();
                 } else {
+                    float s[2][32];
+                    tmem_ld32(s_at, s[0]);
+                    tc::wait_ld();
 #pragma unroll
-                    for (int i = 4; i < kGran; i += 4) {
-                        top0 = fminf(top0, s[i]), top1 = fminf(top1, s[i + 1]), top2 = fminf(top2, s[i + 2]), top3 = fminf(top3, s[i + 3]);
+                    for (int i = 0; i < kGran / 32; ++i) {
+                        if (i + 1 < kGran / 32) {
+                            tmem_ld32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            top[j & 3] = fmaxf(top[j & 3], s[i & 1][j] * sign);
+                        }
+                        tc::wait_ld();
                     }
-                    top0 = fminf(fminf(top0, top1), fminf(top2, top3));
                 }
-                const float top = top0 * f;
-                if (__any_sync(0xffffffffu, top > m + (kSlack + kLift))) {
-                    const float mn = fmaxf(m, top - kLift);
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (f == 1.0f ? 1.0f : f * sign);
+                float s[2][32];
+                tmem_ld32(s_at, s[0]);
+                if (__any_sync(0xffffffffu, most > m + (kSlack + kLift))) {
+                    const float mn = fmaxf(m, most - kLift);
                     const float up = ex2(m - (mn == -INFINITY ? 0.0f : mn));
                     m = mn;
                     l *= up;
                     if (k0 != p.k0) {
                         // the product before has ended: its scores came behind it
-#pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 32) {
                             float o[32];
-                            tmem_ld32(o_at + 32 * i, o);
+                            tmem_ld32(o_at + i, o);
                             tc::wait_ld();
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
                                 o[j] *= up;
                             }
-                            tmem_st32(o_at + 32 * i, o);
+                            tmem_st32(o_at + i, o);
                         }
                     }
                 }
+                // ---- the weights, over the scores ----
                 const float base = m == -INFINITY ? 0.0f : m;
                 float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+                tc::wait_ld();
 #pragma unroll
                 for (int i = 0; i < kGran / 32; ++i) {
+                    if (i + 1 < kGran / 32) {
+                        tmem_ld32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
+                    }
                     uint32_t w2[16];
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        const float p0 = ex2(fmaf(s[32 * i + j], f, -base)), p1 = ex2(fmaf(s[32 * i + j + 1], f, -base));
-                        const float p2 = ex2(fmaf(s[32 * i + j + 2], f, -base)), p3 = ex2(fmaf(s[32 * i + j + 3], f, -base));
+                        const float *x = s[i & 1] + j;
+                        const float p0 = ex2(fmaf(x[0], f, -base)), p1 = ex2(fmaf(x[1], f, -base));
+                        const float p2 = ex2(fmaf(x[2], f, -base)), p3 = ex2(fmaf(x[3], f, -base));
                         l0 += p0, l1 += p1, l2 += p2, l3 += p3;
                         w2[j / 2] = pack2<kRows>(p0, p1);
                         w2[j / 2 + 1] = pack2<kRows>(p2, p3);
                     }
+                    tc::wait_ld();
                     tc::tmem_st16(s_at + 16 * i, w2);
                 }
                 l += (l0 + l1) + (l2 + l3);
@@ -400,6 +462,9 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 if (lane == 0) {
                     arrive(&sm.p_full[w]);
                 }
+            }
+            if (next.active) {
+                publish_q();
             }
         }
         // ---- the end of the tile ----

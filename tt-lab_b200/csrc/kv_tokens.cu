@@ -74,12 +74,6 @@ __device__ __forceinline__ void consumer_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -485,7 +479,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int c = 8 * n + 2 * t + (j & 1), key = key0 + g + (j >> 1) * 8;
-                            s[n][j] = score_log2(s[n][j], scale[n][j & 1], cap_log2, two_over_cap, sm.slope[c], abs(sm.pos[c] - key));
+                            const float x = cap_log2 != 0.0f ? capped(s[n][j], scale[n][j & 1] * two_over_cap, cap_log2) : s[n][j] * scale[n][j & 1];
+                            s[n][j] = fmaf(-sm.slope[c], float(abs(sm.pos[c] - key)), x);
                         }
                     }
                 }
