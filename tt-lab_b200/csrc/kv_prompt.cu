@@ -35,17 +35,28 @@ namespace {
 constexpr int kGran = 128;
 constexpr int kHalf = 128;                 // columns of a warpgroup
 constexpr int kLoader = 8, kIssuer = 9;    // warps
-constexpr int kThreads = 384;
-// Registers a thread: 168 at launch (384 threads); the softmax warpgroups keep a
-// granule's 128 scores in them.  256 * 208 + 128 * 80 = 63488 <= 384 * 168.
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+constexpr int kExpander = 12;              // first of the four warps that expand a 4-bit cache
 constexpr uint32_t kTmemCols = 512;
 
-template <int D> struct PromptSmem {
+// Threads, and registers of the softmax warpgroups, of the loader's and of the
+// expanders': a warpgroup may only take what the launch holds (168 or 128 a
+// thread), 256 * 208 + 128 * 80 <= 384 * 168 and 256 * 168 + 128 * 64 + 128 * 104
+// <= 512 * 128.
+template <int kCache> struct PromptShape {
+    static constexpr bool kFour = kCache == kMxfp4;
+    static constexpr int kThreads = kFour ? 512 : 384;
+    static constexpr int kSoftmaxRegs = kFour ? 168 : 208, kOtherRegs = kFour ? 64 : 80, kExpandRegs = 104;
+    static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs + (kFour ? 128 * kExpandRegs : 0) <= kThreads * (kFour ? 128 : 168), "registers");
+};
+
+template <int kCache, int D> struct PromptSmem {
     static constexpr int kStages = D == 64 ? 3 : 2;
+    static constexpr uint32_t kRawBytes = kCache == kMxfp4 ? 2 * kGran * row_bytes(kMxfp4, D) : 16;  // a granule as the cache holds it
     alignas(1024) uint8_t q[2][kHalf * D * 2];
     alignas(1024) uint8_t k[kStages][kGran * D * 2];
     alignas(1024) uint8_t v[kStages][kGran * D * 2];
+    alignas(16) uint8_t raw[2][kRawBytes];
+    uint64_t raw_full[2], raw_empty[2];
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
     uint32_t tmem;
@@ -131,10 +142,13 @@ template <int kType> __device__ __forceinline__ uint32_t pack2(float lo, float h
     }
 }
 
-template <int D> __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &plan, const CUtensorMap *map, PromptSmem<D> &sm) {
+template <int kCache, int D>
+__device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &plan, const CUtensorMap *map, PromptSmem<kCache, D> &sm) {
     const int lane = threadIdx.x & 31;
-    const int seg = min(1 << a.page_shift, 64), segs = kGran / seg, copies = segs * (D / 64);
-    const int s = lane / (D / 64), x = lane % (D / 64);
+    // 16 bits: boxes of 64 values x up to 64 keys; 4 bits: a head's whole part of a page
+    constexpr int kParts = kCache == kMxfp4 ? 1 : D / 64;
+    const int seg = min(1 << a.page_shift, kCache == kMxfp4 ? kGran : 64), segs = kGran / seg, copies = segs * kParts;
+    const int s = lane / kParts, x = lane % kParts;
     int stage = 0;
     uint32_t phase = 0;
     Walker walk(a.walk, int(blockIdx.x));
@@ -158,6 +172,27 @@ template <int D> __device__ __forceinline__ void load_granules(const AttendArgs 
             }
             const int key = k0 + (lane < copies ? s : 0) * seg;
             const int page = __shfl_sync(0xffffffffu, id, (key >> a.page_shift) - base);
+            if constexpr (kCache == kMxfp4) {
+                const bool ok = wait_or_abort(&sm.raw_empty[stage], phase ^ 1, &sm.abort, a.status);
+                if (__all_sync(0xffffffffu, ok)) {
+                    if (lane == 0) {
+                        tc::mbar_expect_tx(&sm.raw_full[stage], PromptSmem<kCache, D>::kRawBytes);
+                    }
+                    __syncwarp();
+                    if (lane < copies) {
+                        const uint8_t *src = a.pool + (size_t(page) * a.kv_heads + p.head) * a.block_bytes;
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                         tc::smem_u32(sm.raw[stage] + lane * a.block_bytes)),
+                                     "l"(src), "r"(a.block_bytes), "r"(tc::smem_u32(&sm.raw_full[stage]))
+                                     : "memory");
+                    }
+                }
+                if (++stage == 2) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+                continue;
+            }
             const int y = ((page * a.kv_heads + p.head) * 2) * (1 << a.page_shift) + (key & ((1 << a.page_shift) - 1));
             const uint32_t to = uint32_t(x * kGran + s * seg) * 128;
             bool ok = wait_or_abort(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
@@ -180,7 +215,61 @@ template <int D> __device__ __forceinline__ void load_granules(const AttendArgs 
                     tc::tma_load_2d(sm.v[stage] + to, map, 64 * x, y + (1 << a.page_shift), &sm.v_full[stage]);
                 }
             }
-            if (++stage == PromptSmem<D>::kStages) {
+            if (++stage == PromptSmem<kCache, D>::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+    }
+}
+
+// A granule of a 4-bit cache to bf16, which holds every code times its scale
+// exactly: a thread per key, K then V, into the places that TMA fills for a
+// 16-bit cache.
+template <int kCache, int D> __device__ __forceinline__ void expand(const AttendArgs &a, PromptSmem<kCache, D> &sm) {
+    const int key = threadIdx.x - 32 * kExpander;
+    int stage = 0, raw = 0;
+    uint32_t phase = 0, raw_phase = 0;
+    const int tokens = 1 << a.page_shift;
+    const uint32_t at = uint32_t(key >> a.page_shift) * a.block_bytes;
+    const int t = key & (tokens - 1);
+    auto half = [&](const uint8_t *src, uint8_t *dst) {
+        const uint8_t *scales = src + tokens * (D / 2) + t * (D / 32);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+            const uint32_t e = scales[b];
+            const float f = e == 255u ? __uint_as_float(0x7fffffffu) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
+            const uint4 w = *reinterpret_cast<const uint4 *>(src + t * (D / 2) + 16 * b);
+            const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 v = __half22float2(e2m1x2_to_half2((c[i] >> (8 * j)) & 255u));
+                    o[j] = pack2<kBf16>(v.x * f, v.y * f);
+                }
+                const int chunk = 4 * (b & 1) + i;
+                *reinterpret_cast<uint4 *>(dst + (b / 2) * (kGran * 128) + key * 128 + ((chunk ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    };
+    Walker walk(a.walk, int(blockIdx.x));
+    Piece p;
+    while (walk.next(p)) {
+        for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
+            wait_or_abort(&sm.raw_full[raw], raw_phase, &sm.abort, a.status);
+            wait_or_abort(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
+            half(sm.raw[raw] + at, sm.k[stage]);
+            arrive(&sm.k_full[stage]);
+            wait_or_abort(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
+            half(sm.raw[raw] + at + (a.block_bytes >> 1), sm.v[stage]);
+            arrive(&sm.v_full[stage]);
+            arrive(&sm.raw_empty[raw]);
+            raw_phase ^= uint32_t(raw);
+            raw ^= 1;
+            if (++stage == PromptSmem<kCache, D>::kStages) {
                 stage = 0;
                 phase ^= 1;
             }
@@ -189,8 +278,8 @@ template <int D> __device__ __forceinline__ void load_granules(const AttendArgs 
 }
 
 // The matrix instructions, from one thread.
-template <int kRows, int D> __device__ __forceinline__ void issue(const AttendArgs &a, PromptSmem<D> &sm, uint32_t tmem) {
-    constexpr int kStages = PromptSmem<D>::kStages;
+template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(const AttendArgs &a, PromptSmem<kCache, D> &sm, uint32_t tmem) {
+    constexpr int kStages = PromptSmem<kCache, D>::kStages;
     constexpr uint32_t kSDesc = f16_desc<kRows>(kGran, false), kODesc = f16_desc<kRows>(D, true);
     const uint32_t s_at[2] = {tmem, tmem + 128}, o_at[2] = {tmem + 256, tmem + 256 + D};
     int ks = 0, vs = 0;
@@ -264,8 +353,8 @@ template <int kRows, int D> __device__ __forceinline__ void issue(const AttendAr
 }
 
 // A warpgroup: the columns [128 w, 128 w + 128) of each tile, one per thread.
-template <int kRows, int D>
-__device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, PromptSmem<D> &sm, uint32_t tmem) {
+template <int kRows, int kCache, int D>
+__device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, PromptSmem<kCache, D> &sm, uint32_t tmem) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w = warp >> 2;
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // (32 * quadrant) << 16
     const uint32_t s_at = tmem + 128 * w + lanes, o_at = tmem + 256 + D * w + lanes;
@@ -520,23 +609,26 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
             while (redo) {
                 const int src = __ffs(redo) - 1;
                 redo &= redo - 1;
-                attend_column<kRows, kRows, D>(a, plan, p.head, p.seq, __shfl_sync(0xffffffffu, row, src),
+                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, __shfl_sync(0xffffffffu, row, src),
                                                __shfl_sync(0xffffffffu, qhead, src));
             }
         }
         if (!whole) {
             if (arrive_last(a, p, &sm.last, softmax_sync)) {
-                merge_tile<kRows, kRows, D>(a, plan, p, warp, 8, kPromptWidth);
+                merge_tile<kRows, kCache, D>(a, plan, p, warp, 8, kPromptWidth);
             }
             softmax_sync();
         }
     }
 }
 
-template <int kRows, int D>
-__global__ void __launch_bounds__(kThreads, 1) kv_attend_prompt_kernel(AttendArgs a, const __grid_constant__ CUtensorMap map) {
+template <int kRows, int kCache, int D>
+__global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
+    kv_attend_prompt_kernel(AttendArgs a, const __grid_constant__ CUtensorMap map) {
+    using Shape = PromptShape<kCache>;
+    using Smem = PromptSmem<kCache, D>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    PromptSmem<D> &sm = *reinterpret_cast<PromptSmem<D> *>(smem_raw);
+    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5;
     const Plan &plan = *a.walk.plan;
     if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kPromptWidth || a.walk.list->gran != kGran) {
@@ -546,13 +638,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_prompt_kernel(AttendArg
         return;
     }
     if (tid == 0) {
-        for (int i = 0; i < PromptSmem<D>::kStages; ++i) {
-            tc::mbar_init(&sm.k_full[i], 1);
+        for (int i = 0; i < Smem::kStages; ++i) {
+            tc::mbar_init(&sm.k_full[i], Shape::kFour ? 128 : 1);
             tc::mbar_init(&sm.k_empty[i], 1);
-            tc::mbar_init(&sm.v_full[i], 1);
+            tc::mbar_init(&sm.v_full[i], Shape::kFour ? 128 : 1);
             tc::mbar_init(&sm.v_empty[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
+            tc::mbar_init(&sm.raw_full[w], 1);
+            tc::mbar_init(&sm.raw_empty[w], 128);
             tc::mbar_init(&sm.q_full[w], kHalf);
             tc::mbar_init(&sm.s_full[w], 1);
             tc::mbar_init(&sm.p_full[w], 4);
@@ -570,15 +664,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_prompt_kernel(AttendArg
     tc::fence_after_sync();
     const uint32_t tmem = sm.tmem;
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        soften<kRows, D>(a, plan, sm, tmem);
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kSoftmaxRegs));
+        soften<kRows, kCache, D>(a, plan, sm, tmem);
+    } else if (warp < kExpander) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kOtherRegs));
         if (warp == kLoader) {
-            load_granules<D>(a, plan, &map, sm);
+            load_granules<kCache, D>(a, plan, &map, sm);
         } else if (threadIdx.x == 32 * kIssuer) {
-            issue<kRows, D>(a, sm, tmem);
+            issue<kRows, kCache, D>(a, sm, tmem);
         }
+    } else if constexpr (Shape::kFour) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kExpandRegs));
+        expand<kCache, D>(a, sm);
     }
     __syncwarp();
     tc::fence_before_sync();
@@ -586,12 +683,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_prompt_kernel(AttendArg
     if (warp == kIssuer) {
         if (*const_cast<volatile int *>(&sm.abort)) {
             // copies and products that are still in flight end before their memory goes
-            for (int i = 0; i < PromptSmem<D>::kStages; ++i) {
-                for (uint32_t ph = 0; ph < 2; ++ph) {
+            for (uint32_t ph = 0; ph < 2; ++ph) {
+                for (int i = 0; i < Smem::kStages; ++i) {
                     tc::mbar_wait(&sm.k_full[i], ph, 1000000ull);
                     tc::mbar_wait(&sm.v_full[i], ph, 1000000ull);
                     tc::mbar_wait(&sm.k_empty[i], ph, 1000000ull);
                     tc::mbar_wait(&sm.v_empty[i], ph, 1000000ull);
+                }
+                for (int i = 0; i < 2; ++i) {
+                    tc::mbar_wait(&sm.raw_full[i], ph, 1000000ull);
                 }
             }
         }
@@ -600,21 +700,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_prompt_kernel(AttendArg
     }
 }
 
+// f16 rows over a 4-bit cache stay with the kernel for few columns: bf16, which
+// a 4-bit value times its scale needs for its exponent, would cut their Q.
+template <int kRows, int kCache> constexpr bool built() {
+    return kRows != kF32 && (kCache != kMxfp4 || kRows == kBf16);
+}
+
 template <int kRows, int kCache, int D> cudaError_t launch(const ttl_kv &h, const AttendArgs &a, int layer) {
-    if constexpr (kRows == kF32 || kCache == kMxfp4) {
+    if constexpr (!built<kRows, kCache>()) {
         return cudaErrorInvalidValue;
     } else {
-        kv_attend_prompt_kernel<kRows, D><<<h.ctas[1], kThreads, sizeof(PromptSmem<D>), h.stream>>>(a, h.maps[size_t(layer)]);
+        kv_attend_prompt_kernel<kRows, kCache, D><<<h.ctas[1], PromptShape<kCache>::kThreads, sizeof(PromptSmem<kCache, D>), h.stream>>>(
+            a, h.maps[size_t(layer)]);
         return cudaGetLastError();
     }
 }
 
 template <int kRows, int kCache, int D> cudaError_t configure(ttl_kv &h) {
-    if constexpr (kRows == kF32 || kCache == kMxfp4) {
+    if constexpr (!built<kRows, kCache>()) {
         return cudaSuccess;
     } else {
         h.prompt_ctas = std::min(h.sms, kMaxCtas);
-        return cudaFuncSetAttribute(kv_attend_prompt_kernel<kRows, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PromptSmem<D>)));
+        return cudaFuncSetAttribute(kv_attend_prompt_kernel<kRows, kCache, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    int(sizeof(PromptSmem<kCache, D>)));
     }
 }
 
