@@ -292,7 +292,7 @@ int choose_shapes(const ttl_kv &h, int seqs, int, int max_new, Shape shape[kKind
         return 0;  // one launch: whatever the sequence's rows turn out to be
     }
     const int i = token_index(columns, h.dim);
-    shape[0] = Shape{8 << i, 64, 1, h.token_ctas[i]};
+    shape[0] = Shape{8 << i, 64 * token_sub(h.cache_type, 8 << i), 1, h.token_ctas[i]};
     return prompt ? kFewColumns : 1 << 30;
 }
 

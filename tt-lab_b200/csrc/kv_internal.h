@@ -57,6 +57,13 @@ namespace kv {
 constexpr int kNarrow = 8;         // columns of the narrowest tile
 constexpr int kPromptWidth = 256;  // columns of a prompt tile
 
+// The kernel for few columns: steps of 16 keys that each of its four warps takes
+// at once.  Two over a 4-bit cache (less bookkeeping per byte) where the
+// registers allow it.
+constexpr int token_sub(int cache, int width) {
+    return cache == kMxfp4 && width == 8 ? 2 : 1;
+}
+
 // Shape of one kind's launch.
 struct Shape {
     int width, gran, cost, ctas;   // columns per tile, keys per granule, granules a tile's ends cost, CTAs (0: no launch)

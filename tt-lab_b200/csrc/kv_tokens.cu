@@ -48,14 +48,15 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * (kWarps + 1);
-constexpr int kGran = 64;
 
 template <int kRows, int kCache, int D, int NT> struct TokenShape {
     static constexpr int kCols = 8 * NT;
     static constexpr bool kFour = kCache == kMxfp4;
+    static constexpr int kSub = token_sub(kCache, 8 * NT);  // steps of 16 keys a warp takes at once
+    static constexpr int kGran = 16 * kWarps * kSub;
     static constexpr uint32_t kStageBytes = kFour ? 2 * kGran * row_bytes(kMxfp4, D) : 2 * kGran * D * 2;
     // enough in flight to cover HBM's latency at its full rate over the CTAs of an SM (about 48 KB per SM)
-    static constexpr int kStages = kFour ? 6 : (D == 64 ? 4 : 3);
+    static constexpr int kStages = kFour ? 4 : (D == 64 ? 4 : 3);
     static constexpr int kOPitch = D + 4;
 };
 
@@ -115,13 +116,12 @@ template <int kType> __device__ __forceinline__ uint32_t pack2(float lo, float h
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
-__device__ __forceinline__ uint32_t half2_of_codes(uint32_t byte) {
-    const __half2 h = e2m1x2_to_half2(byte);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// 2^(e - 127) of an E8M0 byte; 255 is NaN.
-__device__ __forceinline__ float e8m0(uint32_t e) {
-    return e == 255u ? __uint_as_float(0x7fffffffu) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
+// Eight E2M1 codes to four f16 pairs.
+__device__ __forceinline__ void halves8(uint32_t codes, uint32_t &h0, uint32_t &h1, uint32_t &h2, uint32_t &h3) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h0), "=r"(h1), "=r"(h2), "=r"(h3)
+        : "r"(codes));
 }
 // 2^d for |d| beyond f32's exponents too (0 or infinity there).
 __device__ __forceinline__ float pow2i(int d) {
@@ -153,11 +153,12 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, vo
     return true;
 }
 
-// The loader: one warp, 64 keys a step.
-template <class Smem, int kCache, int D, int kStages, uint32_t kStageBytes>
+// The loader: one warp, a granule a step.
+template <class Smem, int kCache, int D, int kGran, int kStages, uint32_t kStageBytes>
 __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &plan, const CUtensorMap *map, Smem &sm) {
     const int lane = threadIdx.x & 31;
-    const int seg = min(1 << a.page_shift, kGran);       // keys of one copy
+    const int seg = min(1 << a.page_shift, kGran);       // keys of one copy (a TMA box has up to 64 rows)
+    static_assert(kCache == kMxfp4 || kGran == 64, "box rows");
     const int segs = kGran / seg;
     int stage = 0;
     uint32_t phase = 0;
@@ -172,7 +173,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
         for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
             const int first = k0 >> a.page_shift;
             const int need = (k0 + kGran - 1) >> a.page_shift;
-            if (need >= base + 32 || base < 0) {
+            if (need >= base + 32) {
                 base = first;
                 id = len > 0 ? table[min(base + lane, last)] : 0;
                 if (uint32_t(id) >= uint32_t(a.pages)) {
@@ -200,7 +201,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                         tc::tma_load_2d(sm.stage[stage] + ((is_v * (D / 64) + x) * kGran + s * seg) * 128, map, 64 * x, y, &sm.full[stage]);
                     }
                 } else {
-                    // pages of up to 64 keys: one copy of a head's block; of 128: its four parts
+                    // pages up to a granule: one copy of a head's block; larger: its four parts
                     const bool whole = (1 << a.page_shift) <= kGran;
                     const int copies = whole ? segs : 4;
                     const int c = lane;
@@ -243,12 +244,12 @@ __global__ void __launch_bounds__(kThreads)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     constexpr int kCols = T::kCols;
-    constexpr int kBlocks = D / 32;
+    constexpr int kBlocks = D / 32, kSub = T::kSub;
     constexpr int kMma = kCache == kMxfp4 ? kF16 : kRows;
     constexpr int kMTiles = D / 16;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Plan &plan = *a.walk.plan;
-    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kCols || a.walk.list->gran != kGran) {
+    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kCols || a.walk.list->gran != T::kGran) {
         if (tid == 0) {
             set_status(a.status, kKvStalePlan);
         }
@@ -264,13 +265,15 @@ __global__ void __launch_bounds__(kThreads)
     }
     __syncthreads();
     if (warp == kWarps) {
-        load_granules<Smem, kCache, D, T::kStages, T::kStageBytes>(a, plan, &map, sm);
+        load_granules<Smem, kCache, D, T::kGran, T::kStages, T::kStageBytes>(a, plan, &map, sm);
         return;
     }
     const int g = lane >> 2, t = lane & 3;
     const float cap_log2 = a.cap * kLog2e;
     const float two_over_cap = a.cap != 0.0f ? 2.0f / a.cap : 0.0f;
-    const int seg_shift = min(a.page_shift, 6), seg = 1 << seg_shift;
+    // 4 bits: keys and bytes of a copied part
+    const int seg_shift = min(a.page_shift, T::kGran == 64 ? 6 : 7), seg = 1 << seg_shift;
+    const uint32_t block = 2u * uint32_t(seg) * row_bytes(kMxfp4, D);
     // largest weight 2^(kSlack + kLift), times 2^kScaleSlack over a 4-bit cache: 2^15 in f16
     constexpr float kSlack = kMma == kF16 ? 4.0f : 8.0f;
     constexpr int kScaleSlack = 2;
@@ -367,7 +370,7 @@ __global__ void __launch_bounds__(kThreads)
         }
         float scale[NT][2], m[NT][2], l[NT][2];
         float o[NT][kMTiles][4];
-        int ref[kCache == kMxfp4 ? NT : 1][2][kBlocks];  // 4 bits: the scale exponent that o is in units of
+        float unit[kCache == kMxfp4 ? NT : 1][2][kBlocks];  // 4 bits: 1 / the scale that o is in units of
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(kThreads)
                 if constexpr (kCache == kMxfp4) {
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b) {
-                        ref[n][c][b] = -1000;
+                        unit[n][c][b] = __uint_as_float(0x7e800000u);  // of the smallest scale
                     }
                 }
             }
@@ -389,125 +392,150 @@ __global__ void __launch_bounds__(kThreads)
                 }
             }
         }
-        for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
+        for (int k0 = p.k0; k0 < p.k1; k0 += T::kGran) {
             wait_or_abort(&sm.full[stage], phase, &sm.abort, a.status);
-            const int key0 = k0 + 16 * warp;
-            if (key0 < hi_max && key0 + 16 > lo_min) {
+            const int key0 = k0 + 16 * kSub * warp;
+            if (key0 < hi_max && key0 + 16 * kSub > lo_min) {
                 const uint32_t buf = tc::smem_u32(sm.stage[stage]);
-                float s[NT][4];
-                uint32_t sv[kCache == kMxfp4 ? 2 : 1][kBlocks];  // V's scale bytes of keys g, g + 8
-                uint32_t vcodes = 0;
+                float s[kSub][NT][4];
+                float sv[kSub][2][kBlocks];  // 4 bits: V's scales of keys g, g + 8
+                uint32_t vcodes[kSub];
+                float sv_max[kBlocks];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s[n][j] = 0.0f;
-                    }
-                }
-                if constexpr (kCache != kMxfp4) {
-                    const int row = 16 * warp + (lane & 15);
-#pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) {
-                        uint32_t ka[4];
-                        const int chunk = (2 * ks + (lane >> 4)) & 7, x = ks >> 2;
-                        ldmatrix4(ka, buf + (x * kGran + row) * 128 + ((chunk ^ (row & 7)) << 4));
+                for (int u = 0; u < kSub; ++u) {
+                    const int at = 16 * (kSub * warp + u);  // first key in the granule
+                    if constexpr (kCache != kMxfp4) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma<kMma>(s[n], ka, q[n][ks][0], q[n][ks][1]);
-                        }
-                    }
-                } else {
-                    const int in_seg = (16 * warp) & (seg - 1);
-                    const uint32_t block = 2u * uint32_t(seg) * row_bytes(kMxfp4, D);
-                    const uint32_t kc = buf + uint32_t(16 * warp >> seg_shift) * block;
-                    const uint32_t ksc = kc + uint32_t(seg) * (D / 2);
-                    vcodes = kc + (block >> 1);
-                    const uint32_t vsc = vcodes + uint32_t(seg) * (D / 2);
-                    vcodes += uint32_t(in_seg) * (D / 2);
-                    float sk[2][kBlocks];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t at = uint32_t(in_seg + g + 8 * h) * kBlocks;
-                        uint32_t bk, bv;
-                        if constexpr (kBlocks == 2) {
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bk) : "r"(ksc + at));
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bv) : "r"(vsc + at));
-                        } else {
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bk) : "r"(ksc + at));
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bv) : "r"(vsc + at));
+                            for (int j = 0; j < 4; ++j) {
+                                s[u][n][j] = 0.0f;
+                            }
+                        }
+                        const int row = at + (lane & 15);
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            uint32_t ka[4];
+                            const int chunk = (2 * ks + (lane >> 4)) & 7, x = ks >> 2;
+                            ldmatrix4(ka, buf + (x * T::kGran + row) * 128 + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                mma<kMma>(s[u][n], ka, q[n][ks][0], q[n][ks][1]);
+                            }
+                        }
+                    } else {
+                        const int in_seg = at & (seg - 1);
+                        const uint32_t kc = buf + uint32_t(at >> seg_shift) * block;
+                        const uint32_t ksc = kc + uint32_t(seg) * (D / 2);
+                        const uint32_t vc = kc + (block >> 1), vsc = vc + uint32_t(seg) * (D / 2);
+                        vcodes[u] = vc + uint32_t(in_seg) * (D / 2);
+                        float sk[2][kBlocks];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t from = uint32_t(in_seg + g + 8 * h) * kBlocks;
+                            uint32_t bk, bv;
+                            if constexpr (kBlocks == 2) {
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bk) : "r"(ksc + from));
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=r"(bv) : "r"(vsc + from));
+                            } else {
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bk) : "r"(ksc + from));
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bv) : "r"(vsc + from));
+                            }
+                            // 2^(e - 127): the byte is the float's exponent (0: below f32's
+                            // normal range, taken as 0; 255: infinity here, NaN below)
+                            float nan = 0.0f;
+#pragma unroll
+                            for (int b = 0; b < kBlocks; ++b) {
+                                sk[h][b] = __uint_as_float(((bk >> (8 * b)) & 255u) << 23);
+                                sv[u][h][b] = __uint_as_float(((bv >> (8 * b)) & 255u) << 23);
+                                nan += sk[h][b] - sk[h][b];
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                s[u][n][2 * h] = s[u][n][2 * h + 1] = nan;
+                            }
                         }
 #pragma unroll
                         for (int b = 0; b < kBlocks; ++b) {
-                            sk[h][b] = e8m0((bk >> (8 * b)) & 255u);
-                            sv[h][b] = (bv >> (8 * b)) & 255u;
-                        }
-                    }
+                            const float top = fmaxf(sv[u][0][b], sv[u][1][b]);
+                            sv_max[b] = u == 0 ? top : fmaxf(sv_max[b], top);
+                            uint32_t w0, w1, a0[4], a1[4];
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(kc + uint32_t(in_seg + g) * (D / 2) + 16 * b + 4 * t));
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(kc + uint32_t(in_seg + g + 8) * (D / 2) + 16 * b + 4 * t));
+                            halves8(w0, a0[0], a0[2], a1[0], a1[2]);
+                            halves8(w1, a0[1], a0[3], a1[1], a1[3]);
 #pragma unroll
-                    for (int b = 0; b < kBlocks; ++b) {
-                        uint32_t w0, w1;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(kc + uint32_t(in_seg + g) * (D / 2) + 16 * b + 4 * t));
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(kc + uint32_t(in_seg + g + 8) * (D / 2) + 16 * b + 4 * t));
-                        const uint32_t a0[4] = {half2_of_codes(w0 & 255u), half2_of_codes(w1 & 255u), half2_of_codes((w0 >> 8) & 255u),
-                                                half2_of_codes((w1 >> 8) & 255u)};
-                        const uint32_t a1[4] = {half2_of_codes((w0 >> 16) & 255u), half2_of_codes((w1 >> 16) & 255u),
-                                                half2_of_codes(w0 >> 24), half2_of_codes(w1 >> 24)};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma<kMma>(c, a0, q[n][2 * b][0], q[n][2 * b][1]);
-                            mma<kMma>(c, a1, q[n][2 * b + 1][0], q[n][2 * b + 1][1]);
-                            s[n][0] = fmaf(c[0], sk[0][b], s[n][0]);
-                            s[n][1] = fmaf(c[1], sk[0][b], s[n][1]);
-                            s[n][2] = fmaf(c[2], sk[1][b], s[n][2]);
-                            s[n][3] = fmaf(c[3], sk[1][b], s[n][3]);
+                            for (int n = 0; n < NT; ++n) {
+                                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma<kMma>(c, a0, q[n][2 * b][0], q[n][2 * b][1]);
+                                mma<kMma>(c, a1, q[n][2 * b + 1][0], q[n][2 * b + 1][1]);
+                                s[u][n][0] = fmaf(c[0], sk[0][b], s[u][n][0]);
+                                s[u][n][1] = fmaf(c[1], sk[0][b], s[u][n][1]);
+                                s[u][n][2] = fmaf(c[2], sk[1][b], s[u][n][2]);
+                                s[u][n][3] = fmaf(c[3], sk[1][b], s[u][n][3]);
+                            }
                         }
                     }
                 }
                 // ---- scores in log2 units ----
-                const bool masked = key0 < lo_max || key0 + 16 > hi_min;
+                const bool masked = key0 < lo_max || key0 + 16 * kSub > hi_min;
                 if (cap_log2 == 0.0f && !a.slopes) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
+                    for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            s[n][j] *= scale[n][j & 1];
+                        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                s[u][n][j] *= scale[n][j & 1];
+                            }
                         }
                     }
                 } else {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
+                    for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int c = 8 * n + 2 * t + (j & 1), key = key0 + g + (j >> 1) * 8;
-                            const float x = cap_log2 != 0.0f ? capped(s[n][j], scale[n][j & 1] * two_over_cap, cap_log2) : s[n][j] * scale[n][j & 1];
-                            s[n][j] = fmaf(-sm.slope[c], float(abs(sm.pos[c] - key)), x);
+                        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int c = 8 * n + 2 * t + (j & 1), key = key0 + 16 * u + g + (j >> 1) * 8;
+                                const float f = scale[n][j & 1];
+                                const float x = cap_log2 != 0.0f ? capped(s[u][n][j], f * two_over_cap, cap_log2) : s[u][n][j] * f;
+                                s[u][n][j] = fmaf(-sm.slope[c], float(abs(sm.pos[c] - key)), x);
+                            }
                         }
                     }
                 }
                 if (masked) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
+                    for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int c = 8 * n + 2 * t + (j & 1), key = key0 + g + (j >> 1) * 8;
-                            s[n][j] = key >= sm.lo[c] && key < sm.hi[c] ? s[n][j] : -INFINITY;
+                        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int c = 8 * n + 2 * t + (j & 1), key = key0 + 16 * u + g + (j >> 1) * 8;
+                                s[u][n][j] = key >= sm.lo[c] && key < sm.hi[c] ? s[u][n][j] : -INFINITY;
+                            }
                         }
                     }
                 }
                 // ---- the running maximum ----
                 bool move = false;
+                float top[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        move = move || fmaxf(s[n][c], s[n][c + 2]) > m[n][c] + (kSlack + kLift);
+                        top[n][c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
+#pragma unroll
+                        for (int u = 1; u < kSub; ++u) {
+                            top[n][c] = fmaxf(top[n][c], fmaxf(s[u][n][c], s[u][n][c + 2]));
+                        }
+                        move = move || top[n][c] > m[n][c] + (kSlack + kLift);
                         if constexpr (kCache == kMxfp4) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                                for (int b = 0; b < kBlocks; ++b) {
-                                    move = move || (int(sv[h][b]) > ref[n][c][b] + kScaleSlack && sv[h][b] != 255u && s[n][c + 2 * h] != -INFINITY);
-                                }
+                            for (int b = 0; b < kBlocks; ++b) {
+                                // unseen keys may ask for nothing; the scale moves by seen ones below
+                                move = move || sv_max[b] * unit[n][c][b] > float(1 << kScaleSlack);
                             }
                         }
                     }
@@ -518,13 +546,13 @@ __global__ void __launch_bounds__(kThreads)
                         float up[2];
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaxf(s[n][c], s[n][c + 2]);
+                            float most = top[n][c];
 #pragma unroll
                             for (int off = 4; off < 32; off <<= 1) {
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
                             }
                             // m is what weights are relative to: the maximum less the lift
-                            const float mn = fmaxf(m[n][c], top - kLift);
+                            const float mn = fmaxf(m[n][c], most - kLift);
                             up[c] = ex2(m[n][c] - (mn == -INFINITY ? 0.0f : mn));
                             m[n][c] = mn;
                             l[n][c] *= up[c];
@@ -535,18 +563,25 @@ __global__ void __launch_bounds__(kThreads)
                                 float f[2];
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
-                                    int e = -1000;
+                                    // the largest finite scale of a seen key
+                                    float e = 0.0f;
 #pragma unroll
-                                    for (int h = 0; h < 2; ++h) {
-                                        e = sv[h][b] != 255u && s[n][c + 2 * h] != -INFINITY ? max(e, int(sv[h][b])) : e;
+                                    for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+                                        for (int h = 0; h < 2; ++h) {
+                                            e = s[u][n][c + 2 * h] != -INFINITY && sv[u][h][b] < INFINITY ? fmaxf(e, sv[u][h][b]) : e;
+                                        }
                                     }
 #pragma unroll
                                     for (int off = 4; off < 32; off <<= 1) {
-                                        e = max(e, __shfl_xor_sync(0xffffffffu, e, off));
+                                        e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, off));
                                     }
-                                    const int r = max(ref[n][c][b], e);
-                                    f[c] = up[c] * pow2i(ref[n][c][b] - r);
-                                    ref[n][c][b] = r;
+                                    // the unit's reciprocal: 2^(254 - byte) as a float's exponent; a byte
+                                    // that a finite value has is at most 252
+                                    const float r = __uint_as_float(0x7f000000u - max(__float_as_uint(e), 0x00800000u));
+                                    const float less = fminf(unit[n][c][b], r);
+                                    f[c] = up[c] * (less == unit[n][c][b] ? 1.0f : pow2i(int(__float_as_uint(less) >> 23) - int(__float_as_uint(unit[n][c][b]) >> 23)));
+                                    unit[n][c][b] = less;
                                 }
 #pragma unroll
                                 for (int i = 2 * b; i < 2 * b + 2; ++i) {
@@ -565,59 +600,61 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float mm = m[n][j & 1];
-                        s[n][j] = ex2(s[n][j] - (mm == -INFINITY ? 0.0f : mm));
-                        l[n][j & 1] += s[n][j];
-                    }
-                }
-                if constexpr (kCache != kMxfp4) {
-                    uint32_t w[NT][2];
+                    for (int c = 0; c < 2; ++c) {
+                        const float mm = m[n][c] == -INFINITY ? 0.0f : m[n][c];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        w[n][0] = transpose8(pack2<kMma>(s[n][0], s[n][1]));
-                        w[n][1] = transpose8(pack2<kMma>(s[n][2], s[n][3]));
-                    }
-                    const uint32_t vbuf = buf + (D / 64) * kGran * 128;
-                    const int row = 16 * warp + (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-                    for (int i = 0; i < kMTiles; ++i) {
-                        uint32_t va[4];
-                        const int chunk = (2 * i + ((lane >> 3) & 1)) & 7, x = i >> 2;
-                        ldmatrix4_trans(va, vbuf + (x * kGran + row) * 128 + ((chunk ^ (row & 7)) << 4));
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma<kMma>(o[n][i], va, w[n][0], w[n][1]);
+                        for (int u = 0; u < kSub; ++u) {
+                            s[u][n][c] = ex2(s[u][n][c] - mm);
+                            s[u][n][c + 2] = ex2(s[u][n][c + 2] - mm);
+                            l[n][c] += s[u][n][c] + s[u][n][c + 2];
                         }
                     }
-                } else {
+                }
 #pragma unroll
-                    for (int b = 0; b < kBlocks; ++b) {
-                        // 8 x 8 b16 of 4 codes each: keys 0-7 and 8-15, the block's 32 values
-                        uint32_t r0, r1;
-                        ldmatrix2_trans(r0, r1, vcodes + uint32_t(lane & 15) * (D / 2) + 16 * b);
-                        // r: codes 4g .. 4g + 3 of keys 2t (low half) and 2t + 1; to bytes of (key 2t, key 2t + 1)
-                        const uint32_t x0 = (r0 & 0x0F0Fu) | ((r0 >> 12) & 0xF0F0u), y0 = ((r0 >> 4) & 0x0F0Fu) | ((r0 >> 16) & 0xF0F0u);
-                        const uint32_t x1 = (r1 & 0x0F0Fu) | ((r1 >> 12) & 0xF0F0u), y1 = ((r1 >> 4) & 0x0F0Fu) | ((r1 >> 16) & 0xF0F0u);
-                        // rows 0-7: value 4g + 2i, rows 8-15: value 4g + 2i + 1
-                        const uint32_t va0[4] = {half2_of_codes(x0 & 255u), half2_of_codes(y0 & 255u), half2_of_codes(x1 & 255u), half2_of_codes(y1 & 255u)};
-                        const uint32_t va1[4] = {half2_of_codes(x0 >> 8), half2_of_codes(y0 >> 8), half2_of_codes(x1 >> 8), half2_of_codes(y1 >> 8)};
+                for (int u = 0; u < kSub; ++u) {
+                    if constexpr (kCache != kMxfp4) {
+                        uint32_t w[NT][2];
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            float z[4];
+                            w[n][0] = transpose8(pack2<kMma>(s[u][n][0], s[u][n][1]));
+                            w[n][1] = transpose8(pack2<kMma>(s[u][n][2], s[u][n][3]));
+                        }
+                        const uint32_t vbuf = buf + (D / 64) * T::kGran * 128;
+                        const int row = 16 * (kSub * warp + u) + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint32_t e = sv[j >> 1][b];
-                                // 2^(e - ref), at most 2^kScaleSlack where the weight is not 0 (a NaN scale of an unseen
-                                // key makes the column NaN, and so computed again)
-                                const int d = int(e) - ref[n][j & 1][b];
-                                const float f = e == 255u ? __uint_as_float(0x7fffffffu)
-                                                          : (d < -126 ? 0.0f : __uint_as_float(uint32_t(min(d, 100) + 127) << 23));
-                                z[j] = s[n][j] * f;
+                        for (int i = 0; i < kMTiles; ++i) {
+                            uint32_t va[4];
+                            const int chunk = (2 * i + ((lane >> 3) & 1)) & 7, x = i >> 2;
+                            ldmatrix4_trans(va, vbuf + (x * T::kGran + row) * 128 + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                mma<kMma>(o[n][i], va, w[n][0], w[n][1]);
                             }
-                            const uint32_t w0 = transpose8(pack2<kF16>(z[0], z[1])), w1 = transpose8(pack2<kF16>(z[2], z[3]));
-                            mma<kF16>(o[n][2 * b], va0, w0, w1);
-                            mma<kF16>(o[n][2 * b + 1], va1, w0, w1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < kBlocks; ++b) {
+                            // 8 x 8 b16 of 4 codes each: keys 0-7 and 8-15, the block's 32 values
+                            uint32_t r0, r1, va0[4], va1[4];
+                            ldmatrix2_trans(r0, r1, vcodes[u] + uint32_t(lane & 15) * (D / 2) + 16 * b);
+                            // r: codes 4g .. 4g + 3 of key 2t (low half) and of key 2t + 1, to
+                            // bytes of a value's two keys: rows 0-7 of a tile are values 4g + 2i,
+                            // rows 8-15 values 4g + 2i + 1
+                            const uint32_t x0 = (r0 & 0x0F0Fu) | ((r0 >> 12) & 0xF0F0u), y0 = ((r0 >> 4) & 0x0F0Fu) | ((r0 >> 16) & 0xF0F0u);
+                            const uint32_t x1 = (r1 & 0x0F0Fu) | ((r1 >> 12) & 0xF0F0u), y1 = ((r1 >> 4) & 0x0F0Fu) | ((r1 >> 16) & 0xF0F0u);
+                            halves8(x0 | y0 << 16, va0[0], va1[0], va0[1], va1[1]);
+                            halves8(x1 | y1 << 16, va0[2], va1[2], va0[3], va1[3]);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                // the scale over the unit: at most 2^kScaleSlack where the key is seen
+                                // (a NaN scale makes infinity or NaN here, and the column is computed again)
+                                const float f0 = sv[u][0][b] * unit[n][0][b], f1 = sv[u][0][b] * unit[n][1][b];
+                                const float f2 = sv[u][1][b] * unit[n][0][b], f3 = sv[u][1][b] * unit[n][1][b];
+                                const uint32_t w0 = transpose8(pack2<kF16>(s[u][n][0] * f0, s[u][n][1] * f1));
+                                const uint32_t w1 = transpose8(pack2<kF16>(s[u][n][2] * f2, s[u][n][3] * f3));
+                                mma<kF16>(o[n][2 * b], va0, w0, w1);
+                                mma<kF16>(o[n][2 * b + 1], va1, w0, w1);
+                            }
                         }
                     }
                 }
@@ -652,7 +689,7 @@ __global__ void __launch_bounds__(kThreads)
                     const int c = 8 * n + 2 * t + (j & 1);
                     if constexpr (kCache == kMxfp4) {
                         const int d = 32 * (i >> 1) + 4 * g + 2 * (i & 1) + (j >> 1);
-                        sm.o[warp][c][d] = o[n][i][j] * pow2i(ref[n][j & 1][i >> 1] - 127);
+                        sm.o[warp][c][d] = o[n][i][j] * __uint_as_float(0x7f000000u - __float_as_uint(unit[n][j & 1][i >> 1]));
                     } else {
                         sm.o[warp][c][16 * i + g + 8 * (j >> 1)] = o[n][i][j];
                     }
