@@ -29,7 +29,6 @@ struct PlanArgs {
     int32_t *prefix[2][2];
     Cut *cuts[2][2];
     int4 *row[2];
-    int4 *seq;
     uint32_t *counters;
     uint32_t *status;
     const int32_t *row_start, *length, *pages, *first, *prefix_len;
@@ -175,9 +174,6 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             const int columns = q.n * a.group;
             const bool mine = (columns <= a.few) == (kind == 0);
             count = (mine && columns > 0) ? (columns + width - 1) / width : 0;
-            if (blockIdx.x == 0) {
-                a.seq[s] = make_int4(q.row0, q.n, q.len, 0);
-            }
         }
         int sum;
         const int at = block_scan(count, &sum, sums);
@@ -239,7 +235,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             const int g0 = begin < end ? begin / gran : 0;
             // at least one granule: a tile whose rows see nothing is written too
             n = begin < end ? (end + gran - 1) / gran - g0 : 1;
-            tiles[t] = Tile{lo, col0, g0, uint32_t(ncols) | uint32_t(n) << 9};
+            tiles[t] = Tile{lo, col0, g0, uint32_t(ncols) | uint32_t(n) << 9, q.row0, q.len, {0, 0}};
             n += cost;
         }
         int sum;
@@ -319,14 +315,32 @@ struct AppendArgs {
     size_t k_stride, v_stride, q_stride, q_out_stride;
     uint8_t *pool;  // this layer
     const double *turns;
-    float rope_scale;
+    const double2 *table;      // cosine and sine of -1, -1 + 1/64 .. 1 half turns
+    double rope_scale;
     uint32_t *status;
     int rows, q_heads, kv_heads, page_shift, pages, half, interleaved;  // half: rotated pairs (0: none)
     uint32_t block_bytes;
+    // Blocks [0, q_blocks) take Q, the others K and V: [0] and [1] below.
+    int q_blocks;
+    int deep;                  // rows of a thread, up to kAppendRows
+    int subs[2];               // groups of threads that share a CTA, each with its own rows
+    int units[2];              // of a row
+    uint32_t unit_div[2], pair_div;  // ceil(2^32 / n) of units and of half
 };
 
 constexpr int kAppendThreads = 256;
+// Rows of a thread at most (f32: half as many, as their values take twice the
+// registers), groups of threads of a CTA at most.
+constexpr int kAppendRows = 4, kAppendSubs = 4;
+__host__ __device__ constexpr int append_rows(int rows_type) {
+    return rows_type == kF32 ? kAppendRows / 2 : kAppendRows;
+}
 constexpr int kMaxPairs = 64;
+
+// i / n by the reciprocal above: exact while i * n < 2^32.
+__device__ __forceinline__ int quotient(int i, uint32_t div) {
+    return int(__umulhi(uint32_t(i), div));
+}
 
 // The slot of a row: the block of (page, head 0) and the token in it, or
 // nullptr for padding and for a page outside the pool.
@@ -350,236 +364,290 @@ __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
     return out;
 }
 
-// f64 -> f32 rounded to odd: keeps the order against every f32 with an even
-// last bit, so that rounding the result to E2M1 (whose borders are such
-// numbers) equals rounding the f64 at once.
-__device__ __forceinline__ float to_odd(double x) {
-    const float f = __double2float_rz(x);
-    return double(f) == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
+// hi + lo (hi their sum to nearest) as one f32 rounded to odd: the f32 below in
+// size, its last bit set unless lo is 0.  It keeps the order against every f32
+// with an even last bit, so that rounding it to E2M1, whose borders are such
+// numbers, and taking its exponent equals doing so with hi + lo.
+__device__ __forceinline__ float to_odd(float hi, float lo) {
+    if (lo == 0.0f || !(fabsf(hi) < INFINITY)) {
+        return hi;
+    }
+    uint32_t b = __float_as_uint(hi);
+    b -= ((__float_as_uint(lo) ^ b) >> 31) && (b << 1) ? 1u : 0u;
+    return __uint_as_float(b | 1u);
 }
 
-// 32 values -> a 16-byte code block and its scale.
-template <class T> __device__ __forceinline__ void quantize_block(const T (&x)[32], uint8_t *codes, uint8_t *scale) {
-    T top = 0;
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const T m = x[i] < 0 ? -x[i] : x[i];
-        top = m > top ? m : top;
-        finite = finite && (m < T(INFINITY));
-    }
-    int e = -127;
-    if constexpr (sizeof(T) == 8) {
-        const int b = int(__double_as_longlong(top) >> 52) & 0x7ff;
-        e = max(b - 1023 - 2, -127);
-    } else {
-        // a subnormal maximum has a scale below the smallest: -127 all the same
-        e = max(int(__float_as_uint(top) >> 23) - 127 - 2, -127);
-    }
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (finite && top > 0) {
-        // x * 2^-e is exact: e is at most 125 and at least -127
-        T inv;
-        if constexpr (sizeof(T) == 8) {
-            inv = __longlong_as_double((long long)(1023 - e) << 52);
-        } else {
-            inv = __uint_as_float(uint32_t(127 - e) << 23);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-            float lo, hi;
-            if constexpr (sizeof(T) == 8) {
-                lo = to_odd(x[i] * inv), hi = to_odd(x[i + 1] * inv);
-            } else {
-                lo = x[i] * inv, hi = x[i + 1] * inv;
-            }
-            w[i / 8] |= e2m1x2(lo, hi) << (4 * (i % 8));
-        }
-    }
-    *reinterpret_cast<uint4 *>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
-    *scale = finite ? uint8_t(e + 127) : uint8_t(255);
+// x c - y s to about 48 bits: c and s as sums of two f32, the products' and the
+// difference's rounding errors kept by fused multiply-adds and a two-sum.
+__device__ __forceinline__ float turned_odd(float x, float y, float ch, float cl, float sh, float sl) {
+    const float p = x * ch, q = -(y * sh);
+    const float ep = fmaf(x, ch, -p), eq = -fmaf(y, sh, q);
+    const float z = p + q;
+    const float t = z - p;
+    const float ez = (p - (z - t)) + (q - t);
+    const float lo = ez + (ep + eq + (x * cl - y * sl));
+    const float hi = z + lo;
+    return to_odd(hi, lo - (hi - z));
 }
 
-// One CTA takes kAppendRows rows: the cosines and sines of the rows' pairs
-// once, for all heads, then every head in units of 16 values (two runs of 8
-// that are rotated with one another).  The angle is a fraction of a
-// revolution in 64 bits (a position times a frequency has lost 7 bits of its
-// fraction at position 131072 in 32), cut to its fractional part there, and
-// its cosine and sine are then good to 32 bits.
+// Eight values of a block of 32 that four neighbouring lanes hold: the block's
+// scale and this lane's codes, stored where `write`.  An infinity or NaN in any
+// of the four marks the block.
+__device__ __forceinline__ void quantize8(const float (&x)[8], int lane, bool write, uint8_t *block, size_t code_at, size_t scale_at) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);  // sizes order like their bits, NaN above infinity
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const bool finite = top < 0x7f800000u;
+    // floor(log2(top)) - 2; a subnormal top has a scale below the smallest
+    const int exp = max(int(top >> 23) - 127 - 2, -127);
+    uint32_t codes = 0;
+    if (finite) {
+        const float inv = __uint_as_float(uint32_t(127 - exp) << 23);  // exact: exp is -127 .. 125
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            codes |= e2m1x2(x[j] * inv, x[j + 1] * inv) << (4 * j);
+        }
+    }
+    if (write) {
+        *reinterpret_cast<uint32_t *>(block + code_at) = codes;
+        if ((lane & 3) == 0) {
+            block[scale_at] = finite ? uint8_t(exp + 127) : uint8_t(255);
+        }
+    }
+}
+
+// Cosine and sine of `turn` half turns, |turn| <= 1, to about 2^-52: a table of the
+// angles of 1/64 half turn (kTurnSteps + 1 entries from -1 on), and the rest of at
+// most 1/128 half turn (0.0246 rad) by Taylor's series, whose next terms are
+// below 2^-60.
+constexpr int kTurnSteps = 128;
+__device__ __forceinline__ void cos_sin(double turn, const double2 *table, double &c, double &s) {
+    const double k = rint(turn * 64.0);
+    const double x = (turn - k * 0.015625) * 3.14159265358979323846;
+    const double2 t = table[int(k) + 64];
+    const double z = x * x;
+    const double sx = x * fma(z, fma(z, fma(z, -1.0 / 5040.0, 1.0 / 120.0), -1.0 / 6.0), 1.0);
+    const double cx = fma(z, fma(z, fma(z, fma(z, 1.0 / 40320.0, -1.0 / 720.0), 1.0 / 24.0), -0.5), 1.0);
+    c = t.x * cx - t.y * sx;
+    s = t.y * cx + t.x * sx;
+}
+
+// A CTA takes a few rows' Q, or their K and V: the cosines and sines of the rows'
+// pairs once, for all heads, then every head in units of 16 values (two runs of
+// 8 that are rotated with one another).  A thread keeps its unit and goes
+// through the rows with it, their loads in flight together and before the
+// cosines are computed, so that what depends on the unit is computed once.  The
+// angle is a fraction of a revolution in 64 bits (in 32, position times
+// frequency has lost 7 bits of its fraction at position 131072), cut to its
+// fractional part there; its cosine and sine are then good to 32 bits.
+// Over a 4-bit cache, K and V go in units of 8 values, four lanes to a block of
+// 32; K's cosines and sines are pairs of f32 and its codes are rounded once,
+// from about 48 bits, so that they are those of the exact rotation.
 // Memory-bound: every row is read and written once.
-template <int kRows>
-__device__ __forceinline__ void rotate_unit(const void *src, size_t base, int u, int half, int interleaved, const float2 *cs,
-                                            float (&x)[8], float (&y)[8], int &at_x, int &at_y) {
-    // rotated dims are a multiple of 16, so a unit is rotated whole or not at all
-    if (half && !interleaved && 8 * u < half) {
-        at_x = 8 * u, at_y = half + 8 * u;
-    } else {
-        at_x = 16 * u, at_y = 16 * u + 8;
-    }
-    load8<kRows>(src, base + at_x, x);
-    load8<kRows>(src, base + at_y, y);
-    if (16 * u >= 2 * half) {
-        return;
-    }
-    if (!interleaved) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 t = cs[8 * u + j];
-            const float a = x[j], b = y[j];
-            x[j] = a * t.x - b * t.y;
-            y[j] = a * t.y + b * t.x;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 t = cs[8 * u + j], s = cs[8 * u + 4 + j];
-            float a = x[2 * j], b = x[2 * j + 1];
-            x[2 * j] = a * t.x - b * t.y;
-            x[2 * j + 1] = a * t.y + b * t.x;
-            a = y[2 * j], b = y[2 * j + 1];
-            y[2 * j] = a * s.x - b * s.y;
-            y[2 * j + 1] = a * s.y + b * s.x;
-        }
-    }
-}
-
 template <int kRows, int kCache, int D>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(AppendArgs a, int rows_per_cta) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    // [rows_per_cta][half]: f64 where the cache is 4 bits (K is rounded to codes
-    // once, from 64 bits), then f32
-    double2 *cs64 = reinterpret_cast<double2 *>(smem);
-    float2 *cs = reinterpret_cast<float2 *>(smem + (kCache == kMxfp4 ? size_t(rows_per_cta) * a.half * sizeof(double2) : 0));
-    const int r0 = blockIdx.x * rows_per_cta;
-    const int count = min(rows_per_cta, a.rows - r0);
-    for (int i = threadIdx.x; i < count * a.half; i += kAppendThreads) {
-        const int r = i / a.half, pair = i - r * a.half;
-        const int4 ri = a.row[r0 + r];
-        const double turn = double(ri.x) * a.turns[pair];
-        const double part = 2.0 * (turn - rint(turn));  // half turns in [-1, 1]
-        if constexpr (kCache == kMxfp4) {
-            double s, c;
-            sincospi(part, &s, &c);
-            cs64[i] = make_double2(c * a.rope_scale, s * a.rope_scale);
-            cs[i] = make_float2(float(c * a.rope_scale), float(s * a.rope_scale));
+__global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(AppendArgs a) {
+    constexpr bool kFour = kCache == kMxfp4;
+    constexpr int kSize = kRows == kF32 ? 4 : 2, kVec = 8 * kSize / 16;  // 16-byte words of a run
+    constexpr int kDeep = append_rows(kRows), kMost = kDeep * kAppendSubs;
+    __shared__ float2 cs[kMost * kMaxPairs];
+    __shared__ float2 low[kFour ? kMost * kMaxPairs : 1];  // what cos and sin lack in f32
+    __shared__ uint8_t *slots[kMost];
+    __shared__ int tokens[kMost], good[kMost];
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
+    const bool is_q = int(blockIdx.x) < a.q_blocks;
+    const int part = is_q ? 0 : 1, block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
+    const int units = a.units[part], subs = a.subs[part], per_cta = a.deep * subs;
+    const int r0 = block * per_cta, count = min(per_cta, a.rows - r0);
+    const int sub = subs > 1 ? quotient(tid, a.unit_div[part]) : 0;
+    const int step = subs > 1 ? units : threads;  // to the next unit of a thread
+    const int mine = sub < subs ? min(a.deep, count - sub * a.deep) : 0;  // this thread's rows
+    const int rs = sub * a.deep;                  // the first of them, in the CTA
+    int i = subs > 1 ? tid - sub * units : tid;
+
+    // What a unit is: 16 values of Q, or of K or V in the rows' type, or 8 of K or V in 4 bits.
+    struct Unit {
+        bool is_v;
+        int head, ax, ay, turn, pair;  // the runs; turn: 0 none, 1 pairs across the runs, 2 pairs inside; first pair
+        const uint8_t *src;
+        size_t stride;
+    };
+    auto decode = [&](int u) {
+        Unit x;
+        const bool four = kFour && !is_q;
+        const int per_head = four ? D / 8 : D / 16, kv = a.kv_heads * per_head;
+        x.is_v = !is_q && u >= kv;
+        u -= x.is_v ? kv : 0;
+        x.head = u / per_head;
+        u -= x.head * per_head;
+        const int half = x.is_v ? 0 : a.half;
+        if (four) {
+            const int d = 8 * u;
+            x.turn = d < 2 * half ? 1 + a.interleaved : 0;
+            x.ax = d;
+            x.ay = d >= half ? d - half : d + half;  // the run it is rotated with
+            x.pair = x.turn == 2 ? d / 2 : (d >= half ? d - half : d);
         } else {
-            float s, c;
-            sincospif(float(part), &s, &c);
-            cs[i] = make_float2(c * a.rope_scale, s * a.rope_scale);
+            // the rotated values are a multiple of 16: a unit is rotated whole or not at all
+            x.turn = 16 * u < 2 * half ? 1 + a.interleaved : 0;
+            x.ax = x.turn == 1 ? 8 * u : 16 * u;
+            x.ay = x.turn == 1 ? half + 8 * u : 16 * u + 8;
+            x.pair = 8 * u;
+        }
+        x.stride = (is_q ? a.q_stride : (x.is_v ? a.v_stride : a.k_stride)) * kSize;
+        x.src = static_cast<const uint8_t *>(is_q ? a.q : (x.is_v ? a.v : a.k)) + size_t(r0 + rs) * x.stride + size_t(x.head) * (D * kSize);
+        return x;
+    };
+    uint4 x[kDeep][kVec], y[kDeep][kVec];
+    auto load = [&](const Unit &u) {
+        const bool both = !(kFour && !is_q) || u.turn == 1;
+#pragma unroll
+        for (int r = 0; r < kDeep; ++r) {
+            if (r < mine) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    x[r][j] = reinterpret_cast<const uint4 *>(u.src + r * u.stride + u.ax * kSize)[j];
+                    if (both) {
+                        y[r][j] = reinterpret_cast<const uint4 *>(u.src + r * u.stride + u.ay * kSize)[j];
+                    }
+                }
+            }
+        }
+    };
+    Unit unit{};
+    if (i < units) {
+        unit = decode(i);
+        load(unit);
+    }
+    for (int r = tid; r < count; r += threads) {
+        const int4 ri = a.row[r0 + r];
+        int token = 0;
+        slots[r] = is_q ? nullptr : row_slot(a, ri, token);
+        tokens[r] = token;
+        good[r] = ri.w >= 0;
+    }
+    for (int n = tid; n < count * a.half; n += threads) {
+        const int r = quotient(n, a.pair_div), pair = n - r * a.half;
+        const double turn = double(a.row[r0 + r].x) * a.turns[pair];
+        const double part_turn = 2.0 * (turn - rint(turn));  // half turns in [-1, 1]
+        if (kFour && !is_q) {
+            double sn, c;
+            cos_sin(part_turn, a.table, c, sn);
+            sn *= a.rope_scale, c *= a.rope_scale;
+            const float2 h = make_float2(float(c), float(sn));
+            cs[n] = h;
+            if constexpr (kFour) {
+                low[n] = make_float2(float(c - double(h.x)), float(sn - double(h.y)));
+            }
+        } else {
+            float sn, c;
+            sincospif(float(part_turn), &sn, &c);
+            cs[n] = make_float2(c * float(a.rope_scale), sn * float(a.rope_scale));
         }
     }
     __syncthreads();
-    constexpr int kUnits = D / 16;
-    // Q, and K and V where the cache holds the rows' type
-    const int qu = a.q ? a.q_heads * kUnits : 0;
-    const int per_row = qu + (kCache == kMxfp4 ? 0 : 2 * a.kv_heads * kUnits);
-    for (int i = threadIdx.x; i < count * per_row; i += kAppendThreads) {
-        const int r = i / per_row;
-        int u = i - r * per_row;
-        const int row = r0 + r;
-        const int4 ri = a.row[row];
-        if (ri.w < 0) {
-            continue;
-        }
-        float x[8], y[8];
-        int ax, ay;
-        const float2 *rot = cs + r * a.half;
-        if (u < qu) {
-            const int head = u / kUnits;
-            u -= head * kUnits;
-            rotate_unit<kRows>(a.q, size_t(row) * a.q_stride + size_t(head) * D, u, a.half, a.interleaved, rot, x, y, ax, ay);
-            const size_t to = size_t(row) * a.q_out_stride + size_t(head) * D;
-            store8<kRows>(a.q_out, to + ax, x);
-            store8<kRows>(a.q_out, to + ay, y);
-            continue;
-        }
-        if constexpr (kCache != kMxfp4) {
-            u -= qu;
-            const bool is_v = u >= a.kv_heads * kUnits;
-            u -= is_v ? a.kv_heads * kUnits : 0;
-            const int head = u / kUnits;
-            u -= head * kUnits;
-            int token = 0;
-            uint8_t *slot = row_slot(a, ri, token);
-            if (!slot) {
-                continue;
+    if (!(kFour && !is_q)) {
+        while (i < units) {
+            uint8_t *out = is_q ? static_cast<uint8_t *>(a.q_out) + (size_t(r0 + rs) * a.q_out_stride + size_t(unit.head) * D) * kSize : nullptr;
+            const size_t in_slot = size_t(unit.head) * a.block_bytes + (unit.is_v ? a.block_bytes >> 1 : 0);
+#pragma unroll
+            for (int r = 0; r < kDeep; ++r) {
+                if (r >= mine || !good[rs + r] || (!is_q && !slots[rs + r])) {
+                    continue;
+                }
+                uint8_t *dst = is_q ? out + r * a.q_out_stride * kSize : slots[rs + r] + in_slot + size_t(tokens[rs + r]) * (D * kSize);
+                if (unit.turn) {
+                    const float2 *c = cs + (rs + r) * a.half + unit.pair;
+                    float p[8], q[8];
+                    load8<kRows>(x[r], 0, p);
+                    load8<kRows>(y[r], 0, q);
+                    if (unit.turn == 1) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 t = c[j];
+                            const float v = p[j], w = q[j];
+                            p[j] = v * t.x - w * t.y;
+                            q[j] = v * t.y + w * t.x;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 t = c[j];
+                            float *z = j < 4 ? p + 2 * j : q + 2 * (j - 4);
+                            const float v = z[0], w = z[1];
+                            z[0] = v * t.x - w * t.y;
+                            z[1] = v * t.y + w * t.x;
+                        }
+                    }
+                    store8<kRows>(dst, unit.ax, p);
+                    store8<kRows>(dst, unit.ay, q);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) {
+                        reinterpret_cast<uint4 *>(dst + unit.ax * kSize)[j] = x[r][j];
+                        reinterpret_cast<uint4 *>(dst + unit.ay * kSize)[j] = y[r][j];
+                    }
+                }
             }
-            slot += size_t(head) * a.block_bytes + (is_v ? a.block_bytes >> 1 : 0);
-            if (is_v) {
-                rotate_unit<kRows>(a.v, size_t(row) * a.v_stride + size_t(head) * D, u, 0, 0, rot, x, y, ax, ay);
-            } else {
-                rotate_unit<kRows>(a.k, size_t(row) * a.k_stride + size_t(head) * D, u, a.half, a.interleaved, rot, x, y, ax, ay);
+            i += step;
+            if (subs > 1 || i >= units) {
+                break;
             }
-            store8<kRows>(slot, size_t(token) * D + ax, x);
-            store8<kRows>(slot, size_t(token) * D + ay, y);
+            unit = decode(i);
+            load(unit);
         }
     }
-    if constexpr (kCache == kMxfp4) {
-        // a thread per block of 32 values
-        constexpr int kBlocks = D / 32;
-        const int blocks = 2 * a.kv_heads * kBlocks;
-        for (int i = threadIdx.x; i < count * blocks; i += kAppendThreads) {
-            const int r = i / blocks;
-            int u = i - r * blocks;
-            const int row = r0 + r;
-            const int4 ri = a.row[row];
-            int token = 0;
-            uint8_t *slot = row_slot(a, ri, token);
-            if (!slot) {
-                continue;
-            }
-            const bool is_v = u >= a.kv_heads * kBlocks;
-            u -= is_v ? a.kv_heads * kBlocks : 0;
-            const int head = u / kBlocks, b = u - head * kBlocks;
-            slot += size_t(head) * a.block_bytes + (is_v ? a.block_bytes >> 1 : 0);
-            uint8_t *codes = slot + size_t(token) * (D / 2) + b * 16;
-            uint8_t *scale = slot + (size_t(1) << a.page_shift) * (D / 2) + size_t(token) * (D / 32) + b;
-            float x[32], w[8];
-            if (is_v || a.half == 0 || 32 * b >= 2 * a.half) {
-                const size_t at = is_v ? size_t(row) * a.v_stride : size_t(row) * a.k_stride;
+    if constexpr (kFour) {
+        // four lanes to a block of 32: units, threads and groups are multiples of four, so
+        // a block's lanes are in the loop together; the shuffles name the lanes that are
+        while (!is_q && __any_sync(0xffffffffu, i < units)) {
+            const bool have = i < units;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    load8<kRows>(is_v ? a.v : a.k, at + size_t(head) * D + 32 * b + 8 * j, w);
+            for (int r = 0; r < kDeep; ++r) {
+                const bool row = have && r < mine;
+                if (!__any_sync(0xffffffffu, row)) {
+                    continue;
+                }
+                float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (row) {
+                    load8<kRows>(x[r], 0, z);
+                    const float2 *c = cs + (rs + r) * a.half + unit.pair, *e = low + (rs + r) * a.half + unit.pair;
+                    if (unit.turn == 2) {
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        x[8 * j + t] = w[t];
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 h = c[j], l = e[j];
+                            const float p = z[2 * j], q = z[2 * j + 1];
+                            z[2 * j] = turned_odd(p, q, h.x, l.x, h.y, l.y);
+                            z[2 * j + 1] = turned_odd(q, -p, h.x, l.x, h.y, l.y);
+                        }
+                    } else if (unit.turn == 1) {
+                        float w[8];
+                        load8<kRows>(y[r], 0, w);
+                        const float sign = unit.ax >= a.half ? -1.0f : 1.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 h = c[j], l = e[j];
+                            z[j] = turned_odd(z[j], sign * w[j], h.x, l.x, h.y, l.y);
+                        }
                     }
                 }
-                quantize_block(x, codes, scale);
-                continue;
+                const bool write = row && slots[rs + r] != nullptr;
+                const int token = write ? tokens[rs + r] : 0;
+                quantize8(z, lane, write, write ? slots[rs + r] + size_t(unit.head) * a.block_bytes + (unit.is_v ? a.block_bytes >> 1 : 0) : nullptr,
+                          size_t(token) * (D / 2) + unit.ax / 2,
+                          (size_t(1) << a.page_shift) * (D / 2) + size_t(token) * (D / 32) + unit.ax / 32);
             }
-            double z[32];
-            const double2 *rot = cs64 + r * a.half;
-            const size_t at = size_t(row) * a.k_stride + size_t(head) * D;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d0 = 32 * b + 8 * j;
-                load8<kRows>(a.k, at + d0, w);
-                if (d0 >= 2 * a.half) {
-#pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        z[8 * j + t] = w[t];
-                    }
-                } else if (a.interleaved) {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const double2 c = rot[d0 / 2 + t];
-                        const double p = w[2 * t], q = w[2 * t + 1];
-                        z[8 * j + 2 * t] = p * c.x - q * c.y;
-                        z[8 * j + 2 * t + 1] = p * c.y + q * c.x;
-                    }
-                } else {
-                    const bool second = d0 >= a.half;
-                    float o[8];
-                    load8<kRows>(a.k, at + (second ? d0 - a.half : d0 + a.half), o);
-#pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        const double2 c = rot[(second ? d0 - a.half : d0) + t];
-                        z[8 * j + t] = second ? double(o[t]) * c.y + double(w[t]) * c.x : double(w[t]) * c.x - double(o[t]) * c.y;
-                    }
-                }
+            i += step;
+            if (subs > 1) {
+                break;
             }
-            quantize_block(z, codes, scale);
+            if (i < units) {
+                unit = decode(i);
+                load(unit);
+            }
         }
     }
 }
@@ -595,35 +663,54 @@ struct ReadArgs {
     uint32_t *status;
     int rows, kv_heads, page_shift, pages;
     uint32_t block_bytes;
+    int per_cta;
 };
 
+// A CTA takes a few rows; a thread keeps its 8 values of a head and goes through
+// the rows with them, their loads in flight together.  Memory-bound.
 template <int kRows, int kCache, int D> __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
-    constexpr int kUnits = D / 8;
-    const int per_row = 2 * a.kv_heads * kUnits;
-    const long long all = (long long)(a.rows) * per_row;
-    for (long long i = (long long)(blockIdx.x) * 256 + threadIdx.x; i < all; i += (long long)(gridDim.x) * 256) {
-        const int row = int(i / per_row);
-        int u = int(i - (long long)(row)*per_row);
-        const int4 ri = a.row[row];
+    __shared__ const uint8_t *slots[kAppendRows];
+    __shared__ int tokens[kAppendRows];
+    const int tid = threadIdx.x, r0 = blockIdx.x * a.per_cta;
+    const int count = min(a.per_cta, a.rows - r0);
+    if (tid < count) {
         int token = 0;
-        const uint8_t *slot = row_slot(a, ri, token);
-        if (!slot) {
-            continue;
-        }
-        const bool is_v = u >= a.kv_heads * kUnits;
-        u -= is_v ? a.kv_heads * kUnits : 0;
+        slots[tid] = row_slot(a, a.row[r0 + tid], token);
+        tokens[tid] = token;
+    }
+    __syncthreads();
+    constexpr int kUnits = D / 8;
+    const int ku = a.kv_heads * kUnits;
+    for (int i = tid; i < 2 * ku; i += int(blockDim.x)) {
+        const bool is_v = i >= ku;
+        const int u = is_v ? i - ku : i;
         const int head = u / kUnits, d = 8 * (u - head * kUnits);
-        slot += size_t(head) * a.block_bytes + (is_v ? a.block_bytes >> 1 : 0);
-        float x[8];
-        if constexpr (kCache != kMxfp4) {
-            load8<kCache>(slot, size_t(token) * D + d, x);
-        } else {
+        const size_t in_slot = size_t(head) * a.block_bytes + (is_v ? a.block_bytes >> 1 : 0);
+        const size_t stride = is_v ? a.v_stride : a.k_stride, to = size_t(r0) * stride + size_t(head) * D + d;
+        float x[kAppendRows][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = pool_value<kCache, D>(slot, 1 << a.page_shift, token, d + j);
+        for (int r = 0; r < kAppendRows; ++r) {
+            if (r < count && slots[r]) {
+                const uint8_t *block = slots[r] + in_slot;
+                if constexpr (kCache != kMxfp4) {
+                    load8<kCache>(block, size_t(tokens[r]) * D + d, x[r]);
+                } else {
+                    const uint32_t codes = *reinterpret_cast<const uint32_t *>(block + size_t(tokens[r]) * (D / 2) + d / 2);
+                    const float f = scale_of(block[(size_t(1) << a.page_shift) * (D / 2) + size_t(tokens[r]) * (D / 32) + d / 32]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 v = __half22float2(ttl::e2m1x2_to_half2((codes >> (8 * j)) & 255u));
+                        x[r][2 * j] = v.x * f, x[r][2 * j + 1] = v.y * f;
+                    }
+                }
             }
         }
-        store8<kRows>(is_v ? a.v : a.k, size_t(row) * (is_v ? a.v_stride : a.k_stride) + size_t(head) * D + d, x);
+#pragma unroll
+        for (int r = 0; r < kAppendRows; ++r) {
+            if (r < count && slots[r]) {
+                store8<kRows>(is_v ? a.v : a.k, to + r * stride, x[r]);
+            }
+        }
     }
 }
 
@@ -729,19 +816,46 @@ int check_layer(ttl_kv *h, int layer) {
     return TTL_OK;
 }
 
-template <int kRows, int kCache, int D> cudaError_t launch_append(ttl_kv *h, const AppendArgs &a) {
-    // enough rows for a few hundred units of 16 values, and cosines that fit
-    // 48 KB; one row each while that does not fill the GPU
-    int per = a.rows <= 2 * h->sms ? 1 : 4;
-    const size_t smem = size_t(per) * a.half * (sizeof(float2) + (kCache == kMxfp4 ? sizeof(double2) : 0));
-    kv_append_kernel<kRows, kCache, D><<<(a.rows + per - 1) / per, kAppendThreads, smem, h->stream>>>(a, per);
+uint32_t reciprocal(int n) {
+    return n > 1 ? uint32_t(((uint64_t(1) << 32) + n - 1) / n) : 0;
+}
+
+// Rows of a thread: one while there are too few to fill the GPU.
+int rows_of_a_thread(const ttl_kv *h, int rows) {
+    return rows <= 4 * h->sms ? 1 : append_rows(h->rows_type);
+}
+
+template <int kRows, int kCache, int D> cudaError_t launch_append(ttl_kv *h, const AppendArgs &args) {
+    AppendArgs a = args;
+    a.units[0] = a.q ? a.q_heads * (D / 16) : 0;
+    a.units[1] = 2 * a.kv_heads * (kCache == kMxfp4 ? D / 8 : D / 16);
+    // threads: the wider part's units in equal passes of at most 256; the
+    // narrower part puts several rows side by side
+    const int most = std::max(a.units[0], a.units[1]), passes = (most + kAppendThreads - 1) / kAppendThreads;
+    const int threads = std::max(((most + passes - 1) / passes + 31) / 32 * 32, 64);
+    a.deep = rows_of_a_thread(h, a.rows);
+    int blocks[2] = {0, 0};
+    for (int p = 0; p < 2; ++p) {
+        if (a.units[p] == 0) {
+            a.subs[p] = 1;
+            continue;
+        }
+        // groups of a 4-bit part's lanes stay whole: its units are a multiple of 16
+        a.subs[p] = a.deep > 1 ? std::min(std::max(threads / a.units[p], 1), kAppendSubs) : 1;
+        a.unit_div[p] = reciprocal(a.units[p]);
+        blocks[p] = (a.rows + a.deep * a.subs[p] - 1) / (a.deep * a.subs[p]);
+    }
+    a.q_blocks = blocks[0];
+    a.pair_div = a.half > 1 ? reciprocal(a.half) : 0;
+    kv_append_kernel<kRows, kCache, D><<<blocks[0] + blocks[1], threads, 0, h->stream>>>(a);
     return cudaGetLastError();
 }
 
-template <int kRows, int kCache, int D> cudaError_t launch_read(ttl_kv *h, const ReadArgs &a) {
-    const long long all = (long long)(a.rows) * 2 * a.kv_heads * (D / 8);
-    const long long ctas = std::min<long long>((all + 255) / 256, (long long)(h->sms) * 32);
-    kv_read_kernel<kRows, kCache, D><<<unsigned(ctas), 256, 0, h->stream>>>(a);
+template <int kRows, int kCache, int D> cudaError_t launch_read(ttl_kv *h, const ReadArgs &args) {
+    ReadArgs a = args;
+    a.per_cta = rows_of_a_thread(h, a.rows);
+    const int threads = std::min(256, (2 * a.kv_heads * (D / 8) + 31) / 32 * 32);
+    kv_read_kernel<kRows, kCache, D><<<(a.rows + a.per_cta - 1) / a.per_cta, threads, 0, h->stream>>>(a);
     return cudaGetLastError();
 }
 
@@ -849,7 +963,7 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
     h->rows_type = int(c->rows_type), h->cache_type = int(c->cache_type);
     h->max_seqs = int(c->max_seqs), h->max_rows = int(c->max_rows), h->window = int(c->window);
     h->rope_dims = int(c->rope_dims), h->interleaved = int(c->rope_interleaved);
-    h->rope_scale = c->rope_scale == 0.0 ? 1.0f : float(c->rope_scale);
+    h->rope_scale = c->rope_scale == 0.0 ? 1.0 : c->rope_scale;
     h->block_bytes = 2 * uint32_t(h->page_tokens) * row_bytes(h->cache_type, h->dim);
     h->layer_bytes = size_t(h->pages) * h->kv_heads * h->block_bytes;
     if (c->stream) {
@@ -873,6 +987,7 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
     const size_t part = kv_part_floats(*h);
     int rc = kv_alloc(h, &h->pool, h->layer_bytes * h->layers);
     rc = rc ? rc : kv_alloc(h, &h->turns, size_t(h->rope_dims / 2));
+    rc = rc ? rc : kv_alloc(h, &h->table, kTurnSteps + 1);
     rc = rc ? rc : kv_alloc(h, &h->plan, 1);
     for (int k = 0; k < kKinds && !rc; ++k) {
         for (int w = 0; w < (h->window ? 2 : 1) && !rc; ++w) {
@@ -883,7 +998,6 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
     }
     rc = rc ? rc : kv_alloc(h, &h->row[0], size_t(h->max_rows));
     rc = rc ? rc : kv_alloc(h, &h->row[1], size_t(h->max_rows));
-    rc = rc ? rc : kv_alloc(h, &h->seq, size_t(h->max_seqs));
     rc = rc ? rc : kv_alloc(h, &h->part, part);
     rc = rc ? rc : kv_alloc(h, &h->counters, size_t(kKinds) * kMaxCtas);
     rc = rc ? rc : kv_alloc(h, &h->status, 1);
@@ -895,11 +1009,20 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
     for (int i = 0; i < h->rope_dims / 2; ++i) {
         turns[i] = c->rope_freq[i] / 6.283185307179586476925286766559;
     }
+    double2 table[kTurnSteps + 1];
+    for (int i = 0; i <= kTurnSteps; ++i) {
+        // from the first octant, so that equal angles have equal values
+        const int k = std::abs(i - 64), m = std::min(k, 64 - k), n = std::min(m, 32 - m);
+        const double x = n * (3.141592653589793238462643383279502884 / 64.0);
+        const double c = m <= 16 ? std::cos(x) : std::sin(x), s = m <= 16 ? std::sin(x) : std::cos(x);
+        table[i] = make_double2(k <= 32 ? c : -c, i < 64 ? -s : s);
+    }
     cudaError_t e = cudaMemsetAsync(h->pool, 0, h->layer_bytes * h->layers, h->stream);
     e = e ? e : cudaMemsetAsync(h->plan, 0, sizeof(Plan), h->stream);
     e = e ? e : cudaMemsetAsync(h->counters, 0, sizeof(uint32_t) * kKinds * kMaxCtas, h->stream);
     e = e ? e : cudaMemsetAsync(h->status, 0, sizeof(uint32_t), h->stream);
     e = e ? e : cudaMemcpyAsync(h->turns, turns, sizeof(double) * size_t(h->rope_dims / 2), cudaMemcpyHostToDevice, h->stream);
+    e = e ? e : cudaMemcpyAsync(h->table, table, sizeof(table), cudaMemcpyHostToDevice, h->stream);
     e = e ? e : cudaStreamSynchronize(h->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -943,7 +1066,7 @@ int kv_batch(ttl_kv *h, uint32_t seqs, uint32_t rows, uint32_t max_new, const in
             a.cuts[k][w] = h->cuts[k][w];
         }
     }
-    a.row[0] = h->row[0], a.row[1] = h->row[1], a.seq = h->seq;
+    a.row[0] = h->row[0], a.row[1] = h->row[1];
     a.counters = h->counters, a.status = h->status;
     a.row_start = row_start, a.length = length, a.pages = pages, a.first = first, a.prefix_len = prefix;
     a.page_stride = page_stride;
@@ -994,7 +1117,7 @@ int kv_append(ttl_kv *h, int layer, int rotate, const void *k, size_t k_stride, 
     a.k = k, a.v = v, a.q = q, a.q_out = q_out;
     a.k_stride = k_stride, a.v_stride = v_stride, a.q_stride = q_stride, a.q_out_stride = q_out_stride;
     a.pool = h->pool + size_t(layer) * h->layer_bytes;
-    a.turns = h->turns, a.rope_scale = h->rope_scale, a.status = h->status;
+    a.turns = h->turns, a.table = h->table, a.rope_scale = h->rope_scale, a.status = h->status;
     a.rows = h->rows, a.q_heads = h->q_heads, a.kv_heads = h->kv_heads, a.page_shift = h->page_shift, a.pages = h->pages;
     a.half = rotate ? h->rope_dims / 2 : 0, a.interleaved = h->interleaved, a.block_bytes = h->block_bytes;
     TTL_KV_CUDA(h, TTL_KV_DISPATCH(h, launch_append, h, a));
@@ -1017,7 +1140,7 @@ int kv_read(ttl_kv *h, int layer, void *k, size_t k_stride, void *v, size_t v_st
         return rc;
     }
     ReadArgs a{h->plan, h->row[0], k, v, k_stride, v_stride, h->pool + size_t(layer) * h->layer_bytes, h->status,
-               h->rows, h->kv_heads, h->page_shift, h->pages, h->block_bytes};
+               h->rows, h->kv_heads, h->page_shift, h->pages, h->block_bytes, 0};
     TTL_KV_CUDA(h, TTL_KV_DISPATCH(h, launch_read, h, a));
     return TTL_OK;
 }
@@ -1058,7 +1181,7 @@ int kv_attend(ttl_kv *h, int layer, uint32_t flags, const void *q, size_t q_stri
             continue;
         }
         AttendArgs a{};
-        a.walk = Walk{h->plan, &h->plan->list[kind][w], h->tiles[kind][w], h->cuts[kind][w], h->row[w], h->seq};
+        a.walk = Walk{h->plan, &h->plan->list[kind][w], h->tiles[kind][w], h->cuts[kind][w], h->row[w]};
         a.pool = h->pool + size_t(layer) * h->layer_bytes;
         a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
         a.sinks = sinks, a.slopes = slopes;

@@ -38,9 +38,10 @@ constexpr int kKinds = 2;          // tiles of few columns, tiles of a prompt
 constexpr int kMaxCtas = 1024;     // CTAs of a list (cuts)
 constexpr int kNoSplit = 4;        // a tile of at most this many granules is not cut
 
-struct __align__(16) Tile {
+struct __align__(32) Tile {
     int32_t seq, col0, gran0;
     uint32_t size;                 // columns (9 bits), granules
+    int32_t row0, len, pad[2];     // of the sequence: its first row, its length
 };
 struct __align__(16) Cut {
     int32_t head, tile, gran;      // gran: granules into the tile
@@ -64,7 +65,6 @@ struct Walk {
     const Tile *tiles;
     const Cut *cuts;               // [ctas + 1]
     const int4 *row;               // [rows] {position, lo, hi, seq} of this window; seq -1: padding
-    const int4 *seq;               // [seqs] {row0, rows, length, 0}
 };
 
 struct AttendArgs {
@@ -86,6 +86,11 @@ __host__ __device__ constexpr uint32_t row_bytes(int cache, int d) {
     return cache == kMxfp4 ? uint32_t(d / 2 + d / 32) : uint32_t(cache == kF32 ? 4 * d : 2 * d);
 }
 
+// 2^(e - 127) of an E8M0 byte: 0 is the smallest (a subnormal float), 255 NaN.
+__device__ __forceinline__ float scale_of(uint32_t e) {
+    return e == 255u ? __uint_as_float(0x7fffffffu) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
+}
+
 // ---- the pool: [page][KV head][K rows, V rows] ----
 // f32, f16, bf16: [page_tokens][D].  MXFP4: codes [page_tokens][D / 2] (value k
 // in byte k / 2, low nibble for even k), then scales [page_tokens][D / 32].
@@ -102,9 +107,7 @@ template <int kCache, int D> __device__ __forceinline__ float pool_value(const u
         const uint32_t code = (d & 1) ? byte >> 4 : byte & 15u;
         const uint32_t e = rows[tokens * (D / 2) + t * (D / 32) + d / 32];
         const float2 v = __half22float2(e2m1x2_to_half2(code));
-        // 2^(e - 127); 0 is the smallest scale (a subnormal float), 255 NaN
-        const float s = e == 255u ? __uint_as_float(0x7fffffffu) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
-        return v.x * s;
+        return v.x * scale_of(e);
     }
 }
 
@@ -200,7 +203,7 @@ __device__ __forceinline__ float capped(float dot, float in, float out) {
 // ---- the walk ----
 
 struct Piece {
-    int head, tile, seq, col0, ncols;
+    int head, tile, seq, col0, ncols, row0, len;
     int k0, k1;        // keys of the piece (k1 <= the tile's last granule; clip to the sequence's length)
     int first, last;   // first and last CTA that hold a part of the tile (equal: the whole tile is here)
 };
@@ -226,13 +229,16 @@ struct Walker {
         if (!before(head, tile, gran, end)) {
             return false;
         }
-        const Tile t = w.tiles[tile];
+        const Tile &from = w.tiles[tile];
+        const int4 t4 = *reinterpret_cast<const int4 *>(&from);
+        const int2 t2 = *reinterpret_cast<const int2 *>(&from.row0);
+        const Tile t{t4.x, t4.y, t4.z, uint32_t(t4.w), t2.x, t2.y, {0, 0}};
         const int n = int(t.size >> 9);
         int stop = n;
         if (end.head == head && end.tile == tile) {
             stop = end.gran;  // > gran
         }
-        p.head = head, p.tile = tile, p.seq = t.seq, p.col0 = t.col0, p.ncols = int(t.size & 511u);
+        p.head = head, p.tile = tile, p.seq = t.seq, p.col0 = t.col0, p.row0 = t.row0, p.len = t.len, p.ncols = int(t.size & 511u);
         const int gsize = w.list->gran;
         p.k0 = (t.gran0 + gran) * gsize;
         p.k1 = (t.gran0 + stop) * gsize;
@@ -268,11 +274,10 @@ __device__ __forceinline__ int part_slot(int c, int first) {
 // column whose result is not finite is computed again here, where unseen keys
 // are not touched.
 template <int kRows, int kCache, int D>
-__device__ __noinline__ void attend_column(const AttendArgs &a, const Plan &plan, int head, int seq, int row, int qhead) {
+__device__ __noinline__ void attend_column(const AttendArgs &a, const Plan &plan, int head, int seq, int len, int row, int qhead) {
     const int lane = threadIdx.x & 31;
     constexpr int kPer = D / 32;
     const int4 ri = a.walk.row[row];
-    const int len = a.walk.seq[seq].z;
     const int lo = max(ri.y, 0), hi = min(ri.z, len);
     const float scale_log2 = a.scale * kLog2e;
     const float slope = a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
@@ -328,7 +333,6 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
                                               Value value, Stats stats) {
     constexpr int kLanes = D / 8, kCols = 32 / kLanes;
     const int lane = threadIdx.x & 31;
-    const int4 si = a.walk.seq[p.seq];
     for (int base = warp * kCols; base < p.ncols; base += warps * kCols) {
         const int c = base + lane / kLanes;
         bool bad = false;
@@ -337,9 +341,9 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
             const int cc = p.col0 + c;
             const int i = cc / a.group;
             qhead = p.head * a.group + cc - i * a.group;
-            row = si.x + i;
+            row = p.row0 + i;
             const int4 ri = a.walk.row[row];
-            const bool sees = max(ri.y, 0) < min(ri.z, si.z);
+            const bool sees = max(ri.y, 0) < min(ri.z, p.len);
             const float2 ml = stats(c);
             float m = ml.x, l = ml.y, f = 1.0f;
             if (a.sinks) {
@@ -367,7 +371,7 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
         while (redo) {
             const int src = __ffs(redo) - 1;
             const int r = __shfl_sync(0xffffffffu, row, src), h = __shfl_sync(0xffffffffu, qhead, src);
-            attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, r, h);
+            attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, r, h);
             const int first = src / kLanes * kLanes;
             redo &= ~(((kLanes == 32 ? 0u : (1u << kLanes)) - 1u) << first);
         }
@@ -376,10 +380,89 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
 
 // Merges the partial results of a tile over the CTAs [first, last] that hold
 // them and stores its columns.  part: [slot][width][D + 2] with {max, sum}
-// after the D sums.
+// after the D sums.  Few parts: D / 8 lanes per column as in store_columns.
+// Many (a long sequence): a warp per column, a lane per part for the maxima and
+// sums and four values a lane for the values, so that the loads of many parts
+// are in flight together.
+constexpr int kFewParts = 6;
+
 template <int kRows, int kCache, int D>
 __device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps, int width) {
     const size_t pitch = D + 2;
+    const int parts = p.last - p.first + 1;
+    if (parts > kFewParts) {
+        const int lane = threadIdx.x & 31;
+        constexpr int kSplit = 128 / D;  // parts that a warp reads at once
+        const int d = 4 * (lane % (D / 4)), sub = lane / (D / 4);
+        for (int c = warp; c < p.ncols; c += warps) {
+            const int cc = p.col0 + c, i = cc / a.group;
+            const int qhead = p.head * a.group + cc - i * a.group, row = p.row0 + i;
+            const int4 ri = a.walk.row[row];
+            const float *col = a.part + size_t(c) * pitch;
+            auto slot = [&](int k) { return col + size_t(part_slot(p.first + k, p.first)) * width * pitch; };
+            float m = -INFINITY;
+            for (int k = lane; k < parts; k += 32) {
+                m = fmaxf(m, __ldcg(slot(k) + D));
+            }
+#pragma unroll
+            for (int off = 16; off; off >>= 1) {
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            }
+            const float safe = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int base = 0; base < parts; base += 32) {
+                float f = 0.0f;
+                if (base + lane < parts) {
+                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(base + lane) + D));
+                    f = exp2f(ml.x - safe);
+                    l = fmaf(ml.y, f, l);
+                }
+                const int count = min(32, parts - base);
+#pragma unroll 8
+                for (int k = 0; k < count; k += kSplit) {
+                    const int mine = k + sub;
+                    const float w = __shfl_sync(0xffffffffu, f, mine & 31);
+                    if (mine < count) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(slot(base + mine) + d));
+                        const float2 y = __ldcg(reinterpret_cast<const float2 *>(slot(base + mine) + d + 2));
+                        o[0] = fmaf(x.x, w, o[0]), o[1] = fmaf(x.y, w, o[1]);
+                        o[2] = fmaf(y.x, w, o[2]), o[3] = fmaf(y.y, w, o[3]);
+                    }
+                }
+            }
+            l = warp_sum(l);
+            if constexpr (kSplit == 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    o[j] += __shfl_xor_sync(0xffffffffu, o[j], 16);
+                }
+            }
+            float f = 1.0f;
+            if (a.sinks) {
+                const float sink = a.sinks[qhead] * kLog2e, mn = fmaxf(m, sink), s = mn == -INFINITY ? 0.0f : mn;
+                f = exp2f(m - s);
+                l = l * f + exp2f(sink - s);
+            }
+            f = f / l;
+            const bool sees = max(ri.y, 0) < min(ri.z, p.len), write = row < a.rows && ri.w == p.seq;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = sees ? o[j] * f : 0.0f;
+                bad = bad || !(fabsf(o[j]) < INFINITY);
+            }
+            if (write && sub == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    store_value<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + d + j, o[j]);
+                }
+            }
+            if (write && __any_sync(0xffffffffu, bad)) {
+                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, row, qhead);
+            }
+        }
+        return;
+    }
     store_columns<kRows, kCache, D>(
         a, plan, p, warp, warps,
         [&](int c, int d, float(&v)[8]) {

@@ -63,12 +63,11 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
     Walker walk(a.walk, int(blockIdx.x));
     Piece p;
     while (walk.next(p)) {
-        const int4 si = a.walk.seq[p.seq];
         for (int i = tid; i < CT * (D / 8); i += kSimpleThreads) {
             const int c = i / (D / 8), d = 8 * (i % (D / 8));
             float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (c < p.ncols) {
-                const int cc = p.col0 + c, r = cc / a.group, row = si.x + r;
+                const int cc = p.col0 + c, r = cc / a.group, row = p.row0 + r;
                 if (row < a.rows) {
                     load8<kRows>(a.q, size_t(row) * a.q_stride + size_t(p.head * a.group + cc - r * a.group) * D + d, x);
                 }
@@ -83,20 +82,20 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
             float slope = 0.0f;
             if (c < p.ncols) {
                 const int cc = p.col0 + c, r = cc / a.group;
-                ri = a.walk.row[si.x + r];
+                ri = a.walk.row[p.row0 + r];
                 slope = a.slopes ? a.slopes[p.head * a.group + cc - r * a.group] * kLog2e : 0.0f;
             }
-            sm.pos[c] = ri.x, sm.lo[c] = max(ri.y, 0), sm.hi[c] = min(ri.z, si.z);
+            sm.pos[c] = ri.x, sm.lo[c] = max(ri.y, 0), sm.hi[c] = min(ri.z, p.len);
             sm.slope[c] = slope;
             sm.m[c] = -INFINITY, sm.l[c] = 0.0f;
         }
         float o[kCols][4] = {};
         for (int k0 = p.k0; k0 < p.k1; k0 += kSimpleGran) {
-            const int keys = min(kSimpleGran, si.z - k0);  // <= 0: a tile that sees nothing
+            const int keys = min(kSimpleGran, p.len - k0);  // <= 0: a tile that sees nothing
             __syncthreads();
             if (tid < kSimpleGran / 16) {
                 const int j = k0 + 16 * tid;
-                sm.pages[tid] = j < si.z ? page_of(plan, p.seq, j, a.page_shift, a.pages, a.status) : 0;
+                sm.pages[tid] = j < p.len ? page_of(plan, p.seq, j, a.page_shift, a.pages, a.status) : 0;
             }
             __syncthreads();
             if constexpr (kCache != kMxfp4) {

@@ -13,7 +13,7 @@ struct ttl_kv {
     int device = 0, sms = 148;
     int layers = 0, pages = 0, page_tokens = 0, page_shift = 0, q_heads = 0, kv_heads = 0, dim = 0;
     int rows_type = 0, cache_type = 0, max_seqs = 0, max_rows = 0, window = 0, rope_dims = 0, interleaved = 0;
-    float rope_scale = 1.0f;
+    double rope_scale = 1.0;
     uint32_t block_bytes = 0;      // one KV head of a page
     size_t layer_bytes = 0;
     cudaStream_t stream = nullptr;
@@ -21,12 +21,12 @@ struct ttl_kv {
     std::vector<void *> allocations;
     uint8_t *pool = nullptr;
     double *turns = nullptr;       // [rope_dims / 2] revolutions per position
+    double2 *table = nullptr;      // cosines and sines of 129 angles (append over 4 bits)
     ttl::kv::Plan *plan = nullptr;
     ttl::kv::Tile *tiles[2][2] = {};
     int32_t *prefix[2][2] = {};
     ttl::kv::Cut *cuts[2][2] = {};
     int4 *row[2] = {};
-    int4 *seq = nullptr;
     int tile_cap[2] = {};
     float *part = nullptr;
     uint32_t *counters = nullptr;  // [2 kinds][kMaxCtas]

@@ -154,7 +154,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     Walker walk(a.walk, int(blockIdx.x));
     Piece p;
     while (walk.next(p)) {
-        const int len = a.walk.seq[p.seq].z;
+        const int len = p.len;
         const int32_t *table = plan.pages + size_t(p.seq) * plan.page_stride;
         const int last = max(len - 1, 0) >> a.page_shift;
         int base = -64, id = 0;
@@ -237,8 +237,7 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
         const uint8_t *scales = src + tokens * (D / 2) + t * (D / 32);
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
-            const uint32_t e = scales[b];
-            const float f = e == 255u ? __uint_as_float(0x7fffffffu) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
+            const float f = scale_of(scales[b]);
             const uint4 w = *reinterpret_cast<const uint4 *>(src + t * (D / 2) + 16 * b);
             const uint32_t c[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -383,12 +382,11 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
         c.row = 0, c.qhead = 0, c.slope = 0.0f;
         c.ri = make_int4(0, 0, 1 << 30, -1);
         if (c.have) {
-            const int4 si = a.walk.seq[c.p.seq];
             const int cc = c.p.col0 + tid, r = cc / a.group;
             c.qhead = c.p.head * a.group + cc - r * a.group;
-            c.row = si.x + r;
+            c.row = c.p.row0 + r;
             c.ri = a.walk.row[c.row];
-            c.ri.y = max(c.ri.y, 0), c.ri.z = min(c.ri.z, si.z);
+            c.ri.y = max(c.ri.y, 0), c.ri.z = min(c.ri.z, c.p.len);
             c.slope = a.slopes ? a.slopes[c.qhead] * kLog2e : 0.0f;
         }
     };
@@ -609,7 +607,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
             while (redo) {
                 const int src = __ffs(redo) - 1;
                 redo &= redo - 1;
-                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, __shfl_sync(0xffffffffu, row, src),
+                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, __shfl_sync(0xffffffffu, row, src),
                                                __shfl_sync(0xffffffffu, qhead, src));
             }
         }

@@ -165,7 +165,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     Walker walk(a.walk, int(blockIdx.x));
     Piece p;
     while (walk.next(p)) {
-        const int len = a.walk.seq[p.seq].z;
+        const int len = p.len;
         const int32_t *table = plan.pages + size_t(p.seq) * plan.page_stride;
         const int last = max(len - 1, 0) >> a.page_shift;
         // page ids of 32 pages at a time; past the end the last page stands in
@@ -283,16 +283,15 @@ __global__ void __launch_bounds__(kThreads)
     Walker walk(a.walk, int(blockIdx.x));
     Piece p;
     while (walk.next(p)) {
-        const int4 si = a.walk.seq[p.seq];
         // ---- the columns ----
         if (tid < kCols) {
             int4 ri = make_int4(0, 0, 1 << 30, -1);  // a column past the tile: all keys, so that it asks for no mask
             float slope = 0.0f;
             if (tid < p.ncols) {
                 const int cc = p.col0 + tid, r = cc / a.group;
-                ri = a.walk.row[si.x + r];
+                ri = a.walk.row[p.row0 + r];
                 slope = a.slopes ? a.slopes[p.head * a.group + cc - r * a.group] * kLog2e : 0.0f;
-                ri.y = max(ri.y, 0), ri.z = min(ri.z, si.z);
+                ri.y = max(ri.y, 0), ri.z = min(ri.z, p.len);
             }
             sm.pos[tid] = ri.x, sm.lo[tid] = ri.y, sm.hi[tid] = ri.z;
             sm.slope[tid] = slope;
@@ -301,7 +300,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int c = 8 * n + g;
-            const int cc = p.col0 + c, r = cc / a.group, row = si.x + r;
+            const int cc = p.col0 + c, r = cc / a.group, row = p.row0 + r;
             const bool have = c < p.ncols && row < a.rows;
             const uint16_t *src = static_cast<const uint16_t *>(a.q) + size_t(row) * a.q_stride +
                                   size_t(p.head * a.group + cc - r * a.group) * D;
