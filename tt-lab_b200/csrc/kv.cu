@@ -40,6 +40,7 @@ struct PlanArgs {
 };
 
 constexpr int kPlanThreads = 1024;
+constexpr int kNearTiles = 1024;
 constexpr int kMaxPosition = 1 << 29;  // a tile counts up to 2^23 granules
 
 struct SeqState {
@@ -99,7 +100,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     __shared__ int sums[32];
     __shared__ int starts[4096 + 1];  // first tile of a sequence
     __shared__ Cut shared_cuts[kMaxCtas + 1];
+    __shared__ int near_prefix[kNearTiles + 1];  // the granules before a tile, where there are few tiles
     const int tid = threadIdx.x;
+    wait_previous();
     if (blockIdx.x >= 4) {
         const int r = (blockIdx.x - 4) * kPlanThreads + tid;
         if (r >= a.rows) {
@@ -159,7 +162,6 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     }
     const int width = a.width[kind], gran = a.gran[kind], cost = a.cost[kind];
     Tile *tiles = a.tiles[kind][sliding];
-    int32_t *prefix = a.prefix[kind][sliding];
     Cut *cuts = a.cuts[kind][sliding];
     // tiles of each sequence
     int total = 0;
@@ -196,6 +198,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     }
     __syncthreads();
     // their key ranges
+    int32_t *prefix = total <= kNearTiles ? near_prefix : a.prefix[kind][sliding];
     int line = 0;
     for (int base = 0; base < total; base += kPlanThreads) {
         const int t = base + tid;
@@ -460,6 +463,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(AppendArgs
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
     const bool is_q = int(blockIdx.x) < a.q_blocks;
     const int part = is_q ? 0 : 1, block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
+    wait_previous();
     const int units = a.units[part], subs = a.subs[part], per_cta = a.deep * subs;
     const int r0 = block * per_cta, count = min(per_cta, a.rows - r0);
     const int sub = subs > 1 ? quotient(tid, a.unit_div[part]) : 0;
@@ -671,6 +675,7 @@ struct ReadArgs {
 template <int kRows, int kCache, int D> __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     __shared__ const uint8_t *slots[kAppendRows];
     __shared__ int tokens[kAppendRows];
+    wait_previous();
     const int tid = threadIdx.x, r0 = blockIdx.x * a.per_cta;
     const int count = min(a.per_cta, a.rows - r0);
     if (tid < count) {
@@ -775,16 +780,14 @@ int check_pointer(ttl_kv *h, const void *p, const char *name, size_t align) {
     if (reinterpret_cast<uintptr_t>(p) % align) {
         return kv_fail(h, TTL_ERR_ARGUMENT, std::string(name) + " is not aligned to " + std::to_string(align) + " bytes");
     }
-    cudaPointerAttributes at{};
-    const cudaError_t e = cudaPointerGetAttributes(&at, p);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
+    unsigned kind = 0, managed = 0;
+    int device = -1;
+    CUpointer_attribute what[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, CU_POINTER_ATTRIBUTE_IS_MANAGED};
+    void *into[3] = {&kind, &device, &managed};
+    if (h->attributes(3, what, into, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS || kind == 0) {
         return kv_fail(h, TTL_ERR_ARGUMENT, std::string(name) + " is not a device pointer");
     }
-    if (at.type == cudaMemoryTypeManaged) {
-        return TTL_OK;
-    }
-    if (at.type != cudaMemoryTypeDevice || at.device != h->device) {
+    if (!managed && (kind != CU_MEMORYTYPE_DEVICE || device != h->device)) {
         return kv_fail(h, TTL_ERR_ARGUMENT, std::string(name) + " is not memory of the handle's GPU");
     }
     return TTL_OK;
@@ -847,16 +850,14 @@ template <int kRows, int kCache, int D> cudaError_t launch_append(ttl_kv *h, con
     }
     a.q_blocks = blocks[0];
     a.pair_div = a.half > 1 ? reciprocal(a.half) : 0;
-    kv_append_kernel<kRows, kCache, D><<<blocks[0] + blocks[1], threads, 0, h->stream>>>(a);
-    return cudaGetLastError();
+    return launch_chained(kv_append_kernel<kRows, kCache, D>, blocks[0] + blocks[1], threads, 0, h->stream, a);
 }
 
 template <int kRows, int kCache, int D> cudaError_t launch_read(ttl_kv *h, const ReadArgs &args) {
     ReadArgs a = args;
     a.per_cta = rows_of_a_thread(h, a.rows);
     const int threads = std::min(256, (2 * a.kv_heads * (D / 8) + 31) / 32 * 32);
-    kv_read_kernel<kRows, kCache, D><<<(a.rows + a.per_cta - 1) / a.per_cta, threads, 0, h->stream>>>(a);
-    return cudaGetLastError();
+    return launch_chained(kv_read_kernel<kRows, kCache, D>, (a.rows + a.per_cta - 1) / a.per_cta, threads, 0, h->stream, a);
 }
 
 // Tensor maps of a 16-bit pool, one per layer: rows of head_dim values (K and V
@@ -975,6 +976,14 @@ int kv_create(const ttl_kv_config *c, ttl_kv **out) {
         }
         h->own_stream = true;
     }
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found{};
+    if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &fn, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+        cudaGetLastError();
+        return bail(TTL_ERR_CUDA, "cuPointerGetAttributes is not available");
+    }
+    h->attributes = reinterpret_cast<ttl_kv::Attributes>(fn);
     const int group = h->q_heads / h->kv_heads;
     // tiles of the narrowest width a list can have; see choose_shapes
     h->tile_cap[0] = int(std::min<long long>((long long)(h->max_rows) * group / kNarrow + h->max_seqs, 1 << 28));
@@ -1081,8 +1090,7 @@ int kv_batch(ttl_kv *h, uint32_t seqs, uint32_t rows, uint32_t max_new, const in
         a.ctas[k] = h->ctas[k] = shape[k].ctas;
         a.tile_cap[k] = h->tile_cap[k];
     }
-    kv_plan_kernel<<<4 + (rows + kPlanThreads - 1) / kPlanThreads, kPlanThreads, 0, h->stream>>>(a);
-    TTL_KV_CUDA(h, cudaGetLastError());
+    TTL_KV_CUDA(h, launch_chained(kv_plan_kernel, 4 + int((rows + kPlanThreads - 1) / kPlanThreads), kPlanThreads, 0, h->stream, a));
     h->batched = true;
     h->seqs = int(seqs), h->rows = int(rows);
     return TTL_OK;

@@ -208,20 +208,30 @@ struct Piece {
     int first, last;   // first and last CTA that hold a part of the tile (equal: the whole tile is here)
 };
 
+// The descriptor of the tile after the one handed out is loaded ahead.
 struct Walker {
-    const Walk &w;
+    const Tile *list;
     int head, tile, gran;  // next piece
     Cut end;
     uint32_t start_span;   // of the tile that the CTA's range begins in, where it begins inside
-    int cta;
+    int cta, count, gsize;
+    int4 t4;               // tile `tile`
+    int2 t2;
 
-    __device__ __forceinline__ Walker(const Walk &walk, int cta_) : w(walk), cta(cta_) {
+    __device__ __forceinline__ Walker(const Walk &w, int cta_, int gsize_) : list(w.tiles), cta(cta_), gsize(gsize_) {
         const Cut a = w.cuts[cta];
         end = w.cuts[cta + 1];
+        count = w.list->tiles;
         head = a.head, tile = a.tile, gran = a.gran;
         start_span = a.span;
+        load();
     }
-    // -1, 0, 1: (head, tile, gran) against a cut
+    __device__ __forceinline__ void load() {
+        if (before(head, tile, gran, end)) {
+            t4 = *reinterpret_cast<const int4 *>(list + tile);
+            t2 = *reinterpret_cast<const int2 *>(&list[tile].row0);
+        }
+    }
     __device__ __forceinline__ static bool before(int h, int t, int g, const Cut &c) {
         return h != c.head ? h < c.head : (t != c.tile ? t < c.tile : g < c.gran);
     }
@@ -229,19 +239,15 @@ struct Walker {
         if (!before(head, tile, gran, end)) {
             return false;
         }
-        const Tile &from = w.tiles[tile];
-        const int4 t4 = *reinterpret_cast<const int4 *>(&from);
-        const int2 t2 = *reinterpret_cast<const int2 *>(&from.row0);
-        const Tile t{t4.x, t4.y, t4.z, uint32_t(t4.w), t2.x, t2.y, {0, 0}};
-        const int n = int(t.size >> 9);
+        const int n = int(uint32_t(t4.w) >> 9);
         int stop = n;
         if (end.head == head && end.tile == tile) {
             stop = end.gran;  // > gran
         }
-        p.head = head, p.tile = tile, p.seq = t.seq, p.col0 = t.col0, p.row0 = t.row0, p.len = t.len, p.ncols = int(t.size & 511u);
-        const int gsize = w.list->gran;
-        p.k0 = (t.gran0 + gran) * gsize;
-        p.k1 = (t.gran0 + stop) * gsize;
+        p.head = head, p.tile = tile, p.seq = t4.x, p.col0 = t4.y, p.row0 = t2.x, p.len = t2.y;
+        p.ncols = int(uint32_t(t4.w) & 511u);
+        p.k0 = (t4.z + gran) * gsize;
+        p.k1 = (t4.z + stop) * gsize;
         p.first = p.last = cta;
         const uint32_t span = gran > 0 ? start_span : end.span;
         if (gran > 0 || stop < n) {
@@ -250,16 +256,26 @@ struct Walker {
         }
         if (stop == n) {
             gran = 0;
-            if (++tile == w.list->tiles) {
+            if (++tile == count) {
                 tile = 0;
                 ++head;
             }
         } else {
             gran = stop;
         }
+        load();
         return true;
     }
 };
+
+// Programmatic dependent launch: lets the next kernel on the stream start, and
+// waits for what ran before this one.  Every kernel of the cache waits before it
+// touches global memory, so whatever follows a kernel also follows its
+// predecessors.
+__device__ __forceinline__ void wait_previous() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 // Slot of the partial result that CTA c keeps for a tile whose parts begin in
 // CTA `first`: its own first tile (slot 2c) or the one it begins (2c + 1).
@@ -327,10 +343,21 @@ __device__ __noinline__ void attend_column(const AttendArgs &a, const Plan &plan
 
 // Adds the sink, divides, rounds and stores columns [c0, ncols) step `step` of
 // a tile, by warps: D / 8 lanes per column, eight values a lane.  value(c, d,
-// v) gives the eight unnormalised sums, stats(c) {max, sum} in log2 units.
-template <int kRows, int kCache, int D, class Value, class Stats>
+// v) gives the eight unnormalised sums, stats(c) {max, sum} in log2 units,
+// info(c, row, head) what the column may see.
+struct ColumnInfo {
+    int lo, hi, seq;
+    float sink;
+};
+// From the plan's rows, for kernels that do not keep them.
+__device__ __forceinline__ ColumnInfo column_info(const AttendArgs &a, int row, int qhead) {
+    const int4 ri = a.walk.row[row];
+    return ColumnInfo{ri.y, ri.z, ri.w, a.sinks ? a.sinks[qhead] : 0.0f};
+}
+
+template <int kRows, int kCache, int D, class Value, class Stats, class Info>
 __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps,
-                                              Value value, Stats stats) {
+                                              Value value, Stats stats, Info info) {
     constexpr int kLanes = D / 8, kCols = 32 / kLanes;
     const int lane = threadIdx.x & 31;
     for (int base = warp * kCols; base < p.ncols; base += warps * kCols) {
@@ -342,12 +369,12 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
             const int i = cc / a.group;
             qhead = p.head * a.group + cc - i * a.group;
             row = p.row0 + i;
-            const int4 ri = a.walk.row[row];
-            const bool sees = max(ri.y, 0) < min(ri.z, p.len);
+            const ColumnInfo ci = info(c, row, qhead);
+            const bool sees = max(ci.lo, 0) < min(ci.hi, p.len);
             const float2 ml = stats(c);
             float m = ml.x, l = ml.y, f = 1.0f;
             if (a.sinks) {
-                const float sink = a.sinks[qhead] * kLog2e;
+                const float sink = ci.sink * kLog2e;
                 const float mn = fmaxf(m, sink);
                 const float safe = mn == -INFINITY ? 0.0f : mn;
                 f = exp2f(m - safe);
@@ -361,7 +388,7 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
                 v[j] = sees ? v[j] * f : 0.0f;
                 bad = bad || !(fabsf(v[j]) < INFINITY);
             }
-            if (row < a.rows && ri.w == p.seq) {  // a row that two sequences claim belongs to the first
+            if (row < a.rows && ci.seq == p.seq) {  // a row that two sequences claim belongs to the first
                 store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + (lane % kLanes) * 8, v);
             } else {
                 bad = false;
@@ -498,7 +525,8 @@ __device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan
                 l = fmaf(__ldcg(src + 1), exp2f(__ldcg(src) - safe), l);
             }
             return make_float2(m, l);
-        });
+        },
+        [&](int, int row, int qhead) { return column_info(a, row, qhead); });
 }
 
 // After a CTA wrote its partial result of a tile: counts it, and returns true

@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Plan &plan = *a.walk.plan;
+    wait_previous();
     if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != CT || a.walk.list->gran != kSimpleGran) {
         if (tid == 0) {
             set_status(a.status, kKvStalePlan);
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
     const int col0 = (grp / kKeySplit) * kCols, half = grp % kKeySplit;
     const int tokens = 1 << a.page_shift;
     const float scale_log2 = a.scale * kLog2e;
-    Walker walk(a.walk, int(blockIdx.x));
+    Walker walk(a.walk, int(blockIdx.x), kSimpleGran);
     Piece p;
     while (walk.next(p)) {
         for (int i = tid; i < CT * (D / 8); i += kSimpleThreads) {
@@ -224,7 +225,8 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
                         v[j] = sum[c * D + d + j];
                     }
                 },
-                [&](int c) { return make_float2(sm.m[c], sm.l[c]); });
+                [&](int c) { return make_float2(sm.m[c], sm.l[c]); },
+                [&](int, int row, int qhead) { return column_info(a, row, qhead); });
         } else {
             float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * CT * (D + 2);
             for (int i = tid; i < p.ncols * (D + 2); i += kSimpleThreads) {
@@ -240,8 +242,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
 }
 
 template <int kRows, int kCache, int D, int CT> cudaError_t launch_simple_ct(const ttl_kv &h, const AttendArgs &a, int ctas) {
-    kv_attend_simple_kernel<kRows, kCache, D, CT><<<ctas, kSimpleThreads, sizeof(SimpleSmem<CT, D>), h.stream>>>(a);
-    return cudaGetLastError();
+    return launch_chained(kv_attend_simple_kernel<kRows, kCache, D, CT>, ctas, kSimpleThreads, sizeof(SimpleSmem<CT, D>), h.stream, a);
 }
 
 template <int kRows, int kCache, int D> cudaError_t launch_simple(const ttl_kv &h, const AttendArgs &a) {

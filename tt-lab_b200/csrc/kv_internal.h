@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "kv.cuh"
@@ -16,6 +17,8 @@ struct ttl_kv {
     double rope_scale = 1.0;
     uint32_t block_bytes = 0;      // one KV head of a page
     size_t layer_bytes = 0;
+    typedef CUresult (*Attributes)(unsigned, CUpointer_attribute *, void **, CUdeviceptr);
+    Attributes attributes = nullptr;  // cuPointerGetAttributes
     cudaStream_t stream = nullptr;
     bool own_stream = false;
     std::vector<void *> allocations;
@@ -53,6 +56,23 @@ struct ttl_kv {
 
 namespace ttl {
 namespace kv {
+
+// Launches `kernel` so that it may start while its predecessor on the stream
+// ends (programmatic dependent launch; see wait_previous).
+template <class... Params, class... Args>
+cudaError_t launch_chained(void (*kernel)(Params...), int blocks, int threads, size_t smem, cudaStream_t stream, Args &&...args) {
+    cudaLaunchAttribute chained[1];
+    chained[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    chained[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(unsigned(blocks));
+    c.blockDim = dim3(unsigned(threads));
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    c.attrs = chained;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, std::forward<Args>(args)...);
+}
 
 constexpr int kNarrow = 8;         // columns of the narrowest tile
 constexpr int kPromptWidth = 256;  // columns of a prompt tile

@@ -151,7 +151,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     const int s = lane / kParts, x = lane % kParts;
     int stage = 0;
     uint32_t phase = 0;
-    Walker walk(a.walk, int(blockIdx.x));
+    Walker walk(a.walk, int(blockIdx.x), kGran);
     Piece p;
     while (walk.next(p)) {
         const int len = p.len;
@@ -254,7 +254,7 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
-    Walker walk(a.walk, int(blockIdx.x));
+    Walker walk(a.walk, int(blockIdx.x), kGran);
     Piece p;
     while (walk.next(p)) {
         for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
@@ -292,7 +292,7 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
         }
         tc::mma_commit(&sm.s_full[w]);
     };
-    Walker walk(a.walk, int(blockIdx.x));
+    Walker walk(a.walk, int(blockIdx.x), kGran);
     Piece p, ahead;
     bool any = walk.next(p), more;
     for (; any; any = more, p = ahead) {
@@ -364,7 +364,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
     const float sign = scale < 0.0f ? -1.0f : 1.0f;  // the largest score is the smallest product where the scale is negative
     const bool special = a.cap != 0.0f || a.slopes;
     uint32_t s_phase = 0, o_phase = 0;
-    Walker walk(a.walk, int(blockIdx.x));
+    Walker walk(a.walk, int(blockIdx.x), kGran);
     // The tile after the one in hand is looked up while that one runs, and its Q
     // rows are copied as soon as the last scores of this one are there, so that
     // its first scores are under way before this one has ended.
@@ -629,6 +629,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5;
     const Plan &plan = *a.walk.plan;
+    wait_previous();
     if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kPromptWidth || a.walk.list->gran != kGran) {
         if (tid == 0) {
             set_status(a.status, kKvStalePlan);
@@ -708,9 +709,8 @@ template <int kRows, int kCache, int D> cudaError_t launch(const ttl_kv &h, cons
     if constexpr (!built<kRows, kCache>()) {
         return cudaErrorInvalidValue;
     } else {
-        kv_attend_prompt_kernel<kRows, kCache, D><<<h.ctas[1], PromptShape<kCache>::kThreads, sizeof(PromptSmem<kCache, D>), h.stream>>>(
-            a, h.maps[size_t(layer)]);
-        return cudaGetLastError();
+        return launch_chained(kv_attend_prompt_kernel<kRows, kCache, D>, h.ctas[1], PromptShape<kCache>::kThreads,
+                              sizeof(PromptSmem<kCache, D>), h.stream, a, h.maps[size_t(layer)]);
     }
 }
 

@@ -65,8 +65,11 @@ template <int kRows, int kCache, int D, int NT> struct TokenSmem {
     alignas(1024) uint8_t stage[T::kStages][(T::kStageBytes + 1023) / 1024 * 1024];
     float o[kWarps][T::kCols][T::kOPitch];
     float m[kWarps][T::kCols], l[kWarps][T::kCols];
-    int lo[T::kCols], hi[T::kCols], pos[T::kCols];
-    float slope[T::kCols], scale[T::kCols];
+    // the columns: Q rows (16 bytes of padding keep the fragments' loads from
+    // colliding), and for this tile and the next the plan's row, slope and sink
+    alignas(16) uint16_t q[T::kCols][D + 8];
+    int4 row[2][T::kCols];
+    float slope[2][T::kCols], sink[2][T::kCols];
     uint64_t full[T::kStages], empty[T::kStages];
     int last, abort;
 };
@@ -162,26 +165,33 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     const int segs = kGran / seg;
     int stage = 0;
     uint32_t phase = 0;
-    Walker walk(a.walk, int(blockIdx.x));
-    Piece p;
-    while (walk.next(p)) {
-        const int len = p.len;
-        const int32_t *table = plan.pages + size_t(p.seq) * plan.page_stride;
-        const int last = max(len - 1, 0) >> a.page_shift;
-        // page ids of 32 pages at a time; past the end the last page stands in
-        int base = -64, id = 0;
+    Walker walk(a.walk, int(blockIdx.x), kGran);
+    // Page ids, 32 at a time; past the sequence's end its last page stands in.  The
+    // first of the next tile are loaded while this one is.
+    auto ids = [&](const Piece &p, int base) {
+        const int last = max(p.len - 1, 0) >> a.page_shift;
+        return p.len > 0 ? plan.pages[size_t(p.seq) * plan.page_stride + min(base + lane, last)] : 0;
+    };
+    auto checked = [&](const Piece &p, int base, int id) {
+        if (uint32_t(id) >= uint32_t(a.pages)) {
+            if (base + lane <= min(max(p.len - 1, 0), p.k1 - 1) >> a.page_shift) {
+                set_status(a.status, kKvBadPage);
+            }
+            return 0;
+        }
+        return id;
+    };
+    Piece p, ahead;
+    bool any = walk.next(p), more = false;
+    int first_ids = any ? ids(p, p.k0 >> a.page_shift) : 0;
+    for (; any; any = more, p = ahead) {
+        int base = p.k0 >> a.page_shift, id = checked(p, base, first_ids);
+        more = walk.next(ahead);
+        first_ids = more ? ids(ahead, ahead.k0 >> a.page_shift) : 0;
         for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
-            const int first = k0 >> a.page_shift;
-            const int need = (k0 + kGran - 1) >> a.page_shift;
-            if (need >= base + 32) {
-                base = first;
-                id = len > 0 ? table[min(base + lane, last)] : 0;
-                if (uint32_t(id) >= uint32_t(a.pages)) {
-                    if (base + lane <= last && base + lane <= ((p.k1 - 1) >> a.page_shift)) {
-                        set_status(a.status, kKvBadPage);
-                    }
-                    id = 0;
-                }
+            if (((k0 + kGran - 1) >> a.page_shift) >= base + 32) {
+                base = k0 >> a.page_shift;
+                id = checked(p, base, ids(p, base));
             }
             const bool free = wait_or_abort(&sm.empty[stage], phase ^ 1, &sm.abort, a.status);
             if (__all_sync(0xffffffffu, free)) {
@@ -249,12 +259,6 @@ __global__ void __launch_bounds__(kThreads)
     constexpr int kMTiles = D / 16;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Plan &plan = *a.walk.plan;
-    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kCols || a.walk.list->gran != T::kGran) {
-        if (tid == 0) {
-            set_status(a.status, kKvStalePlan);
-        }
-        return;
-    }
     if (tid == 0) {
         for (int i = 0; i < T::kStages; ++i) {
             tc::mbar_init(&sm.full[i], 1);
@@ -264,6 +268,13 @@ __global__ void __launch_bounds__(kThreads)
         tc::fence_mbar_init();
     }
     __syncthreads();
+    wait_previous();
+    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kCols || a.walk.list->gran != T::kGran) {
+        if (tid == 0) {
+            set_status(a.status, kKvStalePlan);
+        }
+        return;
+    }
     if (warp == kWarps) {
         load_granules<Smem, kCache, D, T::kGran, T::kStages, T::kStageBytes>(a, plan, &map, sm);
         return;
@@ -280,42 +291,61 @@ __global__ void __launch_bounds__(kThreads)
     constexpr float kLift = kMma != kF16 ? 0.0f : (kCache == kMxfp4 ? 9.0f : 11.0f);
     int stage = 0;
     uint32_t phase = 0;
-    Walker walk(a.walk, int(blockIdx.x));
-    Piece p;
-    while (walk.next(p)) {
-        // ---- the columns ----
-        if (tid < kCols) {
-            int4 ri = make_int4(0, 0, 1 << 30, -1);  // a column past the tile: all keys, so that it asks for no mask
-            float slope = 0.0f;
-            if (tid < p.ncols) {
-                const int cc = p.col0 + tid, r = cc / a.group;
-                ri = a.walk.row[p.row0 + r];
-                slope = a.slopes ? a.slopes[p.head * a.group + cc - r * a.group] * kLog2e : 0.0f;
-                ri.y = max(ri.y, 0), ri.z = min(ri.z, p.len);
-            }
-            sm.pos[tid] = ri.x, sm.lo[tid] = ri.y, sm.hi[tid] = ri.z;
-            sm.slope[tid] = slope;
+    Walker walk(a.walk, int(blockIdx.x), T::kGran);
+    // copies a tile's Q rows, and the rest of its columns to side `to`, asynchronously
+    auto fetch = [&](const Piece &p, int to) {
+        for (int i = tid; i < kCols * (D / 8); i += 32 * kWarps) {
+            const int c = i / (D / 8), d = 8 * (i - c * (D / 8));
+            const int cc = p.col0 + c, r = cc / a.group, row = p.row0 + r;
+            const bool have = c < p.ncols && row < a.rows;
+            const uint16_t *src = static_cast<const uint16_t *>(a.q) +
+                                  (have ? size_t(row) * a.q_stride + size_t(p.head * a.group + cc - r * a.group) * D + d : 0);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(&sm.q[c][d])), "l"(src), "r"(have ? 16 : 0)
+                         : "memory");
         }
+        if (tid < kCols) {
+            if (tid < p.ncols) {
+                const int cc = p.col0 + tid, r = cc / a.group, qhead = p.head * a.group + cc - r * a.group;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(&sm.row[to][tid])), "l"(a.walk.row + p.row0 + r) : "memory");
+                if (a.slopes) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(&sm.slope[to][tid])), "l"(a.slopes + qhead) : "memory");
+                }
+                if (a.sinks) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(&sm.sink[to][tid])), "l"(a.sinks + qhead) : "memory");
+                }
+            } else {
+                sm.row[to][tid] = make_int4(0, 0, 1 << 30, -1);  // past the tile: all keys, so that it asks for no mask
+                sm.slope[to][tid] = sm.sink[to][tid] = 0.0f;
+            }
+        }
+    };
+    Piece p, ahead;
+    bool any = walk.next(p), more = false;
+    if (any) {
+        fetch(p, 0);
+    }
+    for (int side = 0; any; any = more, p = ahead, side ^= 1) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        consumer_sync();
+        more = walk.next(ahead);
         uint32_t q[NT][D / 16][2];
+        float scale[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int c = 8 * n + g;
-            const int cc = p.col0 + c, r = cc / a.group, row = p.row0 + r;
-            const bool have = c < p.ncols && row < a.rows;
-            const uint16_t *src = static_cast<const uint16_t *>(a.q) + size_t(row) * a.q_stride +
-                                  size_t(p.head * a.group + cc - r * a.group) * D;
+            const uint16_t *src = sm.q[c];
             if constexpr (kCache != kMxfp4) {
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s) {
-                    q[n][s][0] = have ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * t) : 0u;
-                    q[n][s][1] = have ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * t) : 0u;
+                    q[n][s][0] = *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * t);
+                    q[n][s][1] = *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * t);
                 }
             } else {
                 // values 8t .. 8t + 7 of each block of 32, as the codes' words lie
                 uint4 w[kBlocks];
 #pragma unroll
                 for (int b = 0; b < kBlocks; ++b) {
-                    w[b] = have ? *reinterpret_cast<const uint4 *>(src + 32 * b + 8 * t) : make_uint4(0, 0, 0, 0);
+                    w[b] = *reinterpret_cast<const uint4 *>(src + 32 * b + 8 * t);
                 }
                 float unscale = 1.0f;
                 if constexpr (kRows == kBf16) {
@@ -346,8 +376,10 @@ __global__ void __launch_bounds__(kThreads)
                         w[b] = make_uint4(u[0], u[1], u[2], u[3]);
                     }
                 }
-                if (t == 0 && warp == 0) {
-                    sm.scale[c] = a.scale * kLog2e * unscale;
+                // the column's factor, from the lane that holds it to those that hold its scores
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    scale[n][j] = __shfl_sync(0xffffffffu, a.scale * kLog2e * unscale, 4 * (2 * t + j));
                 }
 #pragma unroll
                 for (int b = 0; b < kBlocks; ++b) {
@@ -356,25 +388,29 @@ __global__ void __launch_bounds__(kThreads)
                 }
             }
         }
-        consumer_sync();
+        consumer_sync();  // every warp has its Q: the next tile's may come
+        if (more) {
+            fetch(ahead, side ^ 1);
+        }
         // lowest and highest borders over the columns
         int lo_min, lo_max, hi_min, hi_max;
         {
-            const int l = lane < kCols ? sm.lo[lane] : 0, h = lane < kCols ? sm.hi[lane] : 0;
+            const int4 ri = sm.row[side][min(lane, kCols - 1)];
+            const int l = max(ri.y, 0), h = min(ri.z, p.len);
             const bool real = lane < p.ncols;
             lo_max = __reduce_max_sync(0xffffffffu, real ? l : 0);
             hi_min = __reduce_min_sync(0xffffffffu, real ? h : 1 << 30);
             lo_min = __reduce_min_sync(0xffffffffu, real && l < h ? l : 1 << 30);
             hi_max = __reduce_max_sync(0xffffffffu, real && l < h ? h : 0);
         }
-        float scale[NT][2], m[NT][2], l[NT][2];
+        float m[NT][2], l[NT][2];
         float o[NT][kMTiles][4];
         float unit[kCache == kMxfp4 ? NT : 1][2][kBlocks];  // 4 bits: 1 / the scale that o is in units of
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                scale[n][c] = kCache == kMxfp4 ? sm.scale[8 * n + 2 * t + c] : a.scale * kLog2e;
+                scale[n][c] = kCache == kMxfp4 ? scale[n][c] : a.scale * kLog2e;
                 m[n][c] = -INFINITY, l[n][c] = 0.0f;
                 if constexpr (kCache == kMxfp4) {
 #pragma unroll
@@ -499,7 +535,7 @@ __global__ void __launch_bounds__(kThreads)
                                 const int c = 8 * n + 2 * t + (j & 1), key = key0 + 16 * u + g + (j >> 1) * 8;
                                 const float f = scale[n][j & 1];
                                 const float x = cap_log2 != 0.0f ? capped(s[u][n][j], f * two_over_cap, cap_log2) : s[u][n][j] * f;
-                                s[u][n][j] = fmaf(-sm.slope[c], float(abs(sm.pos[c] - key)), x);
+                                s[u][n][j] = a.slopes ? fmaf(-kLog2e * sm.slope[side][c], float(abs(sm.row[side][c].x - key)), x) : x;
                             }
                         }
                     }
@@ -512,7 +548,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const int c = 8 * n + 2 * t + (j & 1), key = key0 + 16 * u + g + (j >> 1) * 8;
-                                s[u][n][j] = key >= sm.lo[c] && key < sm.hi[c] ? s[u][n][j] : -INFINITY;
+                                const int4 ri = sm.row[side][c];
+                                s[u][n][j] = key >= ri.y && key < ri.z ? s[u][n][j] : -INFINITY;
                             }
                         }
                     }
@@ -724,7 +761,10 @@ __global__ void __launch_bounds__(kThreads)
             }
         };
         if (p.first == p.last) {
-            store_columns<kRows, kCache, D>(a, plan, p, warp, kWarps, value, stats);
+            store_columns<kRows, kCache, D>(a, plan, p, warp, kWarps, value, stats, [&](int c, int, int) {
+                const int4 ri = sm.row[side][c];
+                return ColumnInfo{ri.y, ri.z, ri.w, sm.sink[side][c]};
+            });
         } else {
             float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * kCols * (D + 2);
             for (int i = tid; i < p.ncols * (D / 8); i += 32 * kWarps) {
@@ -748,9 +788,8 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <int kRows, int kCache, int D, int NT> cudaError_t launch_nt(const ttl_kv &h, const AttendArgs &a, int layer) {
-    kv_attend_tokens_kernel<kRows, kCache, D, NT>
-        <<<h.ctas[0], kThreads, sizeof(TokenSmem<kRows, kCache, D, NT>), h.stream>>>(a, h.maps[size_t(layer)]);
-    return cudaGetLastError();
+    return launch_chained(kv_attend_tokens_kernel<kRows, kCache, D, NT>, h.ctas[0], kThreads,
+                          sizeof(TokenSmem<kRows, kCache, D, NT>), h.stream, a, h.maps[size_t(layer)]);
 }
 
 template <int kRows, int kCache, int D> cudaError_t launch(const ttl_kv &h, const AttendArgs &a, int layer) {

@@ -532,8 +532,12 @@ class KvCache:
         self.h = h
         self.rows_type, self.cache_type = rows, cache or rows
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
-        self._dtype = {"f32": "torch.float32", "f16": "torch.float16", "bf16": "torch.bfloat16"}[rows]
+        import torch
+        self._dtype = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[rows]
+        self._i32, self._f32 = torch.int32, torch.float32
         self._rows = 0
+        L = lib()
+        self._calls = (L.ttl_kv_batch_async, L.ttl_kv_append_async, L.ttl_kv_read_async, L.ttl_kv_attend_async)
 
     def _check(self, rc):
         if rc != TTL_OK:
@@ -562,35 +566,40 @@ class KvCache:
         """Address of an optional contiguous tensor of the given type and shape."""
         if t is None:
             return None
-        if str(t.dtype) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        if t.dtype is not dtype or tuple(t.shape) != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
         return t.data_ptr()
 
     def _row_array(self, t, name, heads):
         """(address, row stride) of [rows, heads, head_dim] rows, each contiguous."""
-        shape, stride = t.shape, t.stride()
         d = self.head_dim
-        if str(t.dtype) != self._dtype or len(shape) != 3 or shape[0] < self._rows or shape[1] != heads or shape[2] != d:
+        if t.dtype is not self._dtype or t.dim() != 3:
             raise ValueError(f"{name} must be a {self._dtype} tensor [{self._rows} rows, {heads}, {d}]")
-        if stride[2] != 1 or (stride[1] != d and heads > 1):
+        n, h, e = t.shape
+        if n < self._rows or h != heads or e != d:
+            raise ValueError(f"{name} must be a {self._dtype} tensor [{self._rows} rows, {heads}, {d}]")
+        row, head, inner = t.stride()
+        if inner != 1 or (head != d and heads > 1):
             raise ValueError(f"{name}: the heads of a row must be contiguous")
-        return t.data_ptr(), stride[0] if shape[0] > 1 else max(stride[0], heads * d)
+        return t.data_ptr(), row if n > 1 else max(row, heads * d)
 
     def batch_async(self, row_start, length, pages, rows, max_new=None, first=None, prefix=None):
         """The batch of the next calls: int32 device tensors row_start
         [seqs + 1], length [seqs], pages [seqs, n], first [rows], prefix
         [seqs]; `rows` in all, at most `max_new` of one sequence (None: rows)."""
         seqs = length.shape[0]
-        i32 = "torch.int32"
-        if pages.dim() != 2 or str(pages.dtype) != i32 or pages.shape[0] < seqs or pages.stride(1) != 1:
+        i32 = self._i32
+        if pages.dim() != 2 or pages.dtype is not i32 or pages.shape[0] < seqs or pages.stride(1) != 1:
             raise ValueError("pages must be an int32 tensor [seqs, n] with contiguous rows")
         stride = pages.stride(0) if pages.shape[0] > 1 else pages.shape[1]
         if stride != pages.shape[1]:
             raise ValueError("pages must be contiguous")
-        self._check(lib().ttl_kv_batch_async(
+        rc = self._calls[0](
             self.h, seqs, rows, rows if max_new is None else max_new, self._array(row_start, "row_start", i32, (seqs + 1,)),
             self._array(length, "length", i32, (seqs,)), pages.data_ptr(), stride,
-            self._array(first, "first", i32, (rows,)), self._array(prefix, "prefix", i32, (seqs,))))
+            self._array(first, "first", i32, (rows,)), self._array(prefix, "prefix", i32, (seqs,)))
+        if rc:
+            self._check(rc)
         self._rows = rows
         self._kept = (row_start, length, pages, first, prefix)  # the batch's arrays live until the next batch
 
@@ -604,22 +613,28 @@ class KvCache:
             qp, qs = self._row_array(q, "q", self.q_heads)
         if q_out is not None:
             op, os_ = self._row_array(q_out, "q_out", self.q_heads)
-        self._check(lib().ttl_kv_append_async(self.h, layer, 1 if rotate else 0, kp, ks, vp, vs, qp, qs, op, os_))
+        rc = self._calls[1](self.h, layer, 1 if rotate else 0, kp, ks, vp, vs, qp, qs, op, os_)
+        if rc:
+            self._check(rc)
 
     def read_async(self, layer, k, v):
         """The batch's rows of K and V as the cache holds them."""
         kp, ks = self._row_array(k, "k", self.kv_heads)
         vp, vs = self._row_array(v, "v", self.kv_heads)
-        self._check(lib().ttl_kv_read_async(self.h, layer, kp, ks, vp, vs))
+        rc = self._calls[2](self.h, layer, kp, ks, vp, vs)
+        if rc:
+            self._check(rc)
 
     def attend_async(self, layer, q, out, scale=0.0, cap=0.0, sinks=None, slopes=None, sliding=False):
         """out = attention of the (rotated) Q rows over the layer's cache."""
         qp, qs = self._row_array(q, "q", self.q_heads)
         op, os_ = self._row_array(out, "out", self.q_heads)
-        self._check(lib().ttl_kv_attend_async(
+        rc = self._calls[3](
             self.h, layer, KV_SLIDING if sliding else 0, qp, qs, op, os_, scale or 0.0, cap,
-            self._array(sinks, "sinks", "torch.float32", (self.q_heads,)),
-            self._array(slopes, "slopes", "torch.float32", (self.q_heads,))))
+            self._array(sinks, "sinks", self._f32, (self.q_heads,)),
+            self._array(slopes, "slopes", self._f32, (self.q_heads,)))
+        if rc:
+            self._check(rc)
 
     def page_bytes(self) -> int:
         return lib().ttl_kv_page_bytes(self.h)
