@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace ttl {
 namespace kv {
@@ -74,7 +75,7 @@ struct AttendArgs {
     void *out;
     size_t q_stride, out_stride;   // elements
     const float *sinks, *slopes;
-    float *part;                   // [2 * ctas][width][D + 2]
+    float *part;                   // [2 * ctas][width][part_pitch(D)]
     uint32_t *counters;            // [ctas]
     uint32_t *status;
     float scale, cap;              // natural units; cap 0: none
@@ -148,6 +149,25 @@ template <int kRows> __device__ __forceinline__ void store8(void *base, size_t i
             }
         }
         *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+// Four values (on their size).
+template <int kRows> __device__ __forceinline__ void store4(void *base, size_t i, const float (&v)[4]) {
+    if constexpr (kRows == kF32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(base) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        uint32_t w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if constexpr (kRows == kF16) {
+                const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(base) + i) = make_uint2(w[0], w[1]);
     }
 }
 template <int kRows> __device__ __forceinline__ void load8(const void *base, size_t i, float (&v)[8]) {
@@ -267,6 +287,46 @@ struct Walker {
         return true;
     }
 };
+
+// Waits for a phase of a barrier unless the CTA has given up; a wait of about two
+// seconds gives the CTA up (every later wait returns at once, so that all warps
+// still meet at their barriers and leave).  kSleep lets the hardware put the
+// warp to sleep for up to a millisecond a try.  It pays where other warps of the
+// scheduler compute meanwhile.
+constexpr long long kWaitClocks = 4000000000ll;
+
+template <bool kSleep> __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *status) {
+    const uint32_t addr = tc::smem_u32(bar);
+    long long start = 0;
+    while (true) {
+        uint32_t ok;
+        if constexpr (kSleep) {
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok)
+                : "r"(addr), "r"(parity), "r"(1000000u)
+                : "memory");
+        } else {
+            ok = tc::mbar_try_wait(bar, parity);
+        }
+        if (ok) {
+            return true;
+        }
+        if (*abort) {
+            return false;
+        }
+        const long long now = clock64();
+        if (start == 0) {
+            start = now;
+        } else if (now - start > kWaitClocks) {
+            set_status(status, kKvWait);
+            *abort = 1;
+            return false;
+        }
+    }
+}
 
 // Programmatic dependent launch: lets the next kernel on the stream start, and
 // waits for what ran before this one.  Every kernel of the cache waits before it
@@ -405,128 +465,95 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
     }
 }
 
-// Merges the partial results of a tile over the CTAs [first, last] that hold
-// them and stores its columns.  part: [slot][width][D + 2] with {max, sum}
-// after the D sums.  Few parts: D / 8 lanes per column as in store_columns.
-// Many (a long sequence): a warp per column, a lane per part for the maxima and
-// sums and four values a lane for the values, so that the loads of many parts
-// are in flight together.
-constexpr int kFewParts = 6;
+// Partial results: [slot][width][part_pitch(D)] floats, a column's D sums, then
+// its maximum and sum; rows of a multiple of 16 bytes.
+__host__ __device__ constexpr int part_pitch(int d) {
+    return d + 4;
+}
 
+// Merges the partial results of a tile over the CTAs [first, last] that hold
+// them, in that order, and stores its columns: D / 4 lanes per column.  The
+// parts come from other SMs through L2, about a microsecond each way, so what
+// counts is how many are asked for at once: eight parts' sums and statistics
+// per lane (one token over 131072 keys, 55 parts per head: two parts at a time
+// cost 20 us).
 template <int kRows, int kCache, int D>
 __device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps, int width) {
-    const size_t pitch = D + 2;
+    constexpr int kLanes = D / 4, kCols = 32 / kLanes, kBatch = 8;
+    const int lane = threadIdx.x & 31, sub = lane / kLanes, d = 4 * (lane % kLanes);
     const int parts = p.last - p.first + 1;
-    if (parts > kFewParts) {
-        const int lane = threadIdx.x & 31;
-        constexpr int kSplit = 128 / D;  // parts that a warp reads at once
-        const int d = 4 * (lane % (D / 4)), sub = lane / (D / 4);
-        for (int c = warp; c < p.ncols; c += warps) {
-            const int cc = p.col0 + c, i = cc / a.group;
-            const int qhead = p.head * a.group + cc - i * a.group, row = p.row0 + i;
-            const int4 ri = a.walk.row[row];
-            const float *col = a.part + size_t(c) * pitch;
-            auto slot = [&](int k) { return col + size_t(part_slot(p.first + k, p.first)) * width * pitch; };
-            float m = -INFINITY;
-            for (int k = lane; k < parts; k += 32) {
+    for (int base = warp * kCols; base < p.ncols; base += warps * kCols) {
+        const int c = min(base + sub, p.ncols - 1);
+        const bool have = base + sub < p.ncols;
+        const int cc = p.col0 + c, i = cc / a.group;
+        const int qhead = p.head * a.group + cc - i * a.group, row = p.row0 + i;
+        const ColumnInfo ci = column_info(a, row, qhead);
+        const float *col = a.part + size_t(c) * part_pitch(D);
+        auto slot = [&](int k) { return col + size_t(part_slot(p.first + k, p.first)) * width * part_pitch(D); };
+        float m = -INFINITY;
+        if (parts > kBatch) {
+            for (int k = lane % kLanes; k < parts; k += kLanes) {
                 m = fmaxf(m, __ldcg(slot(k) + D));
             }
 #pragma unroll
-            for (int off = 16; off; off >>= 1) {
+            for (int off = kLanes / 2; off; off >>= 1) {
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
             }
+        }
+        float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k0 = 0; k0 < parts; k0 += kBatch) {
+            float2 ml[kBatch];
+            float4 x[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                if (k0 + k < parts) {
+                    ml[k] = __ldcg(reinterpret_cast<const float2 *>(slot(k0 + k) + D));
+                    x[k] = __ldcg(reinterpret_cast<const float4 *>(slot(k0 + k) + d));
+                }
+            }
+            if (parts <= kBatch) {
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    m = k < parts ? fmaxf(m, ml[k].x) : m;
+                }
+            }
             const float safe = m == -INFINITY ? 0.0f : m;
-            float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int base = 0; base < parts; base += 32) {
-                float f = 0.0f;
-                if (base + lane < parts) {
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(base + lane) + D));
-                    f = exp2f(ml.x - safe);
-                    l = fmaf(ml.y, f, l);
-                }
-                const int count = min(32, parts - base);
-#pragma unroll 8
-                for (int k = 0; k < count; k += kSplit) {
-                    const int mine = k + sub;
-                    const float w = __shfl_sync(0xffffffffu, f, mine & 31);
-                    if (mine < count) {
-                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(slot(base + mine) + d));
-                        const float2 y = __ldcg(reinterpret_cast<const float2 *>(slot(base + mine) + d + 2));
-                        o[0] = fmaf(x.x, w, o[0]), o[1] = fmaf(x.y, w, o[1]);
-                        o[2] = fmaf(y.x, w, o[2]), o[3] = fmaf(y.y, w, o[3]);
-                    }
-                }
-            }
-            l = warp_sum(l);
-            if constexpr (kSplit == 2) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    o[j] += __shfl_xor_sync(0xffffffffu, o[j], 16);
+            for (int k = 0; k < kBatch; ++k) {
+                if (k0 + k < parts) {
+                    const float w = exp2f(ml[k].x - safe);
+                    l = fmaf(ml[k].y, w, l);
+                    o[0] = fmaf(x[k].x, w, o[0]), o[1] = fmaf(x[k].y, w, o[1]);
+                    o[2] = fmaf(x[k].z, w, o[2]), o[3] = fmaf(x[k].w, w, o[3]);
                 }
-            }
-            float f = 1.0f;
-            if (a.sinks) {
-                const float sink = a.sinks[qhead] * kLog2e, mn = fmaxf(m, sink), s = mn == -INFINITY ? 0.0f : mn;
-                f = exp2f(m - s);
-                l = l * f + exp2f(sink - s);
-            }
-            f = f / l;
-            const bool sees = max(ri.y, 0) < min(ri.z, p.len), write = row < a.rows && ri.w == p.seq;
-            bool bad = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                o[j] = sees ? o[j] * f : 0.0f;
-                bad = bad || !(fabsf(o[j]) < INFINITY);
-            }
-            if (write && sub == 0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    store_value<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + d + j, o[j]);
-                }
-            }
-            if (write && __any_sync(0xffffffffu, bad)) {
-                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, row, qhead);
             }
         }
-        return;
+        float f = 1.0f;
+        if (a.sinks) {
+            const float sink = ci.sink * kLog2e, mn = fmaxf(m, sink), s = mn == -INFINITY ? 0.0f : mn;
+            f = exp2f(m - s);
+            l = l * f + exp2f(sink - s);
+        }
+        f = f / l;
+        const bool sees = max(ci.lo, 0) < min(ci.hi, p.len), write = have && row < a.rows && ci.seq == p.seq;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[j] = sees ? o[j] * f : 0.0f;
+            bad = bad || !(fabsf(o[j]) < INFINITY);
+        }
+        if (write) {
+            store4<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + d, o);
+        }
+        const uint32_t redo = __ballot_sync(0xffffffffu, bad && write);
+#pragma unroll
+        for (int s = 0; s < kCols; ++s) {
+            if (redo & ((kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1u) << (s * kLanes))) {
+                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, __shfl_sync(0xffffffffu, row, s * kLanes),
+                                                __shfl_sync(0xffffffffu, qhead, s * kLanes));
+            }
+        }
     }
-    store_columns<kRows, kCache, D>(
-        a, plan, p, warp, warps,
-        [&](int c, int d, float(&v)[8]) {
-            float m = -INFINITY;
-            for (int k = p.first; k <= p.last; ++k) {
-                m = fmaxf(m, __ldcg(a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch + D));
-            }
-            const float safe = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = 0.0f;
-            }
-            for (int k = p.first; k <= p.last; ++k) {
-                const float *src = a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch;
-                const float f = exp2f(__ldcg(src + D) - safe);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 x = __ldcg(reinterpret_cast<const float2 *>(src + d) + j);
-                    v[2 * j] = fmaf(x.x, f, v[2 * j]);
-                    v[2 * j + 1] = fmaf(x.y, f, v[2 * j + 1]);
-                }
-            }
-        },
-        [&](int c) {
-            float m = -INFINITY;
-            for (int k = p.first; k <= p.last; ++k) {
-                m = fmaxf(m, __ldcg(a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch + D));
-            }
-            const float safe = m == -INFINITY ? 0.0f : m;
-            float l = 0.0f;
-            for (int k = p.first; k <= p.last; ++k) {
-                const float *src = a.part + (size_t(part_slot(k, p.first)) * width + c) * pitch + D;
-                l = fmaf(__ldcg(src + 1), exp2f(__ldcg(src) - safe), l);
-            }
-            return make_float2(m, l);
-        },
-        [&](int, int row, int qhead) { return column_info(a, row, qhead); });
 }
 
 // After a CTA wrote its partial result of a tile: counts it, and returns true

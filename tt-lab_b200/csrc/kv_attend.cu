@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
                 [&](int c) { return make_float2(sm.m[c], sm.l[c]); },
                 [&](int, int row, int qhead) { return column_info(a, row, qhead); });
         } else {
-            float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * CT * (D + 2);
-            for (int i = tid; i < p.ncols * (D + 2); i += kSimpleThreads) {
-                const int c = i / (D + 2), d = i - c * (D + 2);
+            float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * CT * part_pitch(D);
+            for (int i = tid; i < p.ncols * part_pitch(D); i += kSimpleThreads) {
+                const int c = i / part_pitch(D), d = i - c * part_pitch(D);
                 part[i] = d < D ? sum[c * D + d] : (d == D ? sm.m[c] : sm.l[c]);
             }
             if (arrive_last(a, p, &sm.last, [] { __syncthreads(); })) {
@@ -301,7 +301,7 @@ size_t kv_part_floats(const ttl_kv &h) {
     for (int i = 0; i < 3; ++i) {
         most = std::max(most, size_t(h.token_ctas[i]) * (8 << i));
     }
-    return 2 * most * (h.dim + 2);
+    return 2 * most * part_pitch(h.dim);
 }
 
 cudaError_t kv_configure(ttl_kv &h) {

@@ -34,18 +34,19 @@ namespace {
 
 constexpr int kGran = 128;
 constexpr int kHalf = 128;                 // columns of a warpgroup
+constexpr int kKeys = 64;                  // keys of a step: half a granule
 constexpr int kLoader = 8, kIssuer = 9;    // warps
 constexpr int kExpander = 12;              // first of the four warps that expand a 4-bit cache
 constexpr uint32_t kTmemCols = 512;
 
 // Threads, and registers of the softmax warpgroups, of the loader's and of the
 // expanders': a warpgroup may only take what the launch holds (168 or 128 a
-// thread), 256 * 208 + 128 * 80 <= 384 * 168 and 256 * 168 + 128 * 64 + 128 * 104
+// thread), 256 * 208 + 128 * 80 <= 384 * 168 and 256 * 176 + 128 * 64 + 128 * 96
 // <= 512 * 128.
 template <int kCache> struct PromptShape {
     static constexpr bool kFour = kCache == kMxfp4;
     static constexpr int kThreads = kFour ? 512 : 384;
-    static constexpr int kSoftmaxRegs = kFour ? 168 : 208, kOtherRegs = kFour ? 64 : 80, kExpandRegs = 104;
+    static constexpr int kSoftmaxRegs = kFour ? 176 : 208, kOtherRegs = kFour ? 64 : 80, kExpandRegs = 96;
     static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs + (kFour ? 128 * kExpandRegs : 0) <= kThreads * (kFour ? 128 : 168), "registers");
 };
 
@@ -58,25 +59,10 @@ template <int kCache, int D> struct PromptSmem {
     alignas(16) uint8_t raw[2][kRawBytes];
     uint64_t raw_full[2], raw_empty[2];
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [warpgroup][half of a granule]
     uint32_t tmem;
     int last, abort;
 };
-
-__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *status) {
-    if (tc::mbar_try_wait(bar, parity)) {
-        return true;
-    }
-    if (*abort) {
-        return false;
-    }
-    if (!tc::mbar_wait(bar, parity)) {
-        set_status(status, kKvWait);
-        *abort = 1;
-        return false;
-    }
-    return true;
-}
 
 __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
@@ -96,19 +82,35 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
     return uint64_t((saddr >> 4) & 0x3FFFu) | uint64_t((lbo >> 4) & 0x3FFFu) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 |
            uint64_t(2) << 61;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// Issued by the lane with `lead` set, the operands alike in all lanes of the warp:
+// so the compiler can keep them in uniform registers, which the instruction
+// takes.  (Code of one thread that has left its warp costs about 120 clocks per
+// instruction, twice what the tensor pipe needs for it.)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(lead)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(lead)
         : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc::smem_u32(bar)),
+        "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(lead));
+    return lead;
 }
 
 #define KV_R8(a, i) "=f"(a[i]), "=f"(a[i + 1]), "=f"(a[i + 2]), "=f"(a[i + 3]), "=f"(a[i + 4]), "=f"(a[i + 5]), "=f"(a[i + 6]), "=f"(a[i + 7])
@@ -173,7 +175,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
             const int key = k0 + (lane < copies ? s : 0) * seg;
             const int page = __shfl_sync(0xffffffffu, id, (key >> a.page_shift) - base);
             if constexpr (kCache == kMxfp4) {
-                const bool ok = wait_or_abort(&sm.raw_empty[stage], phase ^ 1, &sm.abort, a.status);
+                const bool ok = wait_or_abort<true>(&sm.raw_empty[stage], phase ^ 1, &sm.abort, a.status);
                 if (__all_sync(0xffffffffu, ok)) {
                     if (lane == 0) {
                         tc::mbar_expect_tx(&sm.raw_full[stage], PromptSmem<kCache, D>::kRawBytes);
@@ -195,7 +197,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
             }
             const int y = ((page * a.kv_heads + p.head) * 2) * (1 << a.page_shift) + (key & ((1 << a.page_shift) - 1));
             const uint32_t to = uint32_t(x * kGran + s * seg) * 128;
-            bool ok = wait_or_abort(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
+            bool ok = wait_or_abort<true>(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
             if (__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.k_full[stage], kGran * D * 2);
@@ -205,7 +207,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                     tc::tma_load_2d(sm.k[stage] + to, map, 64 * x, y, &sm.k_full[stage]);
                 }
             }
-            ok = wait_or_abort(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
+            ok = wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
             if (__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.v_full[stage], kGran * D * 2);
@@ -258,11 +260,11 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
     Piece p;
     while (walk.next(p)) {
         for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
-            wait_or_abort(&sm.raw_full[raw], raw_phase, &sm.abort, a.status);
-            wait_or_abort(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
+            wait_or_abort<true>(&sm.raw_full[raw], raw_phase, &sm.abort, a.status);
+            wait_or_abort<true>(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
             half(sm.raw[raw] + at, sm.k[stage]);
             arrive(&sm.k_full[stage]);
-            wait_or_abort(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
+            wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
             half(sm.raw[raw] + at + (a.block_bytes >> 1), sm.v[stage]);
             arrive(&sm.v_full[stage]);
             arrive(&sm.raw_empty[raw]);
@@ -276,76 +278,93 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
     }
 }
 
-// The matrix instructions, from one thread.
+// The matrix instructions: a warp, one lane of which issues them.
 template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(const AttendArgs &a, PromptSmem<kCache, D> &sm, uint32_t tmem) {
     constexpr int kStages = PromptSmem<kCache, D>::kStages;
-    constexpr uint32_t kSDesc = f16_desc<kRows>(kGran, false), kODesc = f16_desc<kRows>(D, true);
-    const uint32_t s_at[2] = {tmem, tmem + 128}, o_at[2] = {tmem + 256, tmem + 256 + D};
+    constexpr uint32_t kSDesc = f16_desc<kRows>(kKeys, false), kODesc = f16_desc<kRows>(D, true);
+    constexpr uint32_t kTileBytes = kGran * D * 2;
+    const uint32_t lead = elected();
+    // descriptors of the first Q, K and V; offsets go to their low bits in units of 16 bytes
+    const uint64_t q_desc = tc::smem_desc_sw128(tc::smem_u32(sm.q[0])), k_desc = tc::smem_desc_sw128(tc::smem_u32(sm.k[0])),
+                   v_desc = desc_mn(tc::smem_u32(sm.v[0]), kGran * 128);
     int ks = 0, vs = 0;
-    uint32_t k_phase = 0, v_phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-    auto scores = [&](int w) {
-        const uint32_t q = tc::smem_u32(sm.q[w]), k = tc::smem_u32(sm.k[ks]);
+    uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;  // q: bit w; p: bit 2 h + w
+    auto scores = [&](int w, int h) {
+        const uint64_t q = q_desc + uint64_t(uint32_t(w) * (kHalf * D * 2) >> 4), k = k_desc + uint64_t((uint32_t(ks) * kTileBytes + h * kKeys * 128) >> 4);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-            const uint32_t off = uint32_t(i / 4) * 128 * 128 + uint32_t(i % 4) * 32;
-            mma_ss(s_at[w], tc::smem_desc_sw128(q + off), tc::smem_desc_sw128(k + off), kSDesc, i > 0);
+            const uint64_t off = (uint32_t(i / 4) * 128 * 128 + uint32_t(i % 4) * 32) >> 4;
+            mma_ss(tmem + 128 * w + h * kKeys, q + off, k + off, kSDesc, i > 0, lead);
         }
-        tc::mma_commit(&sm.s_full[w]);
+        commit(&sm.s_full[w][h], lead);
     };
-    Walker walk(a.walk, int(blockIdx.x), kGran);
-    Piece p, ahead;
-    bool any = walk.next(p), more;
-    for (; any; any = more, p = ahead) {
-        more = walk.next(ahead);
-        const int n = (p.k1 - p.k0) / kGran, halves = p.ncols > kHalf ? 2 : 1;
-        wait_or_abort(&sm.k_full[ks], k_phase, &sm.abort, a.status);
-        for (int w = 0; w < halves; ++w) {
-            wait_or_abort(&sm.q_full[w], q_phase[w], &sm.abort, a.status);
-            q_phase[w] ^= 1;
-            tc::fence_after_sync();
-            if (!*const_cast<volatile int *>(&sm.abort)) {
-                scores(w);
-            }
-        }
-        tc::mma_commit(&sm.k_empty[ks]);
+    auto next_k = [&] {
+        commit(&sm.k_empty[ks], lead);
         if (++ks == kStages) {
             ks = 0;
             k_phase ^= 1;
         }
-        for (int j = 0; j < n; ++j) {
-            wait_or_abort(&sm.v_full[vs], v_phase, &sm.abort, a.status);
-            const uint32_t v = tc::smem_u32(sm.v[vs]);
-            for (int w = 0; w < halves; ++w) {
-                wait_or_abort(&sm.p_full[w], p_phase[w], &sm.abort, a.status);
-                p_phase[w] ^= 1;
-                tc::fence_after_sync();
-                if (j + 1 < n && w == 0) {
-                    wait_or_abort(&sm.k_full[ks], k_phase, &sm.abort, a.status);
-                }
-                if (*const_cast<volatile int *>(&sm.abort)) {
-                    continue;
-                }
+    };
+    Walker walk(a.walk, int(blockIdx.x), kGran);
+    Piece p, ahead;
+    bool any = walk.next(p), more, ok = true;
+    for (; any; any = more, p = ahead) {
+        more = walk.next(ahead);
+        const int n = (p.k1 - p.k0) / kGran, halves = p.ncols > kHalf ? 2 : 1;
+        ok = wait_or_abort<true>(&sm.k_full[ks], k_phase, &sm.abort, a.status) && ok;
 #pragma unroll
-                for (int i = 0; i < kGran / 16; ++i) {
-                    mma_ts(o_at[w], s_at[w] + 8 * i, desc_mn(v + uint32_t(i) * 2048, kGran * 128), kODesc, j > 0 || i > 0);
-                }
-                if (j + 1 < n) {
-                    scores(w);
-                } else {
-                    tc::mma_commit(&sm.o_full[w]);
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                if (w < halves) {
+                    if (h == 0) {
+                        ok = wait_or_abort<true>(&sm.q_full[w], (q_phase >> w) & 1u, &sm.abort, a.status) && ok;
+                        q_phase ^= 1u << w;
+                        tc::fence_after_sync();
+                    }
+                    if (__all_sync(0xffffffffu, ok)) {
+                        scores(w, h);
+                    }
                 }
             }
-            tc::mma_commit(&sm.v_empty[vs]);
+        }
+        next_k();
+        for (int j = 0; j < n; ++j) {
+            ok = wait_or_abort<true>(&sm.v_full[vs], v_phase, &sm.abort, a.status) && ok;
+            if (j + 1 < n) {
+                ok = wait_or_abort<true>(&sm.k_full[ks], k_phase, &sm.abort, a.status) && ok;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint64_t v = v_desc + uint64_t((uint32_t(vs) * kTileBytes + h * kKeys * 128) >> 4);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (w < halves) {
+                        ok = wait_or_abort<true>(&sm.p_full[w][h], (p_phase >> (2 * h + w)) & 1u, &sm.abort, a.status) && ok;
+                        p_phase ^= 1u << (2 * h + w);
+                        tc::fence_after_sync();
+                        if (!__all_sync(0xffffffffu, ok)) {
+                            continue;
+                        }
+#pragma unroll
+                        for (int i = 0; i < kKeys / 16; ++i) {
+                            mma_ts(tmem + 256 + D * w, tmem + 128 * w + h * kKeys + 8 * i, v + uint64_t(i * 2048 >> 4), kODesc,
+                                   j > 0 || h > 0 || i > 0, lead);
+                        }
+                        commit(&sm.o_done[w][h], lead);
+                        if (j + 1 < n) {
+                            scores(w, h);
+                        }
+                    }
+                }
+            }
+            commit(&sm.v_empty[vs], lead);
             if (++vs == kStages) {
                 vs = 0;
                 v_phase ^= 1;
             }
             if (j + 1 < n) {
-                tc::mma_commit(&sm.k_empty[ks]);
-                if (++ks == kStages) {
-                    ks = 0;
-                    k_phase ^= 1;
-                }
+                next_k();
             }
         }
     }
@@ -361,9 +380,8 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
     constexpr float kLift = kRows == kF16 ? 11.0f : 0.0f;
     const float scale = a.scale * kLog2e, cap_log2 = a.cap * kLog2e;
     const float cap_in = a.cap != 0.0f ? scale * 2.0f / a.cap : 0.0f;
-    const float sign = scale < 0.0f ? -1.0f : 1.0f;  // the largest score is the smallest product where the scale is negative
     const bool special = a.cap != 0.0f || a.slopes;
-    uint32_t s_phase = 0, o_phase = 0;
+    uint32_t phase = 0;  // of the granule, for the barriers of both halves
     Walker walk(a.walk, int(blockIdx.x), kGran);
     // The tile after the one in hand is looked up while that one runs, and its Q
     // rows are copied as soon as the last scores of this one are there, so that
@@ -424,89 +442,88 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
         const int4 ri = cur.ri;
         const float slope = cur.slope;
         const bool sees = ri.y < ri.z;
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+        bool ok = true;  // no wait has run out
         if (!active && next.active) {
             copy_q(next);
             publish_q();
         }
         if (active) {
-            for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
-                const bool ok = wait_or_abort(&sm.s_full[w], s_phase, &sm.abort, a.status);
-                s_phase ^= 1;
+            int h = 0;
+            for (int k0 = p.k0; k0 < p.k1; k0 += kKeys, h ^= 1) {
+                const uint32_t now = phase;
+                phase ^= uint32_t(h);
+                ok = wait_or_abort<true>(&sm.s_full[w][h], now, &sm.abort, a.status);
                 if (!__all_sync(0xffffffffu, ok)) {
                     continue;
                 }
                 tc::fence_after_sync();
-                if (k0 + kGran >= p.k1 && next.active) {
+                if (k0 + kKeys >= p.k1 && next.active) {
                     copy_q(next);  // the last scores of this tile: its Q has been read
                 }
-                // ---- the maximum; scores that are capped, biased or masked go back as they then are ----
-                float f = scale, top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                const bool mask = __any_sync(0xffffffffu, k0 < ri.y || k0 + kGran > ri.z);
-                if (mask || special) {
+                const uint32_t at = s_at + kKeys * h;
+                float s[kKeys];
+                tmem_ld32(at, s);
+                tmem_ld32(at + 32, s + 32);
+                tc::wait_ld();
+                float f = scale;
+                if (special) {
                     f = 1.0f;
-                    const int from = ri.y - k0, to = ri.z - k0;
-#pragma unroll 1
-                    for (int i = 0; i < kGran; i += 32) {
-                        float s[32];
-                        tmem_ld32(s_at + i, s);
-                        tc::wait_ld();
-                        if (a.cap != 0.0f) {
+                    if (a.cap != 0.0f) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                s[j] = capped(s[j], cap_in, cap_log2);
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                s[j] *= scale;
-                            }
+                        for (int j = 0; j < kKeys; ++j) {
+                            s[j] = capped(s[j], cap_in, cap_log2);
                         }
-                        if (a.slopes) {
+                    } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                s[j] = fmaf(-slope, fabsf(float(ri.x - k0 - i - j)), s[j]);
-                            }
+                        for (int j = 0; j < kKeys; ++j) {
+                            s[j] *= scale;
                         }
-                        if (mask) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                s[j] = i + j >= from && i + j < to ? s[j] : -INFINITY;
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            top[j & 3] = fmaxf(top[j & 3], s[j]);
-                        }
-                        tmem_st32(s_at + i, s);
                     }
-                    tc::wait_st();
-                } else {
-                    float s[2][32];
-                    tmem_ld32(s_at, s[0]);
-                    tc::wait_ld();
+                    if (a.slopes) {
+                        const float away = float(ri.x - k0);
 #pragma unroll
-                    for (int i = 0; i < kGran / 32; ++i) {
-                        if (i + 1 < kGran / 32) {
-                            tmem_ld32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
+                        for (int j = 0; j < kKeys; ++j) {
+                            s[j] = fmaf(-slope, fabsf(away - float(j)), s[j]);
                         }
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            top[j & 3] = fmaxf(top[j & 3], s[i & 1][j] * sign);
-                        }
-                        tc::wait_ld();
                     }
                 }
-                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (f == 1.0f ? 1.0f : f * sign);
-                float s[2][32];
-                tmem_ld32(s_at, s[0]);
+                if (__any_sync(0xffffffffu, k0 < ri.y || k0 + kKeys > ri.z)) {
+                    const int from = ri.y - k0, to = ri.z - k0;
+#pragma unroll
+                    for (int j = 0; j < kKeys; ++j) {
+                        s[j] = j >= from && j < to ? s[j] : (f < 0.0f ? INFINITY : -INFINITY);  // f turns it
+                    }
+                }
+                // ---- the maximum ----
+                float top[4] = {s[0], s[1], s[2], s[3]};
+                if (f >= 0.0f) {
+#pragma unroll
+                    for (int j = 4; j < kKeys; ++j) {
+                        top[j & 3] = fmaxf(top[j & 3], s[j]);
+                    }
+                    top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                } else {
+#pragma unroll
+                    for (int j = 4; j < kKeys; ++j) {
+                        top[j & 3] = fminf(top[j & 3], s[j]);
+                    }
+                    top[0] = fminf(fminf(top[0], top[1]), fminf(top[2], top[3]));
+                }
+                const float most = f == 0.0f ? 0.0f : top[0] * f;
                 if (__any_sync(0xffffffffu, most > m + (kSlack + kLift))) {
                     const float mn = fmaxf(m, most - kLift);
                     const float up = ex2(m - (mn == -INFINITY ? 0.0f : mn));
                     m = mn;
-                    l *= up;
+                    l0 *= up, l1 *= up, l2 *= up, l3 *= up;
                     if (k0 != p.k0) {
-                        // the product before has ended: its scores came behind it
+                        // The product of the half before ends, and with it those before it:
+                        // rescale their sums.  (A barrier per half: the scores in hand came
+                        // behind this half's last product, so no barrier is ever more than
+                        // the one phase behind that its parity can tell.)
+                        wait_or_abort<true>(&sm.o_done[w][h ^ 1], now ^ uint32_t(h ^ 1), &sm.abort, a.status);
+                        __syncwarp();
+                        tc::fence_after_sync();
 #pragma unroll 1
                         for (int i = 0; i < D; i += 32) {
                             float o[32];
@@ -522,32 +539,21 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 }
                 // ---- the weights, over the scores ----
                 const float base = m == -INFINITY ? 0.0f : m;
-                float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
-                tc::wait_ld();
+                float pairs[kKeys / 2];  // of 16-bit weights
 #pragma unroll
-                for (int i = 0; i < kGran / 32; ++i) {
-                    if (i + 1 < kGran / 32) {
-                        tmem_ld32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
-                    }
-                    uint32_t w2[16];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float *x = s[i & 1] + j;
-                        const float p0 = ex2(fmaf(x[0], f, -base)), p1 = ex2(fmaf(x[1], f, -base));
-                        const float p2 = ex2(fmaf(x[2], f, -base)), p3 = ex2(fmaf(x[3], f, -base));
-                        l0 += p0, l1 += p1, l2 += p2, l3 += p3;
-                        w2[j / 2] = pack2<kRows>(p0, p1);
-                        w2[j / 2 + 1] = pack2<kRows>(p2, p3);
-                    }
-                    tc::wait_ld();
-                    tc::tmem_st16(s_at + 16 * i, w2);
+                for (int j = 0; j < kKeys; j += 4) {
+                    const float p0 = ex2(fmaf(s[j], f, -base)), p1 = ex2(fmaf(s[j + 1], f, -base));
+                    const float p2 = ex2(fmaf(s[j + 2], f, -base)), p3 = ex2(fmaf(s[j + 3], f, -base));
+                    l0 += p0, l1 += p1, l2 += p2, l3 += p3;
+                    pairs[j / 2] = __uint_as_float(pack2<kRows>(p0, p1));
+                    pairs[j / 2 + 1] = __uint_as_float(pack2<kRows>(p2, p3));
                 }
-                l += (l0 + l1) + (l2 + l3);
+                tmem_st32(at, pairs);
                 tc::wait_st();
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    arrive(&sm.p_full[w]);
+                    arrive(&sm.p_full[w][h]);
                 }
             }
             if (next.active) {
@@ -558,11 +564,12 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
         const bool whole = p.first == p.last;
         bool bad = false;
         if (active) {
-            const bool ok = wait_or_abort(&sm.o_full[w], o_phase, &sm.abort, a.status);
-            o_phase ^= 1;
+            ok = wait_or_abort<true>(&sm.o_done[w][0], phase ^ 1, &sm.abort, a.status) && ok;
+            ok = wait_or_abort<true>(&sm.o_done[w][1], phase ^ 1, &sm.abort, a.status) && ok;
             tc::fence_after_sync();
+            const float l = (l0 + l1) + (l2 + l3);
             float g = 1.0f;
-            float *part = a.part + (size_t(part_slot(int(blockIdx.x), p.first)) * kPromptWidth + c) * (D + 2);
+            float *part = a.part + (size_t(part_slot(int(blockIdx.x), p.first)) * kPromptWidth + c) * part_pitch(D);
             if (whole) {
                 float mm = m, ll = l;
                 if (a.sinks && have) {
@@ -594,10 +601,9 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                         if (whole && write) {
                             store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + 32 * i + j, v);
                         } else if (!whole && have) {
-#pragma unroll
-                            for (int t = 0; t < 8; t += 2) {
-                                *reinterpret_cast<float2 *>(part + 32 * i + j + t) = make_float2(v[t], v[t + 1]);
-                            }
+                            float4 *dst = reinterpret_cast<float4 *>(part + 32 * i + j);
+                            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
                         }
                     }
                 }
@@ -647,9 +653,11 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
             tc::mbar_init(&sm.raw_full[w], 1);
             tc::mbar_init(&sm.raw_empty[w], 128);
             tc::mbar_init(&sm.q_full[w], kHalf);
-            tc::mbar_init(&sm.s_full[w], 1);
-            tc::mbar_init(&sm.p_full[w], 4);
-            tc::mbar_init(&sm.o_full[w], 1);
+            for (int h = 0; h < 2; ++h) {
+                tc::mbar_init(&sm.s_full[w][h], 1);
+                tc::mbar_init(&sm.p_full[w][h], 4);
+                tc::mbar_init(&sm.o_done[w][h], 1);
+            }
         }
         sm.abort = 0;
         tc::fence_mbar_init();
@@ -669,7 +677,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kOtherRegs));
         if (warp == kLoader) {
             load_granules<kCache, D>(a, plan, &map, sm);
-        } else if (threadIdx.x == 32 * kIssuer) {
+        } else if (warp == kIssuer) {
             issue<kRows, kCache, D>(a, sm, tmem);
         }
     } else if constexpr (Shape::kFour) {

@@ -138,24 +138,6 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                  : "memory");
 }
 
-// Waits for a phase of a barrier unless the CTA has given up; a wait that runs
-// out gives the CTA up (every later wait returns at once, so that all warps
-// still meet at their barriers and leave).
-__device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *status) {
-    if (tc::mbar_try_wait(bar, parity)) {
-        return true;
-    }
-    if (*abort) {
-        return false;
-    }
-    if (!tc::mbar_wait(bar, parity)) {
-        set_status(status, kKvWait);
-        *abort = 1;
-        return false;
-    }
-    return true;
-}
-
 // The loader: one warp, a granule a step.
 template <class Smem, int kCache, int D, int kGran, int kStages, uint32_t kStageBytes>
 __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &plan, const CUtensorMap *map, Smem &sm) {
@@ -193,7 +175,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                 base = k0 >> a.page_shift;
                 id = checked(p, base, ids(p, base));
             }
-            const bool free = wait_or_abort(&sm.empty[stage], phase ^ 1, &sm.abort, a.status);
+            const bool free = wait_or_abort<false>(&sm.empty[stage], phase ^ 1, &sm.abort, a.status);
             if (__all_sync(0xffffffffu, free)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.full[stage], kStageBytes);
@@ -428,7 +410,7 @@ __global__ void __launch_bounds__(kThreads)
             }
         }
         for (int k0 = p.k0; k0 < p.k1; k0 += T::kGran) {
-            wait_or_abort(&sm.full[stage], phase, &sm.abort, a.status);
+            wait_or_abort<false>(&sm.full[stage], phase, &sm.abort, a.status);
             const int key0 = k0 + 16 * kSub * warp;
             if (key0 < hi_max && key0 + 16 * kSub > lo_min) {
                 const uint32_t buf = tc::smem_u32(sm.stage[stage]);
@@ -766,18 +748,16 @@ __global__ void __launch_bounds__(kThreads)
                 return ColumnInfo{ri.y, ri.z, ri.w, sm.sink[side][c]};
             });
         } else {
-            float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * kCols * (D + 2);
+            float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * kCols * part_pitch(D);
             for (int i = tid; i < p.ncols * (D / 8); i += 32 * kWarps) {
                 const int c = i / (D / 8), d = 8 * (i % (D / 8));
                 float v[8];
                 value(c, d, v);
-                float2 *dst = reinterpret_cast<float2 *>(part + size_t(c) * (D + 2) + d);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    dst[j] = make_float2(v[2 * j], v[2 * j + 1]);
-                }
+                float4 *dst = reinterpret_cast<float4 *>(part + size_t(c) * part_pitch(D) + d);
+                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
                 if (d == 0) {
-                    *reinterpret_cast<float2 *>(part + size_t(c) * (D + 2) + D) = stats(c);
+                    *reinterpret_cast<float2 *>(part + size_t(c) * part_pitch(D) + D) = stats(c);
                 }
             }
             if (arrive_last(a, p, &sm.last, consumer_sync)) {
