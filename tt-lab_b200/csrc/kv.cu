@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             const int g0 = begin < end ? begin / gran : 0;
             // at least one granule: a tile whose rows see nothing is written too
             n = begin < end ? (end + gran - 1) / gran - g0 : 1;
-            tiles[t] = Tile{lo, col0, g0, uint32_t(ncols) | uint32_t(n) << 9, q.row0, q.len, {0, 0}};
+            tiles[t] = Tile{lo, col0, g0, uint32_t(ncols) | uint32_t(n) << 9, q.row0 + r0, col0 - r0 * a.group, q.len, 0};
             n += cost;
         }
         int sum;
@@ -1198,6 +1198,7 @@ int kv_attend(ttl_kv *h, int layer, uint32_t flags, const void *q, size_t q_stri
         a.cap = cap;
         a.rows = h->rows, a.group = h->q_heads / h->kv_heads, a.page_shift = h->page_shift, a.pages = h->pages;
         a.kv_heads = h->kv_heads, a.block_bytes = h->block_bytes;
+        a.group_div = uint32_t(((1 << 20) + a.group - 1) / a.group);
         TTL_KV_CUDA(h, launch_attend(*h, a, kind, layer));
     }
     return TTL_OK;

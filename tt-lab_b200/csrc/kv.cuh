@@ -42,7 +42,7 @@ constexpr int kNoSplit = 4;        // a tile of at most this many granules is no
 struct __align__(32) Tile {
     int32_t seq, col0, gran0;
     uint32_t size;                 // columns (9 bits), granules
-    int32_t row0, len, pad[2];     // of the sequence: its first row, its length
+    int32_t row0, rem, len, pad;   // row and head (in its group) of the first column; the sequence's length
 };
 struct __align__(16) Cut {
     int32_t head, tile, gran;      // gran: granules into the tile
@@ -68,6 +68,12 @@ struct Walk {
     const int4 *row;               // [rows] {position, lo, hi, seq} of this window; seq -1: padding
 };
 
+struct Piece {
+    int head, tile, seq, ncols, row0, rem, len;
+    int k0, k1;        // keys of the piece (k1 <= the tile's last granule; clip to the sequence's length)
+    int first, last;   // first and last CTA that hold a part of the tile (equal: the whole tile is here)
+};
+
 struct AttendArgs {
     Walk walk;
     const uint8_t *pool;           // this layer
@@ -81,6 +87,15 @@ struct AttendArgs {
     float scale, cap;              // natural units; cap 0: none
     int rows, group, page_shift, pages, kv_heads;
     uint32_t block_bytes;          // one KV head of a page
+    uint32_t group_div;            // ceil(2^20 / group)
+
+    // Row and query head of column c of a tile.  (rem + c < 512, so the product
+    // is below 2^29 and the quotient exact for any group up to 256.)
+    __device__ __forceinline__ void column(const Piece &p, int c, int &row, int &qhead) const {
+        const int t = p.rem + c, r = int(uint32_t(t) * group_div >> 20);
+        row = p.row0 + r;
+        qhead = p.head * group + t - r * group;
+    }
 };
 
 __host__ __device__ constexpr uint32_t row_bytes(int cache, int d) {
@@ -222,12 +237,6 @@ __device__ __forceinline__ float capped(float dot, float in, float out) {
 
 // ---- the walk ----
 
-struct Piece {
-    int head, tile, seq, col0, ncols, row0, len;
-    int k0, k1;        // keys of the piece (k1 <= the tile's last granule; clip to the sequence's length)
-    int first, last;   // first and last CTA that hold a part of the tile (equal: the whole tile is here)
-};
-
 // The descriptor of the tile after the one handed out is loaded ahead.
 struct Walker {
     const Tile *list;
@@ -236,7 +245,7 @@ struct Walker {
     uint32_t start_span;   // of the tile that the CTA's range begins in, where it begins inside
     int cta, count, gsize;
     int4 t4;               // tile `tile`
-    int2 t2;
+    int4 t2;
 
     __device__ __forceinline__ Walker(const Walk &w, int cta_, int gsize_) : list(w.tiles), cta(cta_), gsize(gsize_) {
         const Cut a = w.cuts[cta];
@@ -249,7 +258,7 @@ struct Walker {
     __device__ __forceinline__ void load() {
         if (before(head, tile, gran, end)) {
             t4 = *reinterpret_cast<const int4 *>(list + tile);
-            t2 = *reinterpret_cast<const int2 *>(&list[tile].row0);
+            t2 = *reinterpret_cast<const int4 *>(&list[tile].row0);
         }
     }
     __device__ __forceinline__ static bool before(int h, int t, int g, const Cut &c) {
@@ -264,7 +273,7 @@ struct Walker {
         if (end.head == head && end.tile == tile) {
             stop = end.gran;  // > gran
         }
-        p.head = head, p.tile = tile, p.seq = t4.x, p.col0 = t4.y, p.row0 = t2.x, p.len = t2.y;
+        p.head = head, p.tile = tile, p.seq = t4.x, p.row0 = t2.x, p.rem = t2.y, p.len = t2.z;
         p.ncols = int(uint32_t(t4.w) & 511u);
         p.k0 = (t4.z + gran) * gsize;
         p.k1 = (t4.z + stop) * gsize;
@@ -425,10 +434,7 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
         bool bad = false;
         int row = 0, qhead = 0;
         if (c < p.ncols) {
-            const int cc = p.col0 + c;
-            const int i = cc / a.group;
-            qhead = p.head * a.group + cc - i * a.group;
-            row = p.row0 + i;
+            a.column(p, c, row, qhead);
             const ColumnInfo ci = info(c, row, qhead);
             const bool sees = max(ci.lo, 0) < min(ci.hi, p.len);
             const float2 ml = stats(c);
@@ -485,8 +491,8 @@ __device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan
     for (int base = warp * kCols; base < p.ncols; base += warps * kCols) {
         const int c = min(base + sub, p.ncols - 1);
         const bool have = base + sub < p.ncols;
-        const int cc = p.col0 + c, i = cc / a.group;
-        const int qhead = p.head * a.group + cc - i * a.group, row = p.row0 + i;
+        int row, qhead;
+        a.column(p, c, row, qhead);
         const ColumnInfo ci = column_info(a, row, qhead);
         const float *col = a.part + size_t(c) * part_pitch(D);
         auto slot = [&](int k) { return col + size_t(part_slot(p.first + k, p.first)) * width * part_pitch(D); };

@@ -68,9 +68,10 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
             const int c = i / (D / 8), d = 8 * (i % (D / 8));
             float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (c < p.ncols) {
-                const int cc = p.col0 + c, r = cc / a.group, row = p.row0 + r;
+                int row, qhead;
+                a.column(p, c, row, qhead);
                 if (row < a.rows) {
-                    load8<kRows>(a.q, size_t(row) * a.q_stride + size_t(p.head * a.group + cc - r * a.group) * D + d, x);
+                    load8<kRows>(a.q, size_t(row) * a.q_stride + size_t(qhead) * D + d, x);
                 }
             }
 #pragma unroll
@@ -82,9 +83,10 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
             int4 ri = make_int4(0, 0, 0, -1);
             float slope = 0.0f;
             if (c < p.ncols) {
-                const int cc = p.col0 + c, r = cc / a.group;
-                ri = a.walk.row[p.row0 + r];
-                slope = a.slopes ? a.slopes[p.head * a.group + cc - r * a.group] * kLog2e : 0.0f;
+                int row, qhead;
+                a.column(p, c, row, qhead);
+                ri = a.walk.row[row];
+                slope = a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
             }
             sm.pos[c] = ri.x, sm.lo[c] = max(ri.y, 0), sm.hi[c] = min(ri.z, p.len);
             sm.slope[c] = slope;

@@ -400,9 +400,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
         c.row = 0, c.qhead = 0, c.slope = 0.0f;
         c.ri = make_int4(0, 0, 1 << 30, -1);
         if (c.have) {
-            const int cc = c.p.col0 + tid, r = cc / a.group;
-            c.qhead = c.p.head * a.group + cc - r * a.group;
-            c.row = c.p.row0 + r;
+            a.column(c.p, tid, c.row, c.qhead);
             c.ri = a.walk.row[c.row];
             c.ri.y = max(c.ri.y, 0), c.ri.z = min(c.ri.z, c.p.len);
             c.slope = a.slopes ? a.slopes[c.qhead] * kLog2e : 0.0f;

@@ -55,9 +55,21 @@ template <int kRows, int kCache, int D, int NT> struct TokenShape {
     static constexpr int kSub = token_sub(kCache, 8 * NT);  // steps of 16 keys a warp takes at once
     static constexpr int kGran = 16 * kWarps * kSub;
     static constexpr uint32_t kStageBytes = kFour ? 2 * kGran * row_bytes(kMxfp4, D) : 2 * kGran * D * 2;
-    // enough in flight to cover HBM's latency at its full rate over the CTAs of an SM (about 48 KB per SM)
-    static constexpr int kStages = kFour ? 4 : (D == 64 ? 4 : 3);
-    static constexpr int kOPitch = D + 4;
+    // Granules in flight: about 96 KB per SM in its two CTAs.  More reads slower
+    // (128 tokens of 64 values: three granules 151 us, five 158, six 162), less too
+    // (two: 161); with three CTAs on an SM 160.
+    static constexpr int kStages = D == 64 || kFour ? 3 : 2;
+    // A column's sums in shared memory: over a 16-bit cache rows of D values whose
+    // groups of 8 are swapped by the column, over 4 bits rows with 4 values of
+    // padding; either way the accumulators' stores do not collide.
+    static constexpr int kOPitch = kFour ? D + 4 : D;
+    __device__ static __forceinline__ int o_at(int c, int d) {
+        return kFour ? d : d ^ (((c >> 1) & 3) << 3);
+    }
+    // Q rows: 16-byte chunks swapped by the column.
+    __device__ static __forceinline__ int q_at(int c, int d) {
+        return d ^ ((c & 7) << 3);
+    }
 };
 
 template <int kRows, int kCache, int D, int NT> struct TokenSmem {
@@ -65,17 +77,29 @@ template <int kRows, int kCache, int D, int NT> struct TokenSmem {
     alignas(1024) uint8_t stage[T::kStages][(T::kStageBytes + 1023) / 1024 * 1024];
     float o[kWarps][T::kCols][T::kOPitch];
     float m[kWarps][T::kCols], l[kWarps][T::kCols];
-    // the columns: Q rows (16 bytes of padding keep the fragments' loads from
-    // colliding), and for this tile and the next the plan's row, slope and sink
-    alignas(16) uint16_t q[T::kCols][D + 8];
+    // the tile in hand and the next: what it is, its Q rows, the plan's rows, slopes and sinks
+    Piece piece[2];                // ncols 0: no more
+    alignas(16) uint16_t q[2][T::kCols][D];
     int4 row[2][T::kCols];
     float slope[2][T::kCols], sink[2][T::kCols];
+    uint64_t tile_full[2], tile_empty[2];
     uint64_t full[T::kStages], empty[T::kStages];
     int last, abort;
 };
 
 __device__ __forceinline__ void consumer_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+}
+
+// True in all computing warps when it is in any.
+__device__ __forceinline__ bool consumers_any(bool x) {
+    uint32_t y;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(y)
+        : "r"(x ? 1u : 0u), "n"(32 * kWarps)
+        : "memory");
+    return y != 0;
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -139,7 +163,7 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
 }
 
 // The loader: one warp, a granule a step.
-template <class Smem, int kCache, int D, int kGran, int kStages, uint32_t kStageBytes>
+template <class Smem, int kCache, int D, int kCols, int kGran, int kStages, uint32_t kStageBytes>
 __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &plan, const CUtensorMap *map, Smem &sm) {
     const int lane = threadIdx.x & 31;
     const int seg = min(1 << a.page_shift, kGran);       // keys of one copy (a TMA box has up to 64 rows)
@@ -163,9 +187,53 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
         }
         return id;
     };
+    // Hands a tile to the computing warps: its description now, its columns
+    // asynchronously.  A lane arrives once for what it stored and once, by itself,
+    // when its copies are there.
+    int side = 0;
+    uint32_t side_phase = 0;
+    auto hand_over = [&](const Piece &p) {
+        wait_or_abort<false>(&sm.tile_empty[side], side_phase ^ 1, &sm.abort, a.status);
+        __syncwarp();
+        if (lane == 0) {
+            sm.piece[side] = p;
+        }
+        if (p.ncols > 0) {
+            for (int i = lane; i < kCols * (D / 8); i += 32) {
+                const int c = i / (D / 8), d = 8 * (i - c * (D / 8));
+                int row, qhead;
+                a.column(p, c, row, qhead);
+                const bool have = c < p.ncols && row < a.rows;
+                const uint16_t *src = static_cast<const uint16_t *>(a.q) + (have ? size_t(row) * a.q_stride + size_t(qhead) * D + d : 0);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(&sm.q[side][c][d ^ ((c & 7) << 3)])), "l"(src), "r"(have ? 16 : 0)
+                             : "memory");
+            }
+            if (lane < p.ncols) {
+                int row, qhead;
+                a.column(p, lane, row, qhead);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(&sm.row[side][lane])), "l"(a.walk.row + row) : "memory");
+                if (a.slopes) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(&sm.slope[side][lane])), "l"(a.slopes + qhead) : "memory");
+                }
+                if (a.sinks) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(&sm.sink[side][lane])), "l"(a.sinks + qhead) : "memory");
+                }
+            } else if (lane < kCols) {
+                sm.row[side][lane] = make_int4(0, 0, 1 << 30, -1);  // past the tile: all keys, so that it asks for no mask
+                sm.slope[side][lane] = sm.sink[side][lane] = 0.0f;
+            }
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(tc::smem_u32(&sm.tile_full[side])) : "memory");
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&sm.tile_full[side])) : "memory");
+        side_phase ^= uint32_t(side);
+        side ^= 1;
+    };
     Piece p, ahead;
     bool any = walk.next(p), more = false;
     int first_ids = any ? ids(p, p.k0 >> a.page_shift) : 0;
+    if (any) {
+        hand_over(p);
+    }
     for (; any; any = more, p = ahead) {
         int base = p.k0 >> a.page_shift, id = checked(p, base, first_ids);
         more = walk.next(ahead);
@@ -218,7 +286,13 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                 phase ^= 1;
             }
         }
+        if (more) {
+            hand_over(ahead);  // while the last granules of this tile are worked on
+        }
     }
+    p.ncols = 0;
+    hand_over(p);
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (*const_cast<volatile int *>(&sm.abort)) {
         // what is still in flight lands before the shared memory goes away
         for (int i = 0; i < kStages; ++i) {
@@ -229,7 +303,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
 }
 
 template <int kRows, int kCache, int D, int NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 64 ? 3 : 2)
     kv_attend_tokens_kernel(AttendArgs a, const __grid_constant__ CUtensorMap map) {
     using T = TokenShape<kRows, kCache, D, NT>;
     using Smem = TokenSmem<kRows, kCache, D, NT>;
@@ -246,6 +320,10 @@ __global__ void __launch_bounds__(kThreads)
             tc::mbar_init(&sm.full[i], 1);
             tc::mbar_init(&sm.empty[i], kWarps);
         }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&sm.tile_full[i], 64);
+            tc::mbar_init(&sm.tile_empty[i], kWarps);
+        }
         sm.abort = 0;
         tc::fence_mbar_init();
     }
@@ -258,7 +336,7 @@ __global__ void __launch_bounds__(kThreads)
         return;
     }
     if (warp == kWarps) {
-        load_granules<Smem, kCache, D, T::kGran, T::kStages, T::kStageBytes>(a, plan, &map, sm);
+        load_granules<Smem, kCache, D, kCols, T::kGran, T::kStages, T::kStageBytes>(a, plan, &map, sm);
         return;
     }
     const int g = lane >> 2, t = lane & 3;
@@ -273,61 +351,33 @@ __global__ void __launch_bounds__(kThreads)
     constexpr float kLift = kMma != kF16 ? 0.0f : (kCache == kMxfp4 ? 9.0f : 11.0f);
     int stage = 0;
     uint32_t phase = 0;
-    Walker walk(a.walk, int(blockIdx.x), T::kGran);
-    // copies a tile's Q rows, and the rest of its columns to side `to`, asynchronously
-    auto fetch = [&](const Piece &p, int to) {
-        for (int i = tid; i < kCols * (D / 8); i += 32 * kWarps) {
-            const int c = i / (D / 8), d = 8 * (i - c * (D / 8));
-            const int cc = p.col0 + c, r = cc / a.group, row = p.row0 + r;
-            const bool have = c < p.ncols && row < a.rows;
-            const uint16_t *src = static_cast<const uint16_t *>(a.q) +
-                                  (have ? size_t(row) * a.q_stride + size_t(p.head * a.group + cc - r * a.group) * D + d : 0);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(&sm.q[c][d])), "l"(src), "r"(have ? 16 : 0)
-                         : "memory");
+    uint32_t side_phase = 0;
+    for (int side = 0;; side ^= 1) {
+        const bool ok = wait_or_abort<false>(&sm.tile_full[side], side_phase, &sm.abort, a.status);
+        side_phase ^= uint32_t(side);
+        // all warps go on with the tile, or none
+        if (consumers_any(!ok || sm.piece[side].ncols == 0)) {
+            break;
         }
-        if (tid < kCols) {
-            if (tid < p.ncols) {
-                const int cc = p.col0 + tid, r = cc / a.group, qhead = p.head * a.group + cc - r * a.group;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(&sm.row[to][tid])), "l"(a.walk.row + p.row0 + r) : "memory");
-                if (a.slopes) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(&sm.slope[to][tid])), "l"(a.slopes + qhead) : "memory");
-                }
-                if (a.sinks) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(tc::smem_u32(&sm.sink[to][tid])), "l"(a.sinks + qhead) : "memory");
-                }
-            } else {
-                sm.row[to][tid] = make_int4(0, 0, 1 << 30, -1);  // past the tile: all keys, so that it asks for no mask
-                sm.slope[to][tid] = sm.sink[to][tid] = 0.0f;
-            }
-        }
-    };
-    Piece p, ahead;
-    bool any = walk.next(p), more = false;
-    if (any) {
-        fetch(p, 0);
-    }
-    for (int side = 0; any; any = more, p = ahead, side ^= 1) {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        consumer_sync();
-        more = walk.next(ahead);
+        const Piece &p = sm.piece[side];
         uint32_t q[NT][D / 16][2];
         float scale[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int c = 8 * n + g;
-            const uint16_t *src = sm.q[c];
+            const uint16_t *src = sm.q[side][c];
             if constexpr (kCache != kMxfp4) {
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s) {
-                    q[n][s][0] = *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * t);
-                    q[n][s][1] = *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * t);
+                    q[n][s][0] = *reinterpret_cast<const uint32_t *>(src + T::q_at(c, 16 * s) + 2 * t);
+                    q[n][s][1] = *reinterpret_cast<const uint32_t *>(src + T::q_at(c, 16 * s + 8) + 2 * t);
                 }
             } else {
                 // values 8t .. 8t + 7 of each block of 32, as the codes' words lie
                 uint4 w[kBlocks];
 #pragma unroll
                 for (int b = 0; b < kBlocks; ++b) {
-                    w[b] = *reinterpret_cast<const uint4 *>(src + 32 * b + 8 * t);
+                    w[b] = *reinterpret_cast<const uint4 *>(src + T::q_at(c, 32 * b + 8 * t));
                 }
                 float unscale = 1.0f;
                 if constexpr (kRows == kBf16) {
@@ -370,10 +420,6 @@ __global__ void __launch_bounds__(kThreads)
                 }
             }
         }
-        consumer_sync();  // every warp has its Q: the next tile's may come
-        if (more) {
-            fetch(ahead, side ^ 1);
-        }
         // lowest and highest borders over the columns
         int lo_min, lo_max, hi_min, hi_max;
         {
@@ -409,7 +455,8 @@ __global__ void __launch_bounds__(kThreads)
                 }
             }
         }
-        for (int k0 = p.k0; k0 < p.k1; k0 += T::kGran) {
+        const int end = p.k1;
+        for (int k0 = p.k0; k0 < end; k0 += T::kGran) {
             wait_or_abort<false>(&sm.full[stage], phase, &sm.abort, a.status);
             const int key0 = k0 + 16 * kSub * warp;
             if (key0 < hi_max && key0 + 16 * kSub > lo_min) {
@@ -709,7 +756,7 @@ __global__ void __launch_bounds__(kThreads)
                         const int d = 32 * (i >> 1) + 4 * g + 2 * (i & 1) + (j >> 1);
                         sm.o[warp][c][d] = o[n][i][j] * __uint_as_float(0x7f000000u - __float_as_uint(unit[n][j & 1][i >> 1]));
                     } else {
-                        sm.o[warp][c][16 * i + g + 8 * (j >> 1)] = o[n][i][j];
+                        sm.o[warp][c][T::o_at(c, 16 * i + g + 8 * (j >> 1))] = o[n][i][j];
                     }
                 }
             }
@@ -736,8 +783,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float f = ex2(sm.m[w][c] - safe);
-                const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][c][d]);
-                const float4 y = *reinterpret_cast<const float4 *>(&sm.o[w][c][d + 4]);
+                const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][c][T::o_at(c, d)]);
+                const float4 y = *reinterpret_cast<const float4 *>(&sm.o[w][c][T::o_at(c, d + 4)]);
                 v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]), v[2] = fmaf(x.z, f, v[2]), v[3] = fmaf(x.w, f, v[3]);
                 v[4] = fmaf(y.x, f, v[4]), v[5] = fmaf(y.y, f, v[5]), v[6] = fmaf(y.z, f, v[6]), v[7] = fmaf(y.w, f, v[7]);
             }
@@ -763,6 +810,10 @@ __global__ void __launch_bounds__(kThreads)
             if (arrive_last(a, p, &sm.last, consumer_sync)) {
                 merge_tile<kRows, kCache, D>(a, plan, p, warp, kWarps, kCols);
             }
+        }
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&sm.tile_empty[side])) : "memory");
         }
     }
 }
