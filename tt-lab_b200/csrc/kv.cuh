@@ -297,6 +297,40 @@ struct Walker {
     }
 };
 
+// The same for |x / cap| up to kSmallScore: tanh y = y P(y^2) without the
+// special-function unit, P fitted to tanh(y) / y over y <= 0.5 for the least
+// relative error (1.4e-8).  scaled: x in log2 units, ratio: x / cap.
+constexpr float kSmallScore = 0.5f;
+__device__ __forceinline__ float capped_small(float scaled, float ratio) {
+    const float t = ratio * ratio;
+    const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.017134985f, -0.052986064f), 0.13324779f), -0.33333069f), 0.99999999f);
+    return scaled * p;
+}
+
+// Pairs of f32 in one instruction: x * f + c, and a + b.
+__device__ __forceinline__ void fma_pair(float &x0, float &x1, float f, float c) {
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 d, {%3, %3};\n\t"
+        "fma.rn.f32x2 a, a, b, d;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(x0), "+f"(x1)
+        : "f"(f), "f"(c));
+}
+__device__ __forceinline__ void add_pair(float &a0, float &a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
+}
+// Largest and smallest of three (NaN is passed over, as by fmaxf).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Waits for a phase of a barrier unless the CTA has given up; a wait of about two
 // seconds gives the CTA up (every later wait returns at once, so that all warps
 // still meet at their barriers and leave).  kSleep lets the hardware put the

@@ -36,6 +36,7 @@ constexpr int kGran = 128;
 constexpr int kHalf = 128;                 // columns of a warpgroup
 constexpr int kKeys = 64;                  // keys of a step: half a granule
 constexpr int kLoader = 8, kIssuer = 9;    // warps
+constexpr int kScout = 10;                 // two warps
 constexpr int kExpander = 12;              // first of the four warps that expand a 4-bit cache
 constexpr uint32_t kTmemCols = 512;
 
@@ -59,13 +60,25 @@ template <int kCache, int D> struct PromptSmem {
     alignas(16) uint8_t raw[2][kRawBytes];
     uint64_t raw_full[2], raw_empty[2];
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [warpgroup][half of a granule]
+    Piece piece[2];                                         // the tile in hand and the next; ncols 0: no more
+    uint64_t piece_full[2], piece_empty[2], q_full, q_empty;
+    uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [warpgroup][half of a granule]
     uint32_t tmem;
     int last, abort;
 };
 
 __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
+// True in all softmax warps when it is in any.
+__device__ __forceinline__ bool softmax_any(bool x) {
+    uint32_t y;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(y)
+        : "r"(x ? 1u : 0u)
+        : "memory");
+    return y != 0;
 }
 __device__ __forceinline__ void softmax_sync() {
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -288,7 +301,7 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
     const uint64_t q_desc = tc::smem_desc_sw128(tc::smem_u32(sm.q[0])), k_desc = tc::smem_desc_sw128(tc::smem_u32(sm.k[0])),
                    v_desc = desc_mn(tc::smem_u32(sm.v[0]), kGran * 128);
     int ks = 0, vs = 0;
-    uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;  // q: bit w; p: bit 2 h + w
+    uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;  // p: bit 2 h + w
     auto scores = [&](int w, int h) {
         const uint64_t q = q_desc + uint64_t(uint32_t(w) * (kHalf * D * 2) >> 4), k = k_desc + uint64_t((uint32_t(ks) * kTileBytes + h * kKeys * 128) >> 4);
 #pragma unroll
@@ -312,23 +325,22 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
         more = walk.next(ahead);
         const int n = (p.k1 - p.k0) / kGran, halves = p.ncols > kHalf ? 2 : 1;
         ok = wait_or_abort<true>(&sm.k_full[ks], k_phase, &sm.abort, a.status) && ok;
+        ok = wait_or_abort<true>(&sm.q_full, q_phase, &sm.abort, a.status) && ok;
+        q_phase ^= 1;
+        tc::fence_after_sync();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                if (w < halves) {
-                    if (h == 0) {
-                        ok = wait_or_abort<true>(&sm.q_full[w], (q_phase >> w) & 1u, &sm.abort, a.status) && ok;
-                        q_phase ^= 1u << w;
-                        tc::fence_after_sync();
-                    }
-                    if (__all_sync(0xffffffffu, ok)) {
-                        scores(w, h);
-                    }
+                if (w < halves && __all_sync(0xffffffffu, ok)) {
+                    scores(w, h);
                 }
             }
         }
         next_k();
+        if (n == 1) {
+            commit(&sm.q_empty, lead);
+        }
         for (int j = 0; j < n; ++j) {
             ok = wait_or_abort<true>(&sm.v_full[vs], v_phase, &sm.abort, a.status) && ok;
             if (j + 1 < n) {
@@ -366,7 +378,48 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
             if (j + 1 < n) {
                 next_k();
             }
+            if (j + 2 == n) {
+                commit(&sm.q_empty, lead);  // the tile's last scores are under way
+            }
         }
+    }
+}
+
+// Two warps that look the tiles up: each tile's description for the softmax
+// warps, and its Q rows, 16 bytes at a time, swizzled as the matrix instruction
+// reads them, as soon as the last scores of the tile before are computed.
+template <int kCache, int D> __device__ __forceinline__ void scout(const AttendArgs &a, PromptSmem<kCache, D> &sm) {
+    const int lane = threadIdx.x - 32 * kScout;  // 0 .. 63
+    Walker walk(a.walk, int(blockIdx.x), kGran);
+    Piece p;
+    uint32_t side_phase = 0, q_phase = 0;
+    for (int side = 0;; side ^= 1) {
+        const bool more = walk.next(p);
+        p.ncols = more ? p.ncols : 0;
+        wait_or_abort<true>(&sm.piece_empty[side], side_phase ^ 1, &sm.abort, a.status);
+        side_phase ^= uint32_t(side);
+        if (lane == 0) {
+            sm.piece[side] = p;
+        }
+        arrive(&sm.piece_full[side]);
+        if (!more) {
+            break;
+        }
+        wait_or_abort<true>(&sm.q_empty, q_phase ^ 1, &sm.abort, a.status);
+        q_phase ^= 1;
+        const int columns = p.ncols > kHalf ? 2 * kHalf : kHalf;
+        for (int i = lane; i < columns * (D / 8); i += 64) {
+            const int c = i / (D / 8), chunk = i % (D / 8), r = c & (kHalf - 1);
+            int row, qhead;
+            a.column(p, c, row, qhead);
+            const bool have = c < p.ncols && row < a.rows;
+            const uint16_t *src = static_cast<const uint16_t *>(a.q) + (have ? size_t(row) * a.q_stride + size_t(qhead) * D + 8 * chunk : 0);
+            const uint32_t to = tc::smem_u32(sm.q[c / kHalf]) + uint32_t(chunk / 8) * (kHalf * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(have ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        arrive(&sm.q_full);
     }
 }
 
@@ -380,75 +433,34 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
     constexpr float kLift = kRows == kF16 ? 11.0f : 0.0f;
     const float scale = a.scale * kLog2e, cap_log2 = a.cap * kLog2e;
     const float cap_in = a.cap != 0.0f ? scale * 2.0f / a.cap : 0.0f;
+    const float ratio = a.cap != 0.0f ? a.scale / a.cap : 0.0f;
     const bool special = a.cap != 0.0f || a.slopes;
-    uint32_t phase = 0;  // of the granule, for the barriers of both halves
-    Walker walk(a.walk, int(blockIdx.x), kGran);
-    // The tile after the one in hand is looked up while that one runs, and its Q
-    // rows are copied as soon as the last scores of this one are there, so that
-    // its first scores are under way before this one has ended.
-    struct Column {
-        Piece p;
-        bool any, active, have;
-        int row, qhead;
-        int4 ri;
-        float slope;
-    };
-    auto look_up = [&](Column &c) {
-        c.any = walk.next(c.p);
-        c.active = c.any && (w == 0 || c.p.ncols > kHalf);
-        c.have = c.any && tid < c.p.ncols;
-        c.row = 0, c.qhead = 0, c.slope = 0.0f;
-        c.ri = make_int4(0, 0, 1 << 30, -1);
-        if (c.have) {
-            a.column(c.p, tid, c.row, c.qhead);
-            c.ri = a.walk.row[c.row];
-            c.ri.y = max(c.ri.y, 0), c.ri.z = min(c.ri.z, c.p.len);
-            c.slope = a.slopes ? a.slopes[c.qhead] * kLog2e : 0.0f;
+    uint32_t phase = 0;       // of the granule, for the barriers of both halves
+    uint32_t side_phase = 0;
+    for (int side = 0;; side ^= 1) {
+        bool ok = wait_or_abort<true>(&sm.piece_full[side], side_phase, &sm.abort, a.status);
+        side_phase ^= uint32_t(side);
+        const Piece &p = sm.piece[side];
+        // all softmax warps go on with the tile, or none
+        if (softmax_any(!ok || p.ncols == 0)) {
+            break;
         }
-    };
-    // Q, 16 bytes at a time, swizzled as the matrix instruction reads it
-    auto copy_q = [&](const Column &c) {
-        const bool read = c.have && c.row < a.rows;
-        const uint16_t *src = static_cast<const uint16_t *>(a.q) + (read ? size_t(c.row) * a.q_stride + size_t(c.qhead) * D : 0);
-        const int r = tid & (kHalf - 1);
-        const uint32_t to = tc::smem_u32(sm.q[w]) + r * 128;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + uint32_t(i / 8) * (kHalf * 128) + (((i & 7) ^ (r & 7)) << 4)),
-                         "l"(src + (read ? 8 * i : 0)), "r"(read ? 16 : 0)
-                         : "memory");
+        const int c = tid;    // column of the tile
+        const bool active = w == 0 || p.ncols > kHalf, have = c < p.ncols;
+        int4 ri = make_int4(0, 0, 1 << 30, -1);
+        float slope = 0.0f;
+        if (have) {
+            int row, qhead;
+            a.column(p, c, row, qhead);
+            ri = a.walk.row[row];
+            ri.y = max(ri.y, 0), ri.z = min(ri.z, p.len);
+            slope = a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
         }
-    };
-    auto publish_q = [&] {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        tc::fence_before_sync();
-        arrive(&sm.q_full[w]);
-    };
-    Column cur, next;
-    look_up(cur);
-    if (cur.active) {
-        copy_q(cur);
-        publish_q();
-    }
-    for (; cur.any; cur = next) {
-        look_up(next);
-        const Piece &p = cur.p;
-        const int c = tid;  // column of the tile
-        const bool active = cur.active, have = cur.have;
-        const int row = cur.row, qhead = cur.qhead;
-        const int4 ri = cur.ri;
-        const float slope = cur.slope;
-        const bool sees = ri.y < ri.z;
         float m = -INFINITY, l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
-        bool ok = true;  // no wait has run out
-        if (!active && next.active) {
-            copy_q(next);
-            publish_q();
-        }
         if (active) {
+            const int begin = p.k0, end = p.k1;
             int h = 0;
-            for (int k0 = p.k0; k0 < p.k1; k0 += kKeys, h ^= 1) {
+            for (int k0 = begin; k0 < end; k0 += kKeys, h ^= 1) {
                 const uint32_t now = phase;
                 phase ^= uint32_t(h);
                 ok = wait_or_abort<true>(&sm.s_full[w][h], now, &sm.abort, a.status);
@@ -456,9 +468,6 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                     continue;
                 }
                 tc::fence_after_sync();
-                if (k0 + kKeys >= p.k1 && next.active) {
-                    copy_q(next);  // the last scores of this tile: its Q has been read
-                }
                 const uint32_t at = s_at + kKeys * h;
                 float s[kKeys];
                 tmem_ld32(at, s);
@@ -468,9 +477,23 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 if (special) {
                     f = 1.0f;
                     if (a.cap != 0.0f) {
+                        float big[2] = {0.0f, 0.0f};
 #pragma unroll
-                        for (int j = 0; j < kKeys; ++j) {
-                            s[j] = capped(s[j], cap_in, cap_log2);
+                        for (int j = 0; j < kKeys; j += 4) {
+                            big[0] = max3(big[0], fabsf(s[j]), fabsf(s[j + 1]));
+                            big[1] = max3(big[1], fabsf(s[j + 2]), fabsf(s[j + 3]));
+                        }
+                        if (__any_sync(0xffffffffu, fmaxf(big[0], big[1]) * fabsf(ratio) > kSmallScore)) {
+#pragma unroll
+                            for (int j = 0; j < kKeys; ++j) {
+                                s[j] = capped(s[j], cap_in, cap_log2);
+                            }
+                        } else {
+                            // most scores are far below their cap: one special function per score, not three
+#pragma unroll
+                            for (int j = 0; j < kKeys; ++j) {
+                                s[j] = capped_small(s[j] * scale, s[j] * ratio);
+                            }
                         }
                     } else {
 #pragma unroll
@@ -494,19 +517,21 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                     }
                 }
                 // ---- the maximum ----
-                float top[4] = {s[0], s[1], s[2], s[3]};
+                float top[2] = {s[0], s[1]};
                 if (f >= 0.0f) {
 #pragma unroll
-                    for (int j = 4; j < kKeys; ++j) {
-                        top[j & 3] = fmaxf(top[j & 3], s[j]);
+                    for (int j = 2; j + 3 < kKeys; j += 4) {
+                        top[0] = max3(top[0], s[j], s[j + 1]);
+                        top[1] = max3(top[1], s[j + 2], s[j + 3]);
                     }
-                    top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    top[0] = fmaxf(max3(top[0], s[kKeys - 2], s[kKeys - 1]), top[1]);
                 } else {
 #pragma unroll
-                    for (int j = 4; j < kKeys; ++j) {
-                        top[j & 3] = fminf(top[j & 3], s[j]);
+                    for (int j = 2; j + 3 < kKeys; j += 4) {
+                        top[0] = min3(top[0], s[j], s[j + 1]);
+                        top[1] = min3(top[1], s[j + 2], s[j + 3]);
                     }
-                    top[0] = fminf(fminf(top[0], top[1]), fminf(top[2], top[3]));
+                    top[0] = fminf(min3(top[0], s[kKeys - 2], s[kKeys - 1]), top[1]);
                 }
                 const float most = f == 0.0f ? 0.0f : top[0] * f;
                 if (__any_sync(0xffffffffu, most > m + (kSlack + kLift))) {
@@ -514,7 +539,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                     const float up = ex2(m - (mn == -INFINITY ? 0.0f : mn));
                     m = mn;
                     l0 *= up, l1 *= up, l2 *= up, l3 *= up;
-                    if (k0 != p.k0) {
+                    if (k0 != begin) {
                         // The product of the half before ends, and with it those before it:
                         // rescale their sums.  (A barrier per half: the scores in hand came
                         // behind this half's last product, so no barrier is ever more than
@@ -540,9 +565,11 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 float pairs[kKeys / 2];  // of 16-bit weights
 #pragma unroll
                 for (int j = 0; j < kKeys; j += 4) {
-                    const float p0 = ex2(fmaf(s[j], f, -base)), p1 = ex2(fmaf(s[j + 1], f, -base));
-                    const float p2 = ex2(fmaf(s[j + 2], f, -base)), p3 = ex2(fmaf(s[j + 3], f, -base));
-                    l0 += p0, l1 += p1, l2 += p2, l3 += p3;
+                    fma_pair(s[j], s[j + 1], f, -base);
+                    fma_pair(s[j + 2], s[j + 3], f, -base);
+                    const float p0 = ex2(s[j]), p1 = ex2(s[j + 1]), p2 = ex2(s[j + 2]), p3 = ex2(s[j + 3]);
+                    add_pair(l0, l1, p0, p1);
+                    add_pair(l2, l3, p2, p3);
                     pairs[j / 2] = __uint_as_float(pack2<kRows>(p0, p1));
                     pairs[j / 2 + 1] = __uint_as_float(pack2<kRows>(p2, p3));
                 }
@@ -554,12 +581,13 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                     arrive(&sm.p_full[w][h]);
                 }
             }
-            if (next.active) {
-                publish_q();
-            }
         }
         // ---- the end of the tile ----
-        const bool whole = p.first == p.last;
+        const bool whole = p.first == p.last, sees = ri.y < ri.z;
+        int row = 0, qhead = 0;
+        if (have) {
+            a.column(p, c, row, qhead);
+        }
         bool bad = false;
         if (active) {
             ok = wait_or_abort<true>(&sm.o_done[w][0], phase ^ 1, &sm.abort, a.status) && ok;
@@ -621,6 +649,10 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
             }
             softmax_sync();
         }
+        __syncwarp();
+        if (lane == 0) {
+            arrive(&sm.piece_empty[side]);
+        }
     }
 }
 
@@ -650,13 +682,16 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
         for (int w = 0; w < 2; ++w) {
             tc::mbar_init(&sm.raw_full[w], 1);
             tc::mbar_init(&sm.raw_empty[w], 128);
-            tc::mbar_init(&sm.q_full[w], kHalf);
+            tc::mbar_init(&sm.piece_full[w], 64);
+            tc::mbar_init(&sm.piece_empty[w], 8);
             for (int h = 0; h < 2; ++h) {
                 tc::mbar_init(&sm.s_full[w][h], 1);
                 tc::mbar_init(&sm.p_full[w][h], 4);
                 tc::mbar_init(&sm.o_done[w][h], 1);
             }
         }
+        tc::mbar_init(&sm.q_full, 64);
+        tc::mbar_init(&sm.q_empty, 1);
         sm.abort = 0;
         tc::fence_mbar_init();
     }
@@ -677,6 +712,8 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
             load_granules<kCache, D>(a, plan, &map, sm);
         } else if (warp == kIssuer) {
             issue<kRows, kCache, D>(a, sm, tmem);
+        } else {
+            scout<kCache, D>(a, sm);
         }
     } else if constexpr (Shape::kFour) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kExpandRegs));
