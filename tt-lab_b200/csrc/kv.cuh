@@ -301,10 +301,29 @@ struct Walker {
 // special-function unit, P fitted to tanh(y) / y over y <= 0.5 for the least
 // relative error (1.4e-8).  scaled: x in log2 units, ratio: x / cap.
 constexpr float kSmallScore = 0.5f;
-__device__ __forceinline__ float capped_small(float scaled, float ratio) {
-    const float t = ratio * ratio;
-    const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.017134985f, -0.052986064f), 0.13324779f), -0.33333069f), 0.99999999f);
-    return scaled * p;
+//
+// Two at a time (one instruction works on a pair of f32): x, y raw products.
+__device__ __forceinline__ void capped_small(float &x, float &y, float scale, float ratio) {
+    asm("{\n\t.reg .b64 x, r, t, p, c;\n\t"
+        "mov.b64 x, {%0, %1};\n\t"
+        "mov.b64 c, {%3, %3};\n\tmul.rn.f32x2 r, x, c;\n\tmul.rn.f32x2 t, r, r;\n\t"
+        "mov.b64 c, {%2, %2};\n\tmul.rn.f32x2 x, x, c;\n\t"
+        "mov.b64 p, {%4, %4};\n\t"
+        "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mov.b64 c, 0x3f8000003f800000;\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mul.rn.f32x2 x, x, p;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(scale), "f"(ratio), "f"(0.017134985f), "f"(-0.052986064f), "f"(0.13324779f), "f"(-0.33333069f));
+}
+// x += base + slope * j, y += base + slope * (j + 1).
+__device__ __forceinline__ void bias_pair(float &x, float &y, float slope, float base, float j) {
+    asm("{\n\t.reg .b64 x, b, s, j;\n\t"
+        "mov.b64 x, {%0, %1};\n\tmov.b64 b, {%3, %3};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 j, {%4, %5};\n\t"
+        "fma.rn.f32x2 b, s, j, b;\n\tadd.rn.f32x2 x, x, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(slope), "f"(base), "f"(j), "f"(j + 1.0f));
 }
 
 // Pairs of f32 in one instruction: x * f + c, and a + b.
@@ -319,15 +338,40 @@ __device__ __forceinline__ void add_pair(float &a0, float &a1, float b0, float b
         : "+f"(a0), "+f"(a1)
         : "f"(b0), "f"(b1));
 }
-// Largest and smallest of three (NaN is passed over, as by fmaxf).
+// 2^x and 2^y on the multiply-add units, for x, y <= 127; 0 from -127 on.  x = n +
+// f with n the nearest integer (it comes out of the sum with 1.5 * 2^23), 2^f by a
+// polynomial fitted over [-1/2, 1/2] with P(0) = 1 for the least relative error
+// (9e-8), n added to its exponent: at -127 that leaves the zero word.  NaN gives 0:
+// the caller looks for it in the maximum.
+__device__ __forceinline__ void pow2_pair(float x, float y, float &px, float &py) {
+    uint32_t bx, by;
+    asm("{\n\t.reg .b64 x, t, r, p, c;\n\t.reg .b32 tx, ty, qx, qy;\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 c, 0x4b4000004b400000;\n\tadd.rn.f32x2 t, x, c;\n\t"
+        "mov.b64 c, 0xcb400000cb400000;\n\tadd.rn.f32x2 r, t, c;\n\t"
+        "mov.b64 c, 0xbf800000bf800000;\n\tfma.rn.f32x2 x, r, c, x;\n\t"
+        "mov.b64 p, {%4, %4};\n\t"
+        "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, {%8, %8};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, 0x3f8000003f800000;\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 {tx, ty}, t;\n\tmov.b64 {qx, qy}, p;\n\t"
+        "mad.lo.u32 %0, tx, 8388608, qx;\n\tmad.lo.u32 %1, ty, 8388608, qy;\n\t}"
+        : "=r"(bx), "=r"(by)
+        : "f"(fmaxf(x, -127.0f)), "f"(fmaxf(y, -127.0f)), "f"(0.001326472731307149f), "f"(0.009671512991189957f),
+          "f"(0.05550733581185341f), "f"(0.24022242426872253f), "f"(0.6931470036506653f));
+    px = __uint_as_float(bx), py = __uint_as_float(by);
+}
+// Largest and smallest of three; NaN if any is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ float min3(float a, float b, float c) {
     float d;
-    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
@@ -506,7 +550,8 @@ __device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &p
 }
 
 // Partial results: [slot][width][part_pitch(D)] floats, a column's D sums, then
-// its maximum and sum; rows of a multiple of 16 bytes.
+// its maximum and sum; rows of a multiple of 16 bytes.  (Prompts lay the same
+// space out by columns.)
 __host__ __device__ constexpr int part_pitch(int d) {
     return d + 4;
 }
@@ -514,12 +559,13 @@ __host__ __device__ constexpr int part_pitch(int d) {
 // Merges the partial results of a tile over the CTAs [first, last] that hold
 // them, in that order, and stores its columns: D / 4 lanes per column.  The
 // parts come from other SMs through L2, about a microsecond each way, so what
-// counts is how many are asked for at once: eight parts' sums and statistics
-// per lane (one token over 131072 keys, 55 parts per head: two parts at a time
-// cost 20 us).
-template <int kRows, int kCache, int D>
+// counts is how many are asked for at once: kBatch parts' sums and statistics
+// per lane, eight (one token over 131072 keys, 55 parts per head: two parts at a
+// time cost 20 us) unless the registers lack (4 bits, three CTAs per SM: with
+// eight the loop over the keys spills, 64 tokens 104 us, with four 92).
+template <int kRows, int kCache, int D, int kBatch>
 __device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps, int width) {
-    constexpr int kLanes = D / 4, kCols = 32 / kLanes, kBatch = 8;
+    constexpr int kLanes = D / 4, kCols = 32 / kLanes;
     const int lane = threadIdx.x & 31, sub = lane / kLanes, d = 4 * (lane % kLanes);
     const int parts = p.last - p.first + 1;
     for (int base = warp * kCols; base < p.ncols; base += warps * kCols) {

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
                 part[i] = d < D ? sum[c * D + d] : (d == D ? sm.m[c] : sm.l[c]);
             }
             if (arrive_last(a, p, &sm.last, [] { __syncthreads(); })) {
-                merge_tile<kRows, kCache, D>(a, plan, p, warp, kSimpleThreads / 32, CT);
+                merge_tile<kRows, kCache, D, 8>(a, plan, p, warp, kSimpleThreads / 32, CT);
             }
         }
         __syncthreads();

@@ -423,6 +423,79 @@ template <int kCache, int D> __device__ __forceinline__ void scout(const AttendA
     }
 }
 
+// A CTA's partial result of a tile: D / 4 rows of a float4 per column, then a
+// row of {maximum, sum}: a warp, whose threads hold a column each, writes and
+// reads 512 bytes at a time.
+template <int D> __device__ __forceinline__ float *part_of(const AttendArgs &a, int cta, int first) {
+    static_assert(kPromptWidth * (D + 2) <= kPromptWidth * part_pitch(D), "the space of a slot");
+    return a.part + size_t(part_slot(cta, first)) * kPromptWidth * part_pitch(D);
+}
+
+// Merges the parts of a thread's column in the order of the keys, and stores it.
+// What counts is the time of a load through L2: eight are under way per thread
+// (two warps' worth of columns at a time, two loads each, took 30 us for 256
+// columns of 128 values in three parts).
+template <int kRows, int kCache, int D>
+__device__ __forceinline__ void merge_column(const AttendArgs &a, const Plan &plan, const Piece &p, int c, int row, int qhead, bool write,
+                                             bool sees) {
+    float m = -INFINITY, l = 0.0f;
+    for (int k = p.first; k <= p.last; ++k) {
+        const float2 y = __ldcg(reinterpret_cast<const float2 *>(part_of<D>(a, k, p.first) + kPromptWidth * D) + c);
+        const float mn = fmaxf(m, y.x), safe = mn == -INFINITY ? 0.0f : mn;
+        l = l * exp2f(m - safe) + y.y * exp2f(y.x - safe);
+        m = mn;
+    }
+    const float safe = m == -INFINITY ? 0.0f : m;
+    float g = 1.0f;
+    if (a.sinks && write) {
+        const float sink = a.sinks[qhead] * kLog2e, mn = fmaxf(m, sink), s = mn == -INFINITY ? 0.0f : mn;
+        g = exp2f(m - s);
+        l = l * g + exp2f(sink - s);
+    }
+    g = g / l;
+    bool bad = false;
+#pragma unroll 1
+    for (int i = 0; i < D / 4; i += 8) {
+        float o[32] = {};
+#pragma unroll 1
+        for (int k = p.first; k <= p.last; ++k) {
+            const float *part = part_of<D>(a, k, p.first);
+            const float4 *src = reinterpret_cast<const float4 *>(part) + i * kPromptWidth + c;
+            float4 x[8];
+            const float y = __ldcg(part + kPromptWidth * D + 2 * c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = __ldcg(src + j * kPromptWidth);
+            }
+            const float w = exp2f(y - safe);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                o[4 * j] = fmaf(x[j].x, w, o[4 * j]), o[4 * j + 1] = fmaf(x[j].y, w, o[4 * j + 1]);
+                o[4 * j + 2] = fmaf(x[j].z, w, o[4 * j + 2]), o[4 * j + 3] = fmaf(x[j].w, w, o[4 * j + 3]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            float v[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                v[t] = sees ? o[j + t] * g : 0.0f;
+                bad = bad || !(fabsf(v[t]) < INFINITY);
+            }
+            if (write) {
+                store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + 4 * i + j, v);
+            }
+        }
+    }
+    uint32_t redo = __ballot_sync(0xffffffffu, bad && write);
+    while (redo) {
+        const int src = __ffs(redo) - 1;
+        redo &= redo - 1;
+        attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, __shfl_sync(0xffffffffu, row, src),
+                                       __shfl_sync(0xffffffffu, qhead, src));
+    }
+}
+
 // A warpgroup: the columns [128 w, 128 w + 128) of each tile, one per thread.
 template <int kRows, int kCache, int D>
 __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, PromptSmem<kCache, D> &sm, uint32_t tmem) {
@@ -483,7 +556,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                             big[0] = max3(big[0], fabsf(s[j]), fabsf(s[j + 1]));
                             big[1] = max3(big[1], fabsf(s[j + 2]), fabsf(s[j + 3]));
                         }
-                        if (__any_sync(0xffffffffu, fmaxf(big[0], big[1]) * fabsf(ratio) > kSmallScore)) {
+                        if (__any_sync(0xffffffffu, !(fmaxf(big[0], big[1]) * fabsf(ratio) <= kSmallScore))) {
 #pragma unroll
                             for (int j = 0; j < kKeys; ++j) {
                                 s[j] = capped(s[j], cap_in, cap_log2);
@@ -491,8 +564,8 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                         } else {
                             // most scores are far below their cap: one special function per score, not three
 #pragma unroll
-                            for (int j = 0; j < kKeys; ++j) {
-                                s[j] = capped_small(s[j] * scale, s[j] * ratio);
+                            for (int j = 0; j < kKeys; j += 2) {
+                                capped_small(s[j], s[j + 1], scale, ratio);
                             }
                         }
                     } else {
@@ -503,9 +576,17 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                     }
                     if (a.slopes) {
                         const float away = float(ri.x - k0);
+                        if (__all_sync(0xffffffffu, ri.x - k0 >= kKeys)) {  // all keys lie before their rows
+                            const float base = -slope * away;
 #pragma unroll
-                        for (int j = 0; j < kKeys; ++j) {
-                            s[j] = fmaf(-slope, fabsf(away - float(j)), s[j]);
+                            for (int j = 0; j < kKeys; j += 2) {
+                                bias_pair(s[j], s[j + 1], slope, base, float(j));
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < kKeys; ++j) {
+                                s[j] = fmaf(-slope, fabsf(away - float(j)), s[j]);
+                            }
                         }
                     }
                 }
@@ -524,17 +605,19 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                         top[0] = max3(top[0], s[j], s[j + 1]);
                         top[1] = max3(top[1], s[j + 2], s[j + 3]);
                     }
-                    top[0] = fmaxf(max3(top[0], s[kKeys - 2], s[kKeys - 1]), top[1]);
+                    top[0] = max3(max3(top[0], s[kKeys - 2], s[kKeys - 1]), top[1], top[1]);
                 } else {
 #pragma unroll
                     for (int j = 2; j + 3 < kKeys; j += 4) {
                         top[0] = min3(top[0], s[j], s[j + 1]);
                         top[1] = min3(top[1], s[j + 2], s[j + 3]);
                     }
-                    top[0] = fminf(min3(top[0], s[kKeys - 2], s[kKeys - 1]), top[1]);
+                    top[0] = min3(min3(top[0], s[kKeys - 2], s[kKeys - 1]), top[1], top[1]);
                 }
-                const float most = f == 0.0f ? 0.0f : top[0] * f;
-                if (__any_sync(0xffffffffu, most > m + (kSlack + kLift))) {
+                // NaN where a score is, or the scale a zero in log2 units
+                const float most = top[0] * f;
+                if (__any_sync(0xffffffffu, !(most <= m + (kSlack + kLift)))) {
+                    l0 = most < INFINITY ? l0 : NAN;  // the column is computed again
                     const float mn = fmaxf(m, most - kLift);
                     const float up = ex2(m - (mn == -INFINITY ? 0.0f : mn));
                     m = mn;
@@ -563,11 +646,21 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 // ---- the weights, over the scores ----
                 const float base = m == -INFINITY ? 0.0f : m;
                 float pairs[kKeys / 2];  // of 16-bit weights
+                // A quarter of the exponentials goes to the multiply-add units: the special
+                // functions alone take 16 a clock and SM.  (4096-token prompt 300 us without,
+                // 284 so, 291 with three eighths; with a cap, which already keeps those units
+                // busy, 175 and 179.)
 #pragma unroll
                 for (int j = 0; j < kKeys; j += 4) {
                     fma_pair(s[j], s[j + 1], f, -base);
                     fma_pair(s[j + 2], s[j + 3], f, -base);
-                    const float p0 = ex2(s[j]), p1 = ex2(s[j + 1]), p2 = ex2(s[j + 2]), p3 = ex2(s[j + 3]);
+                    const float p0 = ex2(s[j]), p1 = ex2(s[j + 1]);
+                    float p2, p3;
+                    if (j % 8 == 0) {
+                        pow2_pair(s[j + 2], s[j + 3], p2, p3);
+                    } else {
+                        p2 = ex2(s[j + 2]), p3 = ex2(s[j + 3]);
+                    }
                     add_pair(l0, l1, p0, p1);
                     add_pair(l2, l3, p2, p3);
                     pairs[j / 2] = __uint_as_float(pack2<kRows>(p0, p1));
@@ -595,7 +688,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
             tc::fence_after_sync();
             const float l = (l0 + l1) + (l2 + l3);
             float g = 1.0f;
-            float *part = a.part + (size_t(part_slot(int(blockIdx.x), p.first)) * kPromptWidth + c) * part_pitch(D);
+            float *part = part_of<D>(a, int(blockIdx.x), p.first);
             if (whole) {
                 float mm = m, ll = l;
                 if (a.sinks && have) {
@@ -607,7 +700,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 }
                 g = g / ll;
             } else if (have) {
-                part[D] = m, part[D + 1] = l;
+                reinterpret_cast<float2 *>(part + kPromptWidth * D)[c] = make_float2(m, l);
             }
             const bool write = have && row < a.rows && ri.w == p.seq;
             if (__all_sync(0xffffffffu, ok)) {
@@ -627,9 +720,9 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                         if (whole && write) {
                             store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + 32 * i + j, v);
                         } else if (!whole && have) {
-                            float4 *dst = reinterpret_cast<float4 *>(part + 32 * i + j);
+                            float4 *dst = reinterpret_cast<float4 *>(part) + (8 * i + j / 4) * kPromptWidth + c;
                             dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                            dst[kPromptWidth] = make_float4(v[4], v[5], v[6], v[7]);
                         }
                     }
                 }
@@ -645,7 +738,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
         }
         if (!whole) {
             if (arrive_last(a, p, &sm.last, softmax_sync)) {
-                merge_tile<kRows, kCache, D>(a, plan, p, warp, 8, kPromptWidth);
+                merge_column<kRows, kCache, D>(a, plan, p, c, row, qhead, have && row < a.rows && ri.w == p.seq, sees);
             }
             softmax_sync();
         }

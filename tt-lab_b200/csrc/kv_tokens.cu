@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
                 }
             }
             if (arrive_last(a, p, &sm.last, consumer_sync)) {
-                merge_tile<kRows, kCache, D>(a, plan, p, warp, kWarps, kCols);
+                merge_tile<kRows, kCache, D, kCache == kMxfp4 ? 4 : 8>(a, plan, p, warp, kWarps, kCols);
             }
         }
         __syncwarp();
