@@ -41,6 +41,7 @@ struct PlanArgs {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kNearTiles = 1024;
+constexpr int kFewShare = 4;  // granules of each CTA of the prompt kernel
 constexpr int kMaxPosition = 1 << 29;  // a tile counts up to 2^23 granules
 
 struct SeqState {
@@ -163,6 +164,25 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     const int width = a.width[kind], gran = a.gran[kind], cost = a.cost[kind];
     Tile *tiles = a.tiles[kind][sliding];
     Cut *cuts = a.cuts[kind][sliding];
+    // Where little of the batch's work lies with sequences of few columns, the
+    // prompt kernel takes them too: the other's launch, with nothing to do then,
+    // costs about 3 us instead of the 30 that a pass over one long sequence takes.
+    int few = a.few;
+    if (a.ctas[0] && a.ctas[1]) {
+        int work = 0;
+        for (int base = 0; base < a.seqs; base += kPlanThreads) {
+            int n = 0;
+            if (base + tid < a.seqs) {
+                const SeqState q = load_seq(a, base + tid);
+                const int keys = sliding && !a.prefix_len ? min(q.len, a.window + q.n) : q.len;
+                n = q.n > 0 && q.n * a.group <= a.few ? min(keys / a.gran[1], kMaxCtas) + a.cost[1] : 0;
+            }
+            int sum;
+            block_scan(n, &sum, sums);
+            work += sum;
+        }
+        few = (long long)(work) * a.kv_heads <= kFewShare * a.ctas[1] ? 0 : few;
+    }
     // tiles of each sequence
     int total = 0;
     for (int base = 0; base < a.seqs; base += kPlanThreads) {
@@ -174,7 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
                 ttl::set_status(a.status, kKvBadBatch);
             }
             const int columns = q.n * a.group;
-            const bool mine = (columns <= a.few) == (kind == 0);
+            const bool mine = (columns <= few) == (kind == 0);
             count = (mine && columns > 0) ? (columns + width - 1) / width : 0;
         }
         int sum;
