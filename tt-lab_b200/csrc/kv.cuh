@@ -317,13 +317,13 @@ __device__ __forceinline__ void capped_small(float &x, float &y, float scale, fl
         : "+f"(x), "+f"(y)
         : "f"(scale), "f"(ratio), "f"(0.017134985f), "f"(-0.052986064f), "f"(0.13324779f), "f"(-0.33333069f));
 }
-// x += base + slope * j, y += base + slope * (j + 1).
-__device__ __forceinline__ void bias_pair(float &x, float &y, float slope, float base, float j) {
-    asm("{\n\t.reg .b64 x, b, s, j;\n\t"
-        "mov.b64 x, {%0, %1};\n\tmov.b64 b, {%3, %3};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 j, {%4, %5};\n\t"
-        "fma.rn.f32x2 b, s, j, b;\n\tadd.rn.f32x2 x, x, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
+// x = x * f + (b + c), with b a pair.
+__device__ __forceinline__ void bias_pair(float &x, float &y, float f, float b0, float b1, float c) {
+    asm("{\n\t.reg .b64 x, b, c;\n\t"
+        "mov.b64 x, {%0, %1};\n\tmov.b64 b, {%3, %4};\n\tmov.b64 c, {%5, %5};\n\tadd.rn.f32x2 b, b, c;\n\t"
+        "mov.b64 c, {%2, %2};\n\tfma.rn.f32x2 x, x, c, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
         : "+f"(x), "+f"(y)
-        : "f"(slope), "f"(base), "f"(j), "f"(j + 1.0f));
+        : "f"(f), "f"(b0), "f"(b1), "f"(c));
 }
 
 // Pairs of f32 in one instruction: x * f + c, and a + b.

@@ -248,11 +248,12 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
     const int tokens = 1 << a.page_shift;
     const uint32_t at = uint32_t(key >> a.page_shift) * a.block_bytes;
     const int t = key & (tokens - 1);
+    const __nv_bfloat162 unit = __bfloat162bfloat162(__ushort_as_bfloat16(0x7e80));  // 2^126
     auto half = [&](const uint8_t *src, uint8_t *dst) {
         const uint8_t *scales = src + tokens * (D / 2) + t * (D / 32);
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
-            const float f = scale_of(scales[b]);
+            const __nv_bfloat162 f = __bfloat162bfloat162(__float2bfloat16_rn(scale_of(scales[b])));  // a power of two
             const uint4 w = *reinterpret_cast<const uint4 *>(src + t * (D / 2) + 16 * b);
             const uint32_t c[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -260,8 +261,16 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
                 uint32_t o[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 v = __half22float2(e2m1x2_to_half2((c[i] >> (8 * j)) & 255u));
-                    o[j] = pack2<kBf16>(v.x * f, v.y * f);
+                    // byte j's codes to the top of the halves: sign at bit 15, the three bits of
+                    // exponent and mantissa to bits 6 to 8, a bf16 of 2^-126 times the value
+                    // (0.5 and 0 are subnormal in either format); both products are exact but
+                    // for results below bf16's normal range
+                    const uint32_t x = __byte_perm(c[i] << 4, c[i], j << 4 | (4 + j) << 12);
+                    const uint32_t bits = (x & 0x80008000u) | ((x >> 6) & 0x01c001c0u);
+                    __nv_bfloat162 v;
+                    memcpy(&v, &bits, 4);
+                    v = __hmul2(__hmul2(v, unit), f);
+                    memcpy(&o[j], &v, 4);
                 }
                 const int chunk = 4 * (b & 1) + i;
                 *reinterpret_cast<uint4 *>(dst + (b / 2) * (kGran * 128) + key * 128 + ((chunk ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -568,24 +577,31 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                                 capped_small(s[j], s[j + 1], scale, ratio);
                             }
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < kKeys; ++j) {
-                            s[j] *= scale;
-                        }
                     }
                     if (a.slopes) {
+                        const float by = a.cap != 0.0f ? 1.0f : scale;
                         const float away = float(ri.x - k0);
-                        if (__all_sync(0xffffffffu, ri.x - k0 >= kKeys)) {  // all keys lie before their rows
-                            const float base = -slope * away;
+                        if (__all_sync(0xffffffffu, away <= 0.0f || away >= float(kKeys - 1))) {
+                            // no row lies between the keys: the bias is a line, +-slope (j - away);
+                            // eight keys share its start
+                            const float turn = away <= 0.0f ? -slope : slope;
+                            float step[8];
 #pragma unroll
-                            for (int j = 0; j < kKeys; j += 2) {
-                                bias_pair(s[j], s[j + 1], slope, base, float(j));
+                            for (int j = 0; j < 8; ++j) {
+                                step[j] = turn * float(j);
+                            }
+#pragma unroll
+                            for (int j = 0; j < kKeys; j += 8) {
+                                const float start = turn * (float(j) - away);
+#pragma unroll
+                                for (int t = 0; t < 8; t += 2) {
+                                    bias_pair(s[j + t], s[j + t + 1], by, step[t], step[t + 1], start);
+                                }
                             }
                         } else {
 #pragma unroll
                             for (int j = 0; j < kKeys; ++j) {
-                                s[j] = fmaf(-slope, fabsf(away - float(j)), s[j]);
+                                s[j] = fmaf(-slope, fabsf(away - float(j)), s[j] * by);
                             }
                         }
                     }
