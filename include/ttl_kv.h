@@ -22,7 +22,8 @@
  * the same time on two streams.  A graph that holds an append or attend
  * without its batch call uses the plan of the last batch call that ran on the
  * device; where that plan has another shape of work than the captured one,
- * ttl_kv_sync reports it.
+ * ttl_kv_sync reports it.  It touches as many rows of its arrays as the batch
+ * had when it was captured.
  *
  * What only the device can see (row_start, length, page ids) is checked there:
  * a sequence with bad numbers is skipped (its rows are left as they were), a
@@ -79,8 +80,9 @@ size_t ttl_kv_page_bytes(const ttl_kv *handle);
  *   row_start [seqs + 1]  rows [row_start[s], row_start[s+1]) are sequence s's
  *                         new tokens, in order (none, one or many); rows past
  *                         row_start[seqs] are padding and left as they were
- *   length    [seqs]      tokens of sequence s including its new rows: the
- *                         rows' positions are length - new .. length - 1
+ *   length    [seqs]      tokens of sequence s including its new rows, at most
+ *                         2^29 - 128: the rows' positions are length - new ..
+ *                         length - 1
  *   pages     [seqs][page_stride]  page ids: position p is in slot
  *                         p % page_tokens of page pages[s][p / page_tokens].
  *                         Sequences may share pages that they only read.
@@ -121,8 +123,8 @@ int ttl_kv_read_async(ttl_kv *handle, int layer, void *k, size_t k_stride, void 
  *   the head's sink, which adds to the sum and has no value row
  * A row that sees nothing is zero.  Values of positions a row does not see
  * never reach it, infinities and NaN included.  f16 and bf16 rows: products
- * on the tensor cores, sums in 32 bits, weights rounded to the rows' type (to
- * f16 over a 4-bit cache). */
+ * on the tensor cores, sums in 32 bits, weights rounded to the rows' type (over
+ * a 4-bit cache to f16 or bf16). */
 int ttl_kv_attend_async(ttl_kv *handle, int layer, uint32_t flags, const void *q, size_t q_stride, void *out,
                         size_t out_stride, float scale, float cap, const float *sinks, const float *slopes);
 

@@ -328,6 +328,117 @@ def test_attend_masks(rows, cache, new, length, mask):
         assert (out[sum(new) - 1] == 0).all()
 
 
+@pytest.mark.parametrize("rows,cache,D", [("f16", "f16", 64), ("f16", "f16", 128), ("bf16", "bf16", 128), ("bf16", "mxfp4", 64),
+                                         ("bf16", "mxfp4", 128)])
+@pytest.mark.parametrize("mask", MASKS, ids=lambda m: "-".join(m))
+def test_attend_masks_of_prompts(rows, cache, D, mask):
+    """Prompts over earlier tokens in every type; biases that rise or fall with
+    the distance, before, across and behind the rows' own keys."""
+    m = dict(mask)
+    new, length, H = (90, 2, 33), (330, 200, 200), 8
+    r = np.random.default_rng(6)
+    first = prefix = None
+    if m.pop("docs", False):
+        first = []
+        for n, l in zip(new, length):
+            cuts = [0] + sorted(int(c) for c in r.integers(0, l, 2))
+            first += [max(c for c in cuts if c <= p) for p in range(l - n, l)]
+        first[7] = first[100] = 1 << 30       # rows that see nothing
+    if m.pop("prefix", False):
+        prefix = [320, 0, 190]
+    if m.pop("sinks", False):
+        m["sinks"] = torch.linspace(-2, 3, H)
+    if m.pop("slopes", False):
+        m["slopes"] = torch.linspace(-0.05, 1.2, H)
+    Setup(rows, cache, H, 2, D, 32, new=new, length=length, window=m.pop("window", 0), first=first, prefix=prefix,
+          pad=0 if first else 3).check(**m)
+
+
+@pytest.mark.parametrize("rows,cache,D", [("bf16", "bf16", 64), ("f16", "f16", 128), ("bf16", "mxfp4", 64)])
+def test_tokens_of_many_sequences_beside_a_prompt(rows, cache, D):
+    """Enough cache behind single tokens that they stay with their own kernel,
+    and a prompt in the same batch."""
+    new, length = (1,) * 20 + (90,) + (3,) * 20, (2600,) * 20 + (500,) + (2500,) * 20
+    Setup(rows, cache, 4, 2, D, 64, new=new, length=length, seed=3).check(sinks=torch.linspace(-1, 1, 4))
+
+
+@pytest.mark.parametrize("rows,cache", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "mxfp4"), ("f16", "mxfp4")])
+@pytest.mark.parametrize("new", [1, 70])
+def test_caps_far_from_the_scores(rows, cache, new):
+    """A cap far above the scores changes nothing, one far below leaves the
+    signs."""
+    s = Setup(rows, cache, 8, 2, 64, 16, new=(new,), length=(new + 60,))
+    s.fill().plan()
+    ref, tol = s.reference()
+    for cap in (1e5, 1e12, 1e30):
+        assert ((s.attend(cap=cap).double() - ref).abs() <= tol).all()
+    s.check(cap=1e-3)
+
+
+@pytest.mark.parametrize("rows,cache", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "mxfp4"), ("f16", "mxfp4")])
+@pytest.mark.parametrize("kw", [{}, dict(scale=-0.2), dict(cap=9.0), dict(slopes=0.1)], ids=lambda k: "-".join(k) or "plain")
+def test_a_seen_nan_key_wherever_it_lies(rows, cache, kw):
+    """A row that sees a key of NaN is NaN whole, at any place of the key in
+    its tile; the rows before it are as without it."""
+    n, extra = 70, 16
+    kw = {k: torch.full((4,), v) if k == "slopes" else v for k, v in kw.items()}
+    s = Setup(rows, cache, 4, 1, 64, 16, new=(n,) * extra, length=(n + 64,) * extra)
+    for i in range(extra):
+        s.dev["k"][s.tok0[i] + 70 + i] = math.nan
+    s.fill().plan()
+    out = s.attend(**{k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}).reshape(extra, n, 4, 64)
+    ref, tol = (x.reshape(extra, n, 4, 64) for x in s.reference(**kw))
+    for i in range(extra):
+        sees = 70 + i - 64  # the first of the sequence's rows that does
+        assert torch.isnan(out[i, sees:]).all()
+        assert ((out[i, :sees].double() - ref[i, :sees]).abs() <= tol[i, :sees]).all()
+
+
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("bf16", "mxfp4")])
+def test_the_longest_sequence(rows, cache):
+    """One token at the last position there is: every page is page 0, so the
+    result is the attention over its 128 keys, each as often as the others.
+    Where 2^29 weights are summed one after the other, a part's sums lose up to
+    2^-23 per step of 16 keys, the part being at most 2^29 / 148 keys of which a
+    warp takes a quarter."""
+    n = 2 ** 29 - 128
+    s = Setup(rows, cache, 4, 1, 64, 128, new=(1,), length=(128,), extra_pages=0)
+    s.fill()
+    ref, tol = s.reference()
+    table = torch.zeros(1, 2 ** 22, dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    out = torch.full_like(s.dev["q"], 7.0)
+    s.cache.batch_async(start, torch.tensor([n], dtype=torch.int32).cuda(), table, rows=1)
+    s.cache.attend_async(0, s.dev["q"], out)
+    s.cache.sync()
+    k, v = (kv_plain.held(x.double(), cache) for x in (s.k, s.v))
+    most = float(v.abs().max())
+    steps = 2 ** 29 / 148 / 4 / 16
+    assert ((out.cpu().double() - ref).abs() <= tol + 2 * steps * 2.0 ** -23 * most).all()
+    s.cache.batch_async(start, torch.tensor([n + 1], dtype=torch.int32).cuda(), table, rows=1)
+    out.fill_(7.0)
+    s.cache.attend_async(0, s.dev["q"], out)
+    with pytest.raises(Exception, match="length"):
+        s.cache.sync()
+    assert (out == 7).all()
+
+
+def test_more_work_than_a_plan_counts_is_refused():
+    """257 sequences of the greatest length are 2^31 granules of keys."""
+    import ttl_moe
+    S, n = 257, 2 ** 29 - 128
+    with ttl_moe.KvCache(pages=1, page_tokens=128, q_heads=1, kv_heads=1, rows="f32", max_seqs=S, max_rows=S, device=0,
+                         stream=torch.cuda.current_stream()) as c:
+        table = torch.zeros(S, 2 ** 22, dtype=torch.int32, device="cuda")
+        c.batch_async(torch.arange(S + 1, dtype=torch.int32).cuda(), torch.full((S,), n, dtype=torch.int32).cuda(), table, rows=S)
+        q = torch.zeros(S, 1, 64, device="cuda")
+        out = torch.full_like(q, 7.0)
+        c.attend_async(0, q, out)
+        with pytest.raises(Exception, match="range"):
+            c.sync()
+        assert (out == 7).all()
+
+
 @pytest.mark.parametrize("rows,cache", COMBOS)
 def test_attend_long_sequence_is_split_and_merged(rows, cache):
     """One token over 20011 keys: the work is cut into many parts; the same

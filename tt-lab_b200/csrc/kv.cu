@@ -42,7 +42,7 @@ struct PlanArgs {
 constexpr int kPlanThreads = 1024;
 constexpr int kNearTiles = 1024;
 constexpr int kFewShare = 4;  // granules of each CTA of the prompt kernel
-constexpr int kMaxPosition = 1 << 29;  // a tile counts up to 2^23 granules
+constexpr int kMaxPosition = (1 << 29) - 128;  // a tile counts up to 2^23 - 1 granules
 
 struct SeqState {
     int row0, n, len;
@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     // their key ranges
     int32_t *prefix = total <= kNearTiles ? near_prefix : a.prefix[kind][sliding];
     int line = 0;
+    long long whole_line = 0;
     for (int base = 0; base < total; base += kPlanThreads) {
         const int t = base + tid;
         int n = 0;
@@ -267,6 +268,20 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             prefix[t] = line + at;
         }
         line += sum;
+        if (total > 255) {
+            // the line is counted in 32 bits, which 255 tiles cannot pass: the upper parts'
+            // sum gives the whole to within 2^22, its lower bits the rest
+            int upper;
+            block_scan(n >> 12, &upper, sums);
+            whole_line += ((long long)(upper) << 12) + (uint32_t(sum) - (uint32_t(upper) << 12));
+        }
+    }
+    if (whole_line > 0x7fffffff) {  // more work than weeks: refused
+        if (tid == 0) {
+            ttl::set_status(a.status, kKvBadBatch);
+        }
+        total = line = 0;
+        __syncthreads();
     }
     if (tid == 0) {
         prefix[total] = line;
