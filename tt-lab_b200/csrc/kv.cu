@@ -1117,7 +1117,7 @@ int kv_batch(ttl_kv *h, uint32_t seqs, uint32_t rows, uint32_t max_new, const in
     a.seqs = int(seqs), a.rows = int(rows), a.max_new = int(max_new);
     a.group = h->q_heads / h->kv_heads, a.kv_heads = h->kv_heads, a.window = h->window, a.page_tokens = h->page_tokens;
     Shape shape[kKinds];
-    a.few = choose_shapes(*h, int(seqs), int(rows), int(max_new), shape);
+    a.few = choose_shapes(*h, int(seqs), int(max_new), shape);
     for (int k = 0; k < kKinds; ++k) {
         a.width[k] = h->width[k] = shape[k].width;
         a.gran[k] = shape[k].gran;

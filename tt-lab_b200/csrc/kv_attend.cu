@@ -270,32 +270,44 @@ template <int kRows, int kCache, int D> cudaError_t configure_simple(const ttl_k
 
 }  // namespace
 
-// Sequences of more columns than this go to the prompt kernel.
-constexpr int kFewColumns = 64;
-
 namespace {
+
+// Sequences of more columns than the widest tile of the kernel for few columns
+// go to the prompt kernel: from there on that one would read the cache more
+// than once.  64 sequences of 4096 keys, bf16, 8 KV heads: D = 64, 32 columns
+// 137 us against the prompt kernel's 177, 64 columns 249 against 178; over 4
+// bits 168 and 253, 325 and 252; D = 128, 16 columns 181 and 205, 32 columns 340
+// and 210.
+constexpr int few_columns(int dim) {
+    return dim == 128 ? 16 : 32;
+}
+
 int token_index(int columns, int dim) {
     return columns <= 8 ? 0 : (columns <= 16 || dim == 128 ? 1 : 2);
 }
+
 }  // namespace
 
-int choose_shapes(const ttl_kv &h, int seqs, int, int max_new, Shape shape[kKinds]) {
+int choose_shapes(const ttl_kv &h, int seqs, int max_new, Shape shape[kKinds]) {
     const int group = h.q_heads / h.kv_heads, columns = max_new * group;
     shape[0] = shape[1] = Shape{kPromptWidth, 128, 2, 0};
     if (h.rows_type == kF32) {
         shape[0] = Shape{columns <= 8 ? 8 : 32, kSimpleGran, 1, 2 * h.sms};
         return 1 << 30;
     }
-    const bool prompt = h.prompt_ctas > 0 && columns > kFewColumns;
+    const bool prompt = h.prompt_ctas > 0 && columns > few_columns(h.dim);
     if (prompt) {
         shape[1].ctas = h.prompt_ctas;
     }
     if (prompt && seqs == 1) {
         return 0;  // one launch: whatever the sequence's rows turn out to be
     }
-    const int i = token_index(columns, h.dim);
+    // Beside a prompt most sequences bring one token: a tile is as wide as that
+    // (64 tokens over 8192 keys and a prompt of 512, bf16: 201 us, with tiles of
+    // 32 columns 270; over 4 bits 131 and 348).
+    const int i = token_index(prompt ? std::min(columns, group) : columns, h.dim);
     shape[0] = Shape{8 << i, 64 * token_sub(h.cache_type, 8 << i), 1, h.token_ctas[i]};
-    return prompt ? kFewColumns : 1 << 30;
+    return prompt ? few_columns(h.dim) : 1 << 30;
 }
 
 size_t kv_part_floats(const ttl_kv &h) {

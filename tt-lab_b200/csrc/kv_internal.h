@@ -91,7 +91,7 @@ struct Shape {
 
 // Chooses the kernels of a batch; returns the most columns of a sequence that
 // goes to kind 0.
-int choose_shapes(const ttl_kv &h, int seqs, int rows, int max_new, Shape shape[kKinds]);
+int choose_shapes(const ttl_kv &h, int seqs, int max_new, Shape shape[kKinds]);
 // Floats of the workspace that holds partial results.
 size_t kv_part_floats(const ttl_kv &h);
 // Sets the kernels' attributes once per handle.
