@@ -381,6 +381,19 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
     return d;
 }
 
+// Whether a phase of a barrier is complete, without waiting for it.
+__device__ __forceinline__ bool phase_done(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(tc::smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // Waits for a phase of a barrier unless the CTA has given up; a wait of about two
 // seconds gives the CTA up (every later wait returns at once, so that all warps
 // still meet at their barriers and leave).  kSleep lets the hardware put the

@@ -25,13 +25,13 @@
 // 4-bit cache four turn codes into bf16.  The scores of the half after next are
 // issued right behind the product of this one, over the weights it has just read.
 //
-// Measured: a 4096-token prompt of 64 query and 8 KV heads, D = 64, bf16: 264 us,
-// 521 TFLOP/s of the 1675 that a plain product reaches; the special-function
+// Measured: a 4096-token prompt of 64 query and 8 KV heads, D = 64, bf16: 249 us,
+// 552 TFLOP/s of the 1675 that a plain product reaches; the special-function
 // unit alone needs 88 us, the tensor pipe (25 % busy) 82.  A half takes a warp
-// 2060 clocks: 400 to wait for its scores, 400 for loads and the maximum, 880 for
-// the weights, with one other warp on its scheduler to fill the gaps; the third
+// about 1900 clocks: 400 for loads and the maximum, 900 for the weights, the rest
+// for hand-overs, with one other warp on its scheduler to fill the gaps; the third
 // that would need 576 columns of tensor memory.  Ends of tiles are 7 %.  f16
-// chunks of up to 509 rows, D = 128, a cap: 113 us, 357 TFLOP/s: the cap's
+// chunks of up to 509 rows, D = 128, a cap: 112 us, 358 TFLOP/s: the cap's
 // polynomial is 16 multiply-adds per pair of scores.  A 1500-token prompt over 4
 // bits with a distance bias: 115 us, where the four expanding warps cost about 15.
 #include <cuda.h>
@@ -558,10 +558,11 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
         if (active) {
             const int begin = p.k0, end = p.k1;
             int h = 0;
+            bool ready = false;  // the scores of this half are there
             for (int k0 = begin; k0 < end; k0 += kKeys, h ^= 1) {
                 const uint32_t now = phase;
                 phase ^= uint32_t(h);
-                ok = wait_or_abort<true>(&sm.s_full[w][h], now, &sm.abort, a.status);
+                ok = ready || wait_or_abort<true>(&sm.s_full[w][h], now, &sm.abort, a.status);
                 if (!__all_sync(0xffffffffu, ok)) {
                     continue;
                 }
@@ -684,6 +685,13 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 // busy, 175 and 179.)
 #pragma unroll
                 for (int j = 0; j < kKeys; j += 4) {
+                    // Are the next half's scores there?  Asked here, the answer's way through the
+                    // queue that the special functions fill costs nothing.  (4096-token prompt
+                    // 264 us without, 249 so.  Over 4 bits the expanding warps take the gaps: 112
+                    // us without, 116.)
+                    if (kCache != kMxfp4 && j == kKeys / 2) {
+                        ready = k0 + kKeys < end && phase_done(&sm.s_full[w][h ^ 1], phase);
+                    }
                     fma_pair(s[j], s[j + 1], f, -base);
                     fma_pair(s[j + 2], s[j + 3], f, -base);
                     const float p0 = ex2(s[j]), p1 = ex2(s[j + 1]);
