@@ -726,6 +726,59 @@ def test_graph_replays_follow_the_batch():
                     assert ((out[s:s + 1].cpu().double() - ref).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "mxfp4")])
+def test_two_graphs_of_one_handle_replayed_in_turn(rows, cache):
+    """Two graphs share the handle's plan and workspace: one of many tokens and a
+    prompt, whose short sequences go with the prompt or by themselves as their
+    lengths on the device ask, one of a prompt alone.  Replayed in turn, each
+    gives what its calls give without a graph, bit for bit."""
+    new, length = (1,) * 20 + (90,) + (3,) * 20, (2600,) * 20 + (500,) + (2500,) * 20
+    st = torch.cuda.Stream()
+    s = Setup(rows, cache, 4, 2, 64, 64, new=new, length=length, seed=3, stream=st)
+    s.fill()
+    d = s.dev
+    short = torch.tensor([7 if n < 90 else l for n, l in zip(new, length)], dtype=torch.int32).cuda()
+    full, now = d["length"].clone(), d["length"]
+    one = dict(start=torch.tensor([0, 90], dtype=torch.int32).cuda(), length=torch.tensor([500], dtype=torch.int32).cuda(),
+               table=d["table"][20:21].contiguous(), q=d["q"][20:110].contiguous())
+    out, out1 = torch.zeros_like(d["q"]), torch.zeros_like(one["q"])
+
+    def many():
+        s.cache.batch_async(d["start"], now, d["table"], rows=s.rows, max_new=90)
+        s.cache.attend_async(0, d["q"], out)
+
+    def single():
+        s.cache.batch_async(one["start"], one["length"], one["table"], rows=90, max_new=90)
+        s.cache.attend_async(0, one["q"], out1)
+
+    want = {}
+    for name, lens in (("full", full), ("short", short)):
+        torch.cuda.synchronize()
+        now.copy_(lens)
+        torch.cuda.synchronize()
+        many()
+        s.cache.sync()
+        want[name] = out.clone()
+    single()
+    s.cache.sync()
+    want["one"] = out1.clone()
+    graphs = []
+    for f in (many, single):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=st):
+            f()
+    for name, lens in (("full", full), ("short", short), ("full", full), ("short", short)):
+        torch.cuda.synchronize()
+        out.fill_(0), out1.fill_(0), now.copy_(lens)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graphs[0].replay()
+            graphs[1].replay()
+        s.cache.sync()
+        assert torch.equal(out, want[name]) and torch.equal(out1, want["one"])
+    assert not torch.equal(want["full"], want["short"])
+
+
 def test_two_handles_on_two_streams_at_once():
     a = Setup("bf16", None, 8, 2, 64, 16, new=(1,), length=(9000,), seed=1, stream=torch.cuda.Stream())
     b = Setup("bf16", None, 8, 2, 64, 16, new=(1,), length=(8000,), seed=2, stream=torch.cuda.Stream())
