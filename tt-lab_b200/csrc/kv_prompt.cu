@@ -680,9 +680,9 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 const float base = m == -INFINITY ? 0.0f : m;
                 float pairs[kKeys / 2];  // of 16-bit weights
                 // A quarter of the exponentials goes to the multiply-add units: the special
-                // functions alone take 16 a clock and SM.  (4096-token prompt 300 us without,
-                // 284 so, 291 with three eighths; with a cap, which already keeps those units
-                // busy, 175 and 179.)
+                // functions alone take 16 a clock and SM.  (4096-token prompt 248 us; with an
+                // eighth 256, three eighths 252, half 267.  With a cap, which keeps those units
+                // busy already, 112, with an eighth 111.)
 #pragma unroll
                 for (int j = 0; j < kKeys; j += 4) {
                     // Are the next half's scores there?  Asked here, the answer's way through the
