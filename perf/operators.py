@@ -13,8 +13,10 @@ Three operators of ``ttl_moe.KvCache`` are measured:
             E8M0 scale per 32 values of a head, the format of the framework's
             expert weights.
 
-``step`` runs a serving step's calls one after another: the batch's plan, the
-append of the new tokens and the attention over them.
+``step`` runs a serving step's calls one after another: the append of the new
+tokens and the attention over them.  Every pass of every operator begins with
+the batch's plan, as a new batch does; a program with many layers makes it once
+for all of them.
 
 With ``own`` false, ``run`` computes in elementary torch operations.
 """
@@ -237,7 +239,7 @@ def prepare(case, seed):
 
 
 def _open(st, hist_k, hist_v):
-    """The framework's cache with the same contents, and the batch's plan."""
+    """The framework's cache with the same contents, and the outputs."""
     import sys
     if "tt-lab_b200/python" not in sys.path:
         sys.path.insert(0, "tt-lab_b200/python")
@@ -255,7 +257,6 @@ def _open(st, hist_k, hist_v):
         off = torch.tensor([0] + length).cumsum(0).to(torch.int32).cuda()
         cache.batch_async(off, st["length"], st["table"], rows=sum(length), max_new=max(length))
         cache.append_async(0, hist_k, hist_v, rotate=False)
-    _plan(st)
     st["out"] = torch.empty(st["q"].shape, dtype=st["q"].dtype, device="cuda")
     st["q_out"] = torch.empty_like(st["out"])
     st["k_out"] = torch.empty(st["k"].shape, dtype=st["k"].dtype, device="cuda")
@@ -273,13 +274,13 @@ def run(st):
     kind = st["case"]["kind"]
     if own:
         c = st["cache"]
+        _plan(st)  # a new batch's rows, lengths, masks and pages are part of every pass, as in the plain form
         if kind == "append":
             c.append_async(0, st["k"], st["v"], q=st["q"], q_out=st["q_out"])
             c.read_async(0, st["k_out"], st["v_out"])
             return {"q": st["q_out"], "k": st["k_out"], "v": st["v_out"]}
         q = st["q"]
         if kind == "step":
-            _plan(st)
             c.append_async(0, st["k"], st["v"], q=st["q"], q_out=st["q_out"])
             q = st["q_out"]
         c.attend_async(0, q, st["out"], sinks=st["sinks"], slopes=st["slopes"], cap=st["case"]["cap"],
