@@ -19,11 +19,13 @@
  * nothing, never wait, and may be captured into a CUDA graph (capture on the
  * handle's stream).  Calls on one handle, and graphs captured from them, share
  * the handle's plan and workspace: they must run one after another, never at
- * the same time on two streams.  A graph that holds an append or attend
+ * the same time on two streams.  A graph that holds an append, read or attend
  * without its batch call uses the plan of the last batch call that ran on the
  * device; where that plan has another shape of work than the captured one,
- * ttl_kv_sync reports it.  It touches as many rows of its arrays as the batch
- * had when it was captured.
+ * ttl_kv_sync reports it.  It reads as many rows of its arrays as the batch
+ * had when it was captured; an append or read of another number of rows than
+ * the plan's is reported, and only the rows that both have are stored or
+ * written.
  *
  * What only the device can see (row_start, length, page ids) is checked there:
  * a sequence with bad numbers is skipped (its rows are left as they were), a

@@ -874,6 +874,93 @@ def test_a_plan_of_another_shape_is_reported():
     s.cache.close()
 
 
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f32", "mxfp4"), ("bf16", "mxfp4")])
+@pytest.mark.parametrize("small", [((0, 8), (24,)), ((0, 3), (3,)), ((0, 40, 44), (60, 9))])
+def test_a_graph_of_appends_after_a_batch_of_other_rows(rows, cache, small):
+    """Append and read captured with 32 rows of four sequences, replayed after a
+    batch of fewer or more rows and sequences whose page table is shorter: the
+    rows that both have are stored, no other slot changes, and the difference is
+    reported."""
+    st = torch.cuda.Stream()
+    s = Setup(rows, cache, 4, 2, 64, 16, new=(8, 8, 8, 8), length=(40, 24, 60, 33), stream=st)
+    torch.cuda.synchronize()
+    s.fill()
+    c, d, total = s.cache, s.dev, sum(s.length)
+
+    def whole():
+        """Every token of every sequence, as the cache holds it."""
+        off = torch.tensor(s.tok0, dtype=torch.int32).cuda()
+        kv = [torch.zeros_like(d["k"]), torch.zeros_like(d["v"])]
+        torch.cuda.synchronize()
+        c.batch_async(off, d["length"], d["table"], rows=total)
+        c.read_async(0, *kv)
+        c.sync()
+        return kv
+
+    g = torch.Generator().manual_seed(8)
+    k, v = (torch.randn(32, 2, 64, generator=g).to(s.dt).cuda() for _ in range(2))
+    q, q_out = torch.ones_like(d["q"]), torch.full_like(d["q"], 7.0)
+    k2, v2 = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+    before = whole()
+    s.plan()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        c.append_async(0, k, v, q=q, q_out=q_out)
+        c.read_async(0, k2, v2)
+    start, length = (torch.tensor(x, dtype=torch.int32).cuda() for x in small)
+    table = d["table"][2:2 + len(small[1])].contiguous()  # the third sequence's pages (and the fourth's)
+    torch.cuda.synchronize()
+    n = min(32, small[0][-1])
+    c.batch_async(start, length, table, rows=small[0][-1])
+    with torch.cuda.stream(st):
+        graph.replay()
+    with pytest.raises(RuntimeError, match="another shape"):
+        c.sync()
+    c.sync()  # once
+    held = [kv_plain.held(x.cpu().double(), cache).to(s.dt) for x in (k, v)]
+    for got, want in zip((k2, v2), held):
+        assert torch.equal(got[:n].cpu(), want[:n]) and (got[n:] == 7).all()
+    assert (q_out[:n] == 1).all() and (q_out[n:] == 7).all()
+    at = s.tok0[2] + torch.arange(n) + small[1][0] - (small[0][1] - small[0][0])
+    for now, was, want in zip(whole(), before, held):
+        was[at] = want[:n].cuda()
+        assert torch.equal(now, was)
+
+
+def test_calls_after_a_batch_that_was_only_captured():
+    """A batch call inside a capture runs nothing: append, read and attend after
+    it meet the plan of the batch before, or none, and say so."""
+    st = torch.cuda.Stream()
+    s = Setup("bf16", None, 4, 2, 64, 16, new=(6,), length=(20,), stream=st)
+    k, v = s.dev["k"][:6].contiguous(), s.dev["v"][:6].contiguous()
+    outs = [torch.full_like(x, 7.0) for x in (s.dev["q"], s.dev["q"], k, v)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        s.plan()
+    for earlier in (False, True):
+        for call in (lambda: s.cache.append_async(0, k, v, q=s.dev["q"], q_out=outs[0]),
+                     lambda: s.cache.read_async(0, outs[2], outs[3])):
+            call()
+            with pytest.raises(RuntimeError, match="another shape"):
+                s.cache.sync()
+        n = 2 if earlier else 0
+        for o in (outs[0], outs[2], outs[3]):
+            assert (o[n:] == 7).all()
+        if earlier:
+            break
+        s.cache.batch_async(torch.tensor([0, 2], dtype=torch.int32).cuda(), s.dev["length"], s.dev["table"], rows=2)
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=st):
+            s.plan()
+    # the captured batch, once it has run, is the plan
+    with torch.cuda.stream(st):
+        graph.replay()
+    s.cache.append_async(0, k, v, q=s.dev["q"], q_out=outs[0])
+    s.cache.read_async(0, outs[2], outs[3])
+    s.cache.sync()
+    assert torch.equal(outs[0], s.dev["q"]) and torch.equal(outs[2], k) and torch.equal(outs[3], v)
+
+
 def test_refusals():
     import ttl_moe
     s = Setup("bf16", None, 8, 2, 64, 16, new=(2,), length=(5,))

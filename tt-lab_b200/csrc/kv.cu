@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
         a.plan->pages = a.pages;
         a.plan->page_stride = a.page_stride;
         a.plan->seqs = a.seqs;
+        a.plan->rows = a.rows;
         if (a.row_start[0] != 0) {
             ttl::set_status(a.status, kKvBadBatch);
         }
@@ -382,6 +383,21 @@ __device__ __forceinline__ int quotient(int i, uint32_t div) {
     return int(__umulhi(uint32_t(i), div));
 }
 
+// A row of the plan on the device.  A captured call may have more rows than the
+// batch that ran last: what the table holds behind that batch's rows is another's
+// (or nobody's), and such a row is padding.
+template <class Args> __device__ __forceinline__ int4 planned_row(const Args &a, int r) {
+    int4 x = a.row[r];  // a.rows entries are there, whoever's; neither load waits for the other
+    x.w = r < a.plan->rows ? x.w : -1;
+    return x;
+}
+// Reports a plan of another number of rows (one thread of the grid).
+template <class Args> __device__ __forceinline__ void check_rows_of_plan(const Args &a) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.plan->rows != a.rows) {
+        ttl::set_status(a.status, kKvStalePlan);
+    }
+}
+
 // The slot of a row: the block of (page, head 0) and the token in it, or
 // nullptr for padding and for a page outside the pool.
 template <class Args> __device__ __forceinline__ uint8_t *row_slot(const Args &a, const int4 &ri, int &token) {
@@ -566,8 +582,9 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(AppendArgs
         unit = decode(i);
         load(unit);
     }
+    check_rows_of_plan(a);
     for (int r = tid; r < count; r += threads) {
-        const int4 ri = a.row[r0 + r];
+        const int4 ri = planned_row(a, r0 + r);
         int token = 0;
         slots[r] = is_q ? nullptr : row_slot(a, ri, token);
         tokens[r] = token;
@@ -719,9 +736,10 @@ template <int kRows, int kCache, int D> __global__ void __launch_bounds__(256) k
     wait_previous();
     const int tid = threadIdx.x, r0 = blockIdx.x * a.per_cta;
     const int count = min(a.per_cta, a.rows - r0);
+    check_rows_of_plan(a);
     if (tid < count) {
         int token = 0;
-        slots[tid] = row_slot(a, a.row[r0 + tid], token);
+        slots[tid] = row_slot(a, planned_row(a, r0 + tid), token);
         tokens[tid] = token;
     }
     __syncthreads();

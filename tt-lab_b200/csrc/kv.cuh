@@ -57,7 +57,7 @@ struct List {
 struct Plan {
     const int32_t *pages;
     uint32_t page_stride;
-    int32_t seqs;
+    int32_t seqs, rows;            // rows: entries of Walk::row that are this batch's
     List list[kKinds][2];          // [kind][0 full, 1 sliding]
 };
 
