@@ -21,11 +21,11 @@
  * the handle's plan and workspace: they must run one after another, never at
  * the same time on two streams.  A graph that holds an append, read or attend
  * without its batch call uses the plan of the last batch call that ran on the
- * device; where that plan has another shape of work than the captured one,
- * ttl_kv_sync reports it.  It reads as many rows of its arrays as the batch
- * had when it was captured; an append or read of another number of rows than
- * the plan's is reported, and only the rows that both have are stored or
- * written.
+ * device.  It reads as many rows of its arrays as the batch had when it was
+ * captured; where the plan has another number of rows, ttl_kv_sync reports it,
+ * and only the rows that both have are stored or written.  Where an attend's
+ * plan asks for other kernels than the captured ones (max_new and the number of
+ * sequences choose them), ttl_kv_sync reports it and out is left as it was.
  *
  * What only the device can see (row_start, length, page ids) is checked there:
  * a sequence with bad numbers is skipped (its rows are left as they were), a

@@ -927,6 +927,81 @@ def test_a_graph_of_appends_after_a_batch_of_other_rows(rows, cache, small):
         assert torch.equal(now, was)
 
 
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "mxfp4")])
+@pytest.mark.parametrize("sliding", [False, True])
+def test_a_graph_of_tokens_after_a_batch_with_a_prompt(rows, cache, sliding):
+    """Beside a prompt, tokens have tiles as wide as without one: a graph that
+    launches their kernel alone would leave the prompt out."""
+    st = torch.cuda.Stream()
+    s = Setup(rows, cache, 8, 1, 64, 16, new=(1, 90, 1), length=(150, 140, 200), window=30, stream=st)
+    one = torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()
+    torch.cuda.synchronize()
+    s.fill()
+    d, out = s.dev, torch.full_like(s.dev["q"], 7.0)
+    torch.cuda.synchronize()
+    s.cache.batch_async(one, d["length"], d["table"], rows=s.rows, max_new=1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        s.cache.attend_async(0, d["q"], out, sliding=sliding)
+    with torch.cuda.stream(st):
+        graph.replay()
+    s.cache.sync()  # its own plan
+    assert (out[:3] != 7).any() and (out[3:] == 7).all()
+    out.fill_(7.0)
+    torch.cuda.synchronize()
+    s.plan()
+    with torch.cuda.stream(st):
+        graph.replay()
+    with pytest.raises(RuntimeError, match="another shape"):
+        s.cache.sync()
+    assert (out == 7).all()
+    # and the other way round
+    mixed = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(mixed, stream=st):
+        s.cache.attend_async(0, d["q"], out, sliding=sliding)
+    s.cache.batch_async(one, d["length"], d["table"], rows=s.rows, max_new=1)
+    with torch.cuda.stream(st):
+        mixed.replay()
+    with pytest.raises(RuntimeError, match="another shape"):
+        s.cache.sync()
+    assert (out == 7).all()
+
+
+@pytest.mark.parametrize("rows", ["bf16", "f32"])
+def test_a_graph_of_attention_after_a_batch_of_other_rows(rows):
+    """The same kernels, another number of rows: those that both have are
+    written, and the difference is reported."""
+    st = torch.cuda.Stream()
+    s = Setup(rows, None, 8, 2, 64, 16, new=(1,) * 6, length=(30, 41, 52, 3, 64, 75), stream=st)
+    torch.cuda.synchronize()
+    s.fill()
+    d, out = s.dev, torch.full_like(s.dev["q"], 7.0)
+    ref, tol = s.reference()
+    torch.cuda.synchronize()
+
+    def batch(n):
+        s.cache.batch_async(d["start"][:n + 1].contiguous(), d["length"][:n].contiguous(), d["table"], rows=n, max_new=1)
+
+    batch(4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        s.cache.attend_async(0, d["q"], out)
+    for n in (6, 2, 4):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        batch(n)
+        with torch.cuda.stream(st):
+            graph.replay()
+        if n == 4:
+            s.cache.sync()
+        else:
+            with pytest.raises(RuntimeError, match="another shape"):
+                s.cache.sync()
+        m = min(n, 4)
+        assert ((out[:m].cpu().double() - ref[:m]).abs() <= tol[:m]).all()
+        assert (out[m:] == 7).all()
+
+
 def test_calls_after_a_batch_that_was_only_captured():
     """A batch call inside a capture runs nothing: append, read and attend after
     it meet the plan of the batch before, or none, and say so."""

@@ -1257,6 +1257,7 @@ int kv_attend(ttl_kv *h, int layer, uint32_t flags, const void *q, size_t q_stri
         a.cap = cap;
         a.rows = h->rows, a.group = h->q_heads / h->kv_heads, a.page_shift = h->page_shift, a.pages = h->pages;
         a.kv_heads = h->kv_heads, a.block_bytes = h->block_bytes;
+        a.other_ctas = h->ctas[1 - kind];
         a.group_div = uint32_t(((1 << 20) + a.group - 1) / a.group);
         TTL_KV_CUDA(h, launch_attend(*h, a, kind, layer));
     }

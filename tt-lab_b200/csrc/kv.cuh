@@ -50,7 +50,7 @@ struct __align__(16) Cut {
     int32_t head, tile, gran;      // gran: granules into the tile
     uint32_t span;                 // gran > 0: first and last CTA (<< 16) that hold a part of the tile
 };
-struct List {
+struct __align__(16) List {
     int32_t tiles, ctas, width, gran;
     int32_t pad[4];
 };
@@ -88,6 +88,7 @@ struct AttendArgs {
     uint32_t *status;
     float scale, cap;              // natural units; cap 0: none
     int rows, group, page_shift, pages, kv_heads;
+    int other_ctas;                // of the call's launch of the other kind (0: none)
     uint32_t block_bytes;          // one KV head of a page
     uint32_t group_div;            // ceil(2^20 / group)
 
@@ -239,6 +240,21 @@ __device__ __forceinline__ float capped(float dot, float in, float out) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(e) + 1.0f));
     const float small = out * y * fmaf(t, fmaf(t, 0.12841587f, -0.33321908f), 0.99999958f);
     return t <= 0.0625f ? small : fmaf(-2.0f * out, r, out);
+}
+
+// Whether the plan on the device is of this call's shape; where it is not, says so.
+// A captured call may meet the plan of another batch.  That plan's work may lie
+// with the other kind as well, which the call did not launch, so both kinds are
+// compared; rows that the call's arrays lack are left out and reported.
+__device__ __forceinline__ bool plan_fits(const AttendArgs &a, int width, int gran) {
+    const List *lists = &a.walk.plan->list[0][0];  // [kind][window]
+    const int4 mine = *reinterpret_cast<const int4 *>(a.walk.list);
+    const int other = lists[(a.walk.list - lists) ^ 2].ctas, rows = a.walk.plan->rows;  // three loads at once
+    const bool fits = (mine.y == int(gridDim.x)) & (mine.z == width) & (mine.w == gran) & (other == a.other_ctas);
+    if (threadIdx.x == 0 && (!fits || (blockIdx.x == 0 && rows != a.rows))) {
+        set_status(a.status, kKvStalePlan);
+    }
+    return fits;
 }
 
 // ---- the walk ----

@@ -50,10 +50,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Plan &plan = *a.walk.plan;
     wait_previous();
-    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != CT || a.walk.list->gran != kSimpleGran) {
-        if (tid == 0) {
-            set_status(a.status, kKvStalePlan);
-        }
+    if (!plan_fits(a, CT, kSimpleGran)) {
         return;
     }
     constexpr int kD4 = D / 4;

@@ -799,10 +799,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5;
     const Plan &plan = *a.walk.plan;
     wait_previous();
-    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kPromptWidth || a.walk.list->gran != kGran) {
-        if (tid == 0) {
-            set_status(a.status, kKvStalePlan);
-        }
+    if (!plan_fits(a, kPromptWidth, kGran)) {
         return;
     }
     if (tid == 0) {

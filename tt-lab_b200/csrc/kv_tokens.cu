@@ -339,10 +339,7 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
     }
     __syncthreads();
     wait_previous();
-    if (a.walk.list->ctas != int(gridDim.x) || a.walk.list->width != kCols || a.walk.list->gran != T::kGran) {
-        if (tid == 0) {
-            set_status(a.status, kKvStalePlan);
-        }
+    if (!plan_fits(a, kCols, T::kGran)) {
         return;
     }
     if (warp == kWarps) {
