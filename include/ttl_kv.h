@@ -17,7 +17,9 @@
  * device memory is allocated in ttl_kv_create.  The _async calls take device
  * pointers of the handle's GPU, enqueue on the handle's stream, allocate
  * nothing, never wait, and may be captured into a CUDA graph (capture on the
- * handle's stream).  Calls on one handle, and graphs captured from them, share
+ * handle's stream; a batch call inside a capture sets the row count and the
+ * kernels of the calls that follow it, captured or not, though the plan on the
+ * device is still the earlier one).  Calls on one handle, and graphs captured from them, share
  * the handle's plan and workspace: they must run one after another, never at
  * the same time on two streams.  A graph that holds an append, read or attend
  * without its batch call uses the plan of the last batch call that ran on the

@@ -1015,13 +1015,15 @@ def test_calls_after_a_batch_that_was_only_captured():
         s.plan()
     for earlier in (False, True):
         for call in (lambda: s.cache.append_async(0, k, v, q=s.dev["q"], q_out=outs[0]),
-                     lambda: s.cache.read_async(0, outs[2], outs[3])):
+                     lambda: s.cache.read_async(0, outs[2], outs[3]),
+                     lambda: s.cache.attend_async(0, s.dev["q"], outs[1])):
             call()
             with pytest.raises(RuntimeError, match="another shape"):
                 s.cache.sync()
         n = 2 if earlier else 0
+        assert (outs[1] == 7).all()  # two rows make narrower tiles: other kernels
         for o in (outs[0], outs[2], outs[3]):
-            assert (o[n:] == 7).all()
+            assert (o[n:] == 7).all() and (o[:n] != 7).all()
         if earlier:
             break
         s.cache.batch_async(torch.tensor([0, 2], dtype=torch.int32).cuda(), s.dev["length"], s.dev["table"], rows=2)
