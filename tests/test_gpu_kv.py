@@ -423,6 +423,28 @@ def test_the_longest_sequence(rows, cache):
     assert (out == 7).all()
 
 
+def test_pieces_of_more_than_two_seconds():
+    """A prompt of 40 rows of 256 heads behind 2^29 keys of 64 KV heads: a CTA's part
+    of one head takes longer than the two seconds after which a wait gives up, and the
+    next head's tile waits for its end.  (What 2^29 weights sum to in 32 bits is
+    another matter: the values are one, so the result is at most a part's lost
+    fraction from it.)"""
+    import ttl_moe
+    H, KV, n, new = 256, 64, 2 ** 29 - 128, 40
+    with ttl_moe.KvCache(pages=1, page_tokens=128, q_heads=H, kv_heads=KV, max_rows=128, device=0,
+                         stream=torch.cuda.current_stream()) as c:
+        one = torch.ones(128, H, 64, dtype=torch.bfloat16, device="cuda")
+        i32 = lambda *v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+        c.batch_async(i32(0, 128), i32(128), i32(0)[None], rows=128)
+        c.append_async(0, one[:, :KV].contiguous(), one[:, :KV].contiguous())
+        table = torch.zeros(1, 2 ** 22, dtype=torch.int32, device="cuda")
+        c.batch_async(i32(0, new), i32(n), table, rows=new)
+        out = torch.full((new, H, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        c.attend_async(0, one[:new], out)
+        c.sync()
+        assert (out != 7).all() and torch.isfinite(out).all()
+
+
 def test_more_work_than_a_plan_counts_is_refused():
     """257 sequences of the greatest length are 2^31 granules of keys."""
     import ttl_moe

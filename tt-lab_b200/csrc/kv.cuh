@@ -410,16 +410,33 @@ __device__ __forceinline__ bool phase_done(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Waits for a phase of a barrier unless the CTA has given up; a wait of about two
-// seconds gives the CTA up (every later wait returns at once, so that all warps
-// still meet at their barriers and leave).  kSleep lets the hardware put the
+// Waits for a phase of a barrier unless the CTA has given up; about two seconds in
+// which nothing moves give the CTA up (every later wait returns at once, so that all
+// warps still meet at their barriers and leave).  Some waits last as long as a
+// piece of the plan, which has no limit but its keys': the prompt kernel's next
+// tile waits for the last scores of this one.  So what goes through the keys
+// leaves a sign of life, and a wait with kLong that ran out begins again where there
+// is a new one (or any, the first time: four seconds at most after the last); the
+// keys are finite, and so are the waits.  kSleep lets the hardware put the
 // warp to sleep for up to a millisecond a try.  It pays where other warps of the
 // scheduler compute meanwhile.
 constexpr long long kWaitClocks = 4000000000ll;
 
-template <bool kSleep> __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *status) {
+struct Halt {
+    int abort;  // the CTA has given up
+    int beat;   // changes while the CTA gets on
+    __device__ __forceinline__ bool aborted() const {
+        return *const_cast<const volatile int *>(&abort) != 0;
+    }
+    __device__ __forceinline__ void alive() {
+        *const_cast<volatile int *>(&beat) = int(clock());
+    }
+};
+
+template <bool kSleep, bool kLong = false> __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, Halt *halt, uint32_t *status) {
     const uint32_t addr = tc::smem_u32(bar);
     long long start = 0;
+    int beat = 0;
     while (true) {
         uint32_t ok;
         if constexpr (kSleep) {
@@ -436,16 +453,21 @@ template <bool kSleep> __device__ __forceinline__ bool wait_or_abort(uint64_t *b
         if (ok) {
             return true;
         }
-        if (*abort) {
+        if (halt->aborted()) {
             return false;
         }
         const long long now = clock64();
         if (start == 0) {
             start = now;
         } else if (now - start > kWaitClocks) {
-            set_status(status, kKvWait);
-            *abort = 1;
-            return false;
+            const int last = kLong ? *const_cast<volatile int *>(&halt->beat) : 0;
+            if (last == beat) {
+                set_status(status, kKvWait);
+                *const_cast<volatile int *>(&halt->abort) = 1;
+                return false;
+            }
+            start = now;
+            beat = last;
         }
     }
 }

@@ -80,7 +80,8 @@ template <int kCache, int D> struct PromptSmem {
     uint64_t piece_full[2], piece_empty[2], q_full, q_empty;
     uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [warpgroup][half of a granule]
     uint32_t tmem;
-    int last, abort;
+    int last;
+    Halt halt;
 };
 
 __device__ __forceinline__ void arrive(uint64_t *bar) {
@@ -204,7 +205,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
             const int key = k0 + (lane < copies ? s : 0) * seg;
             const int page = __shfl_sync(0xffffffffu, id, (key >> a.page_shift) - base);
             if constexpr (kCache == kMxfp4) {
-                const bool ok = wait_or_abort<true>(&sm.raw_empty[stage], phase ^ 1, &sm.abort, a.status);
+                const bool ok = wait_or_abort<true, true>(&sm.raw_empty[stage], phase ^ 1, &sm.halt, a.status);
                 if (__all_sync(0xffffffffu, ok)) {
                     if (lane == 0) {
                         tc::mbar_expect_tx(&sm.raw_full[stage], PromptSmem<kCache, D>::kRawBytes);
@@ -226,7 +227,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
             }
             const int y = ((page * a.kv_heads + p.head) * 2) * (1 << a.page_shift) + (key & ((1 << a.page_shift) - 1));
             const uint32_t to = uint32_t(x * kGran + s * seg) * 128;
-            bool ok = wait_or_abort<true>(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
+            bool ok = wait_or_abort<true, true>(&sm.k_empty[stage], phase ^ 1, &sm.halt, a.status);
             if (__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.k_full[stage], kGran * D * 2);
@@ -236,7 +237,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                     tc::tma_load_2d(sm.k[stage] + to, map, 64 * x, y, &sm.k_full[stage]);
                 }
             }
-            ok = wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
+            ok = wait_or_abort<true, true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
             if (__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.v_full[stage], kGran * D * 2);
@@ -298,11 +299,11 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
     Piece p;
     while (walk.next(p)) {
         for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
-            wait_or_abort<true>(&sm.raw_full[raw], raw_phase, &sm.abort, a.status);
-            wait_or_abort<true>(&sm.k_empty[stage], phase ^ 1, &sm.abort, a.status);
+            wait_or_abort<true, true>(&sm.raw_full[raw], raw_phase, &sm.halt, a.status);
+            wait_or_abort<true, true>(&sm.k_empty[stage], phase ^ 1, &sm.halt, a.status);
             half(sm.raw[raw] + at, sm.k[stage]);
             arrive(&sm.k_full[stage]);
-            wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.abort, a.status);
+            wait_or_abort<true, true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
             half(sm.raw[raw] + at + (a.block_bytes >> 1), sm.v[stage]);
             arrive(&sm.v_full[stage]);
             arrive(&sm.raw_empty[raw]);
@@ -349,8 +350,8 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
     for (; any; any = more, p = ahead) {
         more = walk.next(ahead);
         const int n = (p.k1 - p.k0) / kGran, halves = p.ncols > kHalf ? 2 : 1;
-        ok = wait_or_abort<true>(&sm.k_full[ks], k_phase, &sm.abort, a.status) && ok;
-        ok = wait_or_abort<true>(&sm.q_full, q_phase, &sm.abort, a.status) && ok;
+        ok = wait_or_abort<true, true>(&sm.k_full[ks], k_phase, &sm.halt, a.status) && ok;
+        ok = wait_or_abort<true, true>(&sm.q_full, q_phase, &sm.halt, a.status) && ok;
         q_phase ^= 1;
         tc::fence_after_sync();
 #pragma unroll
@@ -367,9 +368,12 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
             commit(&sm.q_empty, lead);
         }
         for (int j = 0; j < n; ++j) {
-            ok = wait_or_abort<true>(&sm.v_full[vs], v_phase, &sm.abort, a.status) && ok;
+            if ((j & 255) == 255 && lead && ok) {
+                sm.halt.alive();  // about twice a millisecond
+            }
+            ok = wait_or_abort<true, true>(&sm.v_full[vs], v_phase, &sm.halt, a.status) && ok;
             if (j + 1 < n) {
-                ok = wait_or_abort<true>(&sm.k_full[ks], k_phase, &sm.abort, a.status) && ok;
+                ok = wait_or_abort<true, true>(&sm.k_full[ks], k_phase, &sm.halt, a.status) && ok;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -377,7 +381,7 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     if (w < halves) {
-                        ok = wait_or_abort<true>(&sm.p_full[w][h], (p_phase >> (2 * h + w)) & 1u, &sm.abort, a.status) && ok;
+                        ok = wait_or_abort<true, true>(&sm.p_full[w][h], (p_phase >> (2 * h + w)) & 1u, &sm.halt, a.status) && ok;
                         p_phase ^= 1u << (2 * h + w);
                         tc::fence_after_sync();
                         if (!__all_sync(0xffffffffu, ok)) {
@@ -421,7 +425,7 @@ template <int kCache, int D> __device__ __forceinline__ void scout(const AttendA
     for (int side = 0;; side ^= 1) {
         const bool more = walk.next(p);
         p.ncols = more ? p.ncols : 0;
-        wait_or_abort<true>(&sm.piece_empty[side], side_phase ^ 1, &sm.abort, a.status);
+        wait_or_abort<true, true>(&sm.piece_empty[side], side_phase ^ 1, &sm.halt, a.status);
         side_phase ^= uint32_t(side);
         if (lane == 0) {
             sm.piece[side] = p;
@@ -430,7 +434,7 @@ template <int kCache, int D> __device__ __forceinline__ void scout(const AttendA
         if (!more) {
             break;
         }
-        wait_or_abort<true>(&sm.q_empty, q_phase ^ 1, &sm.abort, a.status);
+        wait_or_abort<true, true>(&sm.q_empty, q_phase ^ 1, &sm.halt, a.status);
         q_phase ^= 1;
         const int columns = p.ncols > kHalf ? 2 * kHalf : kHalf;
         for (int i = lane; i < columns * (D / 8); i += 64) {
@@ -536,7 +540,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
     uint32_t phase = 0;       // of the granule, for the barriers of both halves
     uint32_t side_phase = 0;
     for (int side = 0;; side ^= 1) {
-        bool ok = wait_or_abort<true>(&sm.piece_full[side], side_phase, &sm.abort, a.status);
+        bool ok = wait_or_abort<true>(&sm.piece_full[side], side_phase, &sm.halt, a.status);
         side_phase ^= uint32_t(side);
         const Piece &p = sm.piece[side];
         // all softmax warps go on with the tile, or none
@@ -562,7 +566,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
             for (int k0 = begin; k0 < end; k0 += kKeys, h ^= 1) {
                 const uint32_t now = phase;
                 phase ^= uint32_t(h);
-                ok = ready || wait_or_abort<true>(&sm.s_full[w][h], now, &sm.abort, a.status);
+                ok = ready || wait_or_abort<true>(&sm.s_full[w][h], now, &sm.halt, a.status);
                 if (!__all_sync(0xffffffffu, ok)) {
                     continue;
                 }
@@ -660,7 +664,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                         // rescale their sums.  (A barrier per half: the scores in hand came
                         // behind this half's last product, so no barrier is ever more than
                         // the one phase behind that its parity can tell.)
-                        wait_or_abort<true>(&sm.o_done[w][h ^ 1], now ^ uint32_t(h ^ 1), &sm.abort, a.status);
+                        wait_or_abort<true>(&sm.o_done[w][h ^ 1], now ^ uint32_t(h ^ 1), &sm.halt, a.status);
                         __syncwarp();
                         tc::fence_after_sync();
 #pragma unroll 1
@@ -723,8 +727,8 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
         }
         bool bad = false;
         if (active) {
-            ok = wait_or_abort<true>(&sm.o_done[w][0], phase ^ 1, &sm.abort, a.status) && ok;
-            ok = wait_or_abort<true>(&sm.o_done[w][1], phase ^ 1, &sm.abort, a.status) && ok;
+            ok = wait_or_abort<true>(&sm.o_done[w][0], phase ^ 1, &sm.halt, a.status) && ok;
+            ok = wait_or_abort<true>(&sm.o_done[w][1], phase ^ 1, &sm.halt, a.status) && ok;
             tc::fence_after_sync();
             const float l = (l0 + l1) + (l2 + l3);
             float g = 1.0f;
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
         }
         tc::mbar_init(&sm.q_full, 64);
         tc::mbar_init(&sm.q_empty, 1);
-        sm.abort = 0;
+        sm.halt = Halt{0, 0};
         tc::fence_mbar_init();
     }
     if (warp == kIssuer) {
@@ -853,7 +857,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
     tc::fence_before_sync();
     __syncthreads();
     if (warp == kIssuer) {
-        if (*const_cast<volatile int *>(&sm.abort)) {
+        if (sm.halt.aborted()) {
             // copies and products that are still in flight end before their memory goes
             for (uint32_t ph = 0; ph < 2; ++ph) {
                 for (int i = 0; i < Smem::kStages; ++i) {

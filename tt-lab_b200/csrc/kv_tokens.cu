@@ -94,7 +94,8 @@ template <int kRows, int kCache, int D, int NT> struct TokenSmem {
     float slope[2][T::kCols], sink[2][T::kCols];
     uint64_t tile_full[2], tile_empty[2];
     uint64_t full[T::kStages], empty[T::kStages];
-    int last, abort;
+    int last;
+    Halt halt;
 };
 
 __device__ __forceinline__ void consumer_sync() {
@@ -203,7 +204,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     int side = 0;
     uint32_t side_phase = 0;
     auto hand_over = [&](const Piece &p) {
-        wait_or_abort<false>(&sm.tile_empty[side], side_phase ^ 1, &sm.abort, a.status);
+        wait_or_abort<false>(&sm.tile_empty[side], side_phase ^ 1, &sm.halt, a.status);
         __syncwarp();
         if (lane == 0) {
             sm.piece[side] = p;
@@ -253,7 +254,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                 base = k0 >> a.page_shift;
                 id = checked(p, base, ids(p, base));
             }
-            const bool free = wait_or_abort<false>(&sm.empty[stage], phase ^ 1, &sm.abort, a.status);
+            const bool free = wait_or_abort<false>(&sm.empty[stage], phase ^ 1, &sm.halt, a.status);
             if (__all_sync(0xffffffffu, free)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.full[stage], kStageBytes);
@@ -303,7 +304,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     p.ncols = 0;
     hand_over(p);
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (*const_cast<volatile int *>(&sm.abort)) {
+    if (sm.halt.aborted()) {
         // what is still in flight lands before the shared memory goes away
         for (int i = 0; i < kStages; ++i) {
             tc::mbar_wait(&sm.full[i], 0, 1000000ull);
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
             tc::mbar_init(&sm.tile_full[i], 64);
             tc::mbar_init(&sm.tile_empty[i], kWarps);
         }
-        sm.abort = 0;
+        sm.halt = Halt{0, 0};
         tc::fence_mbar_init();
     }
     __syncthreads();
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
     uint32_t phase = 0;
     uint32_t side_phase = 0;
     for (int side = 0;; side ^= 1) {
-        const bool ok = wait_or_abort<false>(&sm.tile_full[side], side_phase, &sm.abort, a.status);
+        const bool ok = wait_or_abort<false>(&sm.tile_full[side], side_phase, &sm.halt, a.status);
         side_phase ^= uint32_t(side);
         // all warps go on with the tile, or none
         if (consumers_any(!ok || sm.piece[side].ncols == 0)) {
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
         }
         const int end = p.k1;
         for (int k0 = p.k0; k0 < end; k0 += T::kGran) {
-            wait_or_abort<false>(&sm.full[stage], phase, &sm.abort, a.status);
+            wait_or_abort<false>(&sm.full[stage], phase, &sm.halt, a.status);
             const int key0 = k0 + 16 * kSub * warp;
             if (key0 < hi_max && key0 + 16 * kSub > lo_min) {
                 const uint32_t buf = tc::smem_u32(sm.stage[stage]);
