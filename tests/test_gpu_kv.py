@@ -500,6 +500,82 @@ def test_unseen_infinities_and_nan_do_not_reach_a_row(rows, cache, new):
         assert ((out.double() - ref).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("rows,cache", COMBOS)
+@pytest.mark.parametrize("D,new,length", [(64, (1,), (9000,)), (128, (3, 2), (5003, 700)), (64, (60,), (6000,)), (128, (40, 1), (4100, 300))])
+def test_infinities_and_nan_in_work_that_is_cut(rows, cache, D, new, length):
+    """Sequences that several CTAs share: a NaN key that no row sees, an infinite
+    value that every other row sees, and NaN behind the end of the last page.  The
+    rows that see the value have it in its place (4 bits: in its block of 32), and
+    nothing else has."""
+    H, KV, at = 8, 2, length[0] // 2
+    first = [(at + 1 if i % 2 else at - 300) if i < new[0] else 0 for i in range(sum(new))]
+    s = Setup(rows, cache, H, KV, D, 16, new=new, length=length, first=first, seed=5)
+    s.v[at] = 0
+    s.dev["v"] = s.v.cuda()
+    ref, tol = s.reference()
+    s.dev["k"][100] = math.nan
+    s.dev["v"][at, :, 5] = math.inf
+    s.dev["v"][50] = math.nan
+    s.fill()
+    tail = -length[0] % 16
+    if tail:  # the last page's stale slots
+        nan = torch.full((tail, KV, D), math.nan, dtype=s.dt, device="cuda")
+        s.cache.batch_async(torch.tensor([0, tail], dtype=torch.int32).cuda(),
+                            torch.tensor([length[0] + tail], dtype=torch.int32).cuda(), s.dev["table"][:1].contiguous(), rows=tail)
+        s.cache.append_async(0, nan, nan)
+    s.plan()
+    for _ in range(2):
+        out = s.attend()
+        sees = torch.tensor([i < new[0] and i % 2 == 0 for i in range(sum(new))])
+        place = torch.zeros(D, dtype=torch.bool)
+        place[0:32 if cache == "mxfp4" else 6] = True
+        place[0:0 if cache == "mxfp4" else 5] = False
+        good = ~(sees[:, None, None] & place).expand_as(out)
+        assert ((out.double() - ref).abs() <= tol)[good].all()
+        assert (~torch.isfinite(out))[~good].all()
+
+
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "mxfp4"), ("f16", "mxfp4")])
+@pytest.mark.parametrize("where", ["unseen", "seen"])
+def test_a_nan_in_a_long_prompt_stays_small(rows, cache, where):
+    """320 columns over 65536 keys, every one of which has to be computed again,
+    beside a short sequence: the call ends in time (one column after the other by
+    one warp takes seconds, and a wait then gave the others up), the short
+    sequence is right, and the long one is where it does not see the NaN."""
+    n, new = 65536, 40
+    s = Setup(rows, cache, 8, 1, 64, 64, new=(new, 3), length=(n, 90), first=[1000] * new + [0] * 3, seed=6)
+    s.dev["v"][999 if where == "unseen" else 1000, 0, 40] = math.nan
+    s.fill().plan()
+    s.attend()
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    out = torch.full_like(s.dev["q"], 7.0)
+    begin.record()
+    s.cache.attend_async(0, s.dev["q"], out)
+    end.record()
+    s.cache.sync()
+    assert begin.elapsed_time(end) < 100.0
+    out = out.cpu()
+    ref, tol = s.reference()
+    bad = slice(32, 64) if cache == "mxfp4" else slice(40, 41)
+    if where == "seen":
+        assert torch.isnan(out[:new, :, bad]).all()
+        out[:new, :, bad] = ref[:new, :, bad].to(out.dtype)
+    assert ((out.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("rows,cache", COMBOS)
+@pytest.mark.parametrize("new", [1, 50])
+def test_infinite_sinks(rows, cache, new):
+    """A sink of infinity takes all the weight, one of minus infinity none."""
+    s = Setup(rows, cache, 8, 2, 64, 16, new=(new,), length=(3000,))
+    sinks = torch.tensor([math.inf, -math.inf] * 4)
+    s.fill().plan()
+    out = s.attend(sinks=sinks.cuda())
+    ref, tol = s.reference()
+    assert (out[:, 0::2] == 0).all()
+    assert ((out.double() - ref).abs() <= tol)[:, 1::2].all()
+
+
 @pytest.mark.parametrize("rows,cache", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f16", "mxfp4")])
 def test_seen_infinities_and_nan_do(rows, cache):
     """A row that sees a NaN or infinite value has it in its result, as the

@@ -209,6 +209,21 @@ template <int kRows> __device__ __forceinline__ void load8(const void *base, siz
     }
 }
 
+// Eight values of a pool row, from a multiple of 8 on.
+template <int kCache, int D> __device__ __forceinline__ void pool8(const uint8_t *rows, int tokens, int t, int d, float (&x)[8]) {
+    if constexpr (kCache != kMxfp4) {
+        load8<kCache>(rows, size_t(t) * D + d, x);
+    } else {
+        const uint32_t codes = *reinterpret_cast<const uint32_t *>(rows + t * (D / 2) + d / 2);
+        const float f = scale_of(rows[tokens * (D / 2) + t * (D / 32) + d / 32]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 v = __half22float2(e2m1x2_to_half2((codes >> (8 * j)) & 255u));
+            x[2 * j] = v.x * f, x[2 * j + 1] = v.y * f;
+        }
+    }
+}
+
 // Page id of position `pos` of a sequence; an id outside the pool is reported
 // and read as page 0.  The caller keeps pos below the sequence's length.
 __device__ __forceinline__ int page_of(const Plan &plan, int seq, int pos, int page_shift, int pages, uint32_t *status) {
@@ -410,23 +425,27 @@ __device__ __forceinline__ bool phase_done(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Waits for a phase of a barrier unless the CTA has given up; about two seconds in
-// which nothing moves give the CTA up (every later wait returns at once, so that all
-// warps still meet at their barriers and leave).  Some waits last as long as a
-// piece of the plan, which has no limit but its keys': the prompt kernel's next
-// tile waits for the last scores of this one.  So what goes through the keys
-// leaves a sign of life, and a wait with kLong that ran out begins again where there
-// is a new one (or any, the first time: four seconds at most after the last); the
-// keys are finite, and so are the waits.  kSleep lets the hardware put the
+// Waits for a phase of a barrier unless the CTA has given up; a wait of about two
+// seconds gives the CTA up (every later wait returns at once, so that all warps
+// still meet at their barriers and leave).  kSleep lets the hardware put the
 // warp to sleep for up to a millisecond a try.  It pays where other warps of the
 // scheduler compute meanwhile.
+//
+// Two things take as long as their keys are many, and their time does not count.
+// While warps compute columns again (`Halt::busy`) nobody gives up.  And the prompt
+// kernel's next tile waits for the last scores of the one in hand, over all the keys
+// of its piece: such a wait (kLong) begins again where the beat that goes with the
+// keys has changed.  The keys are finite, and so are these waits.
 constexpr long long kWaitClocks = 4000000000ll;
 
 struct Halt {
-    int abort;  // the CTA has given up
+    int state;  // bit 0: the CTA has given up; above: warps that compute columns again
     int beat;   // changes while the CTA gets on
     __device__ __forceinline__ bool aborted() const {
-        return *const_cast<const volatile int *>(&abort) != 0;
+        return *const_cast<const volatile int *>(&state) & 1;
+    }
+    __device__ __forceinline__ void busy(bool on) {
+        atomicAdd(&state, on ? 2 : -2);
     }
     __device__ __forceinline__ void alive() {
         *const_cast<volatile int *>(&beat) = int(clock());
@@ -453,17 +472,18 @@ template <bool kSleep, bool kLong = false> __device__ __forceinline__ bool wait_
         if (ok) {
             return true;
         }
-        if (halt->aborted()) {
+        const int state = *const_cast<volatile int *>(&halt->state);
+        if (state & 1) {
             return false;
         }
         const long long now = clock64();
-        if (start == 0) {
+        if (start == 0 || state) {
             start = now;
         } else if (now - start > kWaitClocks) {
             const int last = kLong ? *const_cast<volatile int *>(&halt->beat) : 0;
             if (last == beat) {
                 set_status(status, kKvWait);
-                *const_cast<volatile int *>(&halt->abort) = 1;
+                atomicOr(&halt->state, 1);
                 return false;
             }
             start = now;
@@ -487,68 +507,137 @@ __device__ __forceinline__ int part_slot(int c, int first) {
     return 2 * c + (c == first ? 1 : 0);
 }
 
-// ---- rows with infinities or NaN ----
-// One column computed key by key by a warp, over the keys it sees and no
-// others.  The matrix products multiply every value of a tile, so an infinity
-// or NaN in a place that a column does not see reaches its sum as 0 * x; any
-// column whose result is not finite is computed again here, where unseen keys
-// are not touched.
-template <int kRows, int kCache, int D>
-__device__ __noinline__ void attend_column(const AttendArgs &a, const Plan &plan, int head, int seq, int len, int row, int qhead) {
+// ---- the end of a tile ----
+
+// The sink's part of a column: adds it to the sum l of weights relative to m, and
+// returns the factor that brings the column's sums to the same measure.  An
+// infinite sink takes everything.
+__device__ __forceinline__ float add_sink(float m, float &l, float sink) {
+    sink *= kLog2e;
+    const float mn = fmaxf(m, sink), safe = mn == -INFINITY ? 0.0f : mn;
+    const float f = exp2f(m - safe);
+    l = l * f + (sink == INFINITY ? 1.0f : exp2f(sink - safe));
+    return f;
+}
+
+// Partial results: [slot][width][part_pitch(D)] floats, a column's D sums, then
+// its maximum and sum; rows of a multiple of 16 bytes.  (Prompts lay the same
+// space out by columns.)
+__host__ __device__ constexpr int part_pitch(int d) {
+    return d + 4;
+}
+constexpr int kPromptColumns = 256;  // of a prompt tile
+
+// ---- columns with infinities or NaN ----
+// The matrix products multiply every value of a tile, so an infinity or NaN in a
+// place that a column does not see reaches its sums as 0 * x.  A column whose sums
+// over a piece of a tile are not finite is computed again over that piece, by a
+// warp, and unseen keys are not touched.  Being cut as the tiles are, this takes the
+// whole GPU for a long sequence too.  Lanes are keys for the scores (each reads its
+// own K row, Q comes by shuffles) and values of the head for the sums, eight V rows
+// in flight; a hundred clocks a key, most of them waiting.
+//
+// The column's sums go over those in the partial result `part` of the piece, laid out
+// as in the kernel for few columns or (kPrompt) in that for prompts; without `part` the
+// piece is a whole tile, and the column is finished and stored.
+template <int kRows, int kCache, int D, bool kPrompt>
+__device__ __forceinline__ void redo_column(const AttendArgs &a, const Piece &p, int c, float *part) {
+    constexpr int kPer = D / 32, kDeep = 8;
     const int lane = threadIdx.x & 31;
-    constexpr int kPer = D / 32;
+    const Plan &plan = *a.walk.plan;
+    int row, qhead;
+    a.column(p, c, row, qhead);
     const int4 ri = a.walk.row[row];
-    const int lo = max(ri.y, 0), hi = min(ri.z, len);
+    const int lo = max(max(ri.y, 0), p.k0), hi = min(min(ri.z, p.len), p.k1);
     const float scale_log2 = a.scale * kLog2e;
     const float slope = a.slopes ? a.slopes[qhead] * kLog2e : 0.0f;
     const int tokens = 1 << a.page_shift;
+    auto block = [&](int page) { return a.pool + (size_t(page) * a.kv_heads + p.head) * a.block_bytes; };
     float q[kPer], o[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        q[i] = row_value<kRows>(a.q, size_t(row) * a.q_stride + size_t(qhead) * D + lane + 32 * i);
+        q[i] = row_value<kRows>(a.q, size_t(row) * a.q_stride + size_t(qhead) * D + lane * kPer + i);
         o[i] = 0.0f;
     }
     float m = -INFINITY, l = 0.0f;
-    if (a.sinks) {
-        m = a.sinks[qhead] * kLog2e;
-        l = m == -INFINITY ? 0.0f : 1.0f;
-    }
-    for (int j = lo; j < hi; ++j) {
-        const int page = page_of(plan, seq, j, a.page_shift, a.pages, a.status);
-        const uint8_t *kb = a.pool + (size_t(page) * a.kv_heads + head) * a.block_bytes;
-        const uint8_t *vb = kb + (a.block_bytes >> 1);
-        const int t = j & (tokens - 1);
+    for (int base = lo; base < hi; base += 32) {
+        const int j = base + lane, n = min(32, hi - base);
+        const bool seen = lane < n;
+        const int page = seen ? page_of(plan, p.seq, j, a.page_shift, a.pages, a.status) : 0;
+        const uint8_t *kb = block(page);
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            s = fmaf(q[i], pool_value<kCache, D>(kb, tokens, t, lane + 32 * i), s);
+        for (int d = 0; d < D; d += 8) {
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (seen) {
+                pool8<kCache, D>(kb, tokens, j & (tokens - 1), d, x);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s = fmaf(__shfl_sync(0xffffffffu, q[i % kPer], (d + i) / kPer), x[i], s);
+            }
         }
-        s = warp_sum(s);
         const float x = a.cap != 0.0f ? a.cap * tanhf(s * a.scale / a.cap) * kLog2e : s * scale_log2;
-        const float z = x - slope * float(abs(ri.x - j));
-        const float mn = (z > m || z != z) ? z : m;
-        const float safe = mn == -INFINITY ? 0.0f : mn;
-        const float up = exp2f(m - safe), p = exp2f(z - safe);
-        l = l * up + p;
+        const float z = seen ? x - slope * float(abs(ri.x - j)) : -INFINITY;
+        float top = z;  // NaN drops out here and is met in the weight
+#pragma unroll
+        for (int off = 16; off; off >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        }
+        const float mn = fmaxf(m, top), safe = mn == -INFINITY ? 0.0f : mn;
+        const float up = exp2f(m - safe), w = seen ? exp2f(z - safe) : 0.0f;
+        m = mn;
+        l = l * up + warp_sum(w);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            o[i] = o[i] * up + p * pool_value<kCache, D>(vb, tokens, t, lane + 32 * i);
+            o[i] *= up;
         }
-        m = mn;
+#pragma unroll 1
+        for (int k0 = 0; k0 < n; k0 += kDeep) {
+            float v[kDeep][kPer];
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const uint8_t *vb = block(__shfl_sync(0xffffffffu, page, k0 + k)) + (a.block_bytes >> 1);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    v[k][i] = k0 + k < n ? pool_value<kCache, D>(vb, tokens, (base + k0 + k) & (tokens - 1), lane * kPer + i) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, w, k0 + k);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    o[i] = fmaf(wk, v[k][i], o[i]);
+                }
+            }
+        }
     }
+    if (part) {
+        float *dst = kPrompt ? part + 4 * c : part + size_t(c) * part_pitch(D);
+        constexpr int kQuad = kPrompt ? 4 * kPromptColumns : 4;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int d = lane * kPer + i;
+            dst[(d >> 2) * kQuad + (d & 3)] = o[i];
+        }
+        if (lane == 0) {
+            *reinterpret_cast<float2 *>(kPrompt ? part + kPromptColumns * D + 2 * c : dst + D) = make_float2(m, l);
+        }
+        return;
+    }
+    const float f = a.sinks ? add_sink(m, l, a.sinks[qhead]) : 1.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        store_value<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + lane + 32 * i,
-                           lo < hi ? o[i] / l : 0.0f);
+        store_value<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + lane * kPer + i, lo < hi ? o[i] * f / l : 0.0f);
     }
 }
-
-// ---- the end of a tile ----
 
 // Adds the sink, divides, rounds and stores columns [c0, ncols) step `step` of
 // a tile, by warps: D / 8 lanes per column, eight values a lane.  value(c, d,
 // v) gives the eight unnormalised sums, stats(c) {max, sum} in log2 units,
-// info(c, row, head) what the column may see.
+// info(c, row, head) what the column may see.  Returns whether the thread stored
+// something that is not finite.
 struct ColumnInfo {
     int lo, hi, seq;
     float sink;
@@ -559,69 +648,45 @@ __device__ __forceinline__ ColumnInfo column_info(const AttendArgs &a, int row, 
     return ColumnInfo{ri.y, ri.z, ri.w, a.sinks ? a.sinks[qhead] : 0.0f};
 }
 
-template <int kRows, int kCache, int D, class Value, class Stats, class Info>
-__device__ __forceinline__ void store_columns(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps,
-                                              Value value, Stats stats, Info info) {
+template <int kRows, int D, class Value, class Stats, class Info>
+__device__ __forceinline__ bool store_columns(const AttendArgs &a, const Piece &p, int warp, int warps, Value value, Stats stats,
+                                              Info info) {
     constexpr int kLanes = D / 8, kCols = 32 / kLanes;
     const int lane = threadIdx.x & 31;
+    bool bad = false;
     for (int base = warp * kCols; base < p.ncols; base += warps * kCols) {
         const int c = base + lane / kLanes;
-        bool bad = false;
-        int row = 0, qhead = 0;
         if (c < p.ncols) {
+            int row, qhead;
             a.column(p, c, row, qhead);
             const ColumnInfo ci = info(c, row, qhead);
             const bool sees = max(ci.lo, 0) < min(ci.hi, p.len);
             const float2 ml = stats(c);
-            float m = ml.x, l = ml.y, f = 1.0f;
-            if (a.sinks) {
-                const float sink = ci.sink * kLog2e;
-                const float mn = fmaxf(m, sink);
-                const float safe = mn == -INFINITY ? 0.0f : mn;
-                f = exp2f(m - safe);
-                l = l * f + exp2f(sink - safe);
-            }
-            f = f / l;
+            float l = ml.y;
+            const float f = (a.sinks ? add_sink(ml.x, l, ci.sink) : 1.0f) / l;
             float v[8];
             value(c, (lane % kLanes) * 8, v);
+            const bool write = row < a.rows && ci.seq == p.seq;  // a row that two sequences claim belongs to the first
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[j] = sees ? v[j] * f : 0.0f;
-                bad = bad || !(fabsf(v[j]) < INFINITY);
+                bad = bad || (write && !(fabsf(v[j]) < INFINITY));
             }
-            if (row < a.rows && ci.seq == p.seq) {  // a row that two sequences claim belongs to the first
+            if (write) {
                 store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + (lane % kLanes) * 8, v);
-            } else {
-                bad = false;
             }
-        }
-        uint32_t redo = __ballot_sync(0xffffffffu, bad);
-        while (redo) {
-            const int src = __ffs(redo) - 1;
-            const int r = __shfl_sync(0xffffffffu, row, src), h = __shfl_sync(0xffffffffu, qhead, src);
-            attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, r, h);
-            const int first = src / kLanes * kLanes;
-            redo &= ~(((kLanes == 32 ? 0u : (1u << kLanes)) - 1u) << first);
         }
     }
-}
-
-// Partial results: [slot][width][part_pitch(D)] floats, a column's D sums, then
-// its maximum and sum; rows of a multiple of 16 bytes.  (Prompts lay the same
-// space out by columns.)
-__host__ __device__ constexpr int part_pitch(int d) {
-    return d + 4;
+    return bad;
 }
 
 // Merges the partial results of a tile over the CTAs [first, last] that hold
 // them, in that order, and stores its columns: D / 4 lanes per column.  The
 // parts come from other SMs through L2, about a microsecond each way, so what
 // counts is how many are asked for at once: kBatch parts' sums and statistics
-// per lane, eight (one token over 131072 keys, 55 parts per head: two parts at a
-// time cost 20 us) unless the registers lack (4 bits, three CTAs per SM: with
-// eight the loop over the keys spills, 64 tokens 104 us, with four 92).
-template <int kRows, int kCache, int D, int kBatch>
-__device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan, const Piece &p, int warp, int warps, int width) {
+// per lane.
+template <int kRows, int D, int kBatch>
+__device__ __forceinline__ void merge_tile(const AttendArgs &a, const Piece &p, int warp, int warps, int width) {
     constexpr int kLanes = D / 4, kCols = 32 / kLanes;
     const int lane = threadIdx.x & 31, sub = lane / kLanes, d = 4 * (lane % kLanes);
     const int parts = p.last - p.first + 1;
@@ -671,43 +736,34 @@ __device__ __forceinline__ void merge_tile(const AttendArgs &a, const Plan &plan
                 }
             }
         }
-        float f = 1.0f;
-        if (a.sinks) {
-            const float sink = ci.sink * kLog2e, mn = fmaxf(m, sink), s = mn == -INFINITY ? 0.0f : mn;
-            f = exp2f(m - s);
-            l = l * f + exp2f(sink - s);
-        }
-        f = f / l;
-        const bool sees = max(ci.lo, 0) < min(ci.hi, p.len), write = have && row < a.rows && ci.seq == p.seq;
-        bool bad = false;
+        const float f = (a.sinks ? add_sink(m, l, ci.sink) : 1.0f) / l;
+        const bool sees = max(ci.lo, 0) < min(ci.hi, p.len);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             o[j] = sees ? o[j] * f : 0.0f;
-            bad = bad || !(fabsf(o[j]) < INFINITY);
         }
-        if (write) {
+        if (have && row < a.rows && ci.seq == p.seq) {
             store4<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + d, o);
-        }
-        const uint32_t redo = __ballot_sync(0xffffffffu, bad && write);
-#pragma unroll
-        for (int s = 0; s < kCols; ++s) {
-            if (redo & ((kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1u) << (s * kLanes))) {
-                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, __shfl_sync(0xffffffffu, row, s * kLanes),
-                                                __shfl_sync(0xffffffffu, qhead, s * kLanes));
-            }
         }
     }
 }
 
 // After a CTA wrote its partial result of a tile: counts it, and returns true
 // in the CTA that arrived last (all threads that `sync` joins, thread 0 among
-// them), with the others' results visible.  That CTA leaves the tile's counter at zero for the next launch.
-template <class Sync> __device__ __forceinline__ bool arrive_last(const AttendArgs &a, const Piece &p, int *flag, Sync sync) {
+// them), with the others' results visible.  A part that is held back is not counted;
+// it arrives later.  That CTA leaves the tile's counter at zero for the next launch.
+struct NeverHeld {
+    __device__ __forceinline__ bool operator()() const {
+        return false;
+    }
+};
+template <class Sync, class Held = NeverHeld>
+__device__ __forceinline__ bool arrive_last(const AttendArgs &a, const Piece &p, int *flag, Sync sync, Held held = Held()) {
     __threadfence();
     sync();
     if (threadIdx.x == 0) {
         const uint32_t parts = uint32_t(p.last - p.first + 1);
-        const bool is_last = atomicAdd(&a.counters[p.first], 1u) + 1u == parts;
+        const bool is_last = !held() && atomicAdd(&a.counters[p.first], 1u) + 1u == parts;
         if (is_last) {
             a.counters[p.first] = 0;
         }

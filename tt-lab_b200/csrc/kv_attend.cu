@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
                 for (int c = 0; c < kPer; ++c) {
                     const int col = cg * kPer + c, j = k0 + key;
                     const bool sees = j >= sm.lo[col] && j < sm.hi[col];
-                    const float t = a.cap != 0.0f ? a.cap * kLog2e * tanhf(acc[c] * a.scale / a.cap) : acc[c] * scale_log2;
+                    const float t = a.cap != 0.0f ? a.cap * tanhf(acc[c] * a.scale / a.cap) * kLog2e : acc[c] * scale_log2;
                     // -1 in the sign of a weight marks an unseen key below
                     sm.s[col * Smem::kSPitch + key] = sees ? t - sm.slope[col] * float(abs(sm.pos[col] - j)) : __uint_as_float(0xffc00001u);
                 }
@@ -219,8 +219,8 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
             __syncthreads();
         }
         if (p.first == p.last) {
-            store_columns<kRows, kCache, D>(
-                a, plan, p, warp, kSimpleThreads / 32,
+            store_columns<kRows, D>(
+                a, p, warp, kSimpleThreads / 32,
                 [&](int c, int d, float(&v)[8]) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
                     }
                 },
                 [&](int c) { return make_float2(sm.m[c], sm.l[c]); },
-                [&](int, int row, int qhead) { return column_info(a, row, qhead); });
+                [&](int, int row, int qhead) { return column_info(a, row, qhead); });  // unseen values were not touched
         } else {
             float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * CT * part_pitch(D);
             for (int i = tid; i < p.ncols * part_pitch(D); i += kSimpleThreads) {
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
                 part[i] = d < D ? sum[c * D + d] : (d == D ? sm.m[c] : sm.l[c]);
             }
             if (arrive_last(a, p, &sm.last, [] { __syncthreads(); })) {
-                merge_tile<kRows, kCache, D, 8>(a, plan, p, warp, kSimpleThreads / 32, CT);
+                merge_tile<kRows, D, 8>(a, p, warp, kSimpleThreads / 32, CT);
             }
         }
         __syncthreads();

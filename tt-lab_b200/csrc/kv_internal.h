@@ -75,7 +75,7 @@ cudaError_t launch_chained(void (*kernel)(Params...), int blocks, int threads, s
 }
 
 constexpr int kNarrow = 8;         // columns of the narrowest tile
-constexpr int kPromptWidth = 256;  // columns of a prompt tile
+constexpr int kPromptWidth = kPromptColumns;
 
 // The kernel for few columns: steps of 16 keys that each of its four warps takes
 // at once.  Two over a 4-bit cache (less bookkeeping per byte) where the

@@ -205,7 +205,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
             const int key = k0 + (lane < copies ? s : 0) * seg;
             const int page = __shfl_sync(0xffffffffu, id, (key >> a.page_shift) - base);
             if constexpr (kCache == kMxfp4) {
-                const bool ok = wait_or_abort<true, true>(&sm.raw_empty[stage], phase ^ 1, &sm.halt, a.status);
+                const bool ok = wait_or_abort<true>(&sm.raw_empty[stage], phase ^ 1, &sm.halt, a.status);
                 if (__all_sync(0xffffffffu, ok)) {
                     if (lane == 0) {
                         tc::mbar_expect_tx(&sm.raw_full[stage], PromptSmem<kCache, D>::kRawBytes);
@@ -227,7 +227,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
             }
             const int y = ((page * a.kv_heads + p.head) * 2) * (1 << a.page_shift) + (key & ((1 << a.page_shift) - 1));
             const uint32_t to = uint32_t(x * kGran + s * seg) * 128;
-            bool ok = wait_or_abort<true, true>(&sm.k_empty[stage], phase ^ 1, &sm.halt, a.status);
+            bool ok = wait_or_abort<true>(&sm.k_empty[stage], phase ^ 1, &sm.halt, a.status);
             if (__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.k_full[stage], kGran * D * 2);
@@ -237,7 +237,7 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                     tc::tma_load_2d(sm.k[stage] + to, map, 64 * x, y, &sm.k_full[stage]);
                 }
             }
-            ok = wait_or_abort<true, true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
+            ok = wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
             if (__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) {
                     tc::mbar_expect_tx(&sm.v_full[stage], kGran * D * 2);
@@ -299,11 +299,11 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
     Piece p;
     while (walk.next(p)) {
         for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
-            wait_or_abort<true, true>(&sm.raw_full[raw], raw_phase, &sm.halt, a.status);
-            wait_or_abort<true, true>(&sm.k_empty[stage], phase ^ 1, &sm.halt, a.status);
+            wait_or_abort<true>(&sm.raw_full[raw], raw_phase, &sm.halt, a.status);
+            wait_or_abort<true>(&sm.k_empty[stage], phase ^ 1, &sm.halt, a.status);
             half(sm.raw[raw] + at, sm.k[stage]);
             arrive(&sm.k_full[stage]);
-            wait_or_abort<true, true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
+            wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
             half(sm.raw[raw] + at + (a.block_bytes >> 1), sm.v[stage]);
             arrive(&sm.v_full[stage]);
             arrive(&sm.raw_empty[raw]);
@@ -350,8 +350,8 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
     for (; any; any = more, p = ahead) {
         more = walk.next(ahead);
         const int n = (p.k1 - p.k0) / kGran, halves = p.ncols > kHalf ? 2 : 1;
-        ok = wait_or_abort<true, true>(&sm.k_full[ks], k_phase, &sm.halt, a.status) && ok;
-        ok = wait_or_abort<true, true>(&sm.q_full, q_phase, &sm.halt, a.status) && ok;
+        ok = wait_or_abort<true>(&sm.k_full[ks], k_phase, &sm.halt, a.status) && ok;
+        ok = wait_or_abort<true>(&sm.q_full, q_phase, &sm.halt, a.status) && ok;
         q_phase ^= 1;
         tc::fence_after_sync();
 #pragma unroll
@@ -371,9 +371,9 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
             if ((j & 255) == 255 && lead && ok) {
                 sm.halt.alive();  // about twice a millisecond
             }
-            ok = wait_or_abort<true, true>(&sm.v_full[vs], v_phase, &sm.halt, a.status) && ok;
+            ok = wait_or_abort<true>(&sm.v_full[vs], v_phase, &sm.halt, a.status) && ok;
             if (j + 1 < n) {
-                ok = wait_or_abort<true, true>(&sm.k_full[ks], k_phase, &sm.halt, a.status) && ok;
+                ok = wait_or_abort<true>(&sm.k_full[ks], k_phase, &sm.halt, a.status) && ok;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -381,7 +381,7 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     if (w < halves) {
-                        ok = wait_or_abort<true, true>(&sm.p_full[w][h], (p_phase >> (2 * h + w)) & 1u, &sm.halt, a.status) && ok;
+                        ok = wait_or_abort<true>(&sm.p_full[w][h], (p_phase >> (2 * h + w)) & 1u, &sm.halt, a.status) && ok;
                         p_phase ^= 1u << (2 * h + w);
                         tc::fence_after_sync();
                         if (!__all_sync(0xffffffffu, ok)) {
@@ -464,9 +464,8 @@ template <int D> __device__ __forceinline__ float *part_of(const AttendArgs &a, 
 // What counts is the time of a load through L2: eight are under way per thread
 // (two warps' worth of columns at a time, two loads each, took 30 us for 256
 // columns of 128 values in three parts).
-template <int kRows, int kCache, int D>
-__device__ __forceinline__ void merge_column(const AttendArgs &a, const Plan &plan, const Piece &p, int c, int row, int qhead, bool write,
-                                             bool sees) {
+template <int kRows, int D>
+__device__ __forceinline__ void merge_column(const AttendArgs &a, const Piece &p, int c, int row, int qhead, bool write, bool sees) {
     float m = -INFINITY, l = 0.0f;
     for (int k = p.first; k <= p.last; ++k) {
         const float2 y = __ldcg(reinterpret_cast<const float2 *>(part_of<D>(a, k, p.first) + kPromptWidth * D) + c);
@@ -475,14 +474,7 @@ __device__ __forceinline__ void merge_column(const AttendArgs &a, const Plan &pl
         m = mn;
     }
     const float safe = m == -INFINITY ? 0.0f : m;
-    float g = 1.0f;
-    if (a.sinks && write) {
-        const float sink = a.sinks[qhead] * kLog2e, mn = fmaxf(m, sink), s = mn == -INFINITY ? 0.0f : mn;
-        g = exp2f(m - s);
-        l = l * g + exp2f(sink - s);
-    }
-    g = g / l;
-    bool bad = false;
+    const float g = (a.sinks && write ? add_sink(m, l, a.sinks[qhead]) : 1.0f) / l;
 #pragma unroll 1
     for (int i = 0; i < D / 4; i += 8) {
         float o[32] = {};
@@ -509,25 +501,34 @@ __device__ __forceinline__ void merge_column(const AttendArgs &a, const Plan &pl
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 v[t] = sees ? o[j + t] * g : 0.0f;
-                bad = bad || !(fabsf(v[t]) < INFINITY);
             }
             if (write) {
                 store8<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + 4 * i + j, v);
             }
         }
     }
-    uint32_t redo = __ballot_sync(0xffffffffu, bad && write);
-    while (redo) {
-        const int src = __ffs(redo) - 1;
-        redo &= redo - 1;
-        attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, __shfl_sync(0xffffffffu, row, src),
-                                       __shfl_sync(0xffffffffu, qhead, src));
+}
+
+// The columns base + i of the bits i of `bad`, the same in all lanes.
+template <int kRows, int kCache, int D>
+__device__ __noinline__ void redo_columns(const AttendArgs &a, const Piece &p, uint32_t bad, int base, Halt *halt, float *part) {
+    const bool lead = (threadIdx.x & 31) == 0;
+    if (lead) {
+        halt->busy(true);
+    }
+    __syncwarp();  // what is written again was written before by another lane
+    for (; bad; bad &= bad - 1) {
+        redo_column<kRows, kCache, D, true>(a, p, base + __ffs(bad) - 1, part);
+    }
+    __syncwarp();
+    if (lead) {
+        halt->busy(false);
     }
 }
 
 // A warpgroup: the columns [128 w, 128 w + 128) of each tile, one per thread.
 template <int kRows, int kCache, int D>
-__device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, PromptSmem<kCache, D> &sm, uint32_t tmem) {
+__device__ __forceinline__ void soften(const AttendArgs &a, PromptSmem<kCache, D> &sm, uint32_t tmem) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w = warp >> 2;
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // (32 * quadrant) << 16
     const uint32_t s_at = tmem + 128 * w + lanes, o_at = tmem + 256 + D * w + lanes;
@@ -730,21 +731,15 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
             ok = wait_or_abort<true>(&sm.o_done[w][0], phase ^ 1, &sm.halt, a.status) && ok;
             ok = wait_or_abort<true>(&sm.o_done[w][1], phase ^ 1, &sm.halt, a.status) && ok;
             tc::fence_after_sync();
-            const float l = (l0 + l1) + (l2 + l3);
+            float l = (l0 + l1) + (l2 + l3);
             float g = 1.0f;
             float *part = part_of<D>(a, int(blockIdx.x), p.first);
+            float2 *const stats = reinterpret_cast<float2 *>(part + kPromptWidth * D);
             if (whole) {
-                float mm = m, ll = l;
-                if (a.sinks && have) {
-                    const float sink = a.sinks[qhead] * kLog2e;
-                    mm = fmaxf(m, sink);
-                    const float safe = mm == -INFINITY ? 0.0f : mm;
-                    g = exp2f(m - safe);
-                    ll = l * g + exp2f(sink - safe);
-                }
-                g = g / ll;
+                g = (a.sinks && have ? add_sink(m, l, a.sinks[qhead]) : 1.0f) / l;
             } else if (have) {
-                reinterpret_cast<float2 *>(part + kPromptWidth * D)[c] = make_float2(m, l);
+                stats[c] = make_float2(m, l);
+                bad = !(l < INFINITY);
             }
             const bool write = have && row < a.rows && ri.w == p.seq;
             if (__all_sync(0xffffffffu, ok)) {
@@ -772,17 +767,14 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
                 }
             }
             tc::fence_before_sync();
-            uint32_t redo = __ballot_sync(0xffffffffu, bad && whole && write);
-            while (redo) {
-                const int src = __ffs(redo) - 1;
-                redo &= redo - 1;
-                attend_column<kRows, kCache, D>(a, plan, p.head, p.seq, p.len, __shfl_sync(0xffffffffu, row, src),
-                                               __shfl_sync(0xffffffffu, qhead, src));
+            const uint32_t again = __ballot_sync(0xffffffffu, bad && write);
+            if (again) {
+                redo_columns<kRows, kCache, D>(a, p, again, c & ~31, &sm.halt, whole ? nullptr : part);
             }
         }
         if (!whole) {
             if (arrive_last(a, p, &sm.last, softmax_sync)) {
-                merge_column<kRows, kCache, D>(a, plan, p, c, row, qhead, have && row < a.rows && ri.w == p.seq, sees);
+                merge_column<kRows, D>(a, p, c, row, qhead, have && row < a.rows && ri.w == p.seq, sees);
             }
             softmax_sync();
         }
@@ -795,7 +787,7 @@ __device__ __forceinline__ void soften(const AttendArgs &a, const Plan &plan, Pr
 
 template <int kRows, int kCache, int D>
 __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
-    kv_attend_prompt_kernel(AttendArgs a, const __grid_constant__ CUtensorMap map) {
+    kv_attend_prompt_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap map) {
     using Shape = PromptShape<kCache>;
     using Smem = PromptSmem<kCache, D>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -839,7 +831,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
     const uint32_t tmem = sm.tmem;
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kSoftmaxRegs));
-        soften<kRows, kCache, D>(a, plan, sm, tmem);
+        soften<kRows, kCache, D>(a, sm, tmem);
     } else if (warp < kExpander) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kOtherRegs));
         if (warp == kLoader) {

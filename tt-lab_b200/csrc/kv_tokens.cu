@@ -69,6 +69,11 @@ template <int kRows, int kCache, int D, int NT> struct TokenShape {
     // (128 tokens of 64 values: three granules 151 us, five 158, six 162), less too
     // (two: 161); with three CTAs on an SM 160.
     static constexpr int kStages = D == 64 || kFour ? 3 : 2;
+    // Parts that a lane merges at once.  Twice as many take registers from the loop
+    // over the keys: 64 sequences of two rows, D = 128, 189 us, with eight 226 (four
+    // rows, D = 64: 127 and 171; over 4 bits, two rows 99, with four 105); one token
+    // over 131072 keys gains 1 us by eight.
+    static constexpr int kMergeBatch = kFour ? 2 : 4;
     // A column's sums in shared memory: over a 16-bit cache rows of D values whose
     // groups of 8 are swapped by the column, over 4 bits rows with 4 values of
     // padding; either way the accumulators' stores do not collide.
@@ -96,6 +101,8 @@ template <int kRows, int kCache, int D, int NT> struct TokenSmem {
     uint64_t full[T::kStages], empty[T::kStages];
     int last;
     Halt halt;
+    int again;                     // some column has a sum that is not finite
+    int held[2];                   // so it has in the part of a tile that began in an earlier CTA, or begins here
 };
 
 __device__ __forceinline__ void consumer_sync() {
@@ -171,6 +178,11 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                      tc::smem_u32(dst)),
                  "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
                  : "memory");
+}
+
+// Where this CTA leaves its partial result of a tile.
+template <int D, int kCols> __device__ __forceinline__ float *own_part(const AttendArgs &a, const Piece &p) {
+    return a.part + size_t(part_slot(int(blockIdx.x), p.first)) * kCols * part_pitch(D);
 }
 
 // The loader: one warp, a granule a step.
@@ -313,9 +325,51 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     }
 }
 
+// Columns whose sums are not finite, after the CTA's last tile: found by what was
+// left of them, computed again, and the parts held back are counted.  (In the loop
+// over the tiles this would hold registers that the loop over the keys needs: 64
+// tokens over 4 bits 4 us more.)
+template <int kRows, int kCache, int D, int NT>
+__device__ __forceinline__ void redo_pieces(const AttendArgs &a, TokenSmem<kRows, kCache, D, NT> &sm) {
+    using T = TokenShape<kRows, kCache, D, NT>;
+    constexpr int kPer = D / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Walker walk(a.walk, int(blockIdx.x), T::kGran);
+    Piece p;
+    while (walk.next(p)) {
+        const bool whole = p.first == p.last;
+        if (!whole && !sm.held[p.first == int(blockIdx.x)]) {
+            continue;
+        }
+        float *part = whole ? nullptr : own_part<D, T::kCols>(a, p);
+        for (int c = warp; c < p.ncols; c += kWarps) {
+            int row, qhead;
+            a.column(p, c, row, qhead);
+            if (row >= a.rows || a.walk.row[row].w != p.seq) {
+                continue;  // nobody stores it
+            }
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int d = lane + 32 * i;
+                const float x = whole ? row_value<kRows>(a.out, size_t(row) * a.out_stride + size_t(qhead) * D + d)
+                                      : part[size_t(c) * part_pitch(D) + d];
+                bad = bad || !(fabsf(x) < INFINITY);
+            }
+            bad = bad || (!whole && !(part[size_t(c) * part_pitch(D) + D + 1] < INFINITY));
+            if (__any_sync(0xffffffffu, bad)) {
+                redo_column<kRows, kCache, D, false>(a, p, c, part);
+            }
+        }
+        if (!whole && arrive_last(a, p, &sm.last, consumer_sync)) {
+            merge_tile<kRows, D, T::kMergeBatch>(a, p, warp, kWarps, T::kCols);
+        }
+    }
+}
+
 template <int kRows, int kCache, int D, int NT>
 __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 64 ? 3 : 2)
-    kv_attend_tokens_kernel(AttendArgs a, const __grid_constant__ CUtensorMap map) {
+    kv_attend_tokens_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap map) {
     using T = TokenShape<kRows, kCache, D, NT>;
     using Smem = TokenSmem<kRows, kCache, D, NT>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -336,6 +390,7 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
             tc::mbar_init(&sm.tile_empty[i], kWarps);
         }
         sm.halt = Halt{0, 0};
+        sm.again = sm.held[0] = sm.held[1] = 0;
         tc::fence_mbar_init();
     }
     __syncthreads();
@@ -798,12 +853,16 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
             }
         };
         if (p.first == p.last) {
-            store_columns<kRows, kCache, D>(a, plan, p, warp, kWarps, value, stats, [&](int c, int, int) {
+            const bool bad = store_columns<kRows, D>(a, p, warp, kWarps, value, stats, [&](int c, int, int) {
                 const int4 ri = sm.row[side][c];
                 return ColumnInfo{ri.y, ri.z, ri.w, sm.sink[side][c]};
             });
+            if (bad) {
+                sm.again = 1;
+            }
         } else {
-            float *part = a.part + size_t(part_slot(int(blockIdx.x), p.first)) * kCols * part_pitch(D);
+            float *part = own_part<D, kCols>(a, p);
+            bool bad = false;
             for (int i = tid; i < p.ncols * (D / 8); i += 32 * kWarps) {
                 const int c = i / (D / 8), d = 8 * (i % (D / 8));
                 float v[8];
@@ -811,18 +870,32 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
                 float4 *dst = reinterpret_cast<float4 *>(part + size_t(c) * part_pitch(D) + d);
                 dst[0] = make_float4(v[0], v[1], v[2], v[3]);
                 dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    bad = bad || !(fabsf(v[j]) < INFINITY);
+                }
                 if (d == 0) {
-                    *reinterpret_cast<float2 *>(part + size_t(c) * part_pitch(D) + D) = stats(c);
+                    const float2 ml = stats(c);
+                    *reinterpret_cast<float2 *>(part + size_t(c) * part_pitch(D) + D) = ml;
+                    bad = bad || !(ml.y < INFINITY);
                 }
             }
-            if (arrive_last(a, p, &sm.last, consumer_sync)) {
-                merge_tile<kRows, kCache, D, kCache == kMxfp4 ? 4 : 8>(a, plan, p, warp, kWarps, kCols);
+            int &held = sm.held[p.first == int(blockIdx.x)];
+            if (bad) {
+                sm.again = held = 1;
+            }
+            if (arrive_last(a, p, &sm.last, consumer_sync, [&] { return held != 0; })) {
+                merge_tile<kRows, D, T::kMergeBatch>(a, p, warp, kWarps, kCols);
             }
         }
         __syncwarp();
         if (lane == 0) {
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&sm.tile_empty[side])) : "memory");
         }
+    }
+    consumer_sync();
+    if (sm.again && !sm.halt.aborted()) {
+        redo_pieces<kRows, kCache, D, NT>(a, sm);
     }
 }
 
