@@ -90,6 +90,9 @@ size_t ttl_kv_page_bytes(const ttl_kv *handle);
  *   pages     [seqs][page_stride]  page ids: position p is in slot
  *                         p % page_tokens of page pages[s][p / page_tokens].
  *                         Sequences may share pages that they only read.
+ *                         Entries of pages that no call reaches (an attend those
+ *                         whose positions no row sees, an append or read those
+ *                         without rows) may hold anything, -1 for instance
  *   first     [rows] or NULL  lowest position a row may see (a packed
  *                         document's start)
  *   prefix    [seqs] or NULL  every row sees all positions below prefix

@@ -949,6 +949,43 @@ def test_bad_numbers_are_reported_and_skipped():
     s.cache.sync()  # reported once; the handle stays usable
 
 
+@pytest.mark.parametrize("rows,cache", COMBOS)
+@pytest.mark.parametrize("new", [1, 3, 60])
+def test_pages_below_the_window_may_be_gone(rows, cache, new):
+    """A server frees the pages that a window has passed and leaves -1 in the
+    table: a sliding call says nothing, a full one does, and so does a sliding
+    one where a page that it sees is gone."""
+    page, window, n = 16, 40, 391
+    s = Setup(rows, cache, 8, 2, 64, page, new=(new, 1), length=(n, 50), window=window)
+    s.fill()
+    gone = (n - new - window + 1) // page  # pages below the lowest visible position
+    for more, bad in ((0, False), (1, True)):
+        table = s.table.clone()
+        table[0, :gone + more] = torch.tensor([-1, 10 ** 6])[torch.arange(gone + more) % 2].to(torch.int32)
+        s.dev["table"] = table.cuda()
+        s.plan()
+        out = torch.full_like(s.dev["q"], 7.0)
+        s.cache.attend_async(0, s.dev["q"], out, sliding=True)
+        if bad:
+            with pytest.raises(RuntimeError, match="page id"):
+                s.cache.sync()
+            continue
+        s.cache.sync()
+        ref, tol = s.reference(sliding=True)
+        assert ((out.cpu().double() - ref).abs() <= tol).all()
+        s.cache.attend_async(0, s.dev["q"], out)
+        with pytest.raises(RuntimeError, match="page id"):
+            s.cache.sync()
+
+
+def test_rows_that_see_nothing_ask_for_no_page():
+    s = Setup("bf16", None, 8, 2, 64, 16, new=(40, 1), length=(100, 60), first=[1 << 30] * 41)
+    s.fill()
+    s.dev["table"] = torch.full_like(s.dev["table"], -1)
+    s.plan()
+    assert (s.attend() == 0).all()
+
+
 def test_a_plan_of_another_shape_is_reported():
     """A captured attend whose plan was replaced by one of another shape."""
     st = torch.cuda.Stream()

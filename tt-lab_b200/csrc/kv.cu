@@ -262,7 +262,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             const int g0 = begin < end ? begin / gran : 0;
             // at least one granule: a tile whose rows see nothing is written too
             n = begin < end ? (end + gran - 1) / gran - g0 : 1;
-            tiles[t] = Tile{lo, col0, g0, uint32_t(ncols) | uint32_t(n) << 9, q.row0 + r0, col0 - r0 * a.group, q.len, 0};
+            tiles[t] = Tile{lo, col0, g0, uint32_t(ncols) | uint32_t(n) << 9, q.row0 + r0, col0 - r0 * a.group, q.len,
+                            begin < end ? begin : kNoPosition};
             n += cost;
         }
         int sum;

@@ -39,12 +39,14 @@ enum : uint32_t {
 
 constexpr int kKinds = 2;          // tiles of few columns, tiles of a prompt
 constexpr int kMaxCtas = 1024;     // CTAs of a list (cuts)
+constexpr int kNoPosition = 1 << 30;  // above all
 constexpr int kNoSplit = 4;        // a tile of at most this many granules is not cut
 
 struct __align__(32) Tile {
     int32_t seq, col0, gran0;
     uint32_t size;                 // columns (9 bits), granules
-    int32_t row0, rem, len, pad;   // row and head (in its group) of the first column; the sequence's length
+    int32_t row0, rem, len, low;   // row and head (in its group) of the first column; the sequence's length; the
+                                   // lowest position a column sees (kNoPosition: none)
 };
 struct __align__(16) Cut {
     int32_t head, tile, gran;      // gran: granules into the tile
@@ -71,7 +73,7 @@ struct Walk {
 };
 
 struct Piece {
-    int head, tile, seq, ncols, row0, rem, len;
+    int head, tile, seq, ncols, row0, rem, len, low;
     int k0, k1;        // keys of the piece (k1 <= the tile's last granule; clip to the sequence's length)
     int first, last;   // first and last CTA that hold a part of the tile (equal: the whole tile is here)
 };
@@ -224,12 +226,15 @@ template <int kCache, int D> __device__ __forceinline__ void pool8(const uint8_t
     }
 }
 
-// Page id of position `pos` of a sequence; an id outside the pool is reported
-// and read as page 0.  The caller keeps pos below the sequence's length.
-__device__ __forceinline__ int page_of(const Plan &plan, int seq, int pos, int page_shift, int pages, uint32_t *status) {
+// Page id of position `pos` of a sequence; an id outside the pool is read as page 0,
+// and reported unless the whole page lies below position `low`.  The caller keeps
+// pos below the sequence's length.
+__device__ __forceinline__ int page_of(const Plan &plan, int seq, int pos, int low, int page_shift, int pages, uint32_t *status) {
     const int id = plan.pages[size_t(seq) * plan.page_stride + size_t(pos >> page_shift)];
     if (uint32_t(id) >= uint32_t(pages)) {
-        set_status(status, kKvBadPage);
+        if (pos >> page_shift >= low >> page_shift) {
+            set_status(status, kKvBadPage);
+        }
         return 0;
     }
     return id;
@@ -310,7 +315,7 @@ struct Walker {
         if (end.head == head && end.tile == tile) {
             stop = end.gran;  // > gran
         }
-        p.head = head, p.tile = tile, p.seq = t4.x, p.row0 = t2.x, p.rem = t2.y, p.len = t2.z;
+        p.head = head, p.tile = tile, p.seq = t4.x, p.row0 = t2.x, p.rem = t2.y, p.len = t2.z, p.low = t2.w;
         p.ncols = int(uint32_t(t4.w) & 511u);
         p.k0 = (t4.z + gran) * gsize;
         p.k1 = (t4.z + stop) * gsize;
@@ -563,7 +568,7 @@ __device__ __forceinline__ void redo_column(const AttendArgs &a, const Piece &p,
     for (int base = lo; base < hi; base += 32) {
         const int j = base + lane, n = min(32, hi - base);
         const bool seen = lane < n;
-        const int page = seen ? page_of(plan, p.seq, j, a.page_shift, a.pages, a.status) : 0;
+        const int page = seen ? page_of(plan, p.seq, j, 0, a.page_shift, a.pages, a.status) : 0;
         const uint8_t *kb = block(page);
         float s = 0.0f;
 #pragma unroll

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kSimpleThreads) kv_attend_simple_kernel(Attend
             __syncthreads();
             if (tid < kSimpleGran / 16) {
                 const int j = k0 + 16 * tid;
-                sm.pages[tid] = j < p.len ? page_of(plan, p.seq, j, a.page_shift, a.pages, a.status) : 0;
+                sm.pages[tid] = j < p.len ? page_of(plan, p.seq, j, p.low, a.page_shift, a.pages, a.status) : 0;
             }
             __syncthreads();
             if constexpr (kCache != kMxfp4) {

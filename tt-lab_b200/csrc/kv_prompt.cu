@@ -196,7 +196,8 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
                 base = first;
                 id = len > 0 ? table[min(base + lane, last)] : 0;
                 if (uint32_t(id) >= uint32_t(a.pages)) {
-                    if (base + lane <= min(last, (p.k1 - 1) >> a.page_shift)) {
+                    // (a granule may begin on pages below all that the tile sees: not reported)
+                    if (base + lane >= p.low >> a.page_shift && base + lane <= min(last, (p.k1 - 1) >> a.page_shift)) {
                         set_status(a.status, kKvBadPage);
                     }
                     id = 0;

@@ -203,7 +203,8 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
     };
     auto checked = [&](const Piece &p, int base, int id) {
         if (uint32_t(id) >= uint32_t(a.pages)) {
-            if (base + lane <= min(max(p.len - 1, 0), p.k1 - 1) >> a.page_shift) {
+            // (a granule may begin on pages below all that the tile sees: not reported)
+            if (base + lane >= p.low >> a.page_shift && base + lane <= min(max(p.len - 1, 0), p.k1 - 1) >> a.page_shift) {
                 set_status(a.status, kKvBadPage);
             }
             return 0;
