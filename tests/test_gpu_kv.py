@@ -563,6 +563,44 @@ def test_a_nan_in_a_long_prompt_stays_small(rows, cache, where):
     assert ((out.double() - ref).abs() <= tol).all()
 
 
+def fastest(s, n=5, **kw):
+    """Milliseconds of an attend, the least of a few, and its result."""
+    out, best = torch.full_like(s.dev["q"], 7.0), math.inf
+    for _ in range(n):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        s.cache.attend_async(0, s.dev["q"], out, **kw)
+        b.record()
+        s.cache.sync()
+        best = min(best, a.elapsed_time(b))
+    return best, out.cpu()
+
+
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("D,page,new,length", [(64, 64, (1,) * 40, 2100), (128, 32, (1, 2) * 16, 1500), (64, 128, (300, 200), 1700),
+                                              (128, 16, (90, 200), 1801), (64, 16, (130, 3), 129)])
+def test_stale_slots_cost_nothing(rows, cache, D, page, new, length):
+    """NaN in the last pages' slots behind the sequences' ends, left there by
+    others: nothing is computed again for them (that takes 40 times as long and
+    more)."""
+    length = [max(length + 7 * i, n) for i, n in enumerate(new)]
+    s = Setup(rows, cache, 8, 1, D, page, new=new, length=length, seed=7)
+    s.fill().plan()
+    clean, _ = fastest(s)
+    tails = [-l % page for l in length]
+    full = torch.tensor([l + t for l, t in zip(length, tails)], dtype=torch.int32).cuda()
+    start = torch.tensor([0] + list(np.cumsum(tails)), dtype=torch.int32).cuda()
+    nan = torch.full((sum(tails), 1, D), math.nan, dtype=s.dt, device="cuda")
+    assert sum(tails) > 0
+    s.cache.batch_async(start, full, s.dev["table"], rows=sum(tails))
+    s.cache.append_async(0, nan, nan)
+    s.plan()
+    stale, out = fastest(s)
+    ref, tol = s.reference()
+    assert ((out.double() - ref).abs() <= tol).all()
+    assert stale < 3 * clean, (stale, clean)
+
+
 @pytest.mark.parametrize("rows,cache", COMBOS)
 @pytest.mark.parametrize("new", [1, 50])
 def test_infinite_sinks(rows, cache, new):

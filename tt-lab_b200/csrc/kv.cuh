@@ -417,6 +417,16 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
     return d;
 }
 
+// Slots behind a sequence's end hold what was left there, and 0 * NaN is NaN in every
+// column, so V's values there become 0 before the product: by a warp, `rows` rows of
+// 64 values (128 bytes each) from `addr` on in shared memory that copies fill.
+__device__ __forceinline__ void clear_rows(uint32_t addr, int rows) {
+#pragma unroll 1
+    for (int i = (threadIdx.x & 31) * 16; i < rows * 128; i += 512) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr + i), "r"(0) : "memory");
+    }
+}
+
 // Whether a phase of a barrier is complete, without waiting for it.
 __device__ __forceinline__ bool phase_done(uint64_t *bar, uint32_t parity) {
     uint32_t ok;

@@ -76,6 +76,7 @@ template <int kCache, int D> struct PromptSmem {
     alignas(16) uint8_t raw[2][kRawBytes];
     uint64_t raw_full[2], raw_empty[2];
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t v_tail[kStages];                               // V of a granule that passes the sequence's end, as it was read
     Piece piece[2];                                         // the tile in hand and the next; ncols 0: no more
     uint64_t piece_full[2], piece_empty[2], q_full, q_empty;
     uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [warpgroup][half of a granule]
@@ -240,12 +241,13 @@ __device__ __forceinline__ void load_granules(const AttendArgs &a, const Plan &p
             }
             ok = wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
             if (__all_sync(0xffffffffu, ok)) {
+                uint64_t *bar = k0 + kGran > len ? &sm.v_tail[stage] : &sm.v_full[stage];  // the scouts hand a tail on
                 if (lane == 0) {
-                    tc::mbar_expect_tx(&sm.v_full[stage], kGran * D * 2);
+                    tc::mbar_expect_tx(bar, kGran * D * 2);
                 }
                 __syncwarp();
                 if (lane < copies) {
-                    tc::tma_load_2d(sm.v[stage] + to, map, 64 * x, y + (1 << a.page_shift), &sm.v_full[stage]);
+                    tc::tma_load_2d(sm.v[stage] + to, map, 64 * x, y + (1 << a.page_shift), bar);
                 }
             }
             if (++stage == PromptSmem<kCache, D>::kStages) {
@@ -267,12 +269,13 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
     const uint32_t at = uint32_t(key >> a.page_shift) * a.block_bytes;
     const int t = key & (tokens - 1);
     const __nv_bfloat162 unit = __bfloat162bfloat162(__ushort_as_bfloat16(0x7e80));  // 2^126
-    auto half = [&](const uint8_t *src, uint8_t *dst) {
+    // dead: V behind the sequence's end, whatever was left there, becomes 0
+    auto half = [&](const uint8_t *src, uint8_t *dst, bool dead) {
         const uint8_t *scales = src + tokens * (D / 2) + t * (D / 32);
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
-            const __nv_bfloat162 f = __bfloat162bfloat162(__float2bfloat16_rn(scale_of(scales[b])));  // a power of two
-            const uint4 w = *reinterpret_cast<const uint4 *>(src + t * (D / 2) + 16 * b);
+            const __nv_bfloat162 f = __bfloat162bfloat162(__float2bfloat16_rn(dead ? 1.0f : scale_of(scales[b])));  // a power of two
+            const uint4 w = dead ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4 *>(src + t * (D / 2) + 16 * b);
             const uint32_t c[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -302,10 +305,10 @@ template <int kCache, int D> __device__ __forceinline__ void expand(const Attend
         for (int k0 = p.k0; k0 < p.k1; k0 += kGran) {
             wait_or_abort<true>(&sm.raw_full[raw], raw_phase, &sm.halt, a.status);
             wait_or_abort<true>(&sm.k_empty[stage], phase ^ 1, &sm.halt, a.status);
-            half(sm.raw[raw] + at, sm.k[stage]);
+            half(sm.raw[raw] + at, sm.k[stage], false);
             arrive(&sm.k_full[stage]);
             wait_or_abort<true>(&sm.v_empty[stage], phase ^ 1, &sm.halt, a.status);
-            half(sm.raw[raw] + at + (a.block_bytes >> 1), sm.v[stage]);
+            half(sm.raw[raw] + at + (a.block_bytes >> 1), sm.v[stage], k0 + key >= p.len);
             arrive(&sm.v_full[stage]);
             arrive(&sm.raw_empty[raw]);
             raw_phase ^= uint32_t(raw);
@@ -417,12 +420,16 @@ template <int kRows, int kCache, int D> __device__ __forceinline__ void issue(co
 
 // Two warps that look the tiles up: each tile's description for the softmax
 // warps, and its Q rows, 16 bytes at a time, swizzled as the matrix instruction
-// reads them, as soon as the last scores of the tile before are computed.
+// reads them, as soon as the last scores of the tile before are computed.  Over a
+// 16-bit cache the first of them hands V of a granule that passes the sequence's
+// end on, with the slots behind the end set to 0 (over 4 bits the expanders write
+// 0 there): long before its product, and before the next tile's Q can go anywhere.
 template <int kCache, int D> __device__ __forceinline__ void scout(const AttendArgs &a, PromptSmem<kCache, D> &sm) {
     const int lane = threadIdx.x - 32 * kScout;  // 0 .. 63
     Walker walk(a.walk, int(blockIdx.x), kGran);
     Piece p;
-    uint32_t side_phase = 0, q_phase = 0;
+    uint32_t side_phase = 0, q_phase = 0, tail_phase = 0;  // tail: a bit per stage
+    int granules = 0;                                      // before this tile, modulo the stages
     for (int side = 0;; side ^= 1) {
         const bool more = walk.next(p);
         p.ncols = more ? p.ncols : 0;
@@ -450,6 +457,27 @@ template <int kCache, int D> __device__ __forceinline__ void scout(const AttendA
         asm volatile("cp.async.wait_all;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive(&sm.q_full);
+        if constexpr (kCache != kMxfp4) {
+            constexpr int kStages = PromptSmem<kCache, D>::kStages;
+            const int stage = (granules + (p.k1 - p.k0) / kGran - 1) % kStages;  // of the last granule
+            granules = (stage + 1) % kStages;
+            if (lane < 32 && p.k1 > p.len) {
+                const bool ok = wait_or_abort<true, true>(&sm.v_tail[stage], (tail_phase >> stage) & 1u, &sm.halt, a.status);
+                tail_phase ^= 1u << stage;
+                if (__all_sync(0xffffffffu, ok)) {
+                    const int first = max(p.len - (p.k1 - kGran), 0);
+#pragma unroll
+                    for (int x = 0; x < D / 64; ++x) {
+                        clear_rows(tc::smem_u32(sm.v[stage]) + (x * kGran + first) * 128, kGran - first);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        arrive(&sm.v_full[stage]);
+                    }
+                }
+            }
+        }
     }
 }
 
@@ -805,6 +833,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
             tc::mbar_init(&sm.k_empty[i], 1);
             tc::mbar_init(&sm.v_full[i], Shape::kFour ? 128 : 1);
             tc::mbar_init(&sm.v_empty[i], 1);
+            tc::mbar_init(&sm.v_tail[i], 1);
         }
         for (int w = 0; w < 2; ++w) {
             tc::mbar_init(&sm.raw_full[w], 1);
@@ -856,6 +885,7 @@ __global__ void __launch_bounds__(PromptShape<kCache>::kThreads, 1)
                 for (int i = 0; i < Smem::kStages; ++i) {
                     tc::mbar_wait(&sm.k_full[i], ph, 1000000ull);
                     tc::mbar_wait(&sm.v_full[i], ph, 1000000ull);
+                    tc::mbar_wait(&sm.v_tail[i], ph, 1000000ull);
                     tc::mbar_wait(&sm.k_empty[i], ph, 1000000ull);
                     tc::mbar_wait(&sm.v_empty[i], ph, 1000000ull);
                 }

@@ -525,6 +525,17 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
             const int key0 = k0 + 16 * kSub * warp;
             if (key0 < hi_max && key0 + 16 * kSub > lo_min) {
                 const uint32_t buf = tc::smem_u32(sm.stage[stage]);
+                if constexpr (kCache != kMxfp4) {
+                    if (key0 + 16 > p.len) {  // the warp's own 16 rows
+                        const int first = p.len - key0;
+#pragma unroll 1
+                        for (int x = 0; x < D / 64; ++x) {
+                            clear_rows(buf + ((D / 64 + x) * T::kGran + 16 * warp + first) * 128, 16 - first);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                }
                 float s[kSub][NT][4];
                 float sv[kSub][2][kBlocks];  // 4 bits: V's scales of keys g, g + 8
                 uint32_t vcodes[kSub];
