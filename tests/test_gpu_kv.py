@@ -576,7 +576,7 @@ def fastest(s, n=5, **kw):
     return best, out.cpu()
 
 
-@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("rows,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "mxfp4"), ("f16", "mxfp4")])
 @pytest.mark.parametrize("D,page,new,length", [(64, 64, (1,) * 40, 2100), (128, 32, (1, 2) * 16, 1500), (64, 128, (300, 200), 1700),
                                               (128, 16, (90, 200), 1801), (64, 16, (130, 3), 129)])
 def test_stale_slots_cost_nothing(rows, cache, D, page, new, length):
@@ -599,6 +599,27 @@ def test_stale_slots_cost_nothing(rows, cache, D, page, new, length):
     ref, tol = s.reference()
     assert ((out.double() - ref).abs() <= tol).all()
     assert stale < 3 * clean, (stale, clean)
+
+
+@pytest.mark.parametrize("rows,cache", [("bf16", "mxfp4"), ("f16", "mxfp4")])
+@pytest.mark.parametrize("D,new", [(64, 2), (64, 4), (128, 2)])
+def test_large_values_in_4_bits_cost_nothing(rows, cache, D, new):
+    """Values whose scales pass 4 at keys that some of a tile's columns do not see
+    while they have seen none: nothing is computed again for them."""
+    times = []
+    for size in (1.0, 30.0, 30000.0):
+        first = [0 if i == 0 else 100 for i in range(new)] * 64
+        s = Setup(rows, cache, 8, 1, D, 64, new=(new,) * 64, length=(1500,) * 64, first=first, seed=8)
+        s.v = (s.v.clamp(-2, 2).double() * size).to(s.dt)
+        s.dev["v"] = s.v.cuda()
+        s.fill().plan()
+        t, out = fastest(s)
+        times.append(t)
+        rows_checked = slice(0, 2 * new)
+        s.new, s.length = s.new[:2], s.length[:2]
+        ref, tol = s.reference()
+        assert ((out[rows_checked].double() - ref).abs() <= tol).all()
+    assert max(times) < 3 * times[0], times
 
 
 @pytest.mark.parametrize("rows,cache", COMBOS)

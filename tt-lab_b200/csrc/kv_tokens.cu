@@ -497,7 +497,9 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
         }
         float m[NT][2], l[NT][2];
         float o[NT][kMTiles][4];
-        float unit[kCache == kMxfp4 ? NT : 1][2][kBlocks];  // 4 bits: 1 / the scale that o is in units of
+        // 4 bits: 1 / the scale that o is in units of; 0 until the column sees a key, so
+        // that the scales of unseen keys make 0 with it, however large
+        float unit[kCache == kMxfp4 ? NT : 1][2][kBlocks];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
                 if constexpr (kCache == kMxfp4) {
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b) {
-                        unit[n][c][b] = __uint_as_float(0x7e800000u);  // of the smallest scale
+                        unit[n][c][b] = 0.0f;
                     }
                 }
             }
@@ -526,8 +528,8 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
             if (key0 < hi_max && key0 + 16 * kSub > lo_min) {
                 const uint32_t buf = tc::smem_u32(sm.stage[stage]);
                 if constexpr (kCache != kMxfp4) {
-                    if (key0 + 16 > p.len) {  // the warp's own 16 rows
-                        const int first = p.len - key0;
+                    if (key0 + 16 > hi_max) {  // the warp's own rows behind all that the tile sees
+                        const int first = hi_max - key0;
 #pragma unroll 1
                         for (int x = 0; x < D / 64; ++x) {
                             clear_rows(buf + ((D / 64 + x) * T::kGran + 16 * warp + first) * 128, 16 - first);
@@ -656,6 +658,15 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
                                 s[u][n][j] = key >= ri.y && key < ri.z ? s[u][n][j] : -INFINITY;
                             }
                         }
+                        if constexpr (kCache == kMxfp4) {  // behind all that the tile sees: any scale, NaN too
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                                for (int b = 0; b < kBlocks; ++b) {
+                                    sv[u][h][b] = key0 + 16 * u + g + 8 * h < hi_max ? sv[u][h][b] : 0.0f;
+                                }
+                            }
+                        }
                     }
                 }
                 // ---- the running maximum ----
@@ -719,9 +730,10 @@ __global__ void __launch_bounds__(kThreads, kCache == kMxfp4 && NT == 1 && D == 
                                     // the unit's reciprocal: 2^(254 - byte) as a float's exponent; a byte
                                     // that a finite value has is at most 252
                                     const float r = __uint_as_float(0x7f000000u - max(__float_as_uint(e), 0x00800000u));
-                                    const float less = fminf(unit[n][c][b], r);
-                                    f[c] = up[c] * (less == unit[n][c][b] ? 1.0f : pow2i(int(__float_as_uint(less) >> 23) - int(__float_as_uint(unit[n][c][b]) >> 23)));
-                                    unit[n][c][b] = less;
+                                    const bool begun = unit[n][c][b] != 0.0f;
+                                    const float less = begun ? fminf(unit[n][c][b], r) : r;
+                                    f[c] = up[c] * (!begun || less == unit[n][c][b] ? 1.0f : pow2i(int(__float_as_uint(less) >> 23) - int(__float_as_uint(unit[n][c][b]) >> 23)));
+                                    unit[n][c][b] = m[n][c] == -INFINITY ? 0.0f : less;
                                 }
 #pragma unroll
                                 for (int i = 2 * b; i < 2 * b + 2; ++i) {
