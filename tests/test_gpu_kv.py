@@ -730,6 +730,21 @@ def test_offsets_past_32_bits():
             assert ((out[-1].cpu().double() - ref[-1]).abs() <= tol[-1]).all()
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_leading_columns_of_a_wide_page_table(new):
+    """A server's table has room for the longest sequence; a batch takes the
+    columns that it needs."""
+    s = Setup("bf16", None, 8, 2, 64, 16, new=(new, 1, 3), length=(90, 33, 150))
+    s.fill()
+    wide = torch.full((5, 64), -1, dtype=torch.int32)
+    wide[:3, :s.table.shape[1]] = s.table
+    s.dev["table"] = wide.cuda()[:, :s.table.shape[1]]
+    s.plan()
+    out = s.attend()
+    ref, tol = s.reference()
+    assert ((out.double() - ref).abs() <= tol).all()
+
+
 def test_pages_shared_by_sequences():
     """Two sequences over the same first pages."""
     s = Setup("bf16", None, 8, 2, 64, 16, new=(1, 1), length=(40, 40))

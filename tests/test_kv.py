@@ -77,6 +77,35 @@ def test_calls_without_a_handle():
     L.ttl_kv_destroy(None)
 
 
+def bare(**kw):
+    """A KvCache that has no handle, for its checks of tensors."""
+    import torch
+    import ttl_moe
+    c = ttl_moe.KvCache.__new__(ttl_moe.KvCache)
+    c.h, c._i32, c._dtype, c.head_dim, c._rows = None, torch.int32, torch.bfloat16, 64, 1
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def test_page_tables():
+    """A whole table or the leading columns of a wider one; nothing whose rows
+    would be read past the memory that holds them."""
+    import torch
+    c = bare()
+    wide = torch.zeros(4, 10, dtype=torch.int32)
+    assert c._table_stride(wide, 4) == c._table_stride(wide, 2) == 10
+    assert c._table_stride(wide[:, :3], 4) == c._table_stride(wide[:3, :1], 3) == 10
+    assert c._table_stride(wide[2:, :7], 2) == 10
+    assert c._table_stride(wide[1:2, 4:6], 1) == 2      # one row is read as far as it goes
+    assert c._table_stride(wide[:3, 4:6], 3) == 10      # another row follows the last
+    assert c._table_stride(torch.zeros(4, 1, dtype=torch.int32), 4) == 1
+    for bad in (wide[:, 4:6], wide[1:, 1:3], wide[:, ::2], wide.T, wide.long(), wide[0], wide[:3],
+                wide[:1, :2].expand(4, 2), torch.zeros(40, dtype=torch.int32).as_strided((4, 10), (5, 1))):
+        with pytest.raises(ValueError, match="pages must be"):
+            c._table_stride(bad, 4)
+
+
 @pytest.mark.skipif(os.path.exists("/dev/nvidia0"), reason="a GPU is present")
 def test_create_without_gpu_fails_loudly():
     import ttl_moe

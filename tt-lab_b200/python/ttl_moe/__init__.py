@@ -570,6 +570,19 @@ class KvCache:
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
         return t.data_ptr()
 
+    def _table_stride(self, pages, seqs):
+        """Entries between the rows of a page table [seqs, n]: the whole of a
+        tensor, or the leading columns of a wider one (the sequences' lengths may
+        then reach as far as the wider one's rows)."""
+        if pages.dim() != 2 or pages.dtype is not self._i32 or pages.shape[0] < seqs or \
+                (pages.stride(1) != 1 and pages.shape[1] > 1):
+            raise ValueError("pages must be an int32 tensor [seqs, n] with contiguous rows")
+        n = pages.shape[1]
+        stride = pages.stride(0) if pages.shape[0] > 1 else n
+        if stride != n and (stride < n or (pages.storage_offset() + seqs * stride) * 4 > pages.untyped_storage().nbytes()):
+            raise ValueError("pages must be contiguous, or the leading columns of a wider table")
+        return stride
+
     def _row_array(self, t, name, heads):
         """(address, row stride) of [rows, heads, head_dim] rows, each contiguous."""
         d = self.head_dim
@@ -585,15 +598,12 @@ class KvCache:
 
     def batch_async(self, row_start, length, pages, rows, max_new=None, first=None, prefix=None):
         """The batch of the next calls: int32 device tensors row_start
-        [seqs + 1], length [seqs], pages [seqs, n], first [rows], prefix
-        [seqs]; `rows` in all, at most `max_new` of one sequence (None: rows)."""
+        [seqs + 1], length [seqs], pages [seqs, n] (or the leading columns of a
+        wider table), first [rows], prefix [seqs]; `rows` in all, at most
+        `max_new` of one sequence (None: rows)."""
         seqs = length.shape[0]
         i32 = self._i32
-        if pages.dim() != 2 or pages.dtype is not i32 or pages.shape[0] < seqs or pages.stride(1) != 1:
-            raise ValueError("pages must be an int32 tensor [seqs, n] with contiguous rows")
-        stride = pages.stride(0) if pages.shape[0] > 1 else pages.shape[1]
-        if stride != pages.shape[1]:
-            raise ValueError("pages must be contiguous")
+        stride = self._table_stride(pages, seqs)
         rc = self._calls[0](
             self.h, seqs, rows, rows if max_new is None else max_new, self._array(row_start, "row_start", i32, (seqs + 1,)),
             self._array(length, "length", i32, (seqs,)), pages.data_ptr(), stride,
