@@ -77,6 +77,25 @@ def test_calls_without_a_handle():
     L.ttl_kv_destroy(None)
 
 
+def test_the_default_stream_by_its_handle(monkeypatch):
+    """The handle 0, as torch gives it for its default stream, is that stream;
+    only None asks for an own one."""
+    import types
+
+    import ttl_moe
+    seen = []
+
+    def create(cfg, out):
+        seen.append(cfg._obj.stream)
+        return -1
+
+    monkeypatch.setattr(ttl_moe, "lib", lambda: types.SimpleNamespace(ttl_kv_create=create, ttl_kv_last_error=lambda h: b"no"))
+    for stream in (None, 0, 1, 77, types.SimpleNamespace(cuda_stream=0), types.SimpleNamespace(cuda_stream=78)):
+        with pytest.raises(RuntimeError, match="no"):
+            ttl_moe.KvCache(stream=stream)
+    assert seen == [None, 1, 1, 77, 1, 78]
+
+
 def bare(**kw):
     """A KvCache that has no handle, for its checks of tensors."""
     import torch

@@ -508,8 +508,9 @@ class KvCache:
     sequences, in the rows' type or in 4 bits, and the attention over it.
 
     Arrays are torch tensors of the handle's GPU.  Work goes to the handle's
-    stream: `stream` is a torch stream or a cudaStream_t, None an own one.  The
-    caller keeps the tensors of a call alive until its work is done."""
+    stream: `stream` is a torch stream or a cudaStream_t (0: the default stream),
+    None an own one.  The caller keeps the tensors of a call alive until its work
+    is done."""
 
     def __init__(self, layers=1, pages=64, page_tokens=64, q_heads=64, kv_heads=8, head_dim=64, rows="bf16",
                  cache=None, max_seqs=1, max_rows=1, window=0, rope_freq=None, rope_scale=1.0,
@@ -519,8 +520,8 @@ class KvCache:
             if t not in KV_TYPES:
                 raise ValueError(f"{name} must be one of {', '.join(KV_TYPES)}")
         freq = np.ascontiguousarray(rope_freq, np.float64).reshape(-1) if rope_freq is not None else np.zeros(0)
-        if stream is not None and not isinstance(stream, int):
-            stream = stream.cuda_stream or STREAM_LEGACY
+        if stream is not None:  # the default stream's handle is 0, which here would mean an own one
+            stream = (stream if isinstance(stream, int) else stream.cuda_stream) or STREAM_LEGACY
         cfg = KvConfig(layers, pages, page_tokens, q_heads, kv_heads, head_dim, KV_TYPES[rows],
                        KV_TYPES[cache or rows], max_seqs, max_rows, window, 2 * freq.size, int(bool(rope_interleaved)),
                        freq.ctypes.data if freq.size else None, rope_scale, device, stream)
