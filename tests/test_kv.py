@@ -125,6 +125,18 @@ def test_page_tables():
             c._table_stride(bad, 4)
 
 
+def test_one_row_has_no_stride():
+    """A single row of rows that are no multiple of 16 bytes apart, an expanded
+    one, and one whose stride torch made up."""
+    import torch
+    c = bare()
+    x = torch.zeros(3, 700, dtype=torch.bfloat16)
+    for t in (x[:1, :512].unflatten(1, (8, 64)), torch.zeros(1, 1, 8, 64, dtype=torch.bfloat16).expand(1, 1, 8, 64)[0],
+              torch.zeros(8, 64, dtype=torch.bfloat16).as_strided((1, 8, 64), (1, 64, 1))):
+        assert c._row_array(t, "q", 8) == (t.data_ptr(), 512)
+    assert c._row_array(x[:, :512].unflatten(1, (8, 64)), "q", 8) == (x.data_ptr(), 700)
+
+
 @pytest.mark.skipif(os.path.exists("/dev/nvidia0"), reason="a GPU is present")
 def test_create_without_gpu_fails_loudly():
     import ttl_moe

@@ -595,7 +595,7 @@ class KvCache:
         row, head, inner = t.stride()
         if inner != 1 or (head != d and heads > 1):
             raise ValueError(f"{name}: the heads of a row must be contiguous")
-        return t.data_ptr(), row if n > 1 else max(row, heads * d)
+        return t.data_ptr(), row if n > 1 else heads * d  # one row has no next, whatever the tensor says
 
     def batch_async(self, row_start, length, pages, rows, max_new=None, first=None, prefix=None):
         """The batch of the next calls: int32 device tensors row_start
