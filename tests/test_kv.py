@@ -131,7 +131,7 @@ def test_one_row_has_no_stride():
     import torch
     c = bare()
     x = torch.zeros(3, 700, dtype=torch.bfloat16)
-    for t in (x[:1, :512].unflatten(1, (8, 64)), torch.zeros(1, 1, 8, 64, dtype=torch.bfloat16).expand(1, 1, 8, 64)[0],
+    for t in (x.as_strided((1, 8, 64), (700, 64, 1)), x[:1, :512].unflatten(1, (8, 64)), torch.zeros(1, 1, 8, 64, dtype=torch.bfloat16).expand(1, 1, 8, 64)[0],
               torch.zeros(8, 64, dtype=torch.bfloat16).as_strided((1, 8, 64), (1, 64, 1))):
         assert c._row_array(t, "q", 8) == (t.data_ptr(), 512)
     assert c._row_array(x[:, :512].unflatten(1, (8, 64)), "q", 8) == (x.data_ptr(), 700)
