@@ -109,7 +109,9 @@ int ttl_kv_batch_async(ttl_kv *handle, uint32_t seqs, uint32_t rows, uint32_t ma
  * `layer`, K rotated by its position (rotate != 0), and writes Q
  * [rows][q_heads][head_dim], rotated, to q_out (q and q_out NULL: no Q;
  * q_out == q with the same stride rotates in place).  Strides are elements
- * between rows; base pointers and strides are multiples of 16 bytes.  With a
+ * between rows; base pointers and strides are multiples of 16 bytes.  What a
+ * call writes must not overlap the rows that it reads, nor one output another
+ * (views of one array with one stride may lie side by side).  With a
  * 4-bit cache a block's scale is 2^(floor(log2 max|x|) - 2), codes round to
  * nearest, ties to even; a block that holds an infinity or NaN becomes NaN.
  * Two rows must not share a slot. */

@@ -1247,6 +1247,43 @@ def test_calls_after_a_batch_that_was_only_captured():
     assert torch.equal(outs[0], s.dev["q"]) and torch.equal(outs[2], k) and torch.equal(outs[3], v)
 
 
+def test_overlapping_rows_are_refused():
+    """What a call writes and what it reads lie apart; views of one array side by
+    side do."""
+    n, H, KV, D = 5, 4, 2, 64
+    s = Setup("bf16", None, H, KV, D, 16, new=(n,), length=(20,), freq=100.0 ** (-np.arange(32) / 32))
+    s.fill().plan()
+    c = s.cache
+    flat = torch.randn(4 * n * (H + 2 * KV) * D, device="cuda").bfloat16()
+
+    def rows(start, heads, stride, count=n):
+        return flat[start:].as_strided((count, heads, D), (stride, D, 1), start)
+
+    S = (H + 2 * KV) * D
+    q, k, v = rows(0, H, S), rows(H * D, KV, S), rows((H + KV) * D, KV, S)
+    kw, other = dict(k=k, v=v, q=q), torch.empty(n, H, D, dtype=s.dt, device="cuda")
+    for q_out, what in ((rows(D, H, S), "q"), (rows(2 * S, H, S), "q"), (rows(KV * D, H, S), "q"), (rows(S - D, H, S), "q"),
+                        (rows(8, H, H * D), "q"), (rows(H * D + 8, H, S), "q"), (rows(H * D, H, S), "k")):
+        with pytest.raises(RuntimeError, match=f"q_out overlaps {what}"):
+            c.append_async(0, **kw, q_out=q_out)
+    with pytest.raises(RuntimeError, match="q_out overlaps v"):
+        c.append_async(0, k, rows(10 * S, KV, S), q=other, q_out=rows(10 * S, H, S))
+    for out in (rows(D, H, S), rows(S, H, S), rows(8, H, H * D)):
+        with pytest.raises(RuntimeError, match="out overlaps q"):
+            c.attend_async(0, q, out)
+    for v_out in (k, rows(H * D + 8, KV, S), rows(H * D + S, KV, S)):
+        with pytest.raises(RuntimeError, match="v overlaps k"):
+            c.read_async(0, k, v_out)
+    # apart: in place, side by side, behind one another
+    c.append_async(0, **kw, q_out=q)
+    c.attend_async(0, rows(2 * KV * D, H, S), rows(n * S + 2 * KV * D, H, S))
+    c.attend_async(0, rows(0, H, 2 * H * D), rows(H * D, H, 2 * H * D))
+    c.attend_async(0, rows(H * D, H, 2 * H * D), rows(0, H, 2 * H * D))
+    c.read_async(0, rows(0, KV, 2 * KV * D), rows(KV * D, KV, 2 * KV * D))
+    c.read_async(0, rows(0, KV, KV * D), rows(n * KV * D, KV, KV * D))
+    c.sync()
+
+
 def test_refusals():
     import ttl_moe
     s = Setup("bf16", None, 8, 2, 64, 16, new=(2,), length=(5,))

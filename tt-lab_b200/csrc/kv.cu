@@ -869,6 +869,29 @@ int check_rows(ttl_kv *h, const void *p, size_t stride, int heads, const char *n
     return TTL_OK;
 }
 
+// Two row arrays of a call, one of which is written, that share memory: blocks write
+// in no order what others still read.  Rows of one stride may lie side by side (views
+// of one projection); of different strides they must not interleave.
+int check_apart(ttl_kv *h, const void *out, size_t out_stride, int out_heads, const char *out_name, const void *in, size_t in_stride,
+                int in_heads, const char *in_name) {
+    if (h->rows == 0) {
+        return TTL_OK;
+    }
+    const size_t size = type_size(h->rows_type), rows = size_t(h->rows), so = out_stride * size, si = in_stride * size;
+    const size_t wo = size_t(out_heads) * h->dim * size, wi = size_t(in_heads) * h->dim * size;
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
+    if (o + (rows - 1) * so + wo <= i || i + (rows - 1) * si + wi <= o) {
+        return TTL_OK;
+    }
+    if (rows > 1 && so == si) {
+        const size_t from = i >= o ? (i - o) % so : (so - (o - i) % so) % so;  // of in's rows behind out's
+        if (from >= wo && from + wi <= so) {
+            return TTL_OK;
+        }
+    }
+    return kv_fail(h, TTL_ERR_ARGUMENT, std::string(out_name) + " overlaps " + in_name);
+}
+
 int check_layer(ttl_kv *h, int layer) {
     if (layer < 0 || layer >= h->layers) {
         return kv_fail(h, TTL_ERR_ARGUMENT, "layer " + std::to_string(layer) + " out of range");
@@ -1177,6 +1200,9 @@ int kv_append(ttl_kv *h, int layer, int rotate, const void *k, size_t k_stride, 
     rc = rc ? rc : check_rows(h, v, v_stride, h->kv_heads, "v");
     rc = (rc || !q) ? rc : check_rows(h, q, q_stride, h->q_heads, "q");
     rc = (rc || !q) ? rc : check_rows(h, q_out, q_out_stride, h->q_heads, "q_out");
+    rc = (rc || !q || q == q_out) ? rc : check_apart(h, q_out, q_out_stride, h->q_heads, "q_out", q, q_stride, h->q_heads, "q");
+    rc = (rc || !q) ? rc : check_apart(h, q_out, q_out_stride, h->q_heads, "q_out", k, k_stride, h->kv_heads, "k");
+    rc = (rc || !q) ? rc : check_apart(h, q_out, q_out_stride, h->q_heads, "q_out", v, v_stride, h->kv_heads, "v");
     if (rc || h->rows == 0) {
         return rc;
     }
@@ -1204,6 +1230,7 @@ int kv_read(ttl_kv *h, int layer, void *k, size_t k_stride, void *v, size_t v_st
     TTL_KV_CUDA(h, guard.error);
     rc = check_rows(h, k, k_stride, h->kv_heads, "k");
     rc = rc ? rc : check_rows(h, v, v_stride, h->kv_heads, "v");
+    rc = rc ? rc : check_apart(h, v, v_stride, h->kv_heads, "v", k, k_stride, h->kv_heads, "k");
     if (rc || h->rows == 0) {
         return rc;
     }
@@ -1238,6 +1265,7 @@ int kv_attend(ttl_kv *h, int layer, uint32_t flags, const void *q, size_t q_stri
     TTL_KV_CUDA(h, guard.error);
     rc = check_rows(h, q, q_stride, h->q_heads, "q");
     rc = rc ? rc : check_rows(h, out, out_stride, h->q_heads, "out");
+    rc = rc ? rc : check_apart(h, out, out_stride, h->q_heads, "out", q, q_stride, h->q_heads, "q");
     rc = (rc || !sinks) ? rc : check_pointer(h, sinks, "sinks", 4);
     rc = (rc || !slopes) ? rc : check_pointer(h, slopes, "slopes", 4);
     if (rc || h->rows == 0) {
