@@ -33,3 +33,12 @@ def layer32():
 @pytest.fixture(scope="session")
 def layer128():
     return synth_layer(1, 128)
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_pyfunc_call(pyfuncitem):
+    """A test that asks for the compiled reference (oracle/_ref) where it is not
+    built is skipped when it gets there, as those are that ask beforehand."""
+    outcome = yield
+    if outcome.excinfo and isinstance(outcome.excinfo[1], OSError) and "reference oracle not built" in str(outcome.excinfo[1]):
+        outcome.force_exception(pytest.skip.Exception(str(outcome.excinfo[1])))
