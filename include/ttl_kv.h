@@ -17,17 +17,20 @@
  * device memory is allocated in ttl_kv_create.  The _async calls take device
  * pointers of the handle's GPU, enqueue on the handle's stream, allocate
  * nothing, never wait, and may be captured into a CUDA graph (capture on the
- * handle's stream; a batch call inside a capture sets the row count and the
- * kernels of the calls that follow it, captured or not, though the plan on the
- * device is still the earlier one).  Calls on one handle, and graphs captured from them, share
+ * handle's stream).  Calls on one handle, and graphs captured from them, share
  * the handle's plan and workspace: they must run one after another, never at
- * the same time on two streams.  A graph that holds an append, read or attend
- * without its batch call uses the plan of the last batch call that ran on the
- * device.  It reads as many rows of its arrays as the batch had when it was
- * captured; where the plan has another number of rows, ttl_kv_sync reports it,
- * and only the rows that both have are stored or written.  Where an attend's
- * plan asks for other kernels than the captured ones (max_new and the number of
- * sequences choose them), ttl_kv_sync reports it and out is left as it was.
+ * the same time on two streams.
+ *
+ * Graphs.  A graph that holds an append, read or attend without its batch call
+ * uses the plan of the last batch call that ran on the device.  It reads as
+ * many rows of its arrays as the batch had when it was captured; where the plan
+ * has another number of rows, ttl_kv_sync reports it, and only the rows that
+ * both have are stored or written (a call captured with no rows is not in the
+ * graph).  Where an attend's plan asks for other kernels than the captured ones
+ * (max_new and the number of sequences choose them), ttl_kv_sync reports it and
+ * out is left as it was.  A batch call inside a capture sets the row count and
+ * the kernels of the calls that follow it, captured or not, though the plan on
+ * the device is still the earlier one until the graph runs.
  *
  * What only the device can see (row_start, length, page ids) is checked there:
  * a sequence with bad numbers is skipped (its rows are left as they were), a
@@ -132,9 +135,13 @@ int ttl_kv_read_async(ttl_kv *handle, int layer, void *k, size_t k_stride, void 
  *   the head's sink, which adds to the sum and has no value row
  * A row that sees nothing is zero.  Values of positions a row does not see
  * never reach it, infinities and NaN included.  f16 and bf16 rows: products
- * on the tensor cores, sums in 32 bits, weights rounded to the rows' type (over
- * a 4-bit cache to f16 or bf16; of its values, those below 2^-124 may count as
- * zero). */
+ * on the tensor cores, sums in 32 bits, weights rounded to the rows' type.  Over
+ * a 4-bit cache they are rounded to f16 where few rows of a sequence are new and
+ * to bf16 in bf16 prompts, so a row's last bits may depend on the batch that it
+ * is in; of the cache's values, those below 2^-124 may count as zero.  A column
+ * that meets an infinity or NaN in a place that it does not see (but for slots
+ * behind the sequence's end, which cost nothing) or sees one is computed again
+ * in 32-bit arithmetic, which takes up to 300 times as long. */
 int ttl_kv_attend_async(ttl_kv *handle, int layer, uint32_t flags, const void *q, size_t q_stride, void *out,
                         size_t out_stride, float scale, float cap, const float *sinks, const float *slopes);
 

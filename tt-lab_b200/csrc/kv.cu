@@ -505,9 +505,11 @@ __device__ __forceinline__ void cos_sin(double turn, const double2 *table, doubl
 // 32; K's cosines and sines are pairs of f32 and its codes are rounded once,
 // from about 48 bits, so that they are those of the exact rotation.
 // Every row is read and written once.  16384 bf16 rows of 64 query and 8 KV heads
-// of 64 values into 4 bits (311 MB): 75 us, 4.1 TB/s, the integer pipe busy in half
-// of all clocks with the 48-bit rotation and the codes; 509-row chunks of 16 bits
-// 12 us, one token 5 us, of which most is the chain from the page id to the store.
+// of 64 values into 4 bits (311 MB): 75 us, 4.1 TB/s.  No unit is full (issue 55 % of
+// clocks, integer pipe 49 %, a third of the warps): a CTA is one chain of loads,
+// cosines, barrier, rotation and stores, and three of them on an SM do not cover it.
+// 509-row chunks of 16 bits 12 us, one token 5 us, of which most is the chain from
+// the page id to the store.
 template <int kRows, int kCache, int D>
 __global__ void __launch_bounds__(kAppendThreads, 3) kv_append_kernel(AppendArgs a) {
     constexpr bool kFour = kCache == kMxfp4;
@@ -729,8 +731,9 @@ struct ReadArgs {
 };
 
 // A CTA takes a few rows; a thread keeps its 8 values of a head and goes through
-// the rows with them, their loads in flight together.  Memory-bound: 16384 rows
-// of 8 heads of 64 values out of 4 bits to bf16 (43 MB) 16 us.
+// the rows with them, their loads in flight together.  16384 rows of 8 heads of 64
+// values out of 4 bits to bf16 (43 MB) 16 us, 2.7 TB/s, two fifths of a copy's rate:
+// a lane asks for 4 bytes of codes and one of scale at a time.
 template <int kRows, int kCache, int D> __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     __shared__ const uint8_t *slots[kAppendRows];
     __shared__ int tokens[kAppendRows];

@@ -13,7 +13,9 @@
 // whatever the batch's shape, in one wave; a tile cut by a CTA border leaves
 // partial sums in the workspace, and the CTA that arrives last merges them, in
 // the order of the keys, so results do not depend on timing.  (A second kernel
-// for the merges, in place of the last CTA, cost 7 to 10 us more per call.)
+// for the merges, in place of the last CTA, cost 7 to 10 us more per call.)  The
+// plan takes 6 us on the device, once for all layers of a batch; times in these
+// files that say so hold it.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -262,6 +264,83 @@ __device__ __forceinline__ float capped(float dot, float in, float out) {
     return t <= 0.0625f ? small : fmaf(-2.0f * out, r, out);
 }
 
+// The same for |x / cap| up to kSmallScore: tanh y = y P(y^2) without the
+// special-function unit, P fitted to tanh(y) / y over y <= 0.5 for the least
+// relative error (1.4e-8).  Two at a time (one instruction works on a pair of f32):
+// x, y raw products, to log2 units; scale and ratio bring them there and to x / cap.
+constexpr float kSmallScore = 0.5f;
+__device__ __forceinline__ void capped_small(float &x, float &y, float scale, float ratio) {
+    asm("{\n\t.reg .b64 x, r, t, p, c;\n\t"
+        "mov.b64 x, {%0, %1};\n\t"
+        "mov.b64 c, {%3, %3};\n\tmul.rn.f32x2 r, x, c;\n\tmul.rn.f32x2 t, r, r;\n\t"
+        "mov.b64 c, {%2, %2};\n\tmul.rn.f32x2 x, x, c;\n\t"
+        "mov.b64 p, {%4, %4};\n\t"
+        "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mov.b64 c, 0x3f8000003f800000;\n\tfma.rn.f32x2 p, p, t, c;\n\t"
+        "mul.rn.f32x2 x, x, p;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(scale), "f"(ratio), "f"(0.017134985f), "f"(-0.052986064f), "f"(0.13324779f), "f"(-0.33333069f));
+}
+// x = x * f + (b + c), with b a pair.
+__device__ __forceinline__ void bias_pair(float &x, float &y, float f, float b0, float b1, float c) {
+    asm("{\n\t.reg .b64 x, b, c;\n\t"
+        "mov.b64 x, {%0, %1};\n\tmov.b64 b, {%3, %4};\n\tmov.b64 c, {%5, %5};\n\tadd.rn.f32x2 b, b, c;\n\t"
+        "mov.b64 c, {%2, %2};\n\tfma.rn.f32x2 x, x, c, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(f), "f"(b0), "f"(b1), "f"(c));
+}
+
+// Pairs of f32 in one instruction: x * f + c, and a + b.
+__device__ __forceinline__ void fma_pair(float &x0, float &x1, float f, float c) {
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 d, {%3, %3};\n\t"
+        "fma.rn.f32x2 a, a, b, d;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(x0), "+f"(x1)
+        : "f"(f), "f"(c));
+}
+__device__ __forceinline__ void add_pair(float &a0, float &a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
+}
+// 2^x and 2^y on the multiply-add units, for x, y <= 127; 0 from -127 on.  x = n +
+// f with n the nearest integer (it comes out of the sum with 1.5 * 2^23), 2^f by a
+// polynomial fitted over [-1/2, 1/2] with P(0) = 1 for the least relative error
+// (9e-8), n added to its exponent: at -127 that leaves the zero word.  NaN gives 0:
+// the caller looks for it in the maximum.
+__device__ __forceinline__ void pow2_pair(float x, float y, float &px, float &py) {
+    uint32_t bx, by;
+    asm("{\n\t.reg .b64 x, t, r, p, c;\n\t.reg .b32 tx, ty, qx, qy;\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 c, 0x4b4000004b400000;\n\tadd.rn.f32x2 t, x, c;\n\t"
+        "mov.b64 c, 0xcb400000cb400000;\n\tadd.rn.f32x2 r, t, c;\n\t"
+        "mov.b64 c, 0xbf800000bf800000;\n\tfma.rn.f32x2 x, r, c, x;\n\t"
+        "mov.b64 p, {%4, %4};\n\t"
+        "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, {%8, %8};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 c, 0x3f8000003f800000;\n\tfma.rn.f32x2 p, p, x, c;\n\t"
+        "mov.b64 {tx, ty}, t;\n\tmov.b64 {qx, qy}, p;\n\t"
+        "mad.lo.u32 %0, tx, 8388608, qx;\n\tmad.lo.u32 %1, ty, 8388608, qy;\n\t}"
+        : "=r"(bx), "=r"(by)
+        : "f"(fmaxf(x, -127.0f)), "f"(fmaxf(y, -127.0f)), "f"(0.001326472731307149f), "f"(0.009671512991189957f),
+          "f"(0.05550733581185341f), "f"(0.24022242426872253f), "f"(0.6931470036506653f));
+    px = __uint_as_float(bx), py = __uint_as_float(by);
+}
+// Largest and smallest of three; NaN if any is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Whether the plan on the device is of this call's shape; where it is not, says so.
 // A captured call may meet the plan of another batch.  That plan's work may lie
 // with the other kind as well, which the call did not launch, so both kinds are
@@ -338,84 +417,6 @@ struct Walker {
         return true;
     }
 };
-
-// The same for |x / cap| up to kSmallScore: tanh y = y P(y^2) without the
-// special-function unit, P fitted to tanh(y) / y over y <= 0.5 for the least
-// relative error (1.4e-8).  scaled: x in log2 units, ratio: x / cap.
-constexpr float kSmallScore = 0.5f;
-//
-// Two at a time (one instruction works on a pair of f32): x, y raw products.
-__device__ __forceinline__ void capped_small(float &x, float &y, float scale, float ratio) {
-    asm("{\n\t.reg .b64 x, r, t, p, c;\n\t"
-        "mov.b64 x, {%0, %1};\n\t"
-        "mov.b64 c, {%3, %3};\n\tmul.rn.f32x2 r, x, c;\n\tmul.rn.f32x2 t, r, r;\n\t"
-        "mov.b64 c, {%2, %2};\n\tmul.rn.f32x2 x, x, c;\n\t"
-        "mov.b64 p, {%4, %4};\n\t"
-        "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
-        "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
-        "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, t, c;\n\t"
-        "mov.b64 c, 0x3f8000003f800000;\n\tfma.rn.f32x2 p, p, t, c;\n\t"
-        "mul.rn.f32x2 x, x, p;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(x), "+f"(y)
-        : "f"(scale), "f"(ratio), "f"(0.017134985f), "f"(-0.052986064f), "f"(0.13324779f), "f"(-0.33333069f));
-}
-// x = x * f + (b + c), with b a pair.
-__device__ __forceinline__ void bias_pair(float &x, float &y, float f, float b0, float b1, float c) {
-    asm("{\n\t.reg .b64 x, b, c;\n\t"
-        "mov.b64 x, {%0, %1};\n\tmov.b64 b, {%3, %4};\n\tmov.b64 c, {%5, %5};\n\tadd.rn.f32x2 b, b, c;\n\t"
-        "mov.b64 c, {%2, %2};\n\tfma.rn.f32x2 x, x, c, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(x), "+f"(y)
-        : "f"(f), "f"(b0), "f"(b1), "f"(c));
-}
-
-// Pairs of f32 in one instruction: x * f + c, and a + b.
-__device__ __forceinline__ void fma_pair(float &x0, float &x1, float f, float c) {
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 d, {%3, %3};\n\t"
-        "fma.rn.f32x2 a, a, b, d;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(x0), "+f"(x1)
-        : "f"(f), "f"(c));
-}
-__device__ __forceinline__ void add_pair(float &a0, float &a1, float b0, float b1) {
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(a0), "+f"(a1)
-        : "f"(b0), "f"(b1));
-}
-// 2^x and 2^y on the multiply-add units, for x, y <= 127; 0 from -127 on.  x = n +
-// f with n the nearest integer (it comes out of the sum with 1.5 * 2^23), 2^f by a
-// polynomial fitted over [-1/2, 1/2] with P(0) = 1 for the least relative error
-// (9e-8), n added to its exponent: at -127 that leaves the zero word.  NaN gives 0:
-// the caller looks for it in the maximum.
-__device__ __forceinline__ void pow2_pair(float x, float y, float &px, float &py) {
-    uint32_t bx, by;
-    asm("{\n\t.reg .b64 x, t, r, p, c;\n\t.reg .b32 tx, ty, qx, qy;\n\t"
-        "mov.b64 x, {%2, %3};\n\t"
-        "mov.b64 c, 0x4b4000004b400000;\n\tadd.rn.f32x2 t, x, c;\n\t"
-        "mov.b64 c, 0xcb400000cb400000;\n\tadd.rn.f32x2 r, t, c;\n\t"
-        "mov.b64 c, 0xbf800000bf800000;\n\tfma.rn.f32x2 x, r, c, x;\n\t"
-        "mov.b64 p, {%4, %4};\n\t"
-        "mov.b64 c, {%5, %5};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
-        "mov.b64 c, {%6, %6};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
-        "mov.b64 c, {%7, %7};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
-        "mov.b64 c, {%8, %8};\n\tfma.rn.f32x2 p, p, x, c;\n\t"
-        "mov.b64 c, 0x3f8000003f800000;\n\tfma.rn.f32x2 p, p, x, c;\n\t"
-        "mov.b64 {tx, ty}, t;\n\tmov.b64 {qx, qy}, p;\n\t"
-        "mad.lo.u32 %0, tx, 8388608, qx;\n\tmad.lo.u32 %1, ty, 8388608, qy;\n\t}"
-        : "=r"(bx), "=r"(by)
-        : "f"(fmaxf(x, -127.0f)), "f"(fmaxf(y, -127.0f)), "f"(0.001326472731307149f), "f"(0.009671512991189957f),
-          "f"(0.05550733581185341f), "f"(0.24022242426872253f), "f"(0.6931470036506653f));
-    px = __uint_as_float(bx), py = __uint_as_float(by);
-}
-// Largest and smallest of three; NaN if any is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ float min3(float a, float b, float c) {
-    float d;
-    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 
 // Slots behind a sequence's end hold what was left there, and 0 * NaN is NaN in every
 // column, so V's values there become 0 before the product: by a warp, `rows` rows of

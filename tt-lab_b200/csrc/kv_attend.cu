@@ -23,8 +23,10 @@ namespace {
 // into weights (a warp: a column at a time) and adds the weighted values (a
 // thread: four values of CT * D / 1024 columns).  For f32 rows alone, whose
 // products the tensor cores would round.  A single token bounds it by latency:
-// 64 query and 8 KV heads over 1040 keys (4.3 MB) 15.3 us; prompts by the 32-bit
-// multiply-adds, fed from shared memory.
+// 64 query and 8 KV heads over 1040 keys (4.3 MB) 19.8 us with the plan; prompts by
+// the 32-bit multiply-adds, fed from shared memory, with five barriers per granule:
+// 1024 rows 578 us, 15 TFLOP/s.  64 tokens over 4096 keys in 4 bits 729 us, where
+// bf16 rows take 57: a byte is loaded for every code and another for its scale.
 constexpr int kSimpleThreads = 256;
 constexpr int kSimpleGran = 64;
 
@@ -275,9 +277,9 @@ namespace {
 // Sequences of more columns than the widest tile of the kernel for few columns
 // go to the prompt kernel: from there on that one would read the cache more
 // than once.  64 sequences of 4096 keys, bf16, 8 KV heads: D = 64, 32 columns
-// 137 us against the prompt kernel's 177, 64 columns 249 against 178; over 4
-// bits 168 and 253, 325 and 252; D = 128, 16 columns 181 and 205, 32 columns 340
-// and 210.
+// 129 us against the prompt kernel's 171, 64 columns 230 against 173; over 4
+// bits 172 and 243, 316 and 238; D = 128, 16 columns 189 and 210, 32 columns 342
+// and 212.
 constexpr int few_columns(int dim) {
     return dim == 128 ? 16 : 32;
 }

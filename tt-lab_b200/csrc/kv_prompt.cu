@@ -25,15 +25,20 @@
 // 4-bit cache four turn codes into bf16.  The scores of the half after next are
 // issued right behind the product of this one, over the weights it has just read.
 //
-// Measured: a 4096-token prompt of 64 query and 8 KV heads, D = 64, bf16: 249 us,
-// 552 TFLOP/s of the 1675 that a plain product reaches; the special-function
-// unit alone needs 88 us, the tensor pipe (25 % busy) 82.  A half takes a warp
-// about 1900 clocks: 400 for loads and the maximum, 900 for the weights, the rest
-// for hand-overs, with one other warp on its scheduler to fill the gaps; the third
-// that would need 576 columns of tensor memory.  Ends of tiles are 7 %.  f16
-// chunks of up to 509 rows, D = 128, a cap: 112 us, 358 TFLOP/s: the cap's
-// polynomial is 16 multiply-adds per pair of scores.  A 1500-token prompt over 4
-// bits with a distance bias: 115 us, where the four expanding warps cost about 15.
+// Measured, with the plan's 6 us: a 4096-token prompt of 64 query and 8 KV heads, D
+// = 64, bf16: 252 us, 545 TFLOP/s of the 1675 that a plain product reaches; the
+// special-function unit alone needs 88 us (40 % busy), the tensor pipe (27 %) 82.  A
+// half takes a warp about 1900 clocks: 400 for loads and the maximum, 900 for the
+// weights, the rest for hand-overs, with one other warp on its scheduler to fill the
+// gaps; the third that would need 576 columns of tensor memory.  Ends of tiles are
+// 7 %.  f16 chunks of up to 509 rows, D = 128, a cap: 124 us, 323 TFLOP/s.  A
+// 1500-token prompt over 4 bits with a distance bias: 120 us, of which the four
+// expanding warps cost about 15.  In these two a CTA has 20 to 25 granules in two or
+// three pieces: starts, ends and merges weigh more, and the plan's equal shares come
+// out unequal, the last CTA 15 % behind the mean.
+//
+// Registers: 64-wide heads over 16 bits keep everything in them; 128-wide ones spill
+// 32 bytes, over 4 bits 56 (64-wide) and 224.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

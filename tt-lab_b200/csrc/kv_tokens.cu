@@ -33,15 +33,19 @@
 // largest scale a column has seen in the block, so that it stays in f16's
 // range whatever the values' size.
 //
-// Measured: 128 single tokens over 1 to 8192 keys, 64 query and 8 KV heads, D =
-// 64, bf16 (985 MB): 150 to 153 us, 6.5 TB/s, a plain copy's rate.  One token over
-// 131072 keys (268 MB): 53 us, 41 of them at that rate; the rest is the launch,
-// the first loads and the merge of 55 parts a head.  256 tokens with a window of
-// 128 (70 MB): 24.6 us: the two or three granules of a sequence leave nothing to
-// fetch ahead, and each waits for the page ids that name it.  64 tokens over 4
-// bits, up to 16384 keys (287 MB): 91 us, 3.2 TB/s: the schedulers issue in 60 % of
-// all clocks, with the integer pipe busy in 52 %, for taking codes apart, so the
-// bytes, 44 us of them, do not bound it.
+// Measured, with the plan's 6 us: 128 single tokens over 1 to 8192 keys, 64 query
+// and 8 KV heads, D = 64, bf16 (985 MB): 151 to 156 us, 6.3 to 6.5 TB/s, a plain
+// copy's rate.  One token over 131072 keys (268 MB): 58 us, 41 of them at that rate;
+// the rest is two launches, the first loads and the merge of 55 parts a head.  256
+// tokens with a window of 128 (70 MB): 29.5 us: the two or three granules of a
+// sequence leave nothing to fetch ahead, and each waits for the page ids that name
+// it.  64 tokens over 4 bits, up to 16384 keys (287 MB): 96 us, 3 TB/s: the
+// schedulers issue in 58 % of all clocks, with the integer pipe busy in 53 %, for
+// taking codes apart, so the bytes, 44 us of them, do not bound it.
+//
+// Registers: tiles of 8 columns, which single tokens have, keep everything in them.
+// Wider ones spill: 16 columns of 128-wide heads 84 to 164 bytes, 32 columns 104 to
+// 320, in loops that are bound elsewhere or had no narrower form that was faster.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
