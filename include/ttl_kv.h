@@ -135,7 +135,8 @@ int ttl_kv_read_async(ttl_kv *handle, int layer, void *k, size_t k_stride, void 
  *   the head's sink, which adds to the sum and has no value row
  * A row that sees nothing is zero.  Values of positions a row does not see
  * never reach it, infinities and NaN included.  f16 and bf16 rows: products
- * on the tensor cores, sums in 32 bits, weights rounded to the rows' type.  Over
+ * on the tensor cores, sums in 32 bits (over n keys of one CTA's part good to
+ * n * 2^-24 of their size), weights rounded to the rows' type.  Over
  * a 4-bit cache they are rounded to f16 where few rows of a sequence are new and
  * to bf16 in bf16 prompts, so a row's last bits may depend on the batch that it
  * is in; of the cache's values, those below 2^-124 may count as zero.  A column

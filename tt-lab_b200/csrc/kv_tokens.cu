@@ -39,13 +39,13 @@
 // the rest is two launches, the first loads and the merge of 55 parts a head.  256
 // tokens with a window of 128 (70 MB): 29.5 us: the two or three granules of a
 // sequence leave nothing to fetch ahead, and each waits for the page ids that name
-// it.  64 tokens over 4 bits, up to 16384 keys (287 MB): 96 us, 3 TB/s: the
+// it.  64 tokens over 4 bits, up to 16384 keys (287 MB): 95 us, 3 TB/s: the
 // schedulers issue in 58 % of all clocks, with the integer pipe busy in 53 %, for
 // taking codes apart, so the bytes, 44 us of them, do not bound it.
 //
 // Registers: tiles of 8 columns, which single tokens have, keep everything in them.
-// Wider ones spill: 16 columns of 128-wide heads 84 to 164 bytes, 32 columns 104 to
-// 320, in loops that are bound elsewhere or had no narrower form that was faster.
+// Wider ones spill: 16 columns of 128-wide heads 64 to 100 bytes, 32 columns 124 to
+// 228, in loops that are bound elsewhere or had no narrower form that was faster.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -73,11 +73,12 @@ template <int kRows, int kCache, int D, int NT> struct TokenShape {
     // (128 tokens of 64 values: three granules 151 us, five 158, six 162), less too
     // (two: 161); with three CTAs on an SM 160.
     static constexpr int kStages = D == 64 || kFour ? 3 : 2;
-    // Parts that a lane merges at once.  Twice as many take registers from the loop
-    // over the keys: 64 sequences of two rows, D = 128, 189 us, with eight 226 (four
-    // rows, D = 64: 127 and 171; over 4 bits, two rows 99, with four 105); one token
-    // over 131072 keys gains 1 us by eight.
-    static constexpr int kMergeBatch = kFour ? 2 : 4;
+    // Parts that a lane merges at once.  More of them take registers from the loop over
+    // the keys: 64 sequences of two rows, D = 128, 189 us, with eight 226 (four rows, D
+    // = 64: 127 and 171; over 4 bits one row, D = 128, 92, with two 96, with three 100).
+    // Fewer wait longer where parts are many: one token over 131072 keys 2 us more with
+    // two, 4 us with one; over 4 bits, where the loop is what counts, 6 us less.
+    static constexpr int kMergeBatch = kFour ? 1 : 4;
     // A column's sums in shared memory: over a 16-bit cache rows of D values whose
     // groups of 8 are swapped by the column, over 4 bits rows with 4 values of
     // padding; either way the accumulators' stores do not collide.
